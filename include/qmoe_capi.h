@@ -4,7 +4,8 @@
  * expert dispatch (histogram / scan / permute), the grouped SwiGLU expert
  * GEMM (MFMA, prefill) and GEMV (decode), the weighted combine, the QKV
  * projection with per-head RMSNorm + RoPE epilogue, and causal GQA attention
- * over a contiguous KV cache.
+ * over a contiguous KV cache, over a prefix that a batch shares, and over a
+ * cache of bounded size that keeps the entries with the most attention weight.
  *
  * Conventions shared by every entry point
  *   - All tensor arguments are caller-owned device pointers; outputs and
@@ -83,7 +84,10 @@ typedef void* qmoe_stream_t;
  * QMOE_DECODE_BLOCK_STATE_BYTES of call-to-call state (zeroed before first use).
  * 3: qmoe_moe_experts_grouped takes the tile table non-const (word 3 of each
  * live row counts finished gate_up panels during the call), and
- * qmoe_attn_prefill_ws / qmoe_attn_prefill_workspace are new. */
+ * qmoe_attn_prefill_ws / qmoe_attn_prefill_workspace are new.  Entry points
+ * added since leave the earlier ones as they were: qmoe_attn_shared,
+ * qmoe_attn_prefill_scored, qmoe_attn_decode_scored, qmoe_kv_append,
+ * qmoe_kv_evict and their workspace queries. */
 #define QMOE_VERSION 3
 
 int qmoe_version(void);
@@ -518,6 +522,127 @@ int qmoe_attn_decode(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf
                      const int32_t* ctx_len, int64_t B, int64_t Hq, int64_t Hkv, int64_t D,
                      int64_t S_max, float scale, float* partial, qmoe_bf16* out,
                      qmoe_stream_t stream);
+
+/* Attention of a batch whose sequences share their first P tokens.  The
+ * prefix's keys and values are held once (not per sequence); each sequence has
+ * a cache of its own for what follows.  Query s of row b attends to all P
+ * prefix entries and to the first
+ *   clamp(ctx_len[b] + s, 0, min(max_ctx, S_max))
+ * entries of its own cache (decode: S = 1 and ctx_len counts the new token's
+ * entry; a chunk whose tokens start at own entry e: ctx_len = e + 1).  A query
+ * that sees nothing gets zeros.
+ *   q: bf16 [B*S, Hq, D]; k_prefix, v_prefix: bf16 [Hkv, P_max, D], of which
+ *   entries [0, P) are read; k_cache, v_cache: bf16 [B, Hkv, S_max, D]; ctx_len:
+ *   i32 [B]; max_ctx <= S_max: no query sees more own entries (sizes the
+ *   launch, as qmoe_attn_decode_bucket's); scale > 0; workspace:
+ *   qmoe_attn_shared_workspace(B, S, Hq, Hkv, D, P, max_ctx) bytes (NULL when
+ *   that is 0), holding nothing between calls; calls that share one must not
+ *   overlap.  out: bf16 [B*S, Hq*D].
+ *   The entries that some query of a chunk sees have to be finite (a NaN value
+ *   reaches the queries that do not see it); entries past them are not read.
+ *   Deterministic.  Limits: D == 128, Hq / Hkv <= 16, P_max and S_max <= 2^22,
+ *   B * S * Hq < 2^27.
+ * Replaces: the token-generation and context-encoding attention of
+ *   NeuronQwen3MoEAttention (qwen_with_nki.py:9943-9946, 10081-10109) for a
+ *   batch with a common prompt, whose cache rows the reference repeats. */
+int qmoe_attn_shared(const qmoe_bf16* q, const qmoe_bf16* k_prefix, const qmoe_bf16* v_prefix, int64_t P,
+                     int64_t P_max, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache, const int32_t* ctx_len,
+                     int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max, int64_t max_ctx,
+                     float scale, void* workspace, int64_t workspace_bytes, qmoe_bf16* out, qmoe_stream_t stream);
+
+/* Workspace bytes of qmoe_attn_shared on the current device (-1 for bad sizes).
+ * Replaces: nothing in the reference (a sizing helper of this library). */
+int64_t qmoe_attn_shared_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t P,
+                                   int64_t max_ctx);
+
+/* Causal GQA attention of a prompt chunk (as qmoe_attn_prefill: query s sits at
+ * cache index start + s and sees entries [0, start + s]) that also adds, for
+ * every entry j of [0, start + S) and kv head, the attention weight it got:
+ *   scores[b, kvh, j] += sum over queries s < lengths[b] and the q heads of
+ *                        the group of softmax weight(b, s, head, j)
+ *   lengths: i32 [B], the queries of a right-padded row that count (clamped
+ *   into [0, S]; their own outputs are computed all the same), or NULL: all;
+ *   scores: f32 [B, Hkv, S_max]; entries past start + S are not touched;
+ *   workspace: qmoe_attn_prefill_scored_workspace(B, S, Hq, Hkv, D, start)
+ *   bytes, holding nothing between calls; calls that share one must not
+ *   overlap.  Other arguments as qmoe_attn_prefill.  The entries
+ *   [0, start + S) have to be finite.  Deterministic (no atomics).
+ *   Limits: D == 128, Hq / Hkv <= 16, S_max <= 2^22, S * Hq < 2^23,
+ *   B * S * Hq < 2^27, scale > 0.
+ * Replaces: qmoe_attn_prefill's attention (qwen_with_nki.py:25-28, 1251) where
+ *   the cache is cut down afterwards; the scores have no counterpart. */
+int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache, int64_t B,
+                             int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max, int64_t start,
+                             const int32_t* lengths, float scale, void* workspace, int64_t workspace_bytes,
+                             float* scores, qmoe_bf16* out, qmoe_stream_t stream);
+
+/* Workspace bytes of qmoe_attn_prefill_scored on the current device (-1 for bad
+ * sizes).
+ * Replaces: nothing in the reference (a sizing helper of this library). */
+int64_t qmoe_attn_prefill_scored_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t start);
+
+/* Decode attention, one query per row over slots [0, min(ctx_len[b], max_ctx))
+ * (as qmoe_attn_decode_bucket; a row with ctx_len <= 0 gets zeros), that also
+ * adds each slot's attention weight, summed over the group's q heads, to
+ * scores[b, kvh, slot].  Slots past ctx_len are neither read nor scored.
+ *   scores: f32 [B, Hkv, S_max]; workspace:
+ *   qmoe_attn_decode_scored_workspace(B, Hq, D, max_ctx) bytes, holding nothing
+ *   between calls; calls that share one must not overlap.  Deterministic.
+ *   Limits: D == 128, Hq / Hkv <= 16, 0 < max_ctx <= S_max, scale > 0.
+ * Replaces: the token-generation attention (qwen_with_nki.py:9943-9946) over a
+ *   bounded cache; the scores have no counterpart in the reference. */
+int qmoe_attn_decode_scored(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
+                            const int32_t* ctx_len, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max,
+                            int64_t max_ctx, float scale, void* workspace, int64_t workspace_bytes, float* scores,
+                            qmoe_bf16* out, qmoe_stream_t stream);
+
+/* Workspace bytes of qmoe_attn_decode_scored (-1 for bad sizes).
+ * Replaces: nothing in the reference (a sizing helper of this library). */
+int64_t qmoe_attn_decode_scored_workspace(int64_t B, int64_t Hq, int64_t D, int64_t max_ctx);
+
+/* A decode step's projection rows into a cache whose slots are not positions:
+ * per head RMSNorm and RoPE at positions[b] for q and k (as qmoe_qkv_finish), q
+ * to q_out, the K and V rows to slot slots[b] of row b, scores[b, :, slot] = 0
+ * and slot_pos[b, :, slot] = positions[b].  A row whose position is outside
+ * [0, max_pos) or slot outside [0, S_max) writes no cache entry and gets a zero
+ * q.
+ *   qkv: f32 [B, (Hq + 2*Hkv)*D]; positions, slots: i32 [B]; q_out: bf16
+ *   [B, Hq, D]; scores: f32 and slot_pos: i32 [B, Hkv, S_max], each may be
+ *   NULL.  Limits: D == 128.
+ * Replaces: q_layernorm/k_layernorm, RoPE and the KV-cache update of
+ *   NeuronQwen3MoEAttention (qwen_with_nki.py:10102-10103, 10083-10087,
+ *   9943-9946) for a bounded cache. */
+int qmoe_kv_append(const float* qkv, const qmoe_bf16* q_norm_w, const qmoe_bf16* k_norm_w, const float* rope_cos,
+                   const float* rope_sin, int64_t max_pos, const int32_t* positions, const int32_t* slots, int64_t B,
+                   int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max, float eps, qmoe_bf16* q_out,
+                   qmoe_bf16* k_cache, qmoe_bf16* v_cache, float* scores, int32_t* slot_pos, qmoe_stream_t stream);
+
+/* Cuts a cache down to `budget` entries per (row, kv head).  Of a row's
+ * n = clamp(ctx_len[b], 0, S_max) entries, where n > budget, these stay, in this
+ * order of precedence: entries with slot_pos < sink or slot_pos > newest -
+ * recent (newest: the largest slot_pos of the n); then the largest scores (NaN
+ * ranks highest, -0 as 0).  Ties go to the lowest slot.  Kept entries below slot
+ * `budget` stay where they are; the i-th kept entry past it moves to the i-th
+ * freed slot (K, V, score and position).  Afterwards slots [0, min(n, budget))
+ * hold the kept entries; the scores of all other slots are 0 and their
+ * positions -1, their K/V rows as before.  ctx_len is not written.
+ *   k_cache, v_cache: bf16 [B, Hkv, S_max, D]; scores: f32, slot_pos: i32
+ *   [B, Hkv, S_max]; the _out arrays (S_out slots, S_out >= min(budget, S_max))
+ *   are either those same arrays or another cache that does not overlap them,
+ *   in which case the given one is left as it is; 0 <= recent + sink <= budget;
+ *   workspace: qmoe_kv_evict_workspace(B, Hkv, S_max, budget) bytes, holding
+ *   nothing between calls; calls that share one must not overlap.
+ *   Limits: D == 128, B * Hkv < 65536.
+ * Replaces: nothing in the reference, whose cache keeps every token. */
+int qmoe_kv_evict(const qmoe_bf16* k_cache, const qmoe_bf16* v_cache, const float* scores, const int32_t* slot_pos,
+                  const int32_t* ctx_len, int64_t B, int64_t Hkv, int64_t D, int64_t S_max, int64_t budget,
+                  int64_t recent, int64_t sink, void* workspace, int64_t workspace_bytes, int64_t S_out,
+                  qmoe_bf16* k_out, qmoe_bf16* v_out, float* scores_out, int32_t* slot_pos_out,
+                  qmoe_stream_t stream);
+
+/* Workspace bytes of qmoe_kv_evict (-1 for bad sizes).
+ * Replaces: nothing in the reference (a sizing helper of this library). */
+int64_t qmoe_kv_evict_workspace(int64_t B, int64_t Hkv, int64_t S_max, int64_t budget);
 
 /* Token embedding gather into the fp32 residual stream:
  *   out[i, :] = float(table[ids[i], :]);  table: bf16 [V, H]; ids: i64 [n];

@@ -19,6 +19,7 @@
 //                    K/V row is read from HBM once, with every load of the
 //                    wave in flight together; a second kernel merges the
 //                    per-wave partials that hold keys.
+#include "attn_tile.hpp"
 #include "decode_util.hpp"
 #include "gemm.hpp"
 #include "mfma_pipe.hpp"
@@ -28,8 +29,6 @@
 #include <type_traits>
 
 namespace qmoe {
-
-constexpr int HD = 128;  // head_dim
 
 // ====================================================================== QKV
 // Per-(token, head) finish shared by the QKV kernels: PARTS threads (part =
@@ -373,33 +372,9 @@ static int qkv_pipe_launch(const uint16_t* x, const uint16_t* wqkv, const uint16
 
 // ====================================================================== prefill
 constexpr int AP_QT = 128;               // query rows per workgroup (4 waves x 32)
-constexpr int AP_KT = 64;                // keys per step
-constexpr int AP_ROWB = HD * 2;          // bytes per K / V row in LDS (no pad: chunks are swizzled)
-constexpr int AP_TILE = AP_KT * AP_ROWB;  // 16 KB per K or V tile
-constexpr float AP_TAU = 8.0f;           // lazy-max slack (log2 units): p < 2^8 between rescales
 // The tile DMAs address a (batch, kv head) cache slice with 32-bit byte
 // offsets: (S_max + AP_KT) * AP_ROWB must stay below 2^31.
 constexpr int AP_MAX_SMAX = 1 << 22;
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-
-// LDS slot of the 16-byte chunk c of K row r.  A fragment read (ds_read_b128)
-// takes one chunk of 16 consecutive rows; r % 16 puts them on 16 distinct
-// bank groups.
-__device__ __forceinline__ int ap_kslot(int r, int c) { return c ^ (r & 15); }
-// LDS slot of chunk c of V row r.  A transposing read (ds_read_b64_tr_b16)
-// covers, per half-wave, 4 consecutive rows (4-aligned) x 4 consecutive
-// chunks (4-aligned), and per 16-lane group 4 rows x 2 chunks; this XOR keeps
-// both on distinct bank groups.
-__device__ __forceinline__ int ap_vslot(int r, int c) { return c ^ (4 * (r & 3) + 2 * ((r >> 1) & 1)); }
-
-// ds_read_b64_tr_b16: each group of 16 lanes reads a block of 16 x 4 bf16
-// (lane j supplies the address of row j: 4 consecutive elements) and lane i
-// receives column i % 4 of rows i / 4, i / 4 + 4, i / 4 + 8, i / 4 + 12.
-__device__ __forceinline__ s16x4 lds_read_tr16(const uint8_t* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(p));
-}
 
 // start_dev, when not null, holds the chunk start in device memory (read here,
 // clamped into [0, S_max - S]) so a captured graph can replay the same
@@ -800,11 +775,6 @@ constexpr int AD_MAX_G = 16;            // q heads per kv head
 constexpr int AD_VCH = AD_WKEYS * HD / 8 / 64;  // 16-byte V chunks per lane (16)
 constexpr int AD_PSTR = HD + 4;         // partial record: m, l, 2 pad, o[HD] (16-byte aligned o)
 constexpr int AD_MERGE_PF = 16;         // o values the merge requests before the max is known
-
-// Completes this wave's LDS writes before its own lanes read them (a wave's
-// DS instructions run in order; this also keeps the compiler from moving
-// reads above the writes).
-__device__ __forceinline__ void wave_lds_sync() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
 // Query rows: blockIdx.z.  With chunk_start == nullptr each query row is a
 // batch row (cache row = query row) with ctx_len[row] keys; otherwise qpb

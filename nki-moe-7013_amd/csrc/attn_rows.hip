@@ -1,0 +1,551 @@
+// Attention over a cache whose first part a batch shares, and causal attention
+// that also accumulates each cache entry's attention weight (head_dim 128).
+//
+// Query rows are packed: row r of a (batch, kv head) pair is query r / G, head
+// r % G of the GQA group (G = Hq / Hkv), so a 128-row tile reads each key of
+// the kv head once for all of its heads.  Softmax over a concatenation of key
+// runs is associative: a run leaves (m, l, O) with m its maximum, l = sum
+// 2^(s - m) and O = sum 2^(s - m) v; runs join as m = max m_i, l = sum
+// 2^(m_i - m) l_i, O likewise.
+//
+//  attn_rows_kernel   work items of (row tile, key run) over flash_segment.
+//                     Decode (S * G < 128): the prefix is attended by tiles of
+//                     packed rows that span the batch, so its keys are read
+//                     once for every 128 of all B * S * G rows instead of once
+//                     for each sequence; each sequence's own keys are items of
+//                     their own.  Chunks (S * G >= 128): a tile's rows belong
+//                     to one sequence and its item runs over the prefix, then
+//                     over its own keys.
+//  attn_rows_merge_kernel  joins the runs of a row where there are several.
+//  attn_colsum_kernel      w = 2^(s - lse) summed over query rows: the scores
+//                          of a key run against streamed query tiles, after
+//                          the attention left each row's lse = m + log2 l.
+#include "attn_tile.hpp"
+#include "common.hpp"
+
+#include <math.h>
+
+namespace qmoe {
+
+constexpr int AR_ROWS = 128;      // query rows of a tile (4 waves x 32)
+constexpr int AR_REC = HD + 4;    // record of a row's run: m, l, 2 pad, O[HD]
+constexpr int AR_MAX_G = 16;      // q heads per kv head
+constexpr int64_t AR_MAX_KEYS = 1ll << 22;  // keys of one run are addressed with 32-bit byte offsets
+
+struct ArArgs {
+  const uint16_t *q, *kp, *vp, *k, *v;
+  const int32_t* ctx_len;  // own entries that a row's query 0 sees; nullptr: start + 1 for every row
+  const int32_t* lengths;  // queries of a row that count in lse; nullptr: all
+  int P, Pmax, B, S, Hq, Hkv, S_max, max_ctx, start;
+  float scale_log2;
+  uint16_t* out;
+  float* part;  // [B * S * Hq][NS][AR_REC], when NS > 1
+  float* lse;   // [B][Hkv][S * G] or nullptr
+  // NS: runs per row.  n_pre prefix items (rtp row tiles x nsp runs of pt
+  // tiles x Hkv), then items of rts row tiles x nss runs of st tiles x (B, Hkv),
+  // whose key tiles start with the prefix when joint.
+  int NS, n_pre, nsp, pt, rts, nss, st, joint;
+};
+
+// Own entries that query s of batch row b sees.
+__device__ __forceinline__ int ar_sees(const ArArgs& a, int b, int s) {
+  const int c = a.ctx_len ? min(a.ctx_len[b], a.S_max) : a.start + 1;
+  return max(min(c + s, min(a.max_ctx, a.S_max)), 0);
+}
+
+__device__ __forceinline__ float ar_lse(float m, float l) { return l > 0.0f ? m + __log2f(l) : INFINITY; }
+
+__global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];
+  const int lane = threadIdx.x & 63, hl = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const int G = a.Hq / a.Hkv, nPT = (a.P + AP_KT - 1) / AP_KT;
+  const bool pre = int(blockIdx.x) < a.n_pre;
+  int kvh, b = 0, r0, rows, slot, t0, t1;  // key tiles [t0, t1) of the item's list
+  if (pre) {
+    // (kv head, run) fastest: the row tiles of one run sit Hkv * nsp items apart,
+    // on one XCD (and its L2) when that is a multiple of 8
+    const int grp = a.Hkv * a.nsp, x = int(blockIdx.x), y = x % grp;
+    kvh = y % a.Hkv;
+    slot = y / a.Hkv;
+    r0 = x / grp * AR_ROWS;
+    rows = a.B * a.S * G;
+    t0 = slot * a.pt;
+    t1 = min(nPT, t0 + a.pt);
+  } else {
+    // latest row tile (the most keys) first
+    const int grp = a.B * a.Hkv, x = int(blockIdx.x) - a.n_pre, y = x % (grp * a.nss);
+    const int run = y / grp;
+    b = y % grp / a.Hkv;
+    kvh = y % a.Hkv;
+    r0 = (a.rts - 1 - x / (grp * a.nss)) * AR_ROWS;
+    rows = a.S * G;
+    slot = a.nsp + run;
+    const int seen = ar_sees(a, b, min(r0 + AR_ROWS - 1, rows - 1) / G);
+    t0 = run * a.st;
+    t1 = min((a.joint ? nPT : 0) + (seen + AP_KT - 1) / AP_KT, t0 + a.st);
+  }
+  const int rw = r0 + wave * 32;                   // the wave's first row
+  const int row = rw + (lane & 31);                // this lane's row
+  const bool live = row < rows;
+  const int rq = live ? row : rows - 1;            // a row to take the limits of
+  const int sq = rq / G;                           // its query (over the whole batch for prefix items)
+  const int64_t qrow = (pre ? int64_t(sq) : int64_t(b) * a.S + sq) * a.Hq + kvh * G + rq % G;
+  FlashRows st;
+  st.start(live ? a.q + qrow * HD : nullptr, hl);
+  const bool wlive = rw < rows;                    // wave-uniform
+  const int pt1 = pre || a.joint ? min(t1, nPT) : 0, off = a.joint ? nPT : 0;
+  // the list's prefix tiles, then its own-key tiles (one copy of the loop's code)
+#pragma unroll 1
+  for (int seg = 0; seg < 2; ++seg) {
+    const uint16_t *kk = a.kp, *vv = a.vp;
+    int64_t base;
+    int n, lim, first = -1, last = -1;
+    if (seg == 0) {
+      if (t0 >= pt1) continue;
+      const int k0 = t0 * AP_KT;
+      n = min(a.P, pt1 * AP_KT) - k0;
+      base = (int64_t(kvh) * a.Pmax + k0) * HD;
+      lim = first = n - 1;
+      if (wlive) last = n - 1;
+    } else {
+      const int s0 = max(t0, off) - off, s1 = t1 - off;
+      if (pre || s0 >= s1) break;
+      const int k0 = s0 * AP_KT;
+      const int end = min(ar_sees(a, b, min(r0 + AR_ROWS - 1, rows - 1) / G), s1 * AP_KT);
+      n = end - k0;
+      kk = a.k;
+      vv = a.v;
+      base = ((int64_t(b) * a.Hkv + kvh) * a.S_max + k0) * HD;
+      lim = min(ar_sees(a, b, sq), end) - 1 - k0;
+      if (wlive) {
+        first = min(ar_sees(a, b, rw / G), end) - 1 - k0;
+        last = min(ar_sees(a, b, min(rw + 31, rows - 1) / G), end) - 1 - k0;
+      }
+    }
+    flash_segment(smem, kk + base, vv + base, n, lim, __builtin_amdgcn_readfirstlane(first),
+                  __builtin_amdgcn_readfirstlane(last), a.scale_log2, st);
+  }
+  if (!live) return;
+  const float l = st.row_sum();
+  if (a.NS > 1) {
+    float* rec = a.part + (qrow * a.NS + slot) * AR_REC;
+    if (hl == 0) *reinterpret_cast<float2*>(rec) = make_float2(st.m, l);
+    if (l > 0.0f) {
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<float4*>(rec + 4 + db * 32 + g * 8 + hl * 4) =
+              make_float4(st.o[db][g * 4], st.o[db][g * 4 + 1], st.o[db][g * 4 + 2], st.o[db][g * 4 + 3]);
+    }
+    return;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  uint16_t* op = a.out + qrow * HD;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      u32x2 w;
+      w.x = pack_bf16x2(st.o[db][g * 4 + 0] * inv, st.o[db][g * 4 + 1] * inv);
+      w.y = pack_bf16x2(st.o[db][g * 4 + 2] * inv, st.o[db][g * 4 + 3] * inv);
+      *reinterpret_cast<u32x2*>(op + db * 32 + g * 8 + hl * 4) = w;
+    }
+  if (a.lse && hl == 0 && !pre)
+    a.lse[(int64_t(b) * a.Hkv + kvh) * rows + row] =
+        a.lengths && sq >= a.lengths[b] ? INFINITY : ar_lse(st.m, l);
+}
+
+// One wave a row (b, s, head): lane i takes the (m, l) of run i, then two dims
+// of every run that holds keys, in run order.
+__global__ __launch_bounds__(256) void attn_rows_merge_kernel(const ArArgs a) {
+  const int lane = threadIdx.x & 63;
+  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), n = int64_t(a.B) * a.S * a.Hq;
+  if (row >= n) return;
+  const float* p = a.part + row * a.NS * AR_REC;
+  float M = -INFINITY;
+  for (int i = lane; i < a.NS; i += 64) M = fmaxf(M, p[int64_t(i) * AR_REC]);
+  M = wave_max(M);
+  float L = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  for (int c = 0; c < a.NS; c += 64) {
+    float w = 0.0f, wl = 0.0f;
+    if (c + lane < a.NS) {
+      const float2 ml = *reinterpret_cast<const float2*>(p + int64_t(c + lane) * AR_REC);
+      w = ml.y > 0.0f ? __builtin_amdgcn_exp2f(ml.x - M) : 0.0f;
+      wl = ml.y > 0.0f ? w * ml.y : 0.0f;
+    }
+    L += wave_sum(wl);
+    const int cnt = min(64, a.NS - c);
+    for (int i0 = 0; i0 < cnt; i0 += 8) {
+      float2 v[8];
+      float wi[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int i = min(i0 + u, cnt - 1);
+        wi[u] = i0 + u < cnt ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i)) : 0.0f;
+        v[u] = make_float2(0.0f, 0.0f);  // a run without keys stores no O
+        if (wi[u] != 0.0f) v[u] = *reinterpret_cast<const float2*>(p + int64_t(c + i) * AR_REC + 4 + lane * 2);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        o0 = fmaf(wi[u], v[u].x, o0);
+        o1 = fmaf(wi[u], v[u].y, o1);
+      }
+    }
+  }
+  const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+  reinterpret_cast<uint32_t*>(a.out + row * HD)[lane] = pack_bf16x2(o0 * inv, o1 * inv);
+  if (a.lse && lane == 0) {
+    const int G = a.Hq / a.Hkv, head = int(row % a.Hq), s = int(row / a.Hq % a.S), b = int(row / a.Hq / a.S);
+    a.lse[(int64_t(b) * a.Hkv + head / G) * (a.S * G) + s * G + head % G] =
+        a.lengths && s >= a.lengths[b] ? INFINITY : ar_lse(M, L);
+  }
+}
+
+// ====================================================================== column sums
+constexpr int CS_KEYS = 256;  // keys of a workgroup (4 waves x 64)
+constexpr int CS_QT = 64;     // query rows of a streamed tile
+constexpr int CS_BUFS = 3;
+constexpr int CS_QBYTES = CS_QT * AP_ROWB;
+
+struct CsArgs {
+  const uint16_t *q, *k;
+  const float* lse;        // [B][Hkv][S * G]
+  const int32_t* lengths;  // or nullptr
+  int B, S, Hq, Hkv, S_max, start, n_keys, nkt, n_chunk, chunk;
+  uint32_t g_magic;  // ceil(2^32 / G), 0 for G == 1
+  float scale_log2;
+  float* part;    // [n_chunk][B][Hkv][nkt * CS_KEYS]
+  float* scores;  // [B][Hkv][S_max]
+};
+
+// r / G for 0 <= r < 2^32 / G
+__device__ __forceinline__ int cs_div(uint32_t r, uint32_t magic) {
+  return int(magic ? __umulhi(r, magic) : r);
+}
+
+// Item (b, kv head, key tile, chunk of query rows): a wave keeps 64 keys as
+// the B operands of S = Q . K^T, query tiles of 64 packed rows stream through
+// LDS, and since lane l of a 32 x 32 block holds column l % 32, a key's sum
+// over the rows of a tile is an addition within the lane.
+__global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[CS_BUFS * CS_QBYTES];
+  __shared__ __attribute__((aligned(1024))) float ls[CS_BUFS][4][CS_QT];  // a copy for each wave
+  const int t = threadIdx.x, lane = t & 63, hl = lane >> 5, col = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int G = a.Hq / a.Hkv, grp = a.B * a.Hkv;
+  const int x = int(blockIdx.x), bh = x % grp, y = x / grp, kt = y % a.nkt, ch = y / a.nkt;
+  const int b = bh / a.Hkv, kvh = bh % a.Hkv;
+  const int key0 = kt * CS_KEYS;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
+  // rows that see the tile's first key: query >= key0 - start
+  const int live0 = max(key0 - a.start, 0) * G / CS_QT * CS_QT;
+  const int q0 = max(ch * a.chunk, live0), q1 = min((ch + 1) * a.chunk, len * G);
+  if (q0 >= q1) return;  // the reduction knows which chunks a key tile has
+  const int n_t = (q1 - q0 + CS_QT - 1) / CS_QT;
+  // K as B operands: column block cb, k-step ks: key key0 + 64 wave + 32 cb + col
+  bf16x8 kf[2][HD / 16];
+  int rmin[2];  // the first packed row that sees this lane's key
+#pragma unroll
+  for (int cb = 0; cb < 2; ++cb) {
+    const int key = min(key0 + wave * 64 + cb * 32 + col, a.n_keys - 1);
+    rmin[cb] = max(key - a.start, 0) * G;
+    const uint16_t* kp = a.k + ((int64_t(b) * a.Hkv + kvh) * a.S_max + key) * HD + hl * 8;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      const u32x4 v = ld16(kp + ks * 16);
+      kf[cb][ks] = __builtin_bit_cast(bf16x8, v);
+    }
+  }
+  const int wave_rmax = max(min(key0 + wave * 64 + 63, a.n_keys - 1) - a.start, 0) * G;  // past it: no mask
+  // the row (s, g) sits s * Hq + g rows after the base; rows of queries >= len read as zeros
+  const pipe::i32x4 rq = pipe::make_rsrc(a.q + ((int64_t(b) * a.S) * a.Hq + kvh * G) * HD,
+                                         (uint32_t(len - 1) * a.Hq + G) * AP_ROWB);
+  const pipe::i32x4 rl = pipe::make_rsrc(a.lse + (int64_t(b) * a.Hkv + kvh) * (int64_t(a.S) * G),
+                                         uint32_t(q1) * 4u);
+  const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>(smem));
+  const uint32_t lds_l = uint32_t(reinterpret_cast<uintptr_t>(&ls[0][0][0])) + uint32_t(wave * CS_QT * 4);
+  auto dma_q = [&](int i) {
+    const int buf = i % CS_BUFS;
+    const uint32_t dst = lds0 + uint32_t(buf * CS_QBYTES + wave * 4096);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int rr = 16 * wave + 4 * j + (lane >> 4);
+      const uint32_t r = uint32_t(q0 + i * CS_QT + rr);
+      const int s = cs_div(r, a.g_magic), g = int(r) - s * G;
+      const uint32_t off = (uint32_t(s) * a.Hq + g) * AP_ROWB + uint32_t(ap_kslot(rr, lane & 15) * 16);
+      pipe::dma16(dst + j * 1024, s < len ? off : pipe::PAD, rq, 0);
+    }
+    pipe::dma4(lds_l + uint32_t(buf * 4 * CS_QT * 4), uint32_t(q0 + i * CS_QT + lane) * 4u, rl, 0);
+  };
+  float acc[2] = {0.0f, 0.0f};
+  dma_q(0);
+  if (n_t > 1) dma_q(1);
+  for (int i = 0; i < n_t; ++i) {
+    const int buf = i % CS_BUFS, rt = q0 + i * CS_QT;
+    if (i + 1 < n_t)
+      pipe::wait_vm<5>();
+    else
+      pipe::wait_vm<0>();
+    __syncthreads();  // tile i and its lse visible; tile i - 1's buffer free
+    if (i + 2 < n_t) dma_q(i + 2);
+    f32x16 sc[2][2];
+    const uint8_t* qp = smem + buf * CS_QBYTES + col * AP_ROWB;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      const int so = ap_kslot(lane, 2 * ks + hl) * 16;
+      const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(qp + so);
+      const bf16x8 a1 = *reinterpret_cast<const bf16x8*>(qp + 32 * AP_ROWB + so);
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+        sc[0][cb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, kf[cb][ks], ks ? sc[0][cb] : f32x16{}, 0, 0, 0);
+        sc[1][cb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, kf[cb][ks], ks ? sc[1][cb] : f32x16{}, 0, 0, 0);
+      }
+    }
+    const bool mask = rt < wave_rmax || rt + CS_QT > q1;
+#pragma unroll
+    for (int rb = 0; rb < 2; ++rb)
+#pragma unroll
+      for (int g4 = 0; g4 < 4; ++g4) {
+        const float4 le = *reinterpret_cast<const float4*>(&ls[buf][wave][rb * 32 + g4 * 8 + hl * 4]);
+        const float lo[4] = {le.x, le.y, le.z, le.w};
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float w = __builtin_amdgcn_exp2f(fmaf(sc[rb][cb][g4 * 4 + e], a.scale_log2, -lo[e]));
+            if (mask) {
+              const int r = rt + rb * 32 + g4 * 8 + hl * 4 + e;
+              w = r < rmin[cb] || r >= q1 ? 0.0f : w;
+            }
+            acc[cb] += w;
+          }
+      }
+  }
+#pragma unroll
+  for (int cb = 0; cb < 2; ++cb) acc[cb] += __shfl_xor(acc[cb], 32, 64);
+  if (hl == 0) {
+    float* pp = a.part + (int64_t(ch) * grp + bh) * (int64_t(a.nkt) * CS_KEYS) + key0 + wave * 64 + col;
+    pp[0] = acc[0];
+    pp[32] = acc[1];
+  }
+}
+
+// scores += the chunks' sums, in chunk order
+__global__ __launch_bounds__(256) void attn_colsum_add_kernel(const CsArgs a) {
+  const int grp = a.B * a.Hkv, bh = blockIdx.y, key = int(blockIdx.x) * 256 + int(threadIdx.x);
+  if (key >= a.n_keys) return;
+  const int G = a.Hq / a.Hkv, b = bh / a.Hkv;
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
+  const int key0 = key / CS_KEYS * CS_KEYS, live0 = max(key0 - a.start, 0) * G / CS_QT * CS_QT;
+  float sum = 0.0f;
+  bool any = false;
+  for (int ch = live0 / a.chunk; ch * a.chunk < len * G; ++ch)
+    if (max(ch * a.chunk, live0) < min((ch + 1) * a.chunk, len * G)) {
+      sum += a.part[(int64_t(ch) * grp + bh) * (int64_t(a.nkt) * CS_KEYS) + key];
+      any = true;
+    }
+  if (any) a.scores[int64_t(bh) * a.S_max + key] += sum;
+}
+
+// ---------------------------------------------------------------------- host
+static int64_t ar_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Splits the work into key runs of about as many tiles as fill two workgroups
+// on every CU, and at least AR_MIN_RUN (a run's record and its pipeline's
+// start cost about two tiles).  own = own key tiles of a row at most.
+constexpr int64_t AR_MIN_RUN = 2;
+static void ar_plan(ArArgs& a, int64_t own_keys, int64_t* grid) {
+  const int64_t G = a.Hq / a.Hkv, rows = a.S * G;
+  const int64_t nPT = ar_ceil(a.P, AP_KT), nOT = ar_ceil(own_keys, AP_KT);
+  const int64_t slots = 2 * int64_t(std::max(current_device_cus(), 1));
+  a.joint = rows >= AR_ROWS;
+  a.rts = int(ar_ceil(rows, AR_ROWS));
+  const int64_t rtp = ar_ceil(int64_t(a.B) * rows, AR_ROWS), grp = int64_t(a.B) * a.Hkv * a.rts;
+  const int64_t pre_w = a.joint ? 0 : rtp * a.Hkv * nPT, own_w = grp * (nOT + (a.joint ? nPT : 0));
+  const int64_t run = std::max(AR_MIN_RUN, ar_ceil(pre_w + own_w, slots));
+  a.nsp = a.joint ? 0 : int(ar_ceil(nPT, run));
+  a.pt = a.nsp ? int(ar_ceil(nPT, a.nsp)) : 0;
+  if (a.nsp) a.nsp = int(ar_ceil(nPT, a.pt));
+  a.n_pre = a.joint ? 0 : int(rtp * a.Hkv * a.nsp);
+  const int64_t own_t = nOT + (a.joint ? nPT : 0);
+  a.nss = int(std::max<int64_t>(ar_ceil(own_t, run), own_t > 0 || a.nsp == 0 ? 1 : 0));
+  a.st = a.nss ? int(std::max<int64_t>(ar_ceil(own_t, a.nss), 1)) : 0;
+  if (a.nss) a.nss = int(std::max<int64_t>(ar_ceil(own_t, a.st), 1));
+  a.NS = a.nsp + a.nss;
+  *grid = a.n_pre + grp * a.nss;
+}
+
+// A prefix-only decode item's rows span the batch, so one run may be written
+// without a merge as well.
+static int64_t ar_part_bytes(const ArArgs& a) {
+  return a.NS > 1 ? int64_t(a.B) * a.S * a.Hq * a.NS * AR_REC * int64_t(sizeof(float)) : 0;
+}
+
+static int ar_launch(const char* fn, ArArgs& a, int64_t grid, hipStream_t s) {
+  hipLaunchKernelGGL(attn_rows_kernel, dim3(unsigned(grid)), dim3(256), 0, s, a);
+  int rc = hip_status(fn);
+  if (rc || a.NS == 1) return rc;
+  const int64_t rows = int64_t(a.B) * a.S * a.Hq;
+  hipLaunchKernelGGL(attn_rows_merge_kernel, dim3(unsigned(ar_ceil(rows, 4))), dim3(256), 0, s, a);
+  return hip_status(fn);
+}
+
+// Limits shared by both entry points; B * S may be 0.
+static int ar_check(const char* fn, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max,
+                    float scale) {
+  QMOE_REQUIRE(D == HD, "%s: head_dim must be 128 (D=%lld)", fn, (long long)D);
+  QMOE_REQUIRE(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= AR_MAX_G && Hkv < 4096,
+               "%s: need Hq %% Hkv == 0, Hq / Hkv <= 16 and Hkv < 4096", fn);
+  QMOE_REQUIRE(B >= 0 && B < 65536 && S >= 0 && S < (1ll << 22) && B * S * Hq < (1ll << 27),
+               "%s: bad B/S (B * S * Hq must be below 2^27)", fn);
+  QMOE_REQUIRE(S_max > 0 && S_max <= AR_MAX_KEYS, "%s: S_max must be in [1, 2^22]", fn);
+  QMOE_REQUIRE(scale > 0.0f && std::isfinite(scale), "%s: scale must be positive and finite", fn);
+  return QMOE_OK;
+}
+
+static ArArgs ar_args(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_max) {
+  ArArgs a{};
+  a.B = int(B);
+  a.S = int(S);
+  a.Hq = int(Hq);
+  a.Hkv = int(Hkv);
+  a.S_max = int(S_max);
+  return a;
+}
+
+// Chunks of query rows per key tile of the column sums: enough items for four
+// workgroups a CU (half of them see no key of their tile), each of at least
+// 256 rows.
+static void cs_plan(CsArgs& a) {
+  const int64_t G = a.Hq / a.Hkv, rows = a.S * G;
+  a.nkt = int(ar_ceil(a.n_keys, CS_KEYS));
+  const int64_t items = int64_t(a.B) * a.Hkv * a.nkt, want = 4 * int64_t(std::max(current_device_cus(), 1));
+  int64_t n = std::max<int64_t>(1, std::min(ar_ceil(want, items), ar_ceil(rows, 256)));
+  a.chunk = int(ar_ceil(ar_ceil(rows, n), CS_QT) * CS_QT);
+  a.n_chunk = int(ar_ceil(rows, a.chunk));
+  a.g_magic = G == 1 ? 0u : uint32_t(((1ull << 32) + uint64_t(G) - 1) / uint64_t(G));
+}
+
+}  // namespace qmoe
+
+using namespace qmoe;
+
+extern "C" int64_t qmoe_attn_shared_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                              int64_t P, int64_t max_ctx) {
+  if (B < 0 || S < 0 || P < 0 || max_ctx < 0 || max_ctx > AR_MAX_KEYS || P > AR_MAX_KEYS ||
+      ar_check("qmoe_attn_shared_workspace", B, S, Hq, Hkv, D, 1, 1.0f))
+    return -1;
+  if (B == 0 || S == 0) return 0;
+  ArArgs a = ar_args(B, S, Hq, Hkv, 1);
+  int64_t grid;
+  a.P = int(P);
+  ar_plan(a, max_ctx, &grid);
+  return ar_part_bytes(a);
+}
+
+extern "C" int qmoe_attn_shared(const qmoe_bf16* q, const qmoe_bf16* k_prefix, const qmoe_bf16* v_prefix, int64_t P,
+                                int64_t P_max, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
+                                const int32_t* ctx_len, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                int64_t S_max, int64_t max_ctx, float scale, void* workspace,
+                                int64_t workspace_bytes, qmoe_bf16* out, qmoe_stream_t stream) {
+  const char* fn = "qmoe_attn_shared";
+  QMOE_REQUIRE(B == 0 || S == 0 || (q && k_cache && v_cache && ctx_len && out), "%s: null pointer", fn);
+  if (int rc = ar_check(fn, B, S, Hq, Hkv, D, S_max, scale)) return rc;
+  QMOE_REQUIRE(P >= 0 && P <= P_max && P_max <= AR_MAX_KEYS, "%s: need 0 <= P <= P_max <= 2^22", fn);
+  QMOE_REQUIRE(P == 0 || (k_prefix && v_prefix), "%s: null prefix", fn);
+  QMOE_REQUIRE(max_ctx >= 0 && max_ctx <= S_max, "%s: need 0 <= max_ctx <= S_max", fn);
+  if (B == 0 || S == 0) return QMOE_OK;
+  ArArgs a = ar_args(B, S, Hq, Hkv, S_max);
+  a.q = q;
+  a.kp = k_prefix;
+  a.vp = v_prefix;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.ctx_len = ctx_len;
+  a.P = int(P);
+  a.Pmax = int(P_max);
+  a.max_ctx = int(max_ctx);
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.part = static_cast<float*>(workspace);
+  int64_t grid;
+  ar_plan(a, max_ctx, &grid);
+  QMOE_REQUIRE(grid < (1ll << 31), "%s: grid too large", fn);
+  const int64_t need = ar_part_bytes(a);
+  QMOE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: workspace of %lld bytes, need %lld", fn,
+               (long long)workspace_bytes, (long long)need);
+  return ar_launch(fn, a, grid, as_stream(stream));
+}
+
+namespace qmoe {
+static void ps_plan(ArArgs& a, CsArgs& c, int64_t start, int64_t* grid) {
+  a.start = int(start);
+  a.max_ctx = a.S_max;
+  ar_plan(a, start + a.S, grid);
+  c.B = a.B;
+  c.S = a.S;
+  c.Hq = a.Hq;
+  c.Hkv = a.Hkv;
+  c.S_max = a.S_max;
+  c.start = int(start);
+  c.n_keys = int(start + a.S);
+  cs_plan(c);
+}
+static int64_t ps_lse_bytes(const ArArgs& a) { return ar_ceil(int64_t(a.B) * a.S * a.Hq * 4, 256) * 256; }
+static int64_t ps_col_bytes(const CsArgs& c) {
+  return int64_t(c.n_chunk) * c.B * c.Hkv * c.nkt * CS_KEYS * int64_t(sizeof(float));
+}
+}  // namespace qmoe
+
+extern "C" int64_t qmoe_attn_prefill_scored_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                                      int64_t start) {
+  if (start < 0 || S < 0 || start + S > AR_MAX_KEYS ||
+      ar_check("qmoe_attn_prefill_scored_workspace", B, S, Hq, Hkv, D, std::max<int64_t>(start + S, 1), 1.0f))
+    return -1;
+  if (B == 0 || S == 0) return 0;
+  ArArgs a = ar_args(B, S, Hq, Hkv, start + S);
+  CsArgs c{};
+  int64_t grid;
+  ps_plan(a, c, start, &grid);
+  return ps_lse_bytes(a) + std::max(ar_part_bytes(a), ps_col_bytes(c));
+}
+
+extern "C" int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
+                                        int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max,
+                                        int64_t start, const int32_t* lengths, float scale, void* workspace,
+                                        int64_t workspace_bytes, float* scores, qmoe_bf16* out,
+                                        qmoe_stream_t stream) {
+  const char* fn = "qmoe_attn_prefill_scored";
+  QMOE_REQUIRE(k_cache && v_cache && scores && (B == 0 || S == 0 || (q && out)), "%s: null pointer", fn);
+  if (int rc = ar_check(fn, B, S, Hq, Hkv, D, S_max, scale)) return rc;
+  QMOE_REQUIRE(start >= 0 && start + S <= S_max, "%s: need 0 <= start and start + S <= S_max", fn);
+  // a row's queries are addressed with 32-bit byte offsets
+  QMOE_REQUIRE(S * Hq * AP_ROWB < (1ll << 31), "%s: S * Hq must be below 2^23", fn);
+  if (B == 0 || S == 0) return QMOE_OK;
+  ArArgs a = ar_args(B, S, Hq, Hkv, S_max);
+  CsArgs c{};
+  int64_t grid;
+  ps_plan(a, c, start, &grid);
+  const int64_t lse = ps_lse_bytes(a), need = lse + std::max(ar_part_bytes(a), ps_col_bytes(c));
+  QMOE_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %lld bytes, need %lld", fn,
+               (long long)workspace_bytes, (long long)need);
+  const int64_t cgrid = int64_t(B) * Hkv * c.nkt * c.n_chunk;
+  QMOE_REQUIRE(grid < (1ll << 31) && cgrid < (1ll << 31), "%s: grid too large", fn);
+  a.q = c.q = q;
+  a.k = c.k = k_cache;
+  a.v = v_cache;
+  a.lengths = c.lengths = lengths;
+  a.scale_log2 = c.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  c.lse = a.lse = static_cast<float*>(workspace);
+  c.part = a.part = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + lse);
+  c.scores = scores;
+  if (int rc = ar_launch(fn, a, grid, as_stream(stream))) return rc;
+  hipLaunchKernelGGL(attn_colsum_kernel, dim3(unsigned(cgrid)), dim3(256), 0, as_stream(stream), c);
+  if (int rc = hip_status(fn)) return rc;
+  hipLaunchKernelGGL(attn_colsum_add_kernel, dim3(unsigned(c.nkt), unsigned(B * Hkv)), dim3(256), 0,
+                     as_stream(stream), c);
+  return hip_status(fn);
+}

@@ -78,6 +78,15 @@ PROTOTYPES = {
     "qmoe_attn_decode_fused": (c_int, [P, P, P, P, P, I64, P, I64, I64, I64, I64, I64, I64, c_float, c_float, P, P,
                                        P, P, P]),
     "qmoe_attn_decode_chunk": (c_int, [P, P, P, P, I64, I64, I64, I64, I64, I64, c_float, P, P, P]),
+    "qmoe_attn_shared": (c_int, [P, P, P, I64, I64, P, P, P, I64, I64, I64, I64, I64, I64, I64, c_float, P, I64, P, P]),
+    "qmoe_attn_shared_workspace": (c_int64, [I64, I64, I64, I64, I64, I64, I64]),
+    "qmoe_attn_prefill_scored": (c_int, [P, P, P, I64, I64, I64, I64, I64, I64, I64, P, c_float, P, I64, P, P, P]),
+    "qmoe_attn_prefill_scored_workspace": (c_int64, [I64, I64, I64, I64, I64, I64]),
+    "qmoe_attn_decode_scored": (c_int, [P, P, P, P, I64, I64, I64, I64, I64, I64, c_float, P, I64, P, P, P]),
+    "qmoe_attn_decode_scored_workspace": (c_int64, [I64, I64, I64, I64]),
+    "qmoe_kv_append": (c_int, [P, P, P, P, P, I64, P, P, I64, I64, I64, I64, I64, c_float, P, P, P, P, P, P]),
+    "qmoe_kv_evict": (c_int, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, I64, I64, P, P, P, P, P]),
+    "qmoe_kv_evict_workspace": (c_int64, [I64, I64, I64, I64]),
 }
 
 

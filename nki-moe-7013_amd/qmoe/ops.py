@@ -773,6 +773,289 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, c
     return out
 
 
+# ----------------------------------------------------------------- shared prefixes and bounded caches
+def _call(name: str, dev: torch.device, *args) -> None:
+    """One library call on ``dev`` (made current for it) and its current stream."""
+    fn = getattr(lib(), name)
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        check(fn(*args, _stream()), name)
+        return
+    with torch.cuda.device(dev):
+        check(fn(*args, _stream()), name)
+
+
+def _size(name: str, dev: torch.device, *args) -> int:
+    """A workspace query, for the device the call will run on."""
+    fn = getattr(lib(), name)
+    if dev.index is None or dev.index == torch.cuda.current_device():
+        n = int(fn(*args))
+    else:
+        with torch.cuda.device(dev):
+            n = int(fn(*args))
+    if n < 0:
+        raise ValueError(f"{name}: bad sizes {args}")
+    return n
+
+
+def _scratch(workspace: Optional[torch.Tensor], need: int, dev: torch.device) -> Optional[torch.Tensor]:
+    """``workspace`` if it holds ``need`` bytes, a new one if none was given."""
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
+    if workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError(f"workspace: must be contiguous and on {dev}")
+    if _nbytes(workspace) < need:
+        raise ValueError(f"workspace: needs {need} bytes (got {_nbytes(workspace)})")
+    if workspace.data_ptr() % 16:
+        raise ValueError("workspace: must be 16-byte aligned")
+    return workspace
+
+
+def _aligned(*named) -> None:
+    """Rows of 256 bytes are moved 16 bytes at a time."""
+    for name, t in named:
+        if t.data_ptr() % 16:
+            raise ValueError(f"{name}: must be 16-byte aligned")
+
+
+def _check_cache(k_cache, v_cache, B: Optional[int] = None, D: Optional[int] = None, what: str = "cache"):
+    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
+        raise ValueError(f"k_{what} must be [B, Hkv, S_max, D]")
+    if (B is not None and k_cache.shape[0] != B) or (D is not None and k_cache.shape[3] != D):
+        raise ValueError(f"k_{what} must be [B={B}, Hkv, S_max, D={D}] (got {tuple(k_cache.shape)})")
+    _need(k_cache, f"k_{what}", BF16)
+    _need(v_cache, f"v_{what}", BF16, k_cache.shape)
+    _aligned((f"k_{what}", k_cache), (f"v_{what}", v_cache))
+    return k_cache.shape[1], k_cache.shape[2]
+
+
+def _check_heads(Hq: int, Hkv: int) -> None:
+    if Hkv <= 0 or Hq % Hkv or Hq // Hkv > 16:
+        raise ValueError(f"need Hq a multiple of Hkv, by at most 16 (Hq={Hq}, Hkv={Hkv})")
+
+
+def _check_queries(q, rows: int, out):
+    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.shape[0] != rows:
+        raise ValueError(f"q must be [{rows}, Hq, D]")
+    _need(q, "q", BF16)
+    _, Hq, D = q.shape
+    out = torch.empty(rows, Hq * D, dtype=BF16, device=q.device) if out is None else out
+    _need(out, "out", BF16, (rows, Hq * D))
+    _aligned(("q", q), ("out", out))
+    return Hq, D, out
+
+
+def _check_scale(scale: Optional[float], D: int) -> float:
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite (got {scale})")
+    return scale
+
+
+def attn_shared_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, prefix_len: int, max_ctx: int,
+                          device) -> Optional[torch.Tensor]:
+    """Workspace of :func:`attn_shared` (``None`` when it needs none)."""
+    dev = torch.device(device)
+    return _scratch(None, _size("qmoe_attn_shared_workspace", dev, B, S, Hq, Hkv, D, prefix_len, max_ctx), dev)
+
+
+def attn_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_cache: torch.Tensor,
+                v_cache: torch.Tensor, ctx_len: torch.Tensor, B: int, S: int, prefix_len: Optional[int] = None,
+                scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None) -> torch.Tensor:
+    """Attention of ``q[B*S, Hq, D]`` for a batch whose rows share a prefix:
+    query s of row b sees the first ``prefix_len`` (default: all) entries of
+    ``k_prefix/v_prefix[Hkv, P_max, D]``, which the batch reads once, and the
+    first ``ctx_len[b] + s`` entries of its own ``k_cache/v_cache[B, Hkv, S_max,
+    D]``, at most ``max_ctx`` of them (default ``S_max``; a context bucket sizes
+    the launch).  Decode: S = 1 and ``ctx_len`` (i32 ``[B]``, on the device)
+    counts the new entry; a chunk of S tokens whose first one is own entry e:
+    ``ctx_len = e + 1``.  A query that sees nothing gets zeros.  Returns
+    ``[B*S, Hq*D]``."""
+    Hq, D, out = _check_queries(q, B * S, out)
+    Hkv, S_max = _check_cache(k_cache, v_cache, B, D)
+    _check_heads(Hq, Hkv)
+    if not isinstance(k_prefix, torch.Tensor) or k_prefix.dim() != 3 or k_prefix.shape[0] != Hkv \
+            or k_prefix.shape[2] != D:
+        raise ValueError(f"k_prefix must be [Hkv={Hkv}, P_max, D={D}]")
+    _need(k_prefix, "k_prefix", BF16)
+    _need(v_prefix, "v_prefix", BF16, k_prefix.shape)
+    _aligned(("k_prefix", k_prefix), ("v_prefix", v_prefix))
+    _need(ctx_len, "ctx_len", I32, (B,))
+    P_max = k_prefix.shape[1]
+    P = P_max if prefix_len is None else int(prefix_len)
+    if not 0 <= P <= P_max:
+        raise ValueError(f"prefix_len must be in [0, {P_max}] (got {P})")
+    max_ctx = S_max if max_ctx is None else int(max_ctx)
+    if not 0 <= max_ctx <= S_max:
+        raise ValueError(f"max_ctx must be in [0, {S_max}] (got {max_ctx})")
+    scale = _check_scale(scale, D)
+    dev = q.device
+    _same_device(q, k_prefix, v_prefix, k_cache, v_cache, ctx_len, out)
+    ws = _scratch(workspace, _size("qmoe_attn_shared_workspace", dev, B, S, Hq, Hkv, D, P, max_ctx), dev)
+    _call("qmoe_attn_shared", dev, _ptr(q), _ptr(k_prefix), _ptr(v_prefix), P, P_max, _ptr(k_cache), _ptr(v_cache),
+          _ptr(ctx_len), B, S, Hq, Hkv, D, S_max, max_ctx, scale, _ptr(ws), _nbytes(ws), _ptr(out))
+    return out
+
+
+def attn_prefill_scored_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, start: int, device) -> torch.Tensor:
+    """Workspace of :func:`attn_prefill_scored`."""
+    dev = torch.device(device)
+    return _scratch(None, max(16, _size("qmoe_attn_prefill_scored_workspace", dev, B, S, Hq, Hkv, D, start)), dev)
+
+
+def _check_scores(scores, B: int, Hkv: int, S_max: int) -> None:
+    _need(scores, "scores", F32, (B, Hkv, S_max))
+
+
+def attn_prefill_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, B: int,
+                        S: int, start: int = 0, lengths: Optional[torch.Tensor] = None,
+                        scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`attn_prefill` (host ``start``) that also adds the attention weight
+    of every cache entry, summed over the queries and the q heads of each
+    group, to ``scores[B, Hkv, S_max]`` (f32, in place).  ``lengths`` (i32
+    ``[B]``): of a right-padded row only the first ``lengths[b]`` queries count.
+    Returns ``[B*S, Hq*D]``."""
+    Hq, D, out = _check_queries(q, B * S, out)
+    Hkv, S_max = _check_cache(k_cache, v_cache, B, D)
+    _check_heads(Hq, Hkv)
+    _check_scores(scores, B, Hkv, S_max)
+    start = int(start)
+    if start < 0 or start + S > S_max:
+        raise ValueError(f"need 0 <= start and start + S <= S_max={S_max} (start={start}, S={S})")
+    if lengths is not None:
+        _need(lengths, "lengths", I32, (B,))
+    scale = _check_scale(scale, D)
+    dev = q.device
+    _same_device(q, k_cache, v_cache, scores, lengths, out)
+    ws = _scratch(workspace, _size("qmoe_attn_prefill_scored_workspace", dev, B, S, Hq, Hkv, D, start), dev)
+    _call("qmoe_attn_prefill_scored", dev, _ptr(q), _ptr(k_cache), _ptr(v_cache), B, S, Hq, Hkv, D, S_max, start,
+          _ptr(lengths), scale, _ptr(ws), _nbytes(ws), _ptr(scores), _ptr(out))
+    return out
+
+
+def attn_decode_scored_workspace(B: int, Hq: int, D: int, max_ctx: int, device) -> Optional[torch.Tensor]:
+    """Workspace of :func:`attn_decode_scored`."""
+    dev = torch.device(device)
+    return _scratch(None, _size("qmoe_attn_decode_scored_workspace", dev, B, Hq, D, max_ctx), dev)
+
+
+def attn_decode_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx_len: torch.Tensor,
+                       scores: torch.Tensor, scale: Optional[float] = None,
+                       workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                       max_ctx: Optional[int] = None) -> torch.Tensor:
+    """:func:`attn_decode` that also adds each slot's attention weight, summed
+    over the q heads of its group, to ``scores[B, Hkv, S_max]`` (f32, in place).
+    A row with ``ctx_len`` of zero gets zeros.  Returns ``[B, Hq*D]``."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        raise ValueError("q must be [B, Hq, D]")
+    B = q.shape[0]
+    Hq, D, out = _check_queries(q, B, out)
+    Hkv, S_max = _check_cache(k_cache, v_cache, B, D)
+    _check_heads(Hq, Hkv)
+    _check_scores(scores, B, Hkv, S_max)
+    _need(ctx_len, "ctx_len", I32, (B,))
+    max_ctx = S_max if max_ctx is None else int(max_ctx)
+    if not 0 < max_ctx <= S_max:
+        raise ValueError(f"max_ctx must be in [1, {S_max}] (got {max_ctx})")
+    scale = _check_scale(scale, D)
+    dev = q.device
+    _same_device(q, k_cache, v_cache, ctx_len, scores, out)
+    ws = _scratch(workspace, _size("qmoe_attn_decode_scored_workspace", dev, B, Hq, D, max_ctx), dev)
+    _call("qmoe_attn_decode_scored", dev, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(ctx_len), B, Hq, Hkv, D, S_max,
+          max_ctx, scale, _ptr(ws), _nbytes(ws), _ptr(scores), _ptr(out))
+    return out
+
+
+def kv_append(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor, rope_cos: torch.Tensor,
+              rope_sin: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, Hq: int, Hkv: int,
+              k_cache: torch.Tensor, v_cache: torch.Tensor, eps: float, scores: Optional[torch.Tensor] = None,
+              slot_pos: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A decode step's raw projection ``qkv[B, (Hq+2Hkv)*D]`` (f32): q/k RMSNorm
+    and RoPE at ``positions[b]``, the K/V row into slot ``slots[b]`` of row b,
+    whose score becomes 0 and position ``positions[b]``.  A row whose position
+    or slot is out of range writes no entry and gets a zero q.  Returns
+    ``q[B, Hq, D]``."""
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2:
+        raise ValueError("qkv must be [B, (Hq + 2 Hkv) * D]")
+    B, D = qkv.shape[0], q_norm_w.shape[0]
+    _need(qkv, "qkv", F32, (B, (Hq + 2 * Hkv) * D))
+    _need(q_norm_w, "q_norm_w", BF16, (D,))
+    _need(k_norm_w, "k_norm_w", BF16, (D,))
+    max_pos = rope_cos.shape[0]
+    _need(rope_cos, "rope_cos", F32, (max_pos, D // 2))
+    _need(rope_sin, "rope_sin", F32, (max_pos, D // 2))
+    _need(positions, "positions", I32, (B,))
+    _need(slots, "slots", I32, (B,))
+    n_kv, S_max = _check_cache(k_cache, v_cache, B, D)
+    if n_kv != Hkv:
+        raise ValueError(f"k_cache must have Hkv={Hkv} heads (got {n_kv})")
+    if scores is not None:
+        _check_scores(scores, B, Hkv, S_max)
+    if slot_pos is not None:
+        _need(slot_pos, "slot_pos", I32, (B, Hkv, S_max))
+    q_out = torch.empty(B, Hq, D, dtype=BF16, device=qkv.device) if q_out is None else q_out
+    _need(q_out, "q_out", BF16, (B, Hq, D))
+    _same_device(qkv, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slots, k_cache, v_cache, scores, slot_pos,
+                 q_out)
+    _call("qmoe_kv_append", qkv.device, _ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(rope_cos), _ptr(rope_sin),
+          max_pos, _ptr(positions), _ptr(slots), B, Hq, Hkv, D, S_max, float(eps), _ptr(q_out), _ptr(k_cache),
+          _ptr(v_cache), _ptr(scores), _ptr(slot_pos))
+    return q_out
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    x, y = a.data_ptr(), b.data_ptr()
+    return x < y + _nbytes(b) and y < x + _nbytes(a)
+
+
+def kv_evict_workspace(B: int, Hkv: int, S_max: int, budget: int, device) -> Optional[torch.Tensor]:
+    """Workspace of :func:`kv_evict`."""
+    dev = torch.device(device)
+    return _scratch(None, _size("qmoe_kv_evict_workspace", dev, B, Hkv, S_max, budget), dev)
+
+
+def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, slot_pos: torch.Tensor,
+             ctx_len: torch.Tensor, budget: int, recent: int = 0, sink: int = 0,
+             out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]] = None,
+             workspace: Optional[torch.Tensor] = None) -> None:
+    """Cuts every (row, kv head) of a cache with more than ``budget`` entries
+    (``ctx_len``: i32 ``[B]``) down to ``budget``: positions below ``sink`` and
+    the ``recent`` last ones stay, then the largest scores (ties: the lowest
+    slot).  Kept entries past slot ``budget`` move into the freed slots below
+    it, in order; all other slots end with score 0 and position -1.  In place,
+    or into ``out = (k, v, scores, slot_pos)``, another cache with at least
+    ``budget`` slots, leaving this one as it is.  The caller's next ``ctx_len``
+    is ``ctx_len.clamp(max=budget)``."""
+    Hkv, S_max = _check_cache(k_cache, v_cache)
+    B, D = k_cache.shape[0], k_cache.shape[3]
+    _check_scores(scores, B, Hkv, S_max)
+    _need(slot_pos, "slot_pos", I32, (B, Hkv, S_max))
+    _need(ctx_len, "ctx_len", I32, (B,))
+    budget, recent, sink = int(budget), int(recent), int(sink)
+    if budget <= 0 or recent < 0 or sink < 0 or recent + sink > budget:
+        raise ValueError(f"need budget > 0 and 0 <= recent + sink <= budget (budget={budget}, recent={recent}, "
+                         f"sink={sink})")
+    src = (k_cache, v_cache, scores, slot_pos)
+    if out is None:
+        k2, v2, sc2, sp2 = src
+        S_out = S_max
+    else:
+        k2, v2, sc2, sp2 = out
+        n_kv, S_out = _check_cache(k2, v2, B, D, "out")
+        if n_kv != Hkv or S_out < min(budget, S_max):
+            raise ValueError(f"out must be a cache [{B}, {Hkv}, >= {min(budget, S_max)}, {D}] (got {tuple(k2.shape)})")
+        _need(sc2, "scores_out", F32, (B, Hkv, S_out))
+        _need(sp2, "slot_pos_out", I32, (B, Hkv, S_out))
+        if any(_overlap(x, y) for x in src for y in out):
+            raise ValueError("out overlaps the cache (leave it out to evict in place)")
+    dev = k_cache.device
+    _same_device(*src, ctx_len, k2, v2, sc2, sp2)
+    ws = _scratch(workspace, _size("qmoe_kv_evict_workspace", dev, B, Hkv, S_max, budget), dev)
+    _call("qmoe_kv_evict", dev, _ptr(k_cache), _ptr(v_cache), _ptr(scores), _ptr(slot_pos), _ptr(ctx_len), B, Hkv, D,
+          S_max, budget, recent, sink, _ptr(ws), _nbytes(ws), S_out, _ptr(k2), _ptr(v2), _ptr(sc2), _ptr(sp2))
+
+
 # ----------------------------------------------------------------- embedding / greedy argmax
 def embed(ids: torch.Tensor, table: torch.Tensor, out: Optional[torch.Tensor] = None,
           err: Optional[torch.Tensor] = None) -> torch.Tensor:

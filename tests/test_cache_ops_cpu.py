@@ -1,0 +1,144 @@
+"""What the shared-prefix and bounded-cache entry points refuse, without a GPU:
+the C entries before any launch, the Python wrappers before the library."""
+
+import pytest
+import torch
+
+from qmoe import _lib, ops
+
+NONE = None
+ERR = _lib.QMOE_ERR_INVALID
+
+
+def shared(l, q=1, kp=1, vp=1, P=8, P_max=8, k=1, v=1, ctx=1, B=2, S=1, Hq=32, Hkv=4, D=128, S_max=64, max_ctx=64,
+           scale=0.1, ws=1, n=0, out=1):
+    return l.qmoe_attn_shared(q, kp, vp, P, P_max, k, v, ctx, B, S, Hq, Hkv, D, S_max, max_ctx, scale, ws, n, out, NONE)
+
+
+def prompt(l, q=1, k=1, v=1, B=2, S=4, Hq=32, Hkv=4, D=128, S_max=64, start=0, lengths=NONE, scale=0.1, ws=1, n=0,
+           scores=1, out=1):
+    return l.qmoe_attn_prefill_scored(q, k, v, B, S, Hq, Hkv, D, S_max, start, lengths, scale, ws, n, scores, out, NONE)
+
+
+def scored(l, q=1, k=1, v=1, ctx=1, B=2, Hq=32, Hkv=4, D=128, S_max=64, max_ctx=64, scale=0.1, ws=1, n=0, scores=1,
+           out=1):
+    return l.qmoe_attn_decode_scored(q, k, v, ctx, B, Hq, Hkv, D, S_max, max_ctx, scale, ws, n, scores, out, NONE)
+
+
+def append(l, raw=1, qn=1, kn=1, cos=1, sin=1, max_pos=10, pos=1, slots=1, B=2, Hq=32, Hkv=4, D=128, S_max=64,
+           eps=1e-6, q=1, k=1, v=1, scores=NONE, sp=NONE):
+    return l.qmoe_kv_append(raw, qn, kn, cos, sin, max_pos, pos, slots, B, Hq, Hkv, D, S_max, eps, q, k, v, scores, sp,
+                            NONE)
+
+
+def evict(l, k=1, v=2, sc=3, sp=4, ctx=5, B=2, Hkv=4, D=128, S_max=64, budget=32, recent=4, sink=2, ws=6, n=1 << 20,
+          S_out=64, k2=1, v2=2, sc2=3, sp2=4):
+    return l.qmoe_kv_evict(k, v, sc, sp, ctx, B, Hkv, D, S_max, budget, recent, sink, ws, n, S_out, k2, v2, sc2, sp2,
+                           NONE)
+
+
+NAN, INF = float("nan"), float("inf")
+REFUSED = [
+    (shared, dict(q=NONE), "null pointer"), (shared, dict(k=NONE), "null pointer"), (shared, dict(ctx=NONE), "null"),
+    (shared, dict(out=NONE), "null pointer"), (shared, dict(kp=NONE), "null prefix"),
+    (shared, dict(D=64), "head_dim"), (shared, dict(Hq=30), "Hq % Hkv"), (shared, dict(Hq=68), "Hq / Hkv <= 16"),
+    (shared, dict(Hkv=0), "Hq % Hkv"), (shared, dict(B=-1), "bad B/S"), (shared, dict(S=-1), "bad B/S"),
+    (shared, dict(B=65000, S=3000), "below 2^27"), (shared, dict(S_max=0), "S_max"),
+    (shared, dict(S_max=(1 << 22) + 1), "S_max"), (shared, dict(P=9), "P <= P_max"), (shared, dict(P=-1), "0 <= P"),
+    (shared, dict(P_max=(1 << 22) + 1), "2^22"), (shared, dict(max_ctx=65), "max_ctx"),
+    (shared, dict(max_ctx=-1), "max_ctx"), (shared, dict(scale=0.0), "scale"), (shared, dict(scale=-1.0), "scale"),
+    (shared, dict(scale=NAN), "scale"), (shared, dict(scale=INF), "scale"),
+    (shared, dict(), "workspace of 0 bytes"), (shared, dict(ws=NONE, n=1 << 30), "workspace"),
+    (prompt, dict(q=NONE), "null pointer"), (prompt, dict(scores=NONE), "null pointer"),
+    (prompt, dict(D=64), "head_dim"), (prompt, dict(Hq=33), "Hq % Hkv"), (prompt, dict(start=-1), "start"),
+    (prompt, dict(start=61), "start + S"), (prompt, dict(scale=NAN), "scale"), (prompt, dict(), "workspace"),
+    (prompt, dict(S=1 << 18, S_max=1 << 20, B=1), "2^23"), (prompt, dict(B=-2), "bad B/S"),
+    (scored, dict(q=NONE), "null pointer"), (scored, dict(scores=NONE), "null pointer"),
+    (scored, dict(D=256), "head_dim"), (scored, dict(Hq=68), "Hq / Hkv"), (scored, dict(max_ctx=0), "max_ctx"),
+    (scored, dict(max_ctx=65), "max_ctx"), (scored, dict(scale=-0.1), "scale"), (scored, dict(n=64), "workspace"),
+    (scored, dict(ws=NONE, n=1 << 30), "workspace"), (scored, dict(B=-1), "bad B"), (scored, dict(S_max=0), "bad B"),
+    (append, dict(raw=NONE), "null pointer"), (append, dict(k=NONE), "null pointer"), (append, dict(D=64), "head_dim"),
+    (append, dict(Hq=6), "head counts"), (append, dict(max_pos=0), "max_pos"), (append, dict(B=-1), "bad B"),
+    (append, dict(S_max=0), "S_max"),
+    (evict, dict(k=NONE), "null pointer"), (evict, dict(ctx=NONE), "null pointer"), (evict, dict(D=64), "head_dim"),
+    (evict, dict(B=-1), "B * Hkv"), (evict, dict(B=20000), "B * Hkv"), (evict, dict(S_max=0), "bad S_max"),
+    (evict, dict(budget=0), "budget"), (evict, dict(recent=-1), "recent"), (evict, dict(sink=-1), "recent"),
+    (evict, dict(recent=30, sink=3), "recent + sink"), (evict, dict(S_out=31, k2=7, v2=8, sc2=9, sp2=10), "31 slots"),
+    (evict, dict(S_out=63), "exactly this one"), (evict, dict(v2=8), "exactly this one"),
+    (evict, dict(sp2=8), "exactly this one"), (evict, dict(n=1000), "workspace"), (evict, dict(ws=NONE), "workspace"),
+]
+
+
+@pytest.mark.parametrize("fn,change,msg", REFUSED, ids=lambda x: getattr(x, "__name__", None) or str(x)[:40])
+def test_c_entries_refuse(fn, change, msg):
+    assert fn(_lib.lib(), **change) == ERR
+    assert msg in _lib.last_error(), _lib.last_error()
+
+
+def test_empty_batches_launch_nothing():
+    l = _lib.lib()
+    assert shared(l, q=NONE, k=NONE, v=NONE, ctx=NONE, out=NONE, B=0, ws=NONE) == 0
+    assert shared(l, q=NONE, out=NONE, S=0, ws=NONE) == 0
+    assert prompt(l, q=NONE, out=NONE, B=0, ws=NONE) == 0
+    assert prompt(l, q=NONE, out=NONE, S=0, ws=NONE) == 0
+    assert scored(l, q=NONE, k=NONE, v=NONE, ctx=NONE, scores=NONE, out=NONE, B=0, ws=NONE) == 0
+    assert append(l, raw=NONE, pos=NONE, slots=NONE, q=NONE, k=NONE, v=NONE, B=0) == 0
+    assert evict(l, k=NONE, v=NONE, sc=NONE, sp=NONE, ctx=NONE, k2=NONE, v2=NONE, sc2=NONE, sp2=NONE, B=0, ws=NONE) == 0
+
+
+def test_workspace_queries():
+    l = _lib.lib()
+    assert l.qmoe_attn_shared_workspace(0, 1, 32, 4, 128, 100, 10) == 0
+    assert l.qmoe_attn_shared_workspace(2, 1, 32, 4, 128, 1000, 100) > 0
+    for bad in [(-1, 1, 32, 4, 128, 1, 1), (1, 1, 33, 4, 128, 1, 1), (1, 1, 32, 4, 64, 1, 1), (1, 1, 32, 4, 128, -1, 1),
+                (1, 1, 32, 4, 128, 1, -1), (1, 1, 32, 4, 128, 1 << 23, 1), (1, 1, 32, 4, 128, 1, 1 << 23)]:
+        assert l.qmoe_attn_shared_workspace(*bad) == -1, bad
+    assert l.qmoe_attn_prefill_scored_workspace(0, 5, 32, 4, 128, 0) == 0
+    assert l.qmoe_attn_prefill_scored_workspace(1, 5, 32, 4, 128, 0) >= 5 * 32 * 4
+    for bad in [(1, 5, 32, 4, 128, -1), (1, -5, 32, 4, 128, 0), (1, 5, 32, 4, 128, 1 << 22), (1, 5, 32, 3, 128, 0)]:
+        assert l.qmoe_attn_prefill_scored_workspace(*bad) == -1, bad
+    # a record of 132 floats and 256 logits for each of two splits
+    assert l.qmoe_attn_decode_scored_workspace(3, 32, 128, 257) == 3 * 32 * 2 * (132 + 256) * 4
+    assert l.qmoe_attn_decode_scored_workspace(3, 32, 64, 257) == -1
+    assert l.qmoe_attn_decode_scored_workspace(3, 32, 128, -1) == -1
+    assert l.qmoe_kv_evict_workspace(2, 4, 100, 50) == 2 * 2 * 4 * 50 * 4
+    assert l.qmoe_kv_evict_workspace(2, 4, 100, 500) == 2 * 2 * 4 * 100 * 4
+    assert l.qmoe_kv_evict_workspace(2, -4, 100, 50) == -1
+
+
+def _bf(*shape):
+    return torch.zeros(*shape, dtype=torch.bfloat16)
+
+
+def _i(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+def test_wrappers_refuse():
+    q, k, kp = _bf(2, 32, 128), _bf(2, 4, 8, 128), _bf(4, 9, 128)
+    sc, sp, n = torch.zeros(2, 4, 8), _i(2, 4, 8), _i(2)
+    calls = [
+        (lambda: ops.attn_shared(q, kp, kp, k, k, n, 2, 1), "must be on a GPU"),
+        (lambda: ops.attn_shared(q, kp, kp, k, k, n, 3, 1), r"q must be \[3"),
+        (lambda: ops.attn_shared(None, kp, kp, k, k, n, 2, 1), "q must be"),
+        (lambda: ops.attn_prefill_scored(q, k, k, sc, 1, 2), "must be on a GPU"),
+        (lambda: ops.attn_decode_scored(q[0], k, k, n, sc), "q must be"),
+        (lambda: ops.attn_decode_scored(q, k, k, n, sc), "must be on a GPU"),
+        (lambda: ops.kv_append(torch.zeros(2, 5120), _bf(128), _bf(128), torch.zeros(4, 64), torch.zeros(4, 64), n, n,
+                               32, 4, k, k, 1e-6), "must be on a GPU"),
+        (lambda: ops.kv_append(_bf(2), _bf(128), _bf(128), n, n, n, n, 32, 4, k, k, 1e-6), "qkv must be"),
+        (lambda: ops.kv_evict(k, k, sc, sp, n, 4), "must be on a GPU"),
+        (lambda: ops.kv_evict(k[0], k[0], sc, sp, n, 4), "k_cache must be"),
+        (lambda: ops._check_heads(33, 4), "multiple"),
+        (lambda: ops._check_heads(128, 4), "at most 16"),
+        (lambda: ops._check_scale(float("nan"), 128), "scale"),
+        (lambda: ops._check_scale(0.0, 128), "scale"),
+        (lambda: ops._scratch(torch.zeros(4), 17, torch.device("cpu")), "needs 17 bytes"),
+        (lambda: ops._scratch(torch.zeros(64, dtype=torch.uint8)[1:], 8, torch.device("cpu")), "aligned"),
+        (lambda: ops.attn_shared_workspace(1, 1, 33, 4, 128, 1, 1, "cpu"), "bad sizes"),
+    ]
+    for call, msg in calls:
+        with pytest.raises(ValueError, match=msg):
+            call()
+    a = torch.zeros(100)
+    assert ops._overlap(a[:60], a[50:]) and not ops._overlap(a[:50], a[50:])
