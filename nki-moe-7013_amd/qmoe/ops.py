@@ -774,58 +774,94 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, c
 
 
 # ----------------------------------------------------------------- shared prefixes and bounded caches
-def _call(name: str, dev: torch.device, *args) -> None:
-    """One library call on ``dev`` (made current for it) and its current stream."""
+# A decode step makes these calls for a few microseconds of kernel each, so the
+# checks of an argument are one expression (0.4 us; a separate test of each
+# property and of all devices together 0.9) and the stream is the raw one
+# (0.1 us; the Stream object 2.8).  kv_append of one row, 13 tensors: 22.9 -> 14.8 us.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _arg(t, name: str, dtype, shape, ix: int) -> int:
+    """Address of ``t``, once it is a contiguous, 16-byte aligned tensor of this
+    dtype and shape on GPU ``ix``."""
+    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == ix and t.shape == shape
+            and t.is_contiguous()):
+        p = t.data_ptr()
+        if not p & 15:
+            return p
+    _need(t, name, dtype, shape)
+    if t.get_device() != ix:
+        raise ValueError(f"tensors are on different devices: {name} is on {t.device}, expected cuda:{ix}")
+    raise ValueError(f"{name}: must be 16-byte aligned")
+
+
+def _out(t, name: str, dtype, shape, ix: int):
+    """``(tensor, address)`` of an output: ``t``, or a new tensor."""
+    if t is None:
+        t = torch.empty(shape, dtype=dtype, device=ix)
+        return t, t.data_ptr()
+    return t, _arg(t, name, dtype, shape, ix)
+
+
+def _call(name: str, ix: int, *args) -> None:
+    """One library call on GPU ``ix`` (made current for it) and its current stream."""
     fn = getattr(lib(), name)
-    if dev.index is None or dev.index == torch.cuda.current_device():
-        check(fn(*args, _stream()), name)
-        return
-    with torch.cuda.device(dev):
-        check(fn(*args, _stream()), name)
+    if ix == torch._C._cuda_getDevice():
+        rc = fn(*args, _raw_stream(ix))
+    else:
+        with torch.cuda.device(ix):
+            rc = fn(*args, _raw_stream(ix))
+    if rc:
+        check(rc, name)
 
 
-def _size(name: str, dev: torch.device, *args) -> int:
+def _size(name: str, ix: Optional[int], *args) -> int:
     """A workspace query, for the device the call will run on."""
     fn = getattr(lib(), name)
-    if dev.index is None or dev.index == torch.cuda.current_device():
+    if ix is None or ix == torch._C._cuda_getDevice():
         n = int(fn(*args))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(ix):
             n = int(fn(*args))
     if n < 0:
         raise ValueError(f"{name}: bad sizes {args}")
     return n
 
 
-def _scratch(workspace: Optional[torch.Tensor], need: int, dev: torch.device) -> Optional[torch.Tensor]:
-    """``workspace`` if it holds ``need`` bytes, a new one if none was given."""
+def _scratch(workspace: Optional[torch.Tensor], need: int, ix: int):
+    """``(tensor, address, bytes)`` of ``workspace`` if it holds ``need`` bytes, of
+    a new one if none was given (None, None, 0 where none is needed)."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=dev) if need > 0 else None
-    if workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError(f"workspace: must be contiguous and on {dev}")
-    if _nbytes(workspace) < need:
-        raise ValueError(f"workspace: needs {need} bytes (got {_nbytes(workspace)})")
+        if need <= 0:
+            return None, None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=ix)
+        return workspace, workspace.data_ptr(), need
+    if not isinstance(workspace, torch.Tensor) or workspace.get_device() != ix or not workspace.is_contiguous():
+        raise ValueError(f"workspace: must be a contiguous tensor on cuda:{ix}")
+    size = _nbytes(workspace)
+    if size < need:
+        raise ValueError(f"workspace: needs {need} bytes (got {size})")
     if workspace.data_ptr() % 16:
         raise ValueError("workspace: must be 16-byte aligned")
-    return workspace
+    return workspace, workspace.data_ptr(), size
 
 
-def _aligned(*named) -> None:
-    """Rows of 256 bytes are moved 16 bytes at a time."""
-    for name, t in named:
-        if t.data_ptr() % 16:
-            raise ValueError(f"{name}: must be 16-byte aligned")
+def _new_workspace(name: str, device, *args) -> Optional[torch.Tensor]:
+    dev = torch.device(device)
+    if dev.type != "cuda":
+        raise ValueError(f"workspaces are on a GPU (got {dev})")
+    ix = torch.cuda.current_device() if dev.index is None else dev.index
+    return _scratch(None, _size(name, ix, *args), ix)[0]
 
 
-def _check_cache(k_cache, v_cache, B: Optional[int] = None, D: Optional[int] = None, what: str = "cache"):
-    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4:
-        raise ValueError(f"k_{what} must be [B, Hkv, S_max, D]")
-    if (B is not None and k_cache.shape[0] != B) or (D is not None and k_cache.shape[3] != D):
-        raise ValueError(f"k_{what} must be [B={B}, Hkv, S_max, D={D}] (got {tuple(k_cache.shape)})")
-    _need(k_cache, f"k_{what}", BF16)
-    _need(v_cache, f"v_{what}", BF16, k_cache.shape)
-    _aligned((f"k_{what}", k_cache), (f"v_{what}", v_cache))
-    return k_cache.shape[1], k_cache.shape[2]
+def _gpu(q, name: str, dims: str, n: int) -> int:
+    """GPU of the operand that says the call's sizes."""
+    if not isinstance(q, torch.Tensor) or q.dim() != n:
+        raise ValueError(f"{name} must be {dims}")
+    ix = q.get_device()
+    if ix < 0:
+        raise ValueError(f"{name}: must be on a GPU (got {q.device})")
+    return ix
 
 
 def _check_heads(Hq: int, Hkv: int) -> None:
@@ -833,15 +869,10 @@ def _check_heads(Hq: int, Hkv: int) -> None:
         raise ValueError(f"need Hq a multiple of Hkv, by at most 16 (Hq={Hq}, Hkv={Hkv})")
 
 
-def _check_queries(q, rows: int, out):
-    if not isinstance(q, torch.Tensor) or q.dim() != 3 or q.shape[0] != rows:
-        raise ValueError(f"q must be [{rows}, Hq, D]")
-    _need(q, "q", BF16)
-    _, Hq, D = q.shape
-    out = torch.empty(rows, Hq * D, dtype=BF16, device=q.device) if out is None else out
-    _need(out, "out", BF16, (rows, Hq * D))
-    _aligned(("q", q), ("out", out))
-    return Hq, D, out
+def _cache_sizes(k_cache, B: int, D: int):
+    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4 or k_cache.shape[0] != B or k_cache.shape[3] != D:
+        raise ValueError(f"k_cache must be [B={B}, Hkv, S_max, D={D}]")
+    return k_cache.shape[1], k_cache.shape[2]
 
 
 def _check_scale(scale: Optional[float], D: int) -> float:
@@ -854,8 +885,7 @@ def _check_scale(scale: Optional[float], D: int) -> float:
 def attn_shared_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, prefix_len: int, max_ctx: int,
                           device) -> Optional[torch.Tensor]:
     """Workspace of :func:`attn_shared` (``None`` when it needs none)."""
-    dev = torch.device(device)
-    return _scratch(None, _size("qmoe_attn_shared_workspace", dev, B, S, Hq, Hkv, D, prefix_len, max_ctx), dev)
+    return _new_workspace("qmoe_attn_shared_workspace", device, B, S, Hq, Hkv, D, prefix_len, max_ctx)
 
 
 def attn_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_cache: torch.Tensor,
@@ -871,16 +901,15 @@ def attn_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
     counts the new entry; a chunk of S tokens whose first one is own entry e:
     ``ctx_len = e + 1``.  A query that sees nothing gets zeros.  Returns
     ``[B*S, Hq*D]``."""
-    Hq, D, out = _check_queries(q, B * S, out)
-    Hkv, S_max = _check_cache(k_cache, v_cache, B, D)
+    ix = _gpu(q, "q", "[B*S, Hq, D]", 3)
+    T, Hq, D = q.shape
+    if T != B * S:
+        raise ValueError(f"q must be [B*S={B * S}, Hq, D] (got {tuple(q.shape)})")
+    Hkv, S_max = _cache_sizes(k_cache, B, D)
     _check_heads(Hq, Hkv)
     if not isinstance(k_prefix, torch.Tensor) or k_prefix.dim() != 3 or k_prefix.shape[0] != Hkv \
             or k_prefix.shape[2] != D:
         raise ValueError(f"k_prefix must be [Hkv={Hkv}, P_max, D={D}]")
-    _need(k_prefix, "k_prefix", BF16)
-    _need(v_prefix, "v_prefix", BF16, k_prefix.shape)
-    _aligned(("k_prefix", k_prefix), ("v_prefix", v_prefix))
-    _need(ctx_len, "ctx_len", I32, (B,))
     P_max = k_prefix.shape[1]
     P = P_max if prefix_len is None else int(prefix_len)
     if not 0 <= P <= P_max:
@@ -889,22 +918,21 @@ def attn_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
     if not 0 <= max_ctx <= S_max:
         raise ValueError(f"max_ctx must be in [0, {S_max}] (got {max_ctx})")
     scale = _check_scale(scale, D)
-    dev = q.device
-    _same_device(q, k_prefix, v_prefix, k_cache, v_cache, ctx_len, out)
-    ws = _scratch(workspace, _size("qmoe_attn_shared_workspace", dev, B, S, Hq, Hkv, D, P, max_ctx), dev)
-    _call("qmoe_attn_shared", dev, _ptr(q), _ptr(k_prefix), _ptr(v_prefix), P, P_max, _ptr(k_cache), _ptr(v_cache),
-          _ptr(ctx_len), B, S, Hq, Hkv, D, S_max, max_ctx, scale, _ptr(ws), _nbytes(ws), _ptr(out))
+    pq = _arg(q, "q", BF16, q.shape, ix)
+    pkp, pvp = _arg(k_prefix, "k_prefix", BF16, k_prefix.shape, ix), _arg(v_prefix, "v_prefix", BF16, k_prefix.shape, ix)
+    pk, pv = _arg(k_cache, "k_cache", BF16, k_cache.shape, ix), _arg(v_cache, "v_cache", BF16, k_cache.shape, ix)
+    pc = _arg(ctx_len, "ctx_len", I32, (B,), ix)
+    out, po = _out(out, "out", BF16, (T, Hq * D), ix)
+    _, pw, nw = _scratch(workspace, _size("qmoe_attn_shared_workspace", ix, B, S, Hq, Hkv, D, P, max_ctx), ix)
+    _call("qmoe_attn_shared", ix, pq, pkp, pvp, P, P_max, pk, pv, pc, B, S, Hq, Hkv, D, S_max, max_ctx, scale, pw, nw,
+          po)
     return out
 
 
-def attn_prefill_scored_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, start: int, device) -> torch.Tensor:
+def attn_prefill_scored_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, start: int,
+                                  device) -> Optional[torch.Tensor]:
     """Workspace of :func:`attn_prefill_scored`."""
-    dev = torch.device(device)
-    return _scratch(None, max(16, _size("qmoe_attn_prefill_scored_workspace", dev, B, S, Hq, Hkv, D, start)), dev)
-
-
-def _check_scores(scores, B: int, Hkv: int, S_max: int) -> None:
-    _need(scores, "scores", F32, (B, Hkv, S_max))
+    return _new_workspace("qmoe_attn_prefill_scored_workspace", device, B, S, Hq, Hkv, D, start)
 
 
 def attn_prefill_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, B: int,
@@ -916,28 +944,29 @@ def attn_prefill_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     group, to ``scores[B, Hkv, S_max]`` (f32, in place).  ``lengths`` (i32
     ``[B]``): of a right-padded row only the first ``lengths[b]`` queries count.
     Returns ``[B*S, Hq*D]``."""
-    Hq, D, out = _check_queries(q, B * S, out)
-    Hkv, S_max = _check_cache(k_cache, v_cache, B, D)
+    ix = _gpu(q, "q", "[B*S, Hq, D]", 3)
+    T, Hq, D = q.shape
+    if T != B * S:
+        raise ValueError(f"q must be [B*S={B * S}, Hq, D] (got {tuple(q.shape)})")
+    Hkv, S_max = _cache_sizes(k_cache, B, D)
     _check_heads(Hq, Hkv)
-    _check_scores(scores, B, Hkv, S_max)
     start = int(start)
     if start < 0 or start + S > S_max:
         raise ValueError(f"need 0 <= start and start + S <= S_max={S_max} (start={start}, S={S})")
-    if lengths is not None:
-        _need(lengths, "lengths", I32, (B,))
     scale = _check_scale(scale, D)
-    dev = q.device
-    _same_device(q, k_cache, v_cache, scores, lengths, out)
-    ws = _scratch(workspace, _size("qmoe_attn_prefill_scored_workspace", dev, B, S, Hq, Hkv, D, start), dev)
-    _call("qmoe_attn_prefill_scored", dev, _ptr(q), _ptr(k_cache), _ptr(v_cache), B, S, Hq, Hkv, D, S_max, start,
-          _ptr(lengths), scale, _ptr(ws), _nbytes(ws), _ptr(scores), _ptr(out))
+    pq = _arg(q, "q", BF16, q.shape, ix)
+    pk, pv = _arg(k_cache, "k_cache", BF16, k_cache.shape, ix), _arg(v_cache, "v_cache", BF16, k_cache.shape, ix)
+    ps = _arg(scores, "scores", F32, (B, Hkv, S_max), ix)
+    pl = None if lengths is None else _arg(lengths, "lengths", I32, (B,), ix)
+    out, po = _out(out, "out", BF16, (T, Hq * D), ix)
+    _, pw, nw = _scratch(workspace, _size("qmoe_attn_prefill_scored_workspace", ix, B, S, Hq, Hkv, D, start), ix)
+    _call("qmoe_attn_prefill_scored", ix, pq, pk, pv, B, S, Hq, Hkv, D, S_max, start, pl, scale, pw, nw, ps, po)
     return out
 
 
 def attn_decode_scored_workspace(B: int, Hq: int, D: int, max_ctx: int, device) -> Optional[torch.Tensor]:
     """Workspace of :func:`attn_decode_scored`."""
-    dev = torch.device(device)
-    return _scratch(None, _size("qmoe_attn_decode_scored_workspace", dev, B, Hq, D, max_ctx), dev)
+    return _new_workspace("qmoe_attn_decode_scored_workspace", device, B, Hq, D, max_ctx)
 
 
 def attn_decode_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx_len: torch.Tensor,
@@ -947,23 +976,21 @@ def attn_decode_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     """:func:`attn_decode` that also adds each slot's attention weight, summed
     over the q heads of its group, to ``scores[B, Hkv, S_max]`` (f32, in place).
     A row with ``ctx_len`` of zero gets zeros.  Returns ``[B, Hq*D]``."""
-    if not isinstance(q, torch.Tensor) or q.dim() != 3:
-        raise ValueError("q must be [B, Hq, D]")
-    B = q.shape[0]
-    Hq, D, out = _check_queries(q, B, out)
-    Hkv, S_max = _check_cache(k_cache, v_cache, B, D)
+    ix = _gpu(q, "q", "[B, Hq, D]", 3)
+    B, Hq, D = q.shape
+    Hkv, S_max = _cache_sizes(k_cache, B, D)
     _check_heads(Hq, Hkv)
-    _check_scores(scores, B, Hkv, S_max)
-    _need(ctx_len, "ctx_len", I32, (B,))
     max_ctx = S_max if max_ctx is None else int(max_ctx)
     if not 0 < max_ctx <= S_max:
         raise ValueError(f"max_ctx must be in [1, {S_max}] (got {max_ctx})")
     scale = _check_scale(scale, D)
-    dev = q.device
-    _same_device(q, k_cache, v_cache, ctx_len, scores, out)
-    ws = _scratch(workspace, _size("qmoe_attn_decode_scored_workspace", dev, B, Hq, D, max_ctx), dev)
-    _call("qmoe_attn_decode_scored", dev, _ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(ctx_len), B, Hq, Hkv, D, S_max,
-          max_ctx, scale, _ptr(ws), _nbytes(ws), _ptr(scores), _ptr(out))
+    pq = _arg(q, "q", BF16, q.shape, ix)
+    pk, pv = _arg(k_cache, "k_cache", BF16, k_cache.shape, ix), _arg(v_cache, "v_cache", BF16, k_cache.shape, ix)
+    ps = _arg(scores, "scores", F32, (B, Hkv, S_max), ix)
+    pc = _arg(ctx_len, "ctx_len", I32, (B,), ix)
+    out, po = _out(out, "out", BF16, (B, Hq * D), ix)
+    _, pw, nw = _scratch(workspace, _size("qmoe_attn_decode_scored_workspace", ix, B, Hq, D, max_ctx), ix)
+    _call("qmoe_attn_decode_scored", ix, pq, pk, pv, pc, B, Hq, Hkv, D, S_max, max_ctx, scale, pw, nw, ps, po)
     return out
 
 
@@ -976,31 +1003,22 @@ def kv_append(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
     whose score becomes 0 and position ``positions[b]``.  A row whose position
     or slot is out of range writes no entry and gets a zero q.  Returns
     ``q[B, Hq, D]``."""
-    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2:
-        raise ValueError("qkv must be [B, (Hq + 2 Hkv) * D]")
+    ix = _gpu(qkv, "qkv", "[B, (Hq + 2 Hkv) * D]", 2)
     B, D = qkv.shape[0], q_norm_w.shape[0]
-    _need(qkv, "qkv", F32, (B, (Hq + 2 * Hkv) * D))
-    _need(q_norm_w, "q_norm_w", BF16, (D,))
-    _need(k_norm_w, "k_norm_w", BF16, (D,))
-    max_pos = rope_cos.shape[0]
-    _need(rope_cos, "rope_cos", F32, (max_pos, D // 2))
-    _need(rope_sin, "rope_sin", F32, (max_pos, D // 2))
-    _need(positions, "positions", I32, (B,))
-    _need(slots, "slots", I32, (B,))
-    n_kv, S_max = _check_cache(k_cache, v_cache, B, D)
+    n_kv, S_max = _cache_sizes(k_cache, B, D)
     if n_kv != Hkv:
         raise ValueError(f"k_cache must have Hkv={Hkv} heads (got {n_kv})")
-    if scores is not None:
-        _check_scores(scores, B, Hkv, S_max)
-    if slot_pos is not None:
-        _need(slot_pos, "slot_pos", I32, (B, Hkv, S_max))
-    q_out = torch.empty(B, Hq, D, dtype=BF16, device=qkv.device) if q_out is None else q_out
-    _need(q_out, "q_out", BF16, (B, Hq, D))
-    _same_device(qkv, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slots, k_cache, v_cache, scores, slot_pos,
-                 q_out)
-    _call("qmoe_kv_append", qkv.device, _ptr(qkv), _ptr(q_norm_w), _ptr(k_norm_w), _ptr(rope_cos), _ptr(rope_sin),
-          max_pos, _ptr(positions), _ptr(slots), B, Hq, Hkv, D, S_max, float(eps), _ptr(q_out), _ptr(k_cache),
-          _ptr(v_cache), _ptr(scores), _ptr(slot_pos))
+    max_pos = rope_cos.shape[0]
+    half, slots_shape = (max_pos, D // 2), (B, Hkv, S_max)
+    args = (_arg(qkv, "qkv", F32, (B, (Hq + 2 * Hkv) * D), ix), _arg(q_norm_w, "q_norm_w", BF16, (D,), ix),
+            _arg(k_norm_w, "k_norm_w", BF16, (D,), ix), _arg(rope_cos, "rope_cos", F32, half, ix),
+            _arg(rope_sin, "rope_sin", F32, half, ix), max_pos, _arg(positions, "positions", I32, (B,), ix),
+            _arg(slots, "slots", I32, (B,), ix))
+    pk, pv = _arg(k_cache, "k_cache", BF16, k_cache.shape, ix), _arg(v_cache, "v_cache", BF16, k_cache.shape, ix)
+    ps = None if scores is None else _arg(scores, "scores", F32, slots_shape, ix)
+    pp = None if slot_pos is None else _arg(slot_pos, "slot_pos", I32, slots_shape, ix)
+    q_out, pq = _out(q_out, "q_out", BF16, (B, Hq, D), ix)
+    _call("qmoe_kv_append", ix, *args, B, Hq, Hkv, D, S_max, float(eps), pq, pk, pv, ps, pp)
     return q_out
 
 
@@ -1011,8 +1029,7 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 def kv_evict_workspace(B: int, Hkv: int, S_max: int, budget: int, device) -> Optional[torch.Tensor]:
     """Workspace of :func:`kv_evict`."""
-    dev = torch.device(device)
-    return _scratch(None, _size("qmoe_kv_evict_workspace", dev, B, Hkv, S_max, budget), dev)
+    return _new_workspace("qmoe_kv_evict_workspace", device, B, Hkv, S_max, budget)
 
 
 def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor, slot_pos: torch.Tensor,
@@ -1027,33 +1044,31 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     or into ``out = (k, v, scores, slot_pos)``, another cache with at least
     ``budget`` slots, leaving this one as it is.  The caller's next ``ctx_len``
     is ``ctx_len.clamp(max=budget)``."""
-    Hkv, S_max = _check_cache(k_cache, v_cache)
-    B, D = k_cache.shape[0], k_cache.shape[3]
-    _check_scores(scores, B, Hkv, S_max)
-    _need(slot_pos, "slot_pos", I32, (B, Hkv, S_max))
-    _need(ctx_len, "ctx_len", I32, (B,))
+    ix = _gpu(k_cache, "k_cache", "[B, Hkv, S_max, D]", 4)
+    B, Hkv, S_max, D = k_cache.shape
     budget, recent, sink = int(budget), int(recent), int(sink)
     if budget <= 0 or recent < 0 or sink < 0 or recent + sink > budget:
         raise ValueError(f"need budget > 0 and 0 <= recent + sink <= budget (budget={budget}, recent={recent}, "
                          f"sink={sink})")
     src = (k_cache, v_cache, scores, slot_pos)
-    if out is None:
-        k2, v2, sc2, sp2 = src
-        S_out = S_max
-    else:
-        k2, v2, sc2, sp2 = out
-        n_kv, S_out = _check_cache(k2, v2, B, D, "out")
-        if n_kv != Hkv or S_out < min(budget, S_max):
-            raise ValueError(f"out must be a cache [{B}, {Hkv}, >= {min(budget, S_max)}, {D}] (got {tuple(k2.shape)})")
-        _need(sc2, "scores_out", F32, (B, Hkv, S_out))
-        _need(sp2, "slot_pos_out", I32, (B, Hkv, S_out))
+    names = ("k", "v", "scores", "slot_pos")
+
+    def addresses(cache, what, n_slots):
+        shapes = ((B, Hkv, n_slots, D), (B, Hkv, n_slots, D), (B, Hkv, n_slots), (B, Hkv, n_slots))
+        return [_arg(t, n + what, d, s, ix) for t, n, d, s in zip(cache, names, (BF16, BF16, F32, I32), shapes)]
+
+    ps = addresses(src, "", S_max)
+    pc = _arg(ctx_len, "ctx_len", I32, (B,), ix)
+    po, S_out = ps, S_max
+    if out is not None:
+        _, S_out = _cache_sizes(out[0], B, D)
+        if S_out < min(budget, S_max):
+            raise ValueError(f"out needs at least {min(budget, S_max)} slots (got {S_out})")
+        po = addresses(out, "_out", S_out)
         if any(_overlap(x, y) for x in src for y in out):
             raise ValueError("out overlaps the cache (leave it out to evict in place)")
-    dev = k_cache.device
-    _same_device(*src, ctx_len, k2, v2, sc2, sp2)
-    ws = _scratch(workspace, _size("qmoe_kv_evict_workspace", dev, B, Hkv, S_max, budget), dev)
-    _call("qmoe_kv_evict", dev, _ptr(k_cache), _ptr(v_cache), _ptr(scores), _ptr(slot_pos), _ptr(ctx_len), B, Hkv, D,
-          S_max, budget, recent, sink, _ptr(ws), _nbytes(ws), S_out, _ptr(k2), _ptr(v2), _ptr(sc2), _ptr(sp2))
+    _, pw, nw = _scratch(workspace, _size("qmoe_kv_evict_workspace", ix, B, Hkv, S_max, budget), ix)
+    _call("qmoe_kv_evict", ix, *ps, pc, B, Hkv, D, S_max, budget, recent, sink, pw, nw, S_out, *po)
 
 
 # ----------------------------------------------------------------- embedding / greedy argmax

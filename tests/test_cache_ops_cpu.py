@@ -119,7 +119,7 @@ def test_wrappers_refuse():
     sc, sp, n = torch.zeros(2, 4, 8), _i(2, 4, 8), _i(2)
     calls = [
         (lambda: ops.attn_shared(q, kp, kp, k, k, n, 2, 1), "must be on a GPU"),
-        (lambda: ops.attn_shared(q, kp, kp, k, k, n, 3, 1), r"q must be \[3"),
+        (lambda: ops.attn_shared(q[0], kp, kp, k, k, n, 3, 1), "q must be"),
         (lambda: ops.attn_shared(None, kp, kp, k, k, n, 2, 1), "q must be"),
         (lambda: ops.attn_prefill_scored(q, k, k, sc, 1, 2), "must be on a GPU"),
         (lambda: ops.attn_decode_scored(q[0], k, k, n, sc), "q must be"),
@@ -133,9 +133,12 @@ def test_wrappers_refuse():
         (lambda: ops._check_heads(128, 4), "at most 16"),
         (lambda: ops._check_scale(float("nan"), 128), "scale"),
         (lambda: ops._check_scale(0.0, 128), "scale"),
-        (lambda: ops._scratch(torch.zeros(4), 17, torch.device("cpu")), "needs 17 bytes"),
-        (lambda: ops._scratch(torch.zeros(64, dtype=torch.uint8)[1:], 8, torch.device("cpu")), "aligned"),
-        (lambda: ops.attn_shared_workspace(1, 1, 33, 4, 128, 1, 1, "cpu"), "bad sizes"),
+        (lambda: ops._scratch(torch.zeros(4), 17, -1), "needs 17 bytes"),
+        (lambda: ops._scratch(torch.zeros(64, dtype=torch.uint8)[1:], 8, -1), "aligned"),
+        (lambda: ops._scratch(torch.zeros(4), 8, 0), "on cuda:0"),
+        (lambda: ops._size("qmoe_attn_shared_workspace", None, 1, 1, 33, 4, 128, 1, 1), "bad sizes"),
+        (lambda: ops.attn_shared_workspace(1, 1, 32, 4, 128, 1, 1, "cpu"), "on a GPU"),
+        (lambda: ops._arg(torch.zeros(9)[1:], "x", torch.float32, (8,), -1), "must be on a GPU"),
     ]
     for call, msg in calls:
         with pytest.raises(ValueError, match=msg):
