@@ -206,7 +206,7 @@ __global__ __launch_bounds__(256) void attn_rows_merge_kernel(const ArArgs a) {
 // ====================================================================== column sums
 constexpr int CS_KEYS = 256;  // keys of a workgroup (4 waves x 64)
 constexpr int CS_QT = 64;     // query rows of a streamed tile
-constexpr int CS_BUFS = 3;
+constexpr int CS_BUFS = 3, CS_LBUFS = 4;
 constexpr int CS_QBYTES = CS_QT * AP_ROWB;
 
 struct CsArgs {
@@ -231,7 +231,7 @@ __device__ __forceinline__ int cs_div(uint32_t r, uint32_t magic) {
 // over the rows of a tile is an addition within the lane.
 __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[CS_BUFS * CS_QBYTES];
-  __shared__ __attribute__((aligned(1024))) float ls[CS_BUFS][4][CS_QT];  // a copy for each wave
+  __shared__ __attribute__((aligned(1024))) float ls[CS_LBUFS][4][CS_QT];  // a copy for each wave
   const int t = threadIdx.x, lane = t & 63, hl = lane >> 5, col = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const int G = a.Hq / a.Hkv, grp = a.B * a.Hkv;
@@ -277,52 +277,74 @@ __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
       const uint32_t off = (uint32_t(s) * a.Hq + g) * AP_ROWB + uint32_t(ap_kslot(rr, lane & 15) * 16);
       pipe::dma16(dst + j * 1024, s < len ? off : pipe::PAD, rq, 0);
     }
-    pipe::dma4(lds_l + uint32_t(buf * 4 * CS_QT * 4), uint32_t(q0 + i * CS_QT + lane) * 4u, rl, 0);
+    pipe::dma4(lds_l + uint32_t(i % CS_LBUFS * 4 * CS_QT * 4), uint32_t(q0 + i * CS_QT + lane) * 4u, rl, 0);
   };
   float acc[2] = {0.0f, 0.0f};
+  // S of rows [32 rb, 32 rb + 32) of tile i
+  auto qk = [&](int i, int rb, f32x16 (&sc)[2]) {
+    const uint8_t* qp = smem + i % CS_BUFS * CS_QBYTES + (rb * 32 + col) * AP_ROWB;
+#pragma unroll
+    for (int ks = 0; ks < HD / 16; ++ks) {
+      const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(qp + ap_kslot(lane, 2 * ks + hl) * 16);
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+        sc[cb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, kf[cb][ks], ks ? sc[cb] : f32x16{}, 0, 0, 0);
+    }
+  };
+  // their weights into the sums
+  auto add = [&](int i, int rb, f32x16 (&sc)[2], auto masked) {
+    const int r0 = q0 + i * CS_QT + rb * 32 + hl * 4;
+#pragma unroll
+    for (int g4 = 0; g4 < 4; ++g4) {
+      const float4 le = *reinterpret_cast<const float4*>(&ls[i % CS_LBUFS][wave][rb * 32 + g4 * 8 + hl * 4]);
+      const float lo[4] = {le.x, le.y, le.z, le.w};
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float w = __builtin_amdgcn_exp2f(fmaf(sc[cb][g4 * 4 + e], a.scale_log2, -lo[e]));
+          if constexpr (decltype(masked)::value) {
+            const int r = r0 + g4 * 8 + e;
+            w = r < rmin[cb] || r >= q1 ? 0.0f : w;
+          }
+          acc[cb] += w;
+        }
+    }
+  };
+  // S of one half tile is issued before the weights of the half before it
+  auto step = [&](int i, int rb, f32x16 (&cur)[2], int ni, int nrb, f32x16 (&nxt)[2]) {
+    const int rt = q0 + i * CS_QT;
+    if (rt < wave_rmax || rt + CS_QT > q1) {
+      qk(ni, nrb, nxt);
+      add(i, rb, cur, std::true_type{});
+    } else {
+      qk(ni, nrb, nxt);
+      add(i, rb, cur, std::false_type{});
+    }
+  };
+  f32x16 sa[2], sb[2];
   dma_q(0);
-  if (n_t > 1) dma_q(1);
-  for (int i = 0; i < n_t; ++i) {
-    const int buf = i % CS_BUFS, rt = q0 + i * CS_QT;
-    if (i + 1 < n_t)
+  if (n_t > 1) {
+    dma_q(1);
+    pipe::wait_vm<5>();
+  } else {
+    pipe::wait_vm<0>();
+  }
+  __syncthreads();
+  if (n_t > 2) dma_q(2);
+  qk(0, 0, sa);
+  for (int i = 0; i + 1 < n_t; ++i) {
+    step(i, 0, sa, i, 1, sb);
+    if (i + 2 < n_t)
       pipe::wait_vm<5>();
     else
       pipe::wait_vm<0>();
-    __syncthreads();  // tile i and its lse visible; tile i - 1's buffer free
-    if (i + 2 < n_t) dma_q(i + 2);
-    f32x16 sc[2][2];
-    const uint8_t* qp = smem + buf * CS_QBYTES + col * AP_ROWB;
-#pragma unroll
-    for (int ks = 0; ks < HD / 16; ++ks) {
-      const int so = ap_kslot(lane, 2 * ks + hl) * 16;
-      const bf16x8 a0 = *reinterpret_cast<const bf16x8*>(qp + so);
-      const bf16x8 a1 = *reinterpret_cast<const bf16x8*>(qp + 32 * AP_ROWB + so);
-#pragma unroll
-      for (int cb = 0; cb < 2; ++cb) {
-        sc[0][cb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a0, kf[cb][ks], ks ? sc[0][cb] : f32x16{}, 0, 0, 0);
-        sc[1][cb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a1, kf[cb][ks], ks ? sc[1][cb] : f32x16{}, 0, 0, 0);
-      }
-    }
-    const bool mask = rt < wave_rmax || rt + CS_QT > q1;
-#pragma unroll
-    for (int rb = 0; rb < 2; ++rb)
-#pragma unroll
-      for (int g4 = 0; g4 < 4; ++g4) {
-        const float4 le = *reinterpret_cast<const float4*>(&ls[buf][wave][rb * 32 + g4 * 8 + hl * 4]);
-        const float lo[4] = {le.x, le.y, le.z, le.w};
-#pragma unroll
-        for (int cb = 0; cb < 2; ++cb)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float w = __builtin_amdgcn_exp2f(fmaf(sc[rb][cb][g4 * 4 + e], a.scale_log2, -lo[e]));
-            if (mask) {
-              const int r = rt + rb * 32 + g4 * 8 + hl * 4 + e;
-              w = r < rmin[cb] || r >= q1 ? 0.0f : w;
-            }
-            acc[cb] += w;
-          }
-      }
+    __syncthreads();  // tile i + 1 visible, tile i's queries read (its lse not yet: CS_LBUFS)
+    if (i + 3 < n_t) dma_q(i + 3);
+    step(i, 1, sb, i + 1, 0, sa);
   }
+  step(n_t - 1, 0, sa, n_t - 1, 1, sb);
+  add(n_t - 1, 1, sb, std::true_type{});
 #pragma unroll
   for (int cb = 0; cb < 2; ++cb) acc[cb] += __shfl_xor(acc[cb], 32, 64);
   if (hl == 0) {
@@ -332,21 +354,32 @@ __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
   }
 }
 
-// scores += the chunks' sums, in chunk order
+// scores += the chunks' sums: a workgroup takes 64 keys, wave w the chunks w, w +
+// 4, ..., each eight loads at a time, and the waves' sums join in wave order.
 __global__ __launch_bounds__(256) void attn_colsum_add_kernel(const CsArgs a) {
-  const int grp = a.B * a.Hkv, bh = blockIdx.y, key = int(blockIdx.x) * 256 + int(threadIdx.x);
-  if (key >= a.n_keys) return;
+  __shared__ float red[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int grp = a.B * a.Hkv, bh = blockIdx.y, key = int(blockIdx.x) * 64 + lane;
   const int G = a.Hq / a.Hkv, b = bh / a.Hkv;
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
-  const int key0 = key / CS_KEYS * CS_KEYS, live0 = max(key0 - a.start, 0) * G / CS_QT * CS_QT;
+  const int live0 = max(key / CS_KEYS * CS_KEYS - a.start, 0) * G / CS_QT * CS_QT;
+  // chunks with rows in [live0, len * G) (all of a workgroup's keys have one key tile)
+  const int c0 = live0 / a.chunk, c1 = live0 < len * G ? (len * G + a.chunk - 1) / a.chunk : c0;
+  if (c0 >= c1) return;
+  const float* p = a.part + int64_t(bh) * a.nkt * CS_KEYS + key;
+  const int64_t next = int64_t(grp) * a.nkt * CS_KEYS;
   float sum = 0.0f;
-  bool any = false;
-  for (int ch = live0 / a.chunk; ch * a.chunk < len * G; ++ch)
-    if (max(ch * a.chunk, live0) < min((ch + 1) * a.chunk, len * G)) {
-      sum += a.part[(int64_t(ch) * grp + bh) * (int64_t(a.nkt) * CS_KEYS) + key];
-      any = true;
-    }
-  if (any) a.scores[int64_t(bh) * a.S_max + key] += sum;
+  for (int c = c0 + wave; c < c1; c += 32) {
+    float v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = c + 4 * u < c1 ? p[(c + 4 * u) * next] : 0.0f;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) sum += v[u];
+  }
+  red[wave][lane] = sum;
+  __syncthreads();
+  if (wave == 0 && key < a.n_keys)
+    a.scores[int64_t(bh) * a.S_max + key] += (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 }
 
 // ---------------------------------------------------------------------- host
@@ -415,13 +448,13 @@ static ArArgs ar_args(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_m
   return a;
 }
 
-// Chunks of query rows per key tile of the column sums: enough items for four
-// workgroups a CU (half of them see no key of their tile), each of at least
-// 256 rows.
+// Chunks of query rows per key tile of the column sums: half of the items see
+// no key of their tile, and the others end together only if there are several
+// rounds of them, so about 16 items a CU, each of at least 256 rows.
 static void cs_plan(CsArgs& a) {
   const int64_t G = a.Hq / a.Hkv, rows = a.S * G;
   a.nkt = int(ar_ceil(a.n_keys, CS_KEYS));
-  const int64_t items = int64_t(a.B) * a.Hkv * a.nkt, want = 4 * int64_t(std::max(current_device_cus(), 1));
+  const int64_t items = int64_t(a.B) * a.Hkv * a.nkt, want = 16 * int64_t(std::max(current_device_cus(), 1));
   int64_t n = std::max<int64_t>(1, std::min(ar_ceil(want, items), ar_ceil(rows, 256)));
   a.chunk = int(ar_ceil(ar_ceil(rows, n), CS_QT) * CS_QT);
   a.n_chunk = int(ar_ceil(rows, a.chunk));
@@ -545,7 +578,7 @@ extern "C" int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_c
   if (int rc = ar_launch(fn, a, grid, as_stream(stream))) return rc;
   hipLaunchKernelGGL(attn_colsum_kernel, dim3(unsigned(cgrid)), dim3(256), 0, as_stream(stream), c);
   if (int rc = hip_status(fn)) return rc;
-  hipLaunchKernelGGL(attn_colsum_add_kernel, dim3(unsigned(c.nkt), unsigned(B * Hkv)), dim3(256), 0,
-                     as_stream(stream), c);
+  hipLaunchKernelGGL(attn_colsum_add_kernel, dim3(unsigned(c.nkt * (CS_KEYS / 64)), unsigned(B * Hkv)), dim3(256),
+                     0, as_stream(stream), c);
   return hip_status(fn);
 }
