@@ -213,10 +213,10 @@ struct CsArgs {
   const uint16_t *q, *k;
   const float* lse;        // [B][Hkv][S * G]
   const int32_t* lengths;  // or nullptr
-  int B, S, Hq, Hkv, S_max, start, n_keys, nkt, n_chunk, chunk;
+  int B, S, Hq, Hkv, S_max, start, n_keys, nkt, n_chunk, run;
   uint32_t g_magic;  // ceil(2^32 / G), 0 for G == 1
   float scale_log2;
-  float* part;    // [n_chunk][B][Hkv][nkt * CS_KEYS]
+  float* part;    // [n_chunk][B][Hkv][nkt * CS_KEYS]: a sum for each run
   float* scores;  // [B][Hkv][S_max]
 };
 
@@ -225,7 +225,20 @@ __device__ __forceinline__ int cs_div(uint32_t r, uint32_t magic) {
   return int(magic ? __umulhi(r, magic) : r);
 }
 
-// Item (b, kv head, key tile, chunk of query rows): a wave keeps 64 keys as
+// The packed rows that see key tile kt start at (about) row cs_first, a multiple
+// of CS_QT; its row tiles up to the last counted row are cut into runs of
+// equal length, at most `run` tiles.  len: counted queries.
+__device__ __forceinline__ int cs_first(const CsArgs& a, int kt, int G) {
+  return max(kt * CS_KEYS - a.start, 0) * G / CS_QT * CS_QT;
+}
+__device__ __forceinline__ int cs_tiles(const CsArgs& a, int kt, int G, int len) {
+  return max((len * G - cs_first(a, kt, G) + CS_QT - 1) / CS_QT, 0);
+}
+__device__ __forceinline__ int cs_len(const CsArgs& a, int b) {
+  return a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
+}
+
+// Item (b, kv head, key tile, run of query rows): a wave keeps 64 keys as
 // the B operands of S = Q . K^T, query tiles of 64 packed rows stream through
 // LDS, and since lane l of a 32 x 32 block holds column l % 32, a key's sum
 // over the rows of a tile is an addition within the lane.
@@ -238,11 +251,14 @@ __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
   const int x = int(blockIdx.x), bh = x % grp, y = x / grp, kt = y % a.nkt, ch = y / a.nkt;
   const int b = bh / a.Hkv, kvh = bh % a.Hkv;
   const int key0 = kt * CS_KEYS;
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
-  // rows that see the tile's first key: query >= key0 - start
-  const int live0 = max(key0 - a.start, 0) * G / CS_QT * CS_QT;
-  const int q0 = max(ch * a.chunk, live0), q1 = min((ch + 1) * a.chunk, len * G);
-  if (q0 >= q1) return;  // the reduction knows which chunks a key tile has
+  const int len = cs_len(a, b), tiles = cs_tiles(a, kt, G, len), runs = (tiles + a.run - 1) / a.run;
+  if (ch >= runs) return;  // the addition knows how many runs a key tile has
+  const int per = (tiles + runs - 1) / runs;
+  const int q0 = cs_first(a, kt, G) + ch * per * CS_QT, q1 = min(q0 + per * CS_QT, len * G);
+  if (q0 >= q1) {  // rounding left the last run empty
+    a.part[(int64_t(ch) * grp + bh) * (int64_t(a.nkt) * CS_KEYS) + key0 + t] = 0.0f;
+    return;
+  }
   const int n_t = (q1 - q0 + CS_QT - 1) / CS_QT;
   // K as B operands: column block cb, k-step ks: key key0 + 64 wave + 32 cb + col
   bf16x8 kf[2][HD / 16];
@@ -320,6 +336,12 @@ __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
     } else {
       qk(ni, nrb, nxt);
       add(i, rb, cur, std::false_type{});
+#pragma unroll
+      for (int x = 0; x < 16; ++x) {  // an MFMA, then a sixteenth of the weights' work
+        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
+      }
     }
   };
   f32x16 sa[2], sb[2];
@@ -354,22 +376,18 @@ __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
   }
 }
 
-// scores += the chunks' sums: a workgroup takes 64 keys, wave w the chunks w, w +
+// scores += the runs' sums: a workgroup takes 64 keys, wave w the runs w, w +
 // 4, ..., each eight loads at a time, and the waves' sums join in wave order.
 __global__ __launch_bounds__(256) void attn_colsum_add_kernel(const CsArgs a) {
   __shared__ float red[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int grp = a.B * a.Hkv, bh = blockIdx.y, key = int(blockIdx.x) * 64 + lane;
-  const int G = a.Hq / a.Hkv, b = bh / a.Hkv;
-  const int len = a.lengths ? min(max(a.lengths[b], 0), a.S) : a.S;
-  const int live0 = max(key / CS_KEYS * CS_KEYS - a.start, 0) * G / CS_QT * CS_QT;
-  // chunks with rows in [live0, len * G) (all of a workgroup's keys have one key tile)
-  const int c0 = live0 / a.chunk, c1 = live0 < len * G ? (len * G + a.chunk - 1) / a.chunk : c0;
-  if (c0 >= c1) return;
+  const int c1 = (cs_tiles(a, key / CS_KEYS, a.Hq / a.Hkv, cs_len(a, bh / a.Hkv)) + a.run - 1) / a.run;
+  if (c1 == 0) return;
   const float* p = a.part + int64_t(bh) * a.nkt * CS_KEYS + key;
   const int64_t next = int64_t(grp) * a.nkt * CS_KEYS;
   float sum = 0.0f;
-  for (int c = c0 + wave; c < c1; c += 32) {
+  for (int c = wave; c < c1; c += 32) {
     float v[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) v[u] = c + 4 * u < c1 ? p[(c + 4 * u) * next] : 0.0f;
@@ -448,16 +466,28 @@ static ArArgs ar_args(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_m
   return a;
 }
 
-// Chunks of query rows per key tile of the column sums: half of the items see
-// no key of their tile, and the others end together only if there are several
-// rounds of them, so about 16 items a CU, each of at least 256 rows.
+// Length of a run of row tiles in the column sums.  Two workgroups fit a CU;
+// with k rounds of them the runs are about (all row tiles) / (k * places - key
+// tiles) long (each key tile rounds its number of runs up), and a run costs
+// about CS_START tiles more (K loads, the first tiles' round trip).
+constexpr int64_t CS_START = 5;
 static void cs_plan(CsArgs& a) {
-  const int64_t G = a.Hq / a.Hkv, rows = a.S * G;
+  const int64_t G = a.Hq / a.Hkv, tiles = ar_ceil(a.S * G, CS_QT);
   a.nkt = int(ar_ceil(a.n_keys, CS_KEYS));
-  const int64_t items = int64_t(a.B) * a.Hkv * a.nkt, want = 16 * int64_t(std::max(current_device_cus(), 1));
-  int64_t n = std::max<int64_t>(1, std::min(ar_ceil(want, items), ar_ceil(rows, 256)));
-  a.chunk = int(ar_ceil(ar_ceil(rows, n), CS_QT) * CS_QT);
-  a.n_chunk = int(ar_ceil(rows, a.chunk));
+  int64_t sum = 0;  // row tiles over the key tiles of one (row, kv head)
+  for (int64_t kt = 0; kt < a.nkt; ++kt) sum += tiles - std::max<int64_t>(kt * CS_KEYS - a.start, 0) * G / CS_QT;
+  const int64_t places = 2 * int64_t(std::max(current_device_cus(), 1)), grp = int64_t(a.B) * a.Hkv;
+  int64_t best = INT64_MAX;
+  for (int64_t k = 1; k <= 8; ++k) {
+    const int64_t room = k * places / grp - a.nkt;
+    const int64_t run = room > 0 ? std::max<int64_t>(ar_ceil(sum, room), 1) : tiles;
+    const int64_t rounds = ar_ceil(grp * (sum / run + a.nkt), places), cost = rounds * (run + CS_START);
+    if (cost < best) {
+      best = cost;
+      a.run = int(run);
+    }
+  }
+  a.n_chunk = int(ar_ceil(tiles, a.run));
   a.g_magic = G == 1 ? 0u : uint32_t(((1ull << 32) + uint64_t(G) - 1) / uint64_t(G));
 }
 
