@@ -27,25 +27,42 @@
 
 namespace qmoe {
 
-constexpr int AR_ROWS = 128;      // query rows of a tile (4 waves x 32)
 constexpr int AR_REC = HD + 4;    // record of a row's run: m, l, 2 pad, O[HD]
 constexpr int AR_MAX_G = 16;      // q heads per kv head
 constexpr int64_t AR_MAX_KEYS = 1ll << 22;  // keys of one run are addressed with 32-bit byte offsets
+
+// A kind of item: `rows` query rows and runs of `run` steps of `keys` keys.
+// Tiles (128 rows, 64 keys: flash_segment) share each key among four waves'
+// rows; streams (32 rows, 256 keys: stream_segment) share each row among four
+// waves' keys.
+struct ArKind {
+  int stream, rts, runs, run;
+  __host__ __device__ int rows() const { return stream ? 32 : 128; }
+  __host__ __device__ int keys() const { return stream ? 4 * AP_KT : AP_KT; }
+};
 
 struct ArArgs {
   const uint16_t *q, *kp, *vp, *k, *v;
   const int32_t* ctx_len;  // own entries that a row's query 0 sees; nullptr: start + 1 for every row
   const int32_t* lengths;  // queries of a row that count in lse; nullptr: all
   int P, Pmax, B, S, Hq, Hkv, S_max, max_ctx, start;
+  uint32_t g_magic;        // ar_magic(G)
   float scale_log2;
   uint16_t* out;
   float* part;  // [B * S * Hq][NS][AR_REC], when NS > 1
   float* lse;   // [B][Hkv][S * G] or nullptr
-  // NS: runs per row.  n_pre prefix items (rtp row tiles x nsp runs of pt
-  // tiles x Hkv), then items of rts row tiles x nss runs of st tiles x (B, Hkv),
-  // whose key tiles start with the prefix when joint.
-  int NS, n_pre, nsp, pt, rts, nss, st, joint;
+  // n_pre prefix items (pre.rts row tiles over all B * S * G rows x pre.runs x
+  // Hkv), then items of (own.rts row tiles x own.runs x B x Hkv), whose steps
+  // start with the prefix when joint.  NS = pre.runs + own.runs records a row.
+  int NS, n_pre, joint;
+  ArKind pre, own;
 };
+
+// r / G for 0 <= r < 2^32 / G, by a multiplication
+__host__ __device__ __forceinline__ uint32_t ar_magic(uint32_t G) {
+  return G == 1 ? 0u : uint32_t(((1ull << 32) + G - 1) / G);
+}
+__device__ __forceinline__ int ar_div(uint32_t r, uint32_t magic) { return int(magic ? __umulhi(r, magic) : r); }
 
 // Own entries that query s of batch row b sees.
 __device__ __forceinline__ int ar_sees(const ArArgs& a, int b, int s) {
@@ -55,77 +72,82 @@ __device__ __forceinline__ int ar_sees(const ArArgs& a, int b, int s) {
 
 __device__ __forceinline__ float ar_lse(float m, float l) { return l > 0.0f ? m + __log2f(l) : INFINITY; }
 
-__global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];
+template <bool stream>
+__device__ __forceinline__ void ar_item(const ArArgs& a, const ArKind kd, const bool pre, uint8_t* smem) {
   const int lane = threadIdx.x & 63, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-  const int G = a.Hq / a.Hkv, nPT = (a.P + AP_KT - 1) / AP_KT;
-  const bool pre = int(blockIdx.x) < a.n_pre;
-  int kvh, b = 0, r0, rows, slot, t0, t1;  // key tiles [t0, t1) of the item's list
+  const int G = a.Hq / a.Hkv;
+  constexpr int KS = stream ? 4 * AP_KT : AP_KT, ROWS = stream ? 32 : 128;
+  const int nP = (a.P + KS - 1) / KS;  // steps of the prefix
+  int kvh, b = 0, r0, rows, run;
   if (pre) {
-    // (kv head, run) fastest: the row tiles of one run sit Hkv * nsp items apart,
+    // (kv head, run) fastest: the row tiles of one run sit Hkv * runs items apart,
     // on one XCD (and its L2) when that is a multiple of 8
-    const int grp = a.Hkv * a.nsp, x = int(blockIdx.x), y = x % grp;
+    const int grp = a.Hkv * kd.runs, x = int(blockIdx.x), y = x % grp;
     kvh = y % a.Hkv;
-    slot = y / a.Hkv;
-    r0 = x / grp * AR_ROWS;
+    run = y / a.Hkv;
+    r0 = x / grp * ROWS;
     rows = a.B * a.S * G;
-    t0 = slot * a.pt;
-    t1 = min(nPT, t0 + a.pt);
   } else {
     // latest row tile (the most keys) first
-    const int grp = a.B * a.Hkv, x = int(blockIdx.x) - a.n_pre, y = x % (grp * a.nss);
-    const int run = y / grp;
-    b = y % grp / a.Hkv;
-    kvh = y % a.Hkv;
-    r0 = (a.rts - 1 - x / (grp * a.nss)) * AR_ROWS;
+    const int grp = a.B * a.Hkv, x = int(blockIdx.x) - a.n_pre, y = x % (grp * kd.runs), z = y % grp;
+    run = y / grp;
+    b = z / a.Hkv;
+    kvh = z % a.Hkv;
+    r0 = (kd.rts - 1 - x / (grp * kd.runs)) * ROWS;
     rows = a.S * G;
-    slot = a.nsp + run;
-    const int seen = ar_sees(a, b, min(r0 + AR_ROWS - 1, rows - 1) / G);
-    t0 = run * a.st;
-    t1 = min((a.joint ? nPT : 0) + (seen + AP_KT - 1) / AP_KT, t0 + a.st);
   }
-  const int rw = r0 + wave * 32;                   // the wave's first row
+  const int off = pre || a.joint ? nP : 0;  // own steps start here
+  // own keys that the tile's last row sees; the item's steps [t0, t1)
+  const int seen = pre ? 0 : ar_sees(a, b, ar_div(min(r0 + ROWS, rows) - 1, a.g_magic));
+  const int t0 = run * kd.run, t1 = min(off + (seen + KS - 1) / KS, t0 + kd.run);
+  const int rw = r0 + (stream ? 0 : wave * 32);    // the wave's first row
   const int row = rw + (lane & 31);                // this lane's row
-  const bool live = row < rows;
+  const bool live = row < rows, wlive = rw < rows;
   const int rq = live ? row : rows - 1;            // a row to take the limits of
-  const int sq = rq / G;                           // its query (over the whole batch for prefix items)
-  const int64_t qrow = (pre ? int64_t(sq) : int64_t(b) * a.S + sq) * a.Hq + kvh * G + rq % G;
+  const int sq = ar_div(rq, a.g_magic);            // its query (over the whole batch for prefix items)
+  const int64_t qrow = (pre ? int64_t(sq) : int64_t(b) * a.S + sq) * a.Hq + kvh * G + (rq - sq * G);
   FlashRows st;
   st.start(live ? a.q + qrow * HD : nullptr, hl);
-  const bool wlive = rw < rows;                    // wave-uniform
-  const int pt1 = pre || a.joint ? min(t1, nPT) : 0, off = a.joint ? nPT : 0;
-  // the list's prefix tiles, then its own-key tiles (one copy of the loop's code)
+  // the prefix steps of the run, then its own steps (one copy of the loop's code)
 #pragma unroll 1
   for (int seg = 0; seg < 2; ++seg) {
     const uint16_t *kk = a.kp, *vv = a.vp;
     int64_t base;
     int n, lim, first = -1, last = -1;
     if (seg == 0) {
-      if (t0 >= pt1) continue;
-      const int k0 = t0 * AP_KT;
-      n = min(a.P, pt1 * AP_KT) - k0;
+      const int e = min(t1, off);
+      if (t0 >= e) continue;
+      const int k0 = t0 * KS;
+      n = min(a.P, e * KS) - k0;
       base = (int64_t(kvh) * a.Pmax + k0) * HD;
       lim = first = n - 1;
       if (wlive) last = n - 1;
     } else {
       const int s0 = max(t0, off) - off, s1 = t1 - off;
-      if (pre || s0 >= s1) break;
-      const int k0 = s0 * AP_KT;
-      const int end = min(ar_sees(a, b, min(r0 + AR_ROWS - 1, rows - 1) / G), s1 * AP_KT);
+      if (s0 >= s1) break;
+      const int k0 = s0 * KS, end = min(seen, s1 * KS);
       n = end - k0;
       kk = a.k;
       vv = a.v;
       base = ((int64_t(b) * a.Hkv + kvh) * a.S_max + k0) * HD;
       lim = min(ar_sees(a, b, sq), end) - 1 - k0;
       if (wlive) {
-        first = min(ar_sees(a, b, rw / G), end) - 1 - k0;
-        last = min(ar_sees(a, b, min(rw + 31, rows - 1) / G), end) - 1 - k0;
+        first = min(ar_sees(a, b, ar_div(rw, a.g_magic)), end) - 1 - k0;
+        last = min(ar_sees(a, b, ar_div(min(rw + 31, rows - 1), a.g_magic)), end) - 1 - k0;
       }
     }
-    flash_segment(smem, kk + base, vv + base, n, lim, __builtin_amdgcn_readfirstlane(first),
-                  __builtin_amdgcn_readfirstlane(last), a.scale_log2, st);
+    if constexpr (stream)
+      stream_segment(smem, kk + base, vv + base, n, lim, a.scale_log2, st);
+    else
+      flash_segment(smem, kk + base, vv + base, n, lim, __builtin_amdgcn_readfirstlane(first),
+                    __builtin_amdgcn_readfirstlane(last), a.scale_log2, st);
   }
+  if constexpr (stream) {
+    flash_join(smem, st);
+    if (wave) return;
+  }
+  const int slot = (pre ? 0 : a.pre.runs) + run;
   if (!live) return;
   const float l = st.row_sum();
   if (a.NS > 1) {
@@ -155,6 +177,23 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
   if (a.lse && hl == 0 && !pre)
     a.lse[(int64_t(b) * a.Hkv + kvh) * rows + row] =
         a.lengths && sq >= a.lengths[b] ? INFINITY : ar_lse(st.m, l);
+}
+
+// Both kinds of item in one launch: the prefix's tiles are bound by the matrix
+// pipe, the streams by memory, and they share the CUs.
+template <bool TILES, bool STREAMS>
+__global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];
+  const bool pre = int(blockIdx.x) < a.n_pre;
+  const ArKind kd = pre ? a.pre : a.own;
+  if constexpr (TILES && STREAMS) {
+    if (kd.stream)
+      ar_item<true>(a, kd, pre, smem);
+    else
+      ar_item<false>(a, kd, pre, smem);
+  } else {
+    ar_item<STREAMS>(a, kd, pre, smem);
+  }
 }
 
 // One wave a row (b, s, head): lane i takes the (m, l) of run i, then two dims
@@ -214,16 +253,11 @@ struct CsArgs {
   const float* lse;        // [B][Hkv][S * G]
   const int32_t* lengths;  // or nullptr
   int B, S, Hq, Hkv, S_max, start, n_keys, nkt, n_chunk, run;
-  uint32_t g_magic;  // ceil(2^32 / G), 0 for G == 1
+  uint32_t g_magic;  // ar_magic(G)
   float scale_log2;
   float* part;    // [n_chunk][B][Hkv][nkt * CS_KEYS]: a sum for each run
   float* scores;  // [B][Hkv][S_max]
 };
-
-// r / G for 0 <= r < 2^32 / G
-__device__ __forceinline__ int cs_div(uint32_t r, uint32_t magic) {
-  return int(magic ? __umulhi(r, magic) : r);
-}
 
 // The packed rows that see key tile kt start at (about) row cs_first, a multiple
 // of CS_QT; its row tiles up to the last counted row are cut into runs of
@@ -289,7 +323,7 @@ __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
     for (int j = 0; j < 4; ++j) {
       const int rr = 16 * wave + 4 * j + (lane >> 4);
       const uint32_t r = uint32_t(q0 + i * CS_QT + rr);
-      const int s = cs_div(r, a.g_magic), g = int(r) - s * G;
+      const int s = ar_div(r, a.g_magic), g = int(r) - s * G;
       const uint32_t off = (uint32_t(s) * a.Hq + g) * AP_ROWB + uint32_t(ap_kslot(rr, lane & 15) * 16);
       pipe::dma16(dst + j * 1024, s < len ? off : pipe::PAD, rq, 0);
     }
@@ -403,29 +437,38 @@ __global__ __launch_bounds__(256) void attn_colsum_add_kernel(const CsArgs a) {
 // ---------------------------------------------------------------------- host
 static int64_t ar_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Splits the work into key runs of about as many tiles as fill two workgroups
-// on every CU, and at least AR_MIN_RUN (a run's record and its pipeline's
-// start cost about two tiles).  own = own key tiles of a row at most.
+// Cuts the work into items.  own_keys: own keys of a row at most.  Rows of one
+// sequence that fill a tile run over prefix and own keys in one item; fewer
+// rows leave the prefix to tiles (up to 64 rows of the batch: to streams) of its
+// own, read once for all rows of a tile, and take their own keys as streams
+// (more than 64 rows: as tiles).  Run lengths: about two workgroups on every
+// CU, of at least AR_MIN_RUN tile steps or one stream step.
 constexpr int64_t AR_MIN_RUN = 2;
+static void ar_cut(ArKind& kd, int64_t rows, int64_t steps, int64_t run) {
+  kd.rts = int(ar_ceil(rows, kd.rows()));
+  kd.runs = steps > 0 ? int(ar_ceil(steps, run)) : 0;
+  kd.run = kd.runs ? int(ar_ceil(steps, kd.runs)) : 1;
+  kd.runs = int(ar_ceil(steps, kd.run));
+}
 static void ar_plan(ArArgs& a, int64_t own_keys, int64_t* grid) {
-  const int64_t G = a.Hq / a.Hkv, rows = a.S * G;
-  const int64_t nPT = ar_ceil(a.P, AP_KT), nOT = ar_ceil(own_keys, AP_KT);
+  const int64_t G = a.Hq / a.Hkv, rows = a.S * G, all = int64_t(a.B) * rows, groups = int64_t(a.B) * a.Hkv;
   const int64_t slots = 2 * int64_t(std::max(current_device_cus(), 1));
-  a.joint = rows >= AR_ROWS;
-  a.rts = int(ar_ceil(rows, AR_ROWS));
-  const int64_t rtp = ar_ceil(int64_t(a.B) * rows, AR_ROWS), grp = int64_t(a.B) * a.Hkv * a.rts;
-  const int64_t pre_w = a.joint ? 0 : rtp * a.Hkv * nPT, own_w = grp * (nOT + (a.joint ? nPT : 0));
+  a.joint = rows >= 128;
+  a.pre.stream = !a.joint && all <= 64;
+  a.own.stream = rows <= 64;
+  const int64_t pre_steps = a.joint ? 0 : ar_ceil(a.P, a.pre.keys());
+  const int64_t own_steps = ar_ceil(own_keys, a.own.keys()) + (a.joint ? ar_ceil(a.P, a.own.keys()) : 0);
+  // a stream step moves what four tile steps do
+  const int64_t pre_w = pre_steps * (a.pre.stream ? 4 : 1) * ar_ceil(all, a.pre.rows()) * a.Hkv;
+  const int64_t own_w = own_steps * (a.own.stream ? 4 : 1) * ar_ceil(rows, a.own.rows()) * groups;
   const int64_t run = std::max(AR_MIN_RUN, ar_ceil(pre_w + own_w, slots));
-  a.nsp = a.joint ? 0 : int(ar_ceil(nPT, run));
-  a.pt = a.nsp ? int(ar_ceil(nPT, a.nsp)) : 0;
-  if (a.nsp) a.nsp = int(ar_ceil(nPT, a.pt));
-  a.n_pre = a.joint ? 0 : int(rtp * a.Hkv * a.nsp);
-  const int64_t own_t = nOT + (a.joint ? nPT : 0);
-  a.nss = int(std::max<int64_t>(ar_ceil(own_t, run), own_t > 0 || a.nsp == 0 ? 1 : 0));
-  a.st = a.nss ? int(std::max<int64_t>(ar_ceil(own_t, a.nss), 1)) : 0;
-  if (a.nss) a.nss = int(std::max<int64_t>(ar_ceil(own_t, a.st), 1));
-  a.NS = a.nsp + a.nss;
-  *grid = a.n_pre + grp * a.nss;
+  ar_cut(a.pre, all, pre_steps, a.pre.stream ? ar_ceil(run, 4) : run);
+  ar_cut(a.own, rows, own_steps, a.own.stream ? ar_ceil(run, 4) : run);
+  if (a.pre.runs + a.own.runs == 0) a.own.runs = 1;  // nothing to see: items that write zeros
+  a.NS = a.pre.runs + a.own.runs;
+  a.n_pre = int(int64_t(a.pre.rts) * a.Hkv * a.pre.runs);
+  a.g_magic = ar_magic(uint32_t(G));
+  *grid = a.n_pre + groups * a.own.rts * a.own.runs;
 }
 
 // A prefix-only decode item's rows span the batch, so one run may be written
@@ -435,7 +478,15 @@ static int64_t ar_part_bytes(const ArArgs& a) {
 }
 
 static int ar_launch(const char* fn, ArArgs& a, int64_t grid, hipStream_t s) {
-  hipLaunchKernelGGL(attn_rows_kernel, dim3(unsigned(grid)), dim3(256), 0, s, a);
+  const bool own = grid > a.n_pre, tiles = (a.n_pre && !a.pre.stream) || (own && !a.own.stream);
+  const bool streams = (a.n_pre && a.pre.stream) || (own && a.own.stream);
+  const dim3 g{unsigned(grid)}, t{256};
+  if (tiles && streams)
+    hipLaunchKernelGGL((attn_rows_kernel<true, true>), g, t, 0, s, a);
+  else if (tiles)
+    hipLaunchKernelGGL((attn_rows_kernel<true, false>), g, t, 0, s, a);
+  else
+    hipLaunchKernelGGL((attn_rows_kernel<false, true>), g, t, 0, s, a);
   int rc = hip_status(fn);
   if (rc || a.NS == 1) return rc;
   const int64_t rows = int64_t(a.B) * a.S * a.Hq;
@@ -488,7 +539,7 @@ static void cs_plan(CsArgs& a) {
     }
   }
   a.n_chunk = int(ar_ceil(tiles, a.run));
-  a.g_magic = G == 1 ? 0u : uint32_t(((1ull << 32) + uint64_t(G) - 1) / uint64_t(G));
+  a.g_magic = ar_magic(uint32_t(G));
 }
 
 }  // namespace qmoe

@@ -246,4 +246,141 @@ __device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, 
   }
 }
 
+// Few query rows (up to 32) over many keys, where the keys' stream is what costs:
+// every wave of the workgroup holds the same rows and takes its own 64-key tiles
+// w, w + 4, ... of keys [0, n_keys) of k / v.  K rows go from memory straight
+// into A-operand registers and V by DMA into the wave's own LDS tile, every load
+// of a tile in flight at once and no barrier between the waves; flash_join adds
+// up their states.  Lane's row sees keys [0, lim].
+__device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
+                                               int lim, float scale_log2, FlashRows& st) {
+  const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  uint8_t* vb = smem + wave * AP_TILE;
+  const int vg = lane >> 4, ve = (lane >> 2) & 3, vq = lane & 3;
+  const uint32_t vlane = uint32_t((4 * (vg >> 1) + ve) * AP_ROWB +
+                                  (((2 * (vg & 1) + (vq >> 1)) ^ (2 * (ve >> 1))) * 16) + 8 * (vq & 1));
+  const pipe::i32x4 rv = pipe::make_rsrc(v, uint32_t(n_keys) * AP_ROWB);  // rows past the end read as zeros
+  const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>(smem)) + uint32_t(wave * AP_TILE);
+  const uint32_t voff = uint32_t((lane >> 4) * AP_ROWB + ap_vslot(lane >> 4, lane & 15) * 16);
+#pragma unroll 1
+  for (int k0 = wave * AP_KT; k0 < n_keys; k0 += 4 * AP_KT) {
+    const int last = min(AP_KT, n_keys - k0) - 1;  // rows past it repeat it (their p is 0)
+    u32x4 ka[2][HD / 16];
+    wave_lds_sync();  // the last tile's V reads are done
+#pragma unroll
+    for (int i = 0; i < 16; ++i) pipe::dma16(lds + i * 1024, voff + uint32_t(k0 + 4 * i) * AP_ROWB, rv, 0);
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+      const uint16_t* kp = k + int64_t(k0 + min(mb * 32 + col, last)) * HD + hl * 8;
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks) ka[mb][ks] = ld16(kp + ks * 16);
+    }
+    f32x16 sc[2];
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb) {
+      sc[mb] = f32x16{};
+#pragma unroll
+      for (int ks = 0; ks < HD / 16; ++ks)
+        sc[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka[mb][ks]), st.qf[ks], sc[mb], 0,
+                                                         0, 0);
+    }
+    const int see = min(lim - k0, last);
+    float m = -INFINITY;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int key = mb * 32 + (e >> 2) * 8 + hl * 4 + (e & 3);
+        sc[mb][e] = key <= see ? sc[mb][e] * scale_log2 : -INFINITY;
+        m = fmaxf(m, sc[mb][e]);
+      }
+    {
+      const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(m), __float_as_uint(m), false, false);
+      m = fmaxf(fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1])), st.m);
+    }
+    const float mz = m == -INFINITY ? 0.0f : m;  // no key seen yet
+    const float alpha = __builtin_amdgcn_exp2f(st.m - mz);
+    st.m = m;
+    st.l *= alpha;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) st.o[db][i] *= alpha;
+    uint32_t pk[2][8];
+    float l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float p0 = __builtin_amdgcn_exp2f(sc[mb][2 * i] - mz);
+        const float p1 = __builtin_amdgcn_exp2f(sc[mb][2 * i + 1] - mz);
+        l0 += p0;
+        l1 += p1;
+        const bf16x2_t pp = {static_cast<__bf16>(p0), static_cast<__bf16>(p1)};
+        pk[mb][i] = __builtin_bit_cast(uint32_t, pp);
+      }
+    st.l += l0 + l1;
+    pipe::wait_vm<0>();  // V in LDS
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const u32x4 pw = {pk[s >> 1][(s & 1) * 4], pk[s >> 1][(s & 1) * 4 + 1], pk[s >> 1][(s & 1) * 4 + 2],
+                        pk[s >> 1][(s & 1) * 4 + 3]};
+      const bf16x8 pb = __builtin_bit_cast(bf16x8, pw);
+#pragma unroll
+      for (int db = 0; db < 4; ++db) {
+        const uint32_t va = vlane + uint32_t(64 * (db ^ ve));
+        const s16x4 v0 = lds_read_tr16(vb + va + (16 * s) * AP_ROWB);
+        const s16x4 v1 = lds_read_tr16(vb + va + (16 * s + 8) * AP_ROWB);
+        const bf16x8 a = __builtin_bit_cast(bf16x8, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        st.o[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, pb, st.o[db], 0, 0, 0);
+      }
+    }
+  }
+}
+
+// The four waves' states of the same rows into wave 0's, through LDS in register
+// order (18 values of 64 lanes a chunk of 4): waves 2 and 3 into 0 and 1, then
+// wave 1 into 0.
+__device__ __forceinline__ void flash_join(uint8_t* smem, FlashRows& st) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  constexpr int REC = 64 * (4 * 16 + 2);  // floats of a state
+  static_assert(2 * REC * 4 <= FL_SMEM, "two states fit");
+  auto put = [&](float* p) {
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<float4*>(p + ((db * 4 + g) * 64 + lane) * 4) =
+            make_float4(st.o[db][g * 4], st.o[db][g * 4 + 1], st.o[db][g * 4 + 2], st.o[db][g * 4 + 3]);
+    *reinterpret_cast<float2*>(p + 64 * 64 + lane * 2) = make_float2(st.m, st.l);
+  };
+  auto take = [&](const float* p) {
+    const float2 ml = *reinterpret_cast<const float2*>(p + 64 * 64 + lane * 2);
+    const float m = fmaxf(st.m, ml.x), mz = m == -INFINITY ? 0.0f : m;
+    const float a = __builtin_amdgcn_exp2f(st.m - mz), b = __builtin_amdgcn_exp2f(ml.x - mz);
+    st.m = m;
+    st.l = st.l * a + ml.y * b;
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const float4 o = *reinterpret_cast<const float4*>(p + ((db * 4 + g) * 64 + lane) * 4);
+        st.o[db][g * 4] = fmaf(st.o[db][g * 4], a, o.x * b);
+        st.o[db][g * 4 + 1] = fmaf(st.o[db][g * 4 + 1], a, o.y * b);
+        st.o[db][g * 4 + 2] = fmaf(st.o[db][g * 4 + 2], a, o.z * b);
+        st.o[db][g * 4 + 3] = fmaf(st.o[db][g * 4 + 3], a, o.w * b);
+      }
+  };
+  float* buf = reinterpret_cast<float*>(smem);
+  __syncthreads();  // the V tiles are free
+  if (wave >= 2) put(buf + (wave - 2) * REC);
+  __syncthreads();
+  if (wave < 2) take(buf + wave * REC);
+  __syncthreads();
+  if (wave == 1) put(buf);
+  __syncthreads();
+  if (wave == 0) take(buf);
+}
+
 }  // namespace qmoe
