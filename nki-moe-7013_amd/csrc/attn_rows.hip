@@ -370,12 +370,6 @@ __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
     } else {
       qk(ni, nrb, nxt);
       add(i, rb, cur, std::false_type{});
-#pragma unroll
-      for (int x = 0; x < 16; ++x) {  // an MFMA, then a sixteenth of the weights' work
-        __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x2, 4, 0);
-        __builtin_amdgcn_sched_group_barrier(0x400, 2, 0);
-      }
     }
   };
   f32x16 sa[2], sb[2];
