@@ -27,7 +27,11 @@
 
 namespace qmoe {
 
-constexpr int AR_REC = HD + 4;    // record of a row's run: m, l, 2 pad, O[HD]
+// Record of a run of 32 rows: (m, l) of each row, then O in register order: chunk
+// (db, g) holds 4 dims (32 db + 8 g + 4 (lane / 32)) of every lane, so a store
+// (and the merge's load) covers 1 KB of contiguous memory.  Rows stored one
+// after another cost the merge of 20480 rows x 3 runs 11.6 us instead of 6.
+constexpr int AR_REC = 64 + 16 * 64 * 4;
 constexpr int AR_MAX_G = 16;      // q heads per kv head
 constexpr int64_t AR_MAX_KEYS = 1ll << 22;  // keys of one run are addressed with 32-bit byte offsets
 
@@ -49,12 +53,12 @@ struct ArArgs {
   uint32_t g_magic;        // ar_magic(G)
   float scale_log2;
   uint16_t* out;
-  float* part;  // [B * S * Hq][NS][AR_REC], when NS > 1
+  float* part;  // when NS > 1: [pre.runs][Hkv][nb_pre][AR_REC], [own.runs][B * Hkv][nb_own][AR_REC]
   float* lse;   // [B][Hkv][S * G] or nullptr
   // n_pre prefix items (pre.rts row tiles over all B * S * G rows x pre.runs x
   // Hkv), then items of (own.rts row tiles x own.runs x B x Hkv), whose steps
   // start with the prefix when joint.  NS = pre.runs + own.runs records a row.
-  int NS, n_pre, joint;
+  int NS, n_pre, joint, nb_pre, nb_own;  // nb: blocks of 32 rows
   ArKind pre, own;
 };
 
@@ -147,20 +151,19 @@ __device__ __forceinline__ void ar_item(const ArArgs& a, const ArKind kd, const 
     flash_join(smem, st);
     if (wave) return;
   }
-  const int slot = (pre ? 0 : a.pre.runs) + run;
-  if (!live) return;
   const float l = st.row_sum();
+  if (!live) return;
   if (a.NS > 1) {
-    float* rec = a.part + (qrow * a.NS + slot) * AR_REC;
-    if (hl == 0) *reinterpret_cast<float2*>(rec) = make_float2(st.m, l);
-    if (l > 0.0f) {
+    const int64_t blk = pre ? (int64_t(run) * a.Hkv + kvh) * a.nb_pre + rw / 32
+                            : int64_t(a.pre.runs) * a.Hkv * a.nb_pre +
+                                  ((int64_t(run) * a.B + b) * a.Hkv + kvh) * a.nb_own + rw / 32;
+    float* rec = a.part + blk * AR_REC;
+    if (hl == 0) *reinterpret_cast<float2*>(rec + (lane & 31) * 2) = make_float2(st.m, l);
 #pragma unroll
-      for (int db = 0; db < 4; ++db)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<float4*>(rec + 4 + db * 32 + g * 8 + hl * 4) =
-              make_float4(st.o[db][g * 4], st.o[db][g * 4 + 1], st.o[db][g * 4 + 2], st.o[db][g * 4 + 3]);
-    }
+    for (int c = 0; c < 16; ++c)
+      *reinterpret_cast<float4*>(rec + 64 + (c * 64 + lane) * 4) =
+          make_float4(st.o[c >> 2][(c & 3) * 4], st.o[c >> 2][(c & 3) * 4 + 1], st.o[c >> 2][(c & 3) * 4 + 2],
+                      st.o[c >> 2][(c & 3) * 4 + 3]);
     return;
   }
   const float inv = l > 0.0f ? 1.0f / l : 0.0f;
@@ -196,49 +199,98 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
   }
 }
 
-// One wave a row (b, s, head): lane i takes the (m, l) of run i, then two dims
-// of every run that holds keys, in run order.
+// Joins the runs of 32 packed rows of a kv head: a chunk (db, g) of their dims
+// a wave, from every record; the prefix's records hold the same 32 rows, the own
+// ones those of each row's sequence.  WAVES_A_CHUNK = 1: workgroup y takes the
+// four chunks of block db = y.  4: it takes chunk y alone, each wave every fourth
+// run (few rows with many runs: one row of waves would wait for one load after
+// another), and the waves' (m, l, O) join in LDS in wave order.
+constexpr int AR_MANY_RUNS = 6;
+template <int WAVES_A_CHUNK>
 __global__ __launch_bounds__(256) void attn_rows_merge_kernel(const ArArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6), n = int64_t(a.B) * a.S * a.Hq;
-  if (row >= n) return;
-  const float* p = a.part + row * a.NS * AR_REC;
-  float M = -INFINITY;
-  for (int i = lane; i < a.NS; i += 64) M = fmaxf(M, p[int64_t(i) * AR_REC]);
-  M = wave_max(M);
-  float L = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int c = 0; c < a.NS; c += 64) {
-    float w = 0.0f, wl = 0.0f;
-    if (c + lane < a.NS) {
-      const float2 ml = *reinterpret_cast<const float2*>(p + int64_t(c + lane) * AR_REC);
-      w = ml.y > 0.0f ? __builtin_amdgcn_exp2f(ml.x - M) : 0.0f;
-      wl = ml.y > 0.0f ? w * ml.y : 0.0f;
+  constexpr bool MANY = WAVES_A_CHUNK == 4;
+  __shared__ __attribute__((aligned(16))) uint16_t tile[32][36];
+  __shared__ __attribute__((aligned(16))) float red[MANY ? 4 : 1][64][4];
+  __shared__ float2 rml[MANY ? 4 : 1][64];
+  const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5, w = threadIdx.x >> 6;
+  const int chunk = MANY ? int(blockIdx.y) : int(blockIdx.y) * 4 + w;
+  const int G = a.Hq / a.Hkv, kvh = int(blockIdx.x) % a.Hkv, rb = int(blockIdx.x) / a.Hkv, per = a.S * G;
+  const int rows = a.B * per, row = rb * 32 + col, r = min(row, rows - 1);
+  const int sq = ar_div(r, a.g_magic), b = sq / a.S, rib = r - b * per;
+  const int64_t pre_next = int64_t(a.Hkv) * a.nb_pre * AR_REC, own_next = int64_t(a.B) * a.Hkv * a.nb_own * AR_REC;
+  const float* pp = a.part + (int64_t(kvh) * a.nb_pre + rb) * AR_REC;
+  const float* po = a.part + a.pre.runs * pre_next + ((int64_t(b) * a.Hkv + kvh) * a.nb_own + rib / 32) * AR_REC;
+  const int own_lane = rib % 32 + hl * 32;
+  float M = -INFINITY, L = 0.0f;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  // four runs at a time: all their loads, then the joint maximum once
+  for (int i0 = MANY ? w : 0; i0 < a.NS; i0 += 4 * WAVES_A_CHUNK) {
+    float2 ml[4];
+    f32x4 v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int i = i0 + u * WAVES_A_CHUNK, j = min(i, a.NS - 1);
+      const bool pre = j < a.pre.runs;
+      const float* p = pre ? pp + j * pre_next : po + (j - a.pre.runs) * own_next;
+      const int ln = pre ? lane : own_lane;
+      ml[u] = *reinterpret_cast<const float2*>(p + (ln & 31) * 2);
+      v[u] = *reinterpret_cast<const f32x4*>(p + 64 + (chunk * 64 + ln) * 4);
+      if (i >= a.NS) ml[u] = make_float2(-INFINITY, 0.0f);
     }
-    L += wave_sum(wl);
-    const int cnt = min(64, a.NS - c);
-    for (int i0 = 0; i0 < cnt; i0 += 8) {
-      float2 v[8];
-      float wi[8];
+    const float m = fmaxf(fmaxf(fmaxf(ml[0].x, ml[1].x), fmaxf(ml[2].x, ml[3].x)), M), mz = m == -INFINITY ? 0.0f : m;
+    const float al = __builtin_amdgcn_exp2f(M - mz);
+    M = m;
+    L *= al;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const int i = min(i0 + u, cnt - 1);
-        wi[u] = i0 + u < cnt ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i)) : 0.0f;
-        v[u] = make_float2(0.0f, 0.0f);  // a run without keys stores no O
-        if (wi[u] != 0.0f) v[u] = *reinterpret_cast<const float2*>(p + int64_t(c + i) * AR_REC + 4 + lane * 2);
-      }
+    for (int e = 0; e < 4; ++e) o[e] *= al;
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        o0 = fmaf(wi[u], v[u].x, o0);
-        o1 = fmaf(wi[u], v[u].y, o1);
-      }
+    for (int u = 0; u < 4; ++u) {
+      const float wt = __builtin_amdgcn_exp2f(ml[u].x - mz);  // 0 for a run without keys, whose O is 0
+      L = fmaf(wt, ml[u].y, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(wt, v[u][e], o[e]);
     }
   }
+  if constexpr (MANY) {
+    *reinterpret_cast<f32x4*>(red[w][lane]) = o;
+    rml[w][lane] = make_float2(M, L);
+    __syncthreads();
+    if (w) return;
+    float m = M;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) m = fmaxf(m, rml[i][lane].x);
+    const float mz = m == -INFINITY ? 0.0f : m, al = __builtin_amdgcn_exp2f(M - mz);
+    L *= al;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] *= al;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+      const float wt = __builtin_amdgcn_exp2f(rml[i][lane].x - mz);
+      const f32x4 v = *reinterpret_cast<const f32x4*>(red[i][lane]);
+      L = fmaf(wt, rml[i][lane].y, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(wt, v[e], o[e]);
+    }
+    M = m;
+  }
   const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-  reinterpret_cast<uint32_t*>(a.out + row * HD)[lane] = pack_bf16x2(o0 * inv, o1 * inv);
-  if (a.lse && lane == 0) {
-    const int G = a.Hq / a.Hkv, head = int(row % a.Hq), s = int(row / a.Hq % a.S), b = int(row / a.Hq / a.S);
-    a.lse[(int64_t(b) * a.Hkv + head / G) * (a.S * G) + s * G + head % G] =
-        a.lengths && s >= a.lengths[b] ? INFINITY : ar_lse(M, L);
+  u32x2 pk;
+  pk.x = pack_bf16x2(o[0] * inv, o[1] * inv);
+  pk.y = pack_bf16x2(o[2] * inv, o[3] * inv);
+  if (a.lse && chunk == 0 && hl == 0 && row < rows)
+    a.lse[(int64_t(b) * a.Hkv + kvh) * per + rib] =
+        a.lengths && sq - b * a.S >= a.lengths[b] ? INFINITY : ar_lse(M, L);
+  if constexpr (MANY) {
+    if (row < rows)
+      *reinterpret_cast<u32x2*>(a.out + (int64_t(sq) * a.Hq + kvh * G + (row - sq * G)) * HD + chunk * 8 + hl * 4) = pk;
+  } else {  // 64 bytes of a row at a time
+    *reinterpret_cast<u32x2*>(&tile[col][w * 8 + hl * 4]) = pk;
+    __syncthreads();
+    const int orow = rb * 32 + int(threadIdx.x) / 8, oc = int(threadIdx.x) % 8 * 4;
+    if (orow >= rows) return;
+    const int oq = ar_div(orow, a.g_magic);
+    *reinterpret_cast<u32x2*>(a.out + (int64_t(oq) * a.Hq + kvh * G + (orow - oq * G)) * HD + blockIdx.y * 32 + oc) =
+        *reinterpret_cast<const u32x2*>(&tile[threadIdx.x / 8][oc]);
   }
 }
 
@@ -431,44 +483,82 @@ __global__ __launch_bounds__(256) void attn_colsum_add_kernel(const CsArgs a) {
 // ---------------------------------------------------------------------- host
 static int64_t ar_ceil(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Cuts the work into items.  own_keys: own keys of a row at most.  Rows of one
-// sequence that fill a tile run over prefix and own keys in one item; fewer
-// rows leave the prefix to tiles (up to 64 rows of the batch: to streams) of its
-// own, read once for all rows of a tile, and take their own keys as streams
-// (more than 64 rows: as tiles).  Run lengths: about two workgroups on every
-// CU, of at least AR_MIN_RUN tile steps or one stream step.
-constexpr int64_t AR_MIN_RUN = 2;
-static void ar_cut(ArKind& kd, int64_t rows, int64_t steps, int64_t run) {
-  kd.rts = int(ar_ceil(rows, kd.rows()));
-  kd.runs = steps > 0 ? int(ar_ceil(steps, run)) : 0;
-  kd.run = kd.runs ? int(ar_ceil(steps, kd.runs)) : 1;
-  kd.runs = int(ar_ceil(steps, kd.run));
-}
-static void ar_plan(ArArgs& a, int64_t own_keys, int64_t* grid) {
-  const int64_t G = a.Hq / a.Hkv, rows = a.S * G, all = int64_t(a.B) * rows, groups = int64_t(a.B) * a.Hkv;
-  const int64_t slots = 2 * int64_t(std::max(current_device_cus(), 1));
-  a.joint = rows >= 128;
-  a.pre.stream = !a.joint && all <= 64;
-  a.own.stream = rows <= 64;
-  const int64_t pre_steps = a.joint ? 0 : ar_ceil(a.P, a.pre.keys());
-  const int64_t own_steps = ar_ceil(own_keys, a.own.keys()) + (a.joint ? ar_ceil(a.P, a.own.keys()) : 0);
-  // a stream step moves what four tile steps do
-  const int64_t pre_w = pre_steps * (a.pre.stream ? 4 : 1) * ar_ceil(all, a.pre.rows()) * a.Hkv;
-  const int64_t own_w = own_steps * (a.own.stream ? 4 : 1) * ar_ceil(rows, a.own.rows()) * groups;
-  const int64_t run = std::max(AR_MIN_RUN, ar_ceil(pre_w + own_w, slots));
-  ar_cut(a.pre, all, pre_steps, a.pre.stream ? ar_ceil(run, 4) : run);
-  ar_cut(a.own, rows, own_steps, a.own.stream ? ar_ceil(run, 4) : run);
-  if (a.pre.runs + a.own.runs == 0) a.own.runs = 1;  // nothing to see: items that write zeros
-  a.NS = a.pre.runs + a.own.runs;
-  a.n_pre = int(int64_t(a.pre.rts) * a.Hkv * a.pre.runs);
-  a.g_magic = ar_magic(uint32_t(G));
-  *grid = a.n_pre + groups * a.own.rts * a.own.runs;
+// Cuts the work into items.  own_keys: own keys of a row at most.
+//
+// Rows of one sequence that fill a tile (S * G >= 128) run over the prefix and
+// their own keys in one item.  Fewer rows leave the prefix to items of its own,
+// whose rows span the batch, and take their own keys as streams (more than 64
+// rows: as tiles).  The prefix goes as streams, which read its keys again for
+// every 32 rows (from L2) but wait for no barrier, while that is at most
+// AR_STREAM_KEYS keys in all, and as tiles past it (streams / tiles in us: 128 rows
+// on 16000 keys 21.3 / 22.9, on 32768 31.4 / 30.1; 256 rows on 8192 22.4 / 24.4, on
+// 32768 48.6 / 38.7; 320 rows on 3000 16.0 / 20.1; 512 rows on 1000 25.7 / 26.9, on
+// 8192 31.9 / 29.1, on 32768 95 / 65).
+constexpr int64_t AR_MIN_TILES = 4, AR_STREAM_KEYS = 65536;
+
+// A tile step takes about 1.45 us with one workgroup on a CU and 2.14 with two; a
+// second run costs the merge's launch, and every run a record of 528 bytes for
+// each of `rows` rows (of one head), written and read at about 6 MB/us.
+// Measured: 8 x 101 queries on 2900 + 101 keys, 1 run 71.7 us, 2 runs 63.6, 3 72.4;
+// 512 queries on 4000 + 512 keys, 2 runs 62.7, 3 57.4, 4 53.7, 6 69.6; a 640-token
+// prompt, 1 run 34.4 us, 2 38.9.
+static int64_t ar_joint_runs(int64_t items, int64_t steps, int64_t rows, int64_t cus) {
+  int64_t best = 1;
+  double least = 1e30;
+  for (int64_t n = 1; n <= 16 && n <= std::max<int64_t>(steps, 1); ++n) {
+    const double step = items * n <= cus ? 1.45 : 2.14 * double(ar_ceil(items * n, 2 * cus));
+    const double us = double(ar_ceil(steps, n)) * step + (n > 1 ? 4.5 + double(rows * n) * (2 * 528 / 6e6) : 0.0);
+    if (us < least) {
+      least = us;
+      best = n;
+    }
+  }
+  return best;
 }
 
-// A prefix-only decode item's rows span the batch, so one run may be written
-// without a merge as well.
+static void ar_cut(ArKind& kd, int64_t steps, int64_t want) {
+  want = std::max<int64_t>(1, std::min(want, steps / (kd.stream ? 1 : AR_MIN_TILES)));
+  kd.run = int(std::max<int64_t>(1, ar_ceil(steps, want)));
+  kd.runs = int(ar_ceil(steps, kd.run));
+}
+
+static void ar_plan(ArArgs& a, int64_t own_keys, int64_t* grid) {
+  const int64_t G = a.Hq / a.Hkv, rows = a.S * G, all = int64_t(a.B) * rows, groups = int64_t(a.B) * a.Hkv;
+  const int64_t cus = std::max(current_device_cus(), 1);
+  a.joint = rows >= 128;
+  a.pre.stream = !a.joint && ar_ceil(all, 32) * a.P <= AR_STREAM_KEYS;
+  a.own.stream = rows <= 64;
+  a.pre.rts = int(ar_ceil(all, a.pre.rows()));
+  a.own.rts = int(ar_ceil(rows, a.own.rows()));
+  const int64_t pre_items = int64_t(a.pre.rts) * a.Hkv, own_items = a.own.rts * groups;
+  const int64_t pre_steps = a.joint ? 0 : ar_ceil(a.P, a.pre.keys());
+  const int64_t own_steps = ar_ceil(own_keys, a.own.keys()) + (a.joint ? ar_ceil(a.P, a.own.keys()) : 0);
+  // Items of the prefix: one a CU (their records cost more than the CU's second
+  // place gives); long runs of tiles share the CUs' two places with the own items
+  // by the time of each (a tile step 1.07 us of a CU, a stream step about 5, which
+  // is its share of the memory's rate).
+  int64_t places = cus;
+  if (!a.joint && !a.pre.stream && pre_items * pre_steps >= 8 * cus) {
+    const double pre_us = 1.07 * double(pre_items * pre_steps);
+    const double own_us = (a.own.stream ? 5.0 : 1.07) * double(own_items * own_steps);
+    places = int64_t(2.0 * double(cus) * pre_us / (pre_us + own_us));
+  }
+  ar_cut(a.pre, pre_steps, places / pre_items);
+  ar_cut(a.own, own_steps,
+         a.joint ? ar_joint_runs(own_items, own_steps, int64_t(a.B) * a.S * a.Hq, cus) : cus / own_items);
+  if (a.pre.runs + a.own.runs == 0) a.own.runs = 1;  // nothing to see: items that write zeros
+  a.NS = a.pre.runs + a.own.runs;
+  a.n_pre = int(pre_items * a.pre.runs);
+  a.nb_pre = a.pre.runs ? int(ar_ceil(all, 32)) : 0;
+  a.nb_own = a.own.runs ? int(ar_ceil(rows, 32)) : 0;
+  a.g_magic = ar_magic(uint32_t(G));
+  *grid = a.n_pre + own_items * a.own.runs;
+}
+
 static int64_t ar_part_bytes(const ArArgs& a) {
-  return a.NS > 1 ? int64_t(a.B) * a.S * a.Hq * a.NS * AR_REC * int64_t(sizeof(float)) : 0;
+  if (a.NS <= 1) return 0;
+  const int64_t blocks = int64_t(a.pre.runs) * a.Hkv * a.nb_pre + int64_t(a.own.runs) * a.B * a.Hkv * a.nb_own;
+  return blocks * AR_REC * int64_t(sizeof(float));
 }
 
 static int ar_launch(const char* fn, ArArgs& a, int64_t grid, hipStream_t s) {
@@ -483,8 +573,11 @@ static int ar_launch(const char* fn, ArArgs& a, int64_t grid, hipStream_t s) {
     hipLaunchKernelGGL((attn_rows_kernel<false, true>), g, t, 0, s, a);
   int rc = hip_status(fn);
   if (rc || a.NS == 1) return rc;
-  const int64_t rows = int64_t(a.B) * a.S * a.Hq;
-  hipLaunchKernelGGL(attn_rows_merge_kernel, dim3(unsigned(ar_ceil(rows, 4))), dim3(256), 0, s, a);
+  const int64_t blocks = ar_ceil(int64_t(a.B) * a.S * (a.Hq / a.Hkv), 32) * a.Hkv;
+  if (a.NS >= AR_MANY_RUNS)
+    hipLaunchKernelGGL(attn_rows_merge_kernel<4>, dim3(unsigned(blocks), 16), t, 0, s, a);
+  else
+    hipLaunchKernelGGL(attn_rows_merge_kernel<1>, dim3(unsigned(blocks), 4), t, 0, s, a);
   return hip_status(fn);
 }
 
