@@ -10,6 +10,7 @@ attention over the KV cache ``[B, Hkv, S, D]`` (9943-9946) -> o_proj.
 from __future__ import annotations
 
 import math
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -34,11 +35,27 @@ FUSED_DECODE_MAX_ROWS = 64
 CHUNK_DECODE_MAX = 16
 
 
+@dataclass
+class SharedPrefix:
+    """Keys and values of the tokens that every sequence of a batch starts with,
+    held once: ``k``, ``v`` bf16 ``[Hkv, P_max, D]``, of which ``length`` entries."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    length: int
+
+
 class KVCache:
     """Contiguous K/V cache of one layer: ``[B, Hkv, S_max, D]`` bf16 each.
 
     Unpacks like the reference's ``(K, V)`` present-key-value tuple
-    (``k, v = cache``), and :meth:`wrap` takes such a tuple back without a copy."""
+    (``k, v = cache``), and :meth:`wrap` takes such a tuple back without a copy.
+
+    With a ``prefix`` the rows hold only what follows it: a token's cache index
+    (and the ``positions`` of :meth:`Attention.forward`) counts from the
+    prefix's end, and the caller's RoPE tables start there too."""
+
+    prefix: Optional[SharedPrefix] = None
 
     def __init__(self, B: int, n_kv: int, S_max: int, head_dim: int, device):
         self.k = torch.zeros(B, n_kv, S_max, head_dim, dtype=torch.bfloat16, device=device)
@@ -75,6 +92,76 @@ class KVCache:
 
     def __getitem__(self, i):
         return (self.k, self.v)[i]
+
+
+class CacheBudget:
+    """What the bounded caches of all layers have in common: how many entries a
+    row keeps (``budget``: the first ``sink`` positions, the ``recent`` last
+    ones and those with the most attention weight), the slots past it that
+    decode steps fill before the next eviction, and where each row stands.
+
+    ``slots[b]`` (device) is the slot of row b's next token and ``ctx`` is
+    ``slots + 1``, the entries its step sees; ``used`` is the same on the host,
+    so no step has to ask the device.  ``lengths`` are a prompt's real tokens."""
+
+    def __init__(self, B: int, budget: int, recent: int, sink: int, slack: int, device):
+        if budget <= 0 or recent < 0 or sink < 0 or recent + sink > budget or slack < 1:
+            raise ValueError(f"need 0 <= recent + sink <= budget and at least one slot past it (budget={budget}, "
+                             f"recent={recent}, sink={sink}, slack={slack})")
+        self.budget, self.recent, self.sink, self.capacity = budget, recent, sink, budget + slack
+        self.slots = torch.zeros(B, dtype=torch.int32, device=device)
+        self.ctx = torch.ones(B, dtype=torch.int32, device=device)
+        self.lengths = torch.zeros(B, dtype=torch.int32, device=device)
+        self.used = [0] * B
+        self._prompt = None
+
+    def prompt_cache(self, n_kv: int, S: int, head_dim: int):
+        """Scratch cache of a whole prompt (one for all layers, which run one
+        after another) with its scores at zero and its positions."""
+        B, dev = len(self.used), self.slots.device
+        p = self._prompt
+        if p is None or p[0].k.shape[1] != n_kv or p[0].capacity < S:
+            c = KVCache(B, n_kv, S, head_dim, dev)
+            pos = torch.arange(S, dtype=torch.int32, device=dev).repeat(B, n_kv, 1)
+            p = self._prompt = (c, torch.empty(B, n_kv, S, device=dev), pos)
+        p[1].zero_()
+        return p
+
+    def begin(self, lengths: list) -> None:
+        """A prompt of ``lengths[b]`` real tokens a row comes next."""
+        self.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+        self._stand([min(int(n), self.budget) for n in lengths])
+
+    def _stand(self, used: list) -> None:
+        self.used = used
+        self.slots.copy_(torch.tensor(used, dtype=torch.int32))
+        self.ctx.copy_(self.slots + 1)
+
+    def advance(self) -> None:
+        """After a step, on the host (the step itself moves ``slots`` and ``ctx``)."""
+        self.used = [n + 1 for n in self.used]
+
+    def make_room(self, caches) -> None:
+        """Before a step: evicts in every layer once a row's slots are full."""
+        if max(self.used) < self.capacity:
+            return
+        for c in caches:
+            ops.kv_evict(c.k, c.v, c.scores, c.slot_pos, self.slots, self.budget, self.recent, self.sink)
+        self._stand([min(n, self.budget) for n in self.used])
+
+
+class BoundedKVCache(KVCache):
+    """One layer's cache of at most ``state.budget`` entries per row and kv head
+    between evictions, whose slots are not positions: ``scores`` (f32) and
+    ``slot_pos`` (i32) ``[B, Hkv, capacity]`` hold each entry's accumulated
+    attention weight and position."""
+
+    def __init__(self, state: CacheBudget, n_kv: int, head_dim: int):
+        B, dev = len(state.used), state.slots.device
+        super().__init__(B, n_kv, state.capacity, head_dim, dev)
+        self.state = state
+        self.scores = torch.zeros(B, n_kv, state.capacity, device=dev)
+        self.slot_pos = torch.full((B, n_kv, state.capacity), -1, dtype=torch.int32, device=dev)
 
 
 class Attention:
@@ -123,7 +210,28 @@ class Attention:
         ``post_norm = (rms_w, eps)``: returns ``bf16(rmsnorm(residual) * rms_w)``
         of the updated residual, computed with the o_proj's residual add
         (instead of the residual itself).
+
+        A cache with a ``prefix``: positions count from the prefix's end, every
+        query also sees the prefix (``attn_shared``).  A
+        :class:`BoundedKVCache`: a decode row's entry goes to slot
+        ``state.slots[b]`` and the weights of its attention to the scores; a
+        prompt (``start`` 0, ``state.lengths`` real tokens a row) is attended
+        in full and then cut down to the budget.
         """
+        if cache.prefix is not None or isinstance(cache, BoundedKVCache):
+            o = self._special(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
+        else:
+            o = self._plain(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
+        key = ("oproj", o.shape[0])
+        if key not in self._ws:  # split-K scratch for prefill-size token counts (None: not split)
+            self._ws[key] = ops.gemm_workspace(o.shape[0], self.wo.shape[0], self.wo.shape[1], x.device)
+        if post_norm is not None:
+            return ops.gemm_add_rmsnorm(o, self.wo, residual, post_norm[0], post_norm[1], workspace=self._ws[key])
+        ops.gemm(o, self.wo, _lib.GEMM_ADD_F32, out=residual, workspace=self._ws[key])
+        return residual
+
+    def _plain(self, x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm) -> torch.Tensor:
+        """Attention outputs ``[B*S, Hq*D]`` over a contiguous cache."""
         n_ws = ops.qkv_norm_rope_workspace(B * S, x.shape[1], self.n_q, self.n_kv, self.head_dim)
         n_raw = n_ws
         if S == 1 and n_ws == 0 and self._skinny_decode(x, B):
@@ -167,10 +275,42 @@ class Attention:
             else:
                 o = ops.attn_decode(q.view(B, self.n_q, self.head_dim), cache.k, cache.v, positions + 1, self.scale,
                                     self._decode_ws(B, cache, x.device), max_ctx=max_ctx)
-        key = ("oproj", o.shape[0])
-        if key not in self._ws:  # split-K scratch for prefill-size token counts (None: not split)
-            self._ws[key] = ops.gemm_workspace(o.shape[0], self.wo.shape[0], self.wo.shape[1], x.device)
-        if post_norm is not None:
-            return ops.gemm_add_rmsnorm(o, self.wo, residual, post_norm[0], post_norm[1], workspace=self._ws[key])
-        ops.gemm(o, self.wo, _lib.GEMM_ADD_F32, out=residual, workspace=self._ws[key])
-        return residual
+        return o
+
+    def _special(self, x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm) -> torch.Tensor:
+        """Attention outputs ``[B*S, Hq*D]`` over a shared prefix or a bounded cache."""
+        bounded = isinstance(cache, BoundedKVCache)
+        if isinstance(start, torch.Tensor):
+            raise ValueError("a chunk at a device-held position needs a contiguous cache without a prefix")
+        if S > 1:
+            if norm is not None:
+                raise ValueError("the fused input norm takes one fp32 row on the GEMV path")
+            if bounded and start != 0:
+                raise ValueError("a bounded cache takes a prompt from its first token on")
+            n = ops.qkv_norm_rope_workspace(B * S, x.shape[1], self.n_q, self.n_kv, self.head_dim)
+            ws = torch.empty(n // 4, dtype=torch.float32, device=x.device) if n > 0 else None
+            own, scores, pos = cache.state.prompt_cache(self.n_kv, S, self.head_dim) if bounded else (cache, None, None)
+            q = ops.qkv_norm_rope(x, self.wqkv, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, B, S,
+                                  self.n_q, self.n_kv, own.k, own.v, self.eps, workspace=ws)
+            if not bounded:
+                ctx = positions.view(B, S)[:, 0] + 1
+                return ops.attn_shared(q, cache.prefix.k, cache.prefix.v, cache.k, cache.v, ctx, B, S,
+                                       cache.prefix.length, self.scale, max_ctx=min(cache.capacity, start + S))
+            st = cache.state
+            o = ops.attn_prefill_scored(q, own.k, own.v, scores, B, S, 0, st.lengths, self.scale)
+            ops.kv_evict(own.k, own.v, scores, pos, st.lengths, st.budget, st.recent, st.sink,
+                         out=(cache.k, cache.v, cache.scores, cache.slot_pos))
+            return o
+        if norm is not None:
+            raw = ops.gemv_rmsnorm(x, norm[0], norm[1], self.wqkv, _lib.GEMM_STORE_F32)
+        else:
+            raw = ops.gemm(x, self.wqkv, _lib.GEMM_STORE_F32)
+        if not bounded:
+            q = ops.kv_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, positions, self.n_q,
+                              self.n_kv, cache.k, cache.v, self.eps)
+            return ops.attn_shared(q, cache.prefix.k, cache.prefix.v, cache.k, cache.v, positions + 1, B, 1,
+                                   cache.prefix.length, self.scale, max_ctx=max_ctx)
+        st = cache.state
+        q = ops.kv_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, st.slots, self.n_q, self.n_kv,
+                          cache.k, cache.v, self.eps, scores=cache.scores, slot_pos=cache.slot_pos)
+        return ops.attn_decode_scored(q, cache.k, cache.v, st.ctx, cache.scores, self.scale, max_ctx=max_ctx)

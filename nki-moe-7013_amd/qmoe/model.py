@@ -33,7 +33,7 @@ from typing import Any, Callable, Dict, List, Optional
 import torch
 
 from . import _lib, ops, weights
-from .attention import Attention, KVCache, rope_tables
+from .attention import Attention, BoundedKVCache, CacheBudget, KVCache, SharedPrefix, rope_tables
 from .config import Qwen3MoeShape
 from .moe import MoEBlock
 
@@ -66,6 +66,16 @@ class MoENeuronConfig:
         # (the reference ships 5, qwen_with_nki.py:74); 0 or 1 = plain greedy
         self.speculation_length = int(kwargs.pop("speculation_length", 0))
         self.use_hip_graphs = bool(kwargs.pop("use_hip_graphs", True))
+        # entries a row keeps in each layer's cache (0: all of them): the first
+        # kv_cache_sink positions, the kv_cache_recent last ones and those with
+        # the most accumulated attention weight; kv_cache_slack decode steps run
+        # between evictions
+        self.kv_cache_budget = int(kwargs.pop("kv_cache_budget", 0))
+        self.kv_cache_recent = int(kwargs.pop("kv_cache_recent", self.kv_cache_budget // 4))
+        self.kv_cache_sink = int(kwargs.pop("kv_cache_sink", min(4, self.kv_cache_budget)))
+        self.kv_cache_slack = int(kwargs.pop("kv_cache_slack", 64))
+        if self.kv_cache_budget < 0:
+            raise ValueError("kv_cache_budget must be >= 0")
         self.seed = int(kwargs.pop("seed", 0))
         self.extra = kwargs  # every other generate-mode flag, accepted and ignored
 
@@ -252,9 +262,13 @@ class NeuronQwen3MoeDecoderLayer:
         end = int(pos_cpu.max()) + 1
         if past_key_value is not None:
             self.cache = KVCache.wrap(past_key_value)
-        elif (self.cache is None or self.cache.k.shape[0] != B or self.cache.capacity < end) and int(starts.min()) == 0:
+        elif (self.cache is None or self.cache.k.shape[0] != B or self.cache.capacity < end) and int(starts.min()) == 0 \
+                and not _special(self.cache):
             cap = max(end, int(self.config.neuron_config.max_length) + 1)
             self.cache = KVCache(B, self.config.num_key_value_heads, cap, self.config.head_dim, dev)
+        if _special(self.cache):
+            raise ValueError("a cache with a shared prefix or a budget is driven by the model (its indices are not "
+                             "positions): pass a KVCache or a (K, V) pair")
         if self.cache is None or self.cache.k.shape[0] != B:
             raise ValueError("no KV cache for this batch: start at position 0 or pass past_key_value")
         if self.cache.capacity < end:
@@ -271,6 +285,10 @@ class NeuronQwen3MoeDecoderLayer:
             self.run(h, pos, B, 1, rope, 0)
         out = h.view(B, S, H).to(hidden_states.dtype)
         return out, self.cache, rope[0], rope[1], None
+
+
+def _special(cache) -> bool:
+    return cache is not None and (cache.prefix is not None or isinstance(cache, BoundedKVCache))
 
 
 def _check_causal_mask(mask: Optional[torch.Tensor], pos: torch.Tensor) -> None:
@@ -306,12 +324,22 @@ class NeuronQwen3MoeModel:
         self.lm_head = params["lm_head"]
         dev = self.embed_tokens.device
         max_pos = min(int(config.max_position_embeddings), int(config.neuron_config.max_length) + 1)
-        self.rope = rope_tables(config.head_dim, max_pos, float(config.rope_theta), dev)
+        self.rope = self.rope_full = rope_tables(config.head_dim, max_pos, float(config.rope_theta), dev)
+        self.base = 0  # tokens of a shared prefix: the position of cache index 0, where ``rope`` starts
+        self.budget: Optional[CacheBudget] = None
         # set by the embedding gather when a token id is outside the vocabulary
         self.embed_err = torch.zeros(1, dtype=torch.int32, device=dev)
 
     def allocate_cache(self, B: int, S_max: int):
-        c = self.config
+        """A contiguous cache of ``S_max`` entries a row in every layer, or, with
+        ``neuron_config.kv_cache_budget``, a bounded one."""
+        c, n = self.config, self.config.neuron_config
+        if n.kv_cache_budget > 0:
+            self.budget = CacheBudget(B, n.kv_cache_budget, n.kv_cache_recent, n.kv_cache_sink, n.kv_cache_slack,
+                                      self.embed_tokens.device)
+            for l in self.layers:
+                l.cache = BoundedKVCache(self.budget, c.num_key_value_heads, c.head_dim)
+            return
         for l in self.layers:
             l.cache = KVCache(B, c.num_key_value_heads, S_max, c.head_dim, self.embed_tokens.device)
 
@@ -325,6 +353,42 @@ class NeuronQwen3MoeModel:
             x = layer.run(h, positions, B, S, self.rope, start, max_ctx, x_in=x,
                           next_norm=None if nxt is None else (nxt.weight, nxt.eps))
         return h
+
+    def caches(self):
+        return [l.cache for l in self.layers]
+
+    def set_prefix(self, input_ids: torch.Tensor, budget: int = 0, recent: int = 0, sink: int = 0) -> None:
+        """Runs ``input_ids[1, P]`` and makes its keys and values (cut down to
+        ``budget`` entries a kv head, if that is fewer) the prefix of every
+        row's cache; an empty ``input_ids`` takes the prefix away."""
+        P, dev, c = input_ids.shape[1], self.embed_tokens.device, self.config
+        own = self.caches()
+        for cache in own:
+            cache.prefix = None
+        self.base, self.rope = 0, self.rope_full
+        if P == 0:
+            return
+        if P >= self.rope_full[0].shape[0]:
+            raise ValueError(f"a prefix of {P} tokens leaves no position of {self.rope_full[0].shape[0]} to continue at")
+        n = P
+        if 0 < budget < P:
+            state = CacheBudget(1, budget, recent, sink, 1, dev)
+            state.begin([P])
+            made = [BoundedKVCache(state, c.num_key_value_heads, c.head_dim) for _ in own]
+            n = budget
+        else:
+            made = [KVCache(1, c.num_key_value_heads, P, c.head_dim, dev) for _ in own]
+        try:
+            for l, cache in zip(self.layers, made):
+                l.cache = cache
+            self.hidden(input_ids.to(dev), torch.arange(P, dtype=torch.int32, device=dev), 1, P, 0)
+        finally:
+            for l, cache in zip(self.layers, own):
+                l.cache = cache
+        for cache, m in zip(own, made):
+            cache.prefix = SharedPrefix(m.k[0], m.v[0], n)
+        self.base = P
+        self.rope = tuple(t[P:] for t in self.rope_full)
 
     def check_embed(self) -> None:
         """Raise if any token id so far was outside the vocabulary (synchronises)."""
@@ -566,8 +630,45 @@ class NeuronQwen3MoeForCausalLM:
         return random_params(self.config, self.device, seed=self.neuron_config.seed)
 
     def reset(self):
-        """Start a new sequence (the KV cache is overwritten from position 0)."""
+        """Start a new sequence (the KV cache is overwritten from position 0; a
+        shared prefix stays)."""
         self.position = 0
+
+    # -- shared prefix -----------------------------------------------------------
+    def share_prefix(self, prefix_ids: torch.Tensor, budget: int = 0, recent: Optional[int] = None,
+                     sink: int = 4) -> None:
+        """Makes ``prefix_ids`` (``[P]`` or ``[1, P]``) the beginning of every
+        sequence that follows: it runs once, its keys and values are held once,
+        and the prompts of :meth:`prefill` and ``generate`` continue it (their
+        positions start at P, which counts towards ``max_length``).  With
+        ``budget`` every kv head keeps only that many of its entries: the first
+        ``sink``, the ``recent`` last ones (default a quarter of the budget)
+        and those that got the most attention weight within the prefix.  The
+        embedding and the layers run as for any prompt; :meth:`drop_prefix`
+        takes the prefix away."""
+        if self.model is None:
+            raise RuntimeError("load() the model first")
+        if self.model.budget is not None:
+            raise ValueError("a prefix is shared by contiguous caches (kv_cache_budget is set); "
+                             "pass budget here to keep part of the prefix")
+        ids = prefix_ids.reshape(1, -1)
+        if prefix_ids.dim() > 2 or (prefix_ids.dim() == 2 and prefix_ids.shape[0] != 1) or ids.shape[1] == 0:
+            raise ValueError("prefix_ids must be [P] or [1, P] with P > 0")
+        self._graphs.clear()  # captured steps hold the old prefix's addresses
+        self.model.set_prefix(ids, int(budget), int(budget) // 4 if recent is None else int(recent),
+                              min(int(sink), int(budget)))
+        self.model.check_embed()
+        self.reset()
+
+    def drop_prefix(self) -> None:
+        """Sequences start at position 0 again."""
+        if self.model is not None and self.model.base:
+            self._graphs.clear()
+            self.model.set_prefix(torch.empty(1, 0, dtype=torch.long))
+            self.reset()
+
+    def _contiguous(self) -> bool:
+        return self.model.budget is None and not self.model.base
 
     # -- forward ---------------------------------------------------------------
     def prefill(self, input_ids: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -578,7 +679,15 @@ class NeuronQwen3MoeForCausalLM:
         B, S = input_ids.shape
         dev = self.device
         pos = torch.arange(S, device=dev, dtype=torch.int32).repeat(B)
+        budget = self.model.budget
+        if budget is not None:
+            if B != len(budget.used):
+                raise ValueError(f"the bounded caches hold {len(budget.used)} rows (got {B})")
+            # a single token is a decode step into empty caches
+            budget.begin([S] * B if lengths is None else [int(n) for n in lengths]) if S > 1 else budget.begin([0] * B)
         h = self.model.hidden(input_ids.to(dev), pos, B, S, 0)
+        if budget is not None and S == 1:
+            budget.begin([1] * B)
         if lengths is None:
             last = h.view(B, S, -1)[:, -1].contiguous()
         else:
@@ -598,7 +707,14 @@ class NeuronQwen3MoeForCausalLM:
         else:
             pos = positions.to(device=dev, dtype=torch.int32).contiguous()
             self.position = int(pos.max()) + 1
+        budget = self.model.budget
+        if budget is not None:
+            budget.make_room(self.model.caches())
         h = self.model.hidden(token_ids.to(dev).view(B, 1), pos, B, 1, 0)
+        if budget is not None:
+            budget.slots.add_(1)
+            budget.ctx.add_(1)
+            budget.advance()
         return self.model.logits(h)
 
     def forward(self, input_ids: torch.Tensor, attention_mask=None, position_ids=None, **kw) -> CausalLMOutput:
@@ -633,8 +749,15 @@ class NeuronQwen3MoeForCausalLM:
         st["tok"].copy_(first_token.to(self.device).view(B).long())
         st["pos"].copy_(pos0)
         out = torch.empty(B, n_steps, dtype=torch.long, device=self.device)
+        budget = self.model.budget
         for i in range(n_steps):
-            self._decode_graph(B, self._bucket(top + i + 1)).replay()
+            ctx = top + i + 1
+            if budget is not None:
+                budget.make_room(self.model.caches())
+                ctx = max(budget.used) + 1
+            self._decode_graph(B, self._bucket(ctx)).replay()
+            if budget is not None:
+                budget.advance()
             out[:, i].copy_(st["tok"])
         self.position = top + n_steps
         self.model.check_embed()
@@ -680,11 +803,20 @@ class NeuronQwen3MoeForCausalLM:
             m.logits(h, out=st["logits"])
             ops.argmax(st["logits"], out=st["tok"], workspace=st["am_ws"])
             st["pos"].add_(1)
+            if m.budget is not None:
+                m.budget.slots.add_(1)
+                m.budget.ctx.add_(1)
 
         # Warm-up on a side stream (allocations, lazily created workspaces), then
         # capture.  The warm-up writes one K/V cache slot: the slot at the
-        # current step position, which the next real step overwrites.
+        # current step position, which the next real step overwrites.  On bounded
+        # caches it runs with no slot and no entries: its attention's weights
+        # would stay in the scores.
         saved = (st["tok"].clone(), st["pos"].clone())
+        if m.budget is not None:
+            stand = (m.budget.slots.clone(), m.budget.ctx.clone())
+            m.budget.slots.fill_(-1)
+            m.budget.ctx.fill_(0)
         s = torch.cuda.Stream()
         s.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(s):
@@ -696,6 +828,9 @@ class NeuronQwen3MoeForCausalLM:
             step()
         st["tok"].copy_(saved[0])
         st["pos"].copy_(saved[1])
+        if m.budget is not None:
+            m.budget.slots.copy_(stand[0])
+            m.budget.ctx.copy_(stand[1])
         torch.cuda.synchronize()
         self._graphs[key] = g
         return g
@@ -717,6 +852,8 @@ class NeuronQwen3MoeForCausalLM:
             raise ValueError("spec_generate takes one prompt [1, T0]")
         if spec_len < 2:
             raise ValueError("spec_len must be at least 2")
+        if not self._contiguous():
+            raise ValueError("speculation runs on contiguous caches (no shared prefix, no kv_cache_budget)")
         T0 = prompt.shape[1]
         cap = self.model.layers[0].cache.capacity
         if T0 + max_new_tokens > cap:
@@ -813,11 +950,12 @@ class HuggingFaceGenerationAdapter:
         if generation_config is not None and getattr(generation_config, "do_sample", False):
             raise ValueError("only greedy decoding is implemented (set do_sample=False)")
         B, S = input_ids.shape
+        base = m.model.base if m.model is not None else 0  # tokens of a shared prefix
         if max_new_tokens is None:
             limit = max_length if max_length is not None else m.neuron_config.max_length
-            max_new_tokens = max(0, int(limit) - S)
-        if S + max_new_tokens > m.neuron_config.max_length + 1:
-            raise ValueError(f"prompt + new tokens ({S}+{max_new_tokens}) exceed max_length "
+            max_new_tokens = max(0, int(limit) - base - S)
+        if base + S + max_new_tokens > m.neuron_config.max_length + 1:
+            raise ValueError(f"prompt + new tokens ({base + S}+{max_new_tokens}) exceed max_length "
                              f"{m.neuron_config.max_length}")
         # right-padded prompts (main.py:366, 480-486): row b has lengths[b]
         # real tokens; its new tokens continue from position lengths[b] and,
@@ -834,7 +972,7 @@ class HuggingFaceGenerationAdapter:
             if bool((lengths == S).all()):
                 lengths = None
         spec = int(getattr(m.neuron_config, "speculation_length", 0))
-        if spec >= 2 and B == 1 and max_new_tokens > 1:
+        if spec >= 2 and B == 1 and max_new_tokens > 1 and m._contiguous():
             prompt = input_ids if lengths is None else input_ids[:, : int(lengths[0])]
             out, _ = m.spec_generate(prompt, max_new_tokens, spec_len=spec)
             return torch.cat([input_ids.to(m.device), out[:, prompt.shape[1]:].to(m.device)], dim=1)

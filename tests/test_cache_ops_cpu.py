@@ -145,3 +145,47 @@ def test_wrappers_refuse():
             call()
     a = torch.zeros(100)
     assert ops._overlap(a[:60], a[50:]) and not ops._overlap(a[:50], a[50:])
+
+
+def test_cache_budget_bookkeeping(monkeypatch):
+    """Where the rows stand, on the host and on the device, through a prompt, steps
+    and evictions (the eviction itself replaced by a note that it ran)."""
+    from types import SimpleNamespace
+
+    from qmoe.attention import CacheBudget
+
+    b = CacheBudget(2, 10, 3, 2, 4, "cpu")
+    assert b.capacity == 14
+    calls = []
+    monkeypatch.setattr(ops, "kv_evict", lambda k, v, sc, sp, ctx, *a: calls.append((k, ctx.tolist(), a)))
+    caches = [SimpleNamespace(k=i, v=i, scores=i, slot_pos=i) for i in range(3)]
+    b.begin([20, 5])
+    assert b.used == [10, 5] and b.slots.tolist() == [10, 5] and b.ctx.tolist() == [11, 6]
+    assert b.lengths.tolist() == [20, 5]
+    for step in range(5):
+        b.make_room(caches)
+        assert max(b.used) < b.capacity and b.slots.tolist() == b.used
+        b.slots.add_(1)
+        b.ctx.add_(1)
+        b.advance()
+    assert [c[0] for c in calls] == [0, 1, 2] and calls[0][1] == [14, 9] and calls[0][2] == (10, 3, 2)
+    assert b.used == [11, 10]
+    cache, scores, pos = b.prompt_cache(4, 6, 128)
+    scores.fill_(3.0)
+    again = b.prompt_cache(4, 5, 128)
+    assert again[0] is cache and not bool(again[1].any()) and pos[1, 3].tolist() == list(range(6))
+    assert b.prompt_cache(4, 7, 128)[0] is not cache
+    for bad in [(2, 0, 0, 0, 4), (2, 10, 8, 3, 4), (2, 10, -1, 0, 4), (2, 10, 0, 0, 0)]:
+        with pytest.raises(ValueError, match="at least one slot"):
+            CacheBudget(*bad, "cpu")
+
+
+def test_config_of_the_budget():
+    from qmoe.model import MoENeuronConfig
+
+    c = MoENeuronConfig(kv_cache_budget=100)
+    assert (c.kv_cache_recent, c.kv_cache_sink, c.kv_cache_slack) == (25, 4, 64)
+    c = MoENeuronConfig()
+    assert (c.kv_cache_budget, c.kv_cache_recent, c.kv_cache_sink) == (0, 0, 0)
+    with pytest.raises(ValueError, match="kv_cache_budget"):
+        MoENeuronConfig(kv_cache_budget=-1)
