@@ -3,9 +3,11 @@
     python nki-moe-7013_amd/build.py [-j N]
 
 Each csrc/*.hip / *.cpp is compiled by hipcc into _build/*.o (in parallel),
-then linked into qmoe/libqmoe.so next to the Python bindings; probes/*.hip
-(measurement kernels that bench.py uses for measured peaks, not part of the
-C ABI) go into qmoe/libqmoe_probe.so.  Every HIP translation unit is built
+then linked into qmoe/libqmoe.so next to the Python bindings; bind/native.cpp
+(host code against torch's headers) becomes the extension module
+qmoe/_native.so, which links to it; probes/*.hip (measurement kernels that
+bench.py uses for measured peaks, not part of the C ABI) go into
+qmoe/libqmoe_probe.so.  Every HIP translation unit is built
 with packed-FP32 instruction selection disabled.
 """
 
@@ -18,12 +20,15 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 OUT_DIR = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "qmoe", "libqmoe.so")
+NATIVE_SRC = os.path.join(PKG, "bind", "native.cpp")
+NATIVE = os.path.join(PKG, "qmoe", "_native.so")
 PROBES = os.path.join(PKG, "probes")
 PROBE_LIB = os.path.join(PKG, "qmoe", "libqmoe_probe.so")
 BUILD_INFO = os.path.join(PKG, "qmoe", "build_info.json")
@@ -62,6 +67,26 @@ def _compile(src: str) -> str:
     return obj
 
 
+def _build_native() -> None:
+    """The extension module, with the host compiler: no device code in it."""
+    import torch
+    from torch.utils import cpp_extension
+
+    lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.path.dirname(os.path.dirname(hipcc()))
+    includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(rocm, "include"),
+                os.path.join(ROOT, "include")]
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{i}" for i in includes], NATIVE_SRC, "-o", NATIVE + ".tmp", f"-L{lib_dir}", "-ltorch_python",
+           "-ltorch_cpu", "-lc10", "-lc10_hip", f"-L{os.path.dirname(LIB)}", "-l:libqmoe.so", "-Wl,-rpath,$ORIGIN",
+           f"-Wl,-rpath,{lib_dir}"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError("native module failed:\n" + r.stdout + r.stderr)
+    os.replace(NATIVE + ".tmp", NATIVE)
+
+
 def build(jobs: int = 8) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     srcs = sorted(
@@ -75,6 +100,7 @@ def build(jobs: int = 8) -> str:
     if r.returncode != 0:
         raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
     os.replace(tmp, LIB)
+    _build_native()
     # measurement probes (bench.py's measured peaks): a library of their own
     psrcs = sorted(os.path.join(PROBES, f) for f in os.listdir(PROBES) if f.endswith(".hip"))
     pobjs = [_compile(p) for p in psrcs]

@@ -10,6 +10,7 @@ import os
 from ctypes import c_float, c_int, c_int64, c_void_p, c_char_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libqmoe.so")
+NATIVE_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_native.so")
 
 QMOE_OK = 0
 QMOE_ERR_INVALID = 1
@@ -114,6 +115,19 @@ def lib() -> ctypes.CDLL:
         fn.argtypes = args
     _lib = l
     return l
+
+
+def native():
+    """The checked calls of the cache operators (bind/native.cpp), as a module;
+    raise ImportError if it has not been built."""
+    lib()
+    if not os.path.exists(NATIVE_PATH):
+        raise ImportError(f"{NATIVE_PATH} is missing: build it with `python nki-moe-7013_amd/build.py`")
+    import torch  # noqa: F401  (its libraries are what the module links to)
+
+    from . import _native
+
+    return _native
 
 
 def last_error() -> str:

@@ -774,112 +774,28 @@ def attn_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, c
 
 
 # ----------------------------------------------------------------- shared prefixes and bounded caches
-# A decode step makes these calls for a few microseconds of kernel each, so the
-# checks of an argument are one expression (0.4 us; a separate test of each
-# property and of all devices together 0.9) and the stream is the raw one
-# (0.1 us; the Stream object 2.8).  kv_append of one row, 13 tensors: 22.9 -> 14.8 us.
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# A decode step makes these calls for a few microseconds of kernel each, so their
+# checks, outputs and workspaces are native too (bind/native.cpp; a wrapper in
+# Python takes 10 us for the 14 tensors of kv_append).  They run on the operands'
+# GPU and its current stream.
+_native_module = None
 
 
-def _arg(t, name: str, dtype, shape, ix: int) -> int:
-    """Address of ``t``, once it is a contiguous, 16-byte aligned tensor of this
-    dtype and shape on GPU ``ix``."""
-    if (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == ix and t.shape == shape
-            and t.is_contiguous()):
-        p = t.data_ptr()
-        if not p & 15:
-            return p
-    _need(t, name, dtype, shape)
-    if t.get_device() != ix:
-        raise ValueError(f"tensors are on different devices: {name} is on {t.device}, expected cuda:{ix}")
-    raise ValueError(f"{name}: must be 16-byte aligned")
-
-
-def _out(t, name: str, dtype, shape, ix: int):
-    """``(tensor, address)`` of an output: ``t``, or a new tensor."""
-    if t is None:
-        t = torch.empty(shape, dtype=dtype, device=ix)
-        return t, t.data_ptr()
-    return t, _arg(t, name, dtype, shape, ix)
-
-
-def _call(name: str, ix: int, *args) -> None:
-    """One library call on GPU ``ix`` (made current for it) and its current stream."""
-    fn = getattr(lib(), name)
-    if ix == torch._C._cuda_getDevice():
-        rc = fn(*args, _raw_stream(ix))
-    else:
-        with torch.cuda.device(ix):
-            rc = fn(*args, _raw_stream(ix))
-    if rc:
-        check(rc, name)
-
-
-def _size(name: str, ix: Optional[int], *args) -> int:
-    """A workspace query, for the device the call will run on."""
-    fn = getattr(lib(), name)
-    if ix is None or ix == torch._C._cuda_getDevice():
-        n = int(fn(*args))
-    else:
-        with torch.cuda.device(ix):
-            n = int(fn(*args))
-    if n < 0:
-        raise ValueError(f"{name}: bad sizes {args}")
-    return n
-
-
-def _scratch(workspace: Optional[torch.Tensor], need: int, ix: int):
-    """``(tensor, address, bytes)`` of ``workspace`` if it holds ``need`` bytes, of
-    a new one if none was given (None, None, 0 where none is needed)."""
-    if workspace is None:
-        if need <= 0:
-            return None, None, 0
-        workspace = torch.empty(need, dtype=torch.uint8, device=ix)
-        return workspace, workspace.data_ptr(), need
-    if not isinstance(workspace, torch.Tensor) or workspace.get_device() != ix or not workspace.is_contiguous():
-        raise ValueError(f"workspace: must be a contiguous tensor on cuda:{ix}")
-    size = _nbytes(workspace)
-    if size < need:
-        raise ValueError(f"workspace: needs {need} bytes (got {size})")
-    if workspace.data_ptr() % 16:
-        raise ValueError("workspace: must be 16-byte aligned")
-    return workspace, workspace.data_ptr(), size
+def _native():
+    global _native_module
+    if _native_module is None:
+        _native_module = _lib.native()
+    return _native_module
 
 
 def _new_workspace(name: str, device, *args) -> Optional[torch.Tensor]:
+    """A workspace for a call on ``device`` (``None`` when it needs none)."""
     dev = torch.device(device)
     if dev.type != "cuda":
         raise ValueError(f"workspaces are on a GPU (got {dev})")
     ix = torch.cuda.current_device() if dev.index is None else dev.index
-    return _scratch(None, _size(name, ix, *args), ix)[0]
-
-
-def _gpu(q, name: str, dims: str, n: int) -> int:
-    """GPU of the operand that says the call's sizes."""
-    if not isinstance(q, torch.Tensor) or q.dim() != n:
-        raise ValueError(f"{name} must be {dims}")
-    ix = q.get_device()
-    if ix < 0:
-        raise ValueError(f"{name}: must be on a GPU (got {q.device})")
-    return ix
-
-
-def _check_heads(Hq: int, Hkv: int) -> None:
-    if Hkv <= 0 or Hq % Hkv or Hq // Hkv > 16:
-        raise ValueError(f"need Hq a multiple of Hkv, by at most 16 (Hq={Hq}, Hkv={Hkv})")
-
-
-def _cache_sizes(k_cache, B: int, D: int):
-    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4 or k_cache.shape[0] != B or k_cache.shape[3] != D:
-        raise ValueError(f"k_cache must be [B={B}, Hkv, S_max, D={D}]")
-    return k_cache.shape[1], k_cache.shape[2]
-
-
-def _check_scale(scale: Optional[float], D: int) -> float:
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"scale must be positive and finite (got {scale})")
-    return scale
+    with torch.cuda.device(ix):
+        return _native().workspace(getattr(lib(), name)(*args), name, ix)
 
 
 def attn_shared_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, prefix_len: int, max_ctx: int,
@@ -901,32 +817,8 @@ def attn_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
     counts the new entry; a chunk of S tokens whose first one is own entry e:
     ``ctx_len = e + 1``.  A query that sees nothing gets zeros.  Returns
     ``[B*S, Hq*D]``."""
-    ix = _gpu(q, "q", "[B*S, Hq, D]", 3)
-    T, Hq, D = q.shape
-    if T != B * S:
-        raise ValueError(f"q must be [B*S={B * S}, Hq, D] (got {tuple(q.shape)})")
-    Hkv, S_max = _cache_sizes(k_cache, B, D)
-    _check_heads(Hq, Hkv)
-    if not isinstance(k_prefix, torch.Tensor) or k_prefix.dim() != 3 or k_prefix.shape[0] != Hkv \
-            or k_prefix.shape[2] != D:
-        raise ValueError(f"k_prefix must be [Hkv={Hkv}, P_max, D={D}]")
-    P_max = k_prefix.shape[1]
-    P = P_max if prefix_len is None else int(prefix_len)
-    if not 0 <= P <= P_max:
-        raise ValueError(f"prefix_len must be in [0, {P_max}] (got {P})")
-    max_ctx = S_max if max_ctx is None else int(max_ctx)
-    if not 0 <= max_ctx <= S_max:
-        raise ValueError(f"max_ctx must be in [0, {S_max}] (got {max_ctx})")
-    scale = _check_scale(scale, D)
-    pq = _arg(q, "q", BF16, q.shape, ix)
-    pkp, pvp = _arg(k_prefix, "k_prefix", BF16, k_prefix.shape, ix), _arg(v_prefix, "v_prefix", BF16, k_prefix.shape, ix)
-    pk, pv = _arg(k_cache, "k_cache", BF16, k_cache.shape, ix), _arg(v_cache, "v_cache", BF16, k_cache.shape, ix)
-    pc = _arg(ctx_len, "ctx_len", I32, (B,), ix)
-    out, po = _out(out, "out", BF16, (T, Hq * D), ix)
-    _, pw, nw = _scratch(workspace, _size("qmoe_attn_shared_workspace", ix, B, S, Hq, Hkv, D, P, max_ctx), ix)
-    _call("qmoe_attn_shared", ix, pq, pkp, pvp, P, P_max, pk, pv, pc, B, S, Hq, Hkv, D, S_max, max_ctx, scale, pw, nw,
-          po)
-    return out
+    return _native().attn_shared(q, k_prefix, v_prefix, k_cache, v_cache, ctx_len, B, S, prefix_len, scale, workspace,
+                                 out, max_ctx)
 
 
 def attn_prefill_scored_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, start: int,
@@ -944,24 +836,7 @@ def attn_prefill_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     group, to ``scores[B, Hkv, S_max]`` (f32, in place).  ``lengths`` (i32
     ``[B]``): of a right-padded row only the first ``lengths[b]`` queries count.
     Returns ``[B*S, Hq*D]``."""
-    ix = _gpu(q, "q", "[B*S, Hq, D]", 3)
-    T, Hq, D = q.shape
-    if T != B * S:
-        raise ValueError(f"q must be [B*S={B * S}, Hq, D] (got {tuple(q.shape)})")
-    Hkv, S_max = _cache_sizes(k_cache, B, D)
-    _check_heads(Hq, Hkv)
-    start = int(start)
-    if start < 0 or start + S > S_max:
-        raise ValueError(f"need 0 <= start and start + S <= S_max={S_max} (start={start}, S={S})")
-    scale = _check_scale(scale, D)
-    pq = _arg(q, "q", BF16, q.shape, ix)
-    pk, pv = _arg(k_cache, "k_cache", BF16, k_cache.shape, ix), _arg(v_cache, "v_cache", BF16, k_cache.shape, ix)
-    ps = _arg(scores, "scores", F32, (B, Hkv, S_max), ix)
-    pl = None if lengths is None else _arg(lengths, "lengths", I32, (B,), ix)
-    out, po = _out(out, "out", BF16, (T, Hq * D), ix)
-    _, pw, nw = _scratch(workspace, _size("qmoe_attn_prefill_scored_workspace", ix, B, S, Hq, Hkv, D, start), ix)
-    _call("qmoe_attn_prefill_scored", ix, pq, pk, pv, B, S, Hq, Hkv, D, S_max, start, pl, scale, pw, nw, ps, po)
-    return out
+    return _native().attn_prefill_scored(q, k_cache, v_cache, scores, B, S, start, lengths, scale, workspace, out)
 
 
 def attn_decode_scored_workspace(B: int, Hq: int, D: int, max_ctx: int, device) -> Optional[torch.Tensor]:
@@ -976,22 +851,7 @@ def attn_decode_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
     """:func:`attn_decode` that also adds each slot's attention weight, summed
     over the q heads of its group, to ``scores[B, Hkv, S_max]`` (f32, in place).
     A row with ``ctx_len`` of zero gets zeros.  Returns ``[B, Hq*D]``."""
-    ix = _gpu(q, "q", "[B, Hq, D]", 3)
-    B, Hq, D = q.shape
-    Hkv, S_max = _cache_sizes(k_cache, B, D)
-    _check_heads(Hq, Hkv)
-    max_ctx = S_max if max_ctx is None else int(max_ctx)
-    if not 0 < max_ctx <= S_max:
-        raise ValueError(f"max_ctx must be in [1, {S_max}] (got {max_ctx})")
-    scale = _check_scale(scale, D)
-    pq = _arg(q, "q", BF16, q.shape, ix)
-    pk, pv = _arg(k_cache, "k_cache", BF16, k_cache.shape, ix), _arg(v_cache, "v_cache", BF16, k_cache.shape, ix)
-    ps = _arg(scores, "scores", F32, (B, Hkv, S_max), ix)
-    pc = _arg(ctx_len, "ctx_len", I32, (B,), ix)
-    out, po = _out(out, "out", BF16, (B, Hq * D), ix)
-    _, pw, nw = _scratch(workspace, _size("qmoe_attn_decode_scored_workspace", ix, B, Hq, D, max_ctx), ix)
-    _call("qmoe_attn_decode_scored", ix, pq, pk, pv, pc, B, Hq, Hkv, D, S_max, max_ctx, scale, pw, nw, ps, po)
-    return out
+    return _native().attn_decode_scored(q, k_cache, v_cache, ctx_len, scores, scale, workspace, out, max_ctx)
 
 
 def kv_append(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor, rope_cos: torch.Tensor,
@@ -1003,28 +863,8 @@ def kv_append(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
     whose score becomes 0 and position ``positions[b]``.  A row whose position
     or slot is out of range writes no entry and gets a zero q.  Returns
     ``q[B, Hq, D]``."""
-    ix = _gpu(qkv, "qkv", "[B, (Hq + 2 Hkv) * D]", 2)
-    B, D = qkv.shape[0], q_norm_w.shape[0]
-    n_kv, S_max = _cache_sizes(k_cache, B, D)
-    if n_kv != Hkv:
-        raise ValueError(f"k_cache must have Hkv={Hkv} heads (got {n_kv})")
-    max_pos = rope_cos.shape[0]
-    half, slots_shape = (max_pos, D // 2), (B, Hkv, S_max)
-    args = (_arg(qkv, "qkv", F32, (B, (Hq + 2 * Hkv) * D), ix), _arg(q_norm_w, "q_norm_w", BF16, (D,), ix),
-            _arg(k_norm_w, "k_norm_w", BF16, (D,), ix), _arg(rope_cos, "rope_cos", F32, half, ix),
-            _arg(rope_sin, "rope_sin", F32, half, ix), max_pos, _arg(positions, "positions", I32, (B,), ix),
-            _arg(slots, "slots", I32, (B,), ix))
-    pk, pv = _arg(k_cache, "k_cache", BF16, k_cache.shape, ix), _arg(v_cache, "v_cache", BF16, k_cache.shape, ix)
-    ps = None if scores is None else _arg(scores, "scores", F32, slots_shape, ix)
-    pp = None if slot_pos is None else _arg(slot_pos, "slot_pos", I32, slots_shape, ix)
-    q_out, pq = _out(q_out, "q_out", BF16, (B, Hq, D), ix)
-    _call("qmoe_kv_append", ix, *args, B, Hq, Hkv, D, S_max, float(eps), pq, pk, pv, ps, pp)
-    return q_out
-
-
-def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    x, y = a.data_ptr(), b.data_ptr()
-    return x < y + _nbytes(b) and y < x + _nbytes(a)
+    return _native().kv_append(qkv, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slots, Hq, Hkv, k_cache, v_cache,
+                               eps, scores, slot_pos, q_out)
 
 
 def kv_evict_workspace(B: int, Hkv: int, S_max: int, budget: int, device) -> Optional[torch.Tensor]:
@@ -1044,31 +884,7 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     or into ``out = (k, v, scores, slot_pos)``, another cache with at least
     ``budget`` slots, leaving this one as it is.  The caller's next ``ctx_len``
     is ``ctx_len.clamp(max=budget)``."""
-    ix = _gpu(k_cache, "k_cache", "[B, Hkv, S_max, D]", 4)
-    B, Hkv, S_max, D = k_cache.shape
-    budget, recent, sink = int(budget), int(recent), int(sink)
-    if budget <= 0 or recent < 0 or sink < 0 or recent + sink > budget:
-        raise ValueError(f"need budget > 0 and 0 <= recent + sink <= budget (budget={budget}, recent={recent}, "
-                         f"sink={sink})")
-    src = (k_cache, v_cache, scores, slot_pos)
-    names = ("k", "v", "scores", "slot_pos")
-
-    def addresses(cache, what, n_slots):
-        shapes = ((B, Hkv, n_slots, D), (B, Hkv, n_slots, D), (B, Hkv, n_slots), (B, Hkv, n_slots))
-        return [_arg(t, n + what, d, s, ix) for t, n, d, s in zip(cache, names, (BF16, BF16, F32, I32), shapes)]
-
-    ps = addresses(src, "", S_max)
-    pc = _arg(ctx_len, "ctx_len", I32, (B,), ix)
-    po, S_out = ps, S_max
-    if out is not None:
-        _, S_out = _cache_sizes(out[0], B, D)
-        if S_out < min(budget, S_max):
-            raise ValueError(f"out needs at least {min(budget, S_max)} slots (got {S_out})")
-        po = addresses(out, "_out", S_out)
-        if any(_overlap(x, y) for x in src for y in out):
-            raise ValueError("out overlaps the cache (leave it out to evict in place)")
-    _, pw, nw = _scratch(workspace, _size("qmoe_kv_evict_workspace", ix, B, Hkv, S_max, budget), ix)
-    _call("qmoe_kv_evict", ix, *ps, pc, B, Hkv, D, S_max, budget, recent, sink, pw, nw, S_out, *po)
+    _native().kv_evict(k_cache, v_cache, scores, slot_pos, ctx_len, budget, recent, sink, out, workspace)
 
 
 # ----------------------------------------------------------------- embedding / greedy argmax

@@ -371,3 +371,110 @@ def test_kv_evict_past_the_ranks_in_lds(dev):
         assert torch.equal(pos[0, h, :budget].long(), want)
         assert torch.equal(k[0, h, :budget], k0[0, h, want]) and torch.equal(sc[0, h, :budget], sc0[0, h, want])
         assert bool((pos[0, h, budget:] == -1).all()) and not bool(sc[0, h, budget:].any())
+
+
+# ------------------------------------------------------------------ refusals on the GPU
+def test_wrappers_refuse_before_any_launch(dev):
+    """Every argument that does not fit is named; the outputs stay as they were."""
+    announce("refusals")
+    B, S_max, P = 2, 8, 9
+    q = torch.ones(B, 32, D, dtype=torch.bfloat16, device=dev)
+    k, v = torch.ones(2, B, 4, S_max, D, dtype=torch.bfloat16, device=dev)
+    kp = torch.ones(4, P, D, dtype=torch.bfloat16, device=dev)
+    sc, sp = torch.ones(B, 4, S_max, device=dev), torch.ones(B, 4, S_max, dtype=torch.int32, device=dev)
+    n = torch.ones(B, dtype=torch.int32, device=dev)
+    out = torch.full((B, 32 * D), 7.0, dtype=torch.bfloat16, device=dev)
+    raw, w = torch.ones(B, 40 * D, device=dev), torch.ones(D, dtype=torch.bfloat16, device=dev)
+    cos = torch.ones(4, D // 2, device=dev)
+    odd = torch.ones(B * 4 * S_max * D + 8, dtype=torch.bfloat16, device=dev)[1:-7].view(B, 4, S_max, D)
+    tiny = torch.zeros(16, dtype=torch.uint8, device=dev)
+
+    def shared(q=q, kp=kp, vp=kp, k=k, v=v, n=n, B=B, S=1, **kw):
+        return ops.attn_shared(q, kp, vp, k, v, n, B, S, out=kw.pop("out", out), **kw)
+
+    def prompt(q=q, k=k, v=v, sc=sc, B=1, S=2, start=0, **kw):
+        return ops.attn_prefill_scored(q, k, v, sc, B, S, start, out=out, **kw)
+
+    def scored(q=q, k=k, v=v, n=n, sc=sc, **kw):
+        return ops.attn_decode_scored(q, k, v, n, sc, out=out, **kw)
+
+    def append(raw=raw, qn=w, kn=w, cos=cos, sin=cos, pos=n, slots=n, Hq=32, Hkv=4, k=k, v=v, **kw):
+        return ops.kv_append(raw, qn, kn, cos, sin, pos, slots, Hq, Hkv, k, v, 1e-6, **kw)
+
+    def evict(k=k, v=v, sc=sc, sp=sp, n=n, budget=4, **kw):
+        return ops.kv_evict(k, v, sc, sp, n, budget, **kw)
+
+    other = tuple(torch.empty_like(t) for t in (k, v, sc, sp))
+    refused = [
+        (shared, dict(B=3), "q must be"), (shared, dict(q=q.float()), "q: dtype"),
+        (shared, dict(q=q.transpose(0, 1).contiguous().transpose(0, 1)), "q: must be contiguous"),
+        (shared, dict(k=k[:1]), "k_cache must be"), (shared, dict(v=v[:, :, :7].contiguous()), "v_cache: shape"),
+        (shared, dict(v=v.cpu()), "v_cache: must be on a GPU"), (shared, dict(k=odd, v=odd), "16-byte aligned"),
+        (shared, dict(q=q[:, :30].contiguous()), "multiple of Hkv"), (shared, dict(kp=kp[:3]), "k_prefix must be"),
+        (shared, dict(vp=kp[:, :8].contiguous()), "v_prefix: shape"), (shared, dict(n=n.long()), "ctx_len: dtype"),
+        (shared, dict(n=n[:1]), "ctx_len: shape"), (shared, dict(prefix_len=10), "prefix_len"),
+        (shared, dict(prefix_len=-1), "prefix_len"), (shared, dict(max_ctx=9), "max_ctx"),
+        (shared, dict(max_ctx=-1), "max_ctx"), (shared, dict(scale=0.0), "scale"),
+        (shared, dict(scale=NAN), "scale"), (shared, dict(workspace=tiny), "workspace: needs"),
+        (shared, dict(workspace=tiny.cpu()), "workspace: must be"), (shared, dict(out=out[:1]), "out: shape"),
+        (shared, dict(out=out.float()), "out: dtype"),
+        (prompt, dict(B=2, S=2), "q must be"), (prompt, dict(B=1, S=2), "k_cache must be"),
+        (prompt, dict(k=k[:1], v=v[:1]), "scores: shape"),
+        (prompt, dict(k=k[:1], v=v[:1], sc=sc[:1], start=7), "start"),
+        (prompt, dict(k=k[:1], v=v[:1], sc=sc[:1], start=-1), "start"),
+        (prompt, dict(k=k[:1], v=v[:1], sc=sc[:1], lengths=n), "lengths: shape"),
+        (prompt, dict(k=k[:1], v=v[:1], sc=sc[:1], workspace=tiny), "workspace: needs"),
+        (scored, dict(sc=sc.double()), "scores: dtype"), (scored, dict(max_ctx=0), "max_ctx"),
+        (scored, dict(scale=-1.0), "scale"), (scored, dict(workspace=tiny), "workspace: needs"),
+        (append, dict(Hkv=2), "heads"), (append, dict(raw=raw[:1]), "k_cache must be"),
+        (append, dict(sin=cos[:3]), "rope_sin: shape"), (append, dict(qn=w.float()), "q_norm_w: dtype"),
+        (append, dict(scores=sc[:1]), "scores: shape"), (append, dict(slot_pos=sp.long()), "slot_pos: dtype"),
+        (append, dict(q_out=q[:1]), "q_out: shape"), (append, dict(Hq=30), "qkv: shape"),
+        (evict, dict(budget=0), "budget"), (evict, dict(recent=3, sink=2), "recent"),
+        (evict, dict(sp=sp[:1]), "slot_pos: shape"), (evict, dict(out=other[:3]), "out must be"),
+        (evict, dict(out=(k, v, other[2], other[3])), "overlaps"),
+        (evict, dict(out=(other[0], other[1], sc, other[3])), "overlaps"),
+        (evict, dict(out=tuple(t[:, :, :3].contiguous() for t in other)), "at least 4 slots"),
+        (evict, dict(workspace=tiny), "workspace: needs"),
+    ]
+    before = [t.clone() for t in (k, v, sc, sp, out)]
+    for call, change, msg in refused:
+        with pytest.raises(ValueError, match=msg):
+            call(**change)
+    torch.cuda.synchronize()
+    for t, x in zip((k, v, sc, sp, out), before):
+        assert torch.equal(t, x)
+
+
+def test_empty_batches_and_given_workspaces(dev):
+    announce("empty batches")
+    none = torch.empty(0, 32, D, dtype=torch.bfloat16, device=dev)
+    k = torch.zeros(0, 4, 8, D, dtype=torch.bfloat16, device=dev)
+    kp = torch.zeros(4, 9, D, dtype=torch.bfloat16, device=dev)
+    n, sc = torch.zeros(0, dtype=torch.int32, device=dev), torch.zeros(0, 4, 8, device=dev)
+    sp = torch.zeros(0, 4, 8, dtype=torch.int32, device=dev)
+    assert ops.attn_shared(none, kp, kp, k, k, n, 0, 1).shape == (0, 32 * D)
+    assert ops.attn_decode_scored(none, k, k, n, sc).shape == (0, 32 * D)
+    one = torch.zeros(1, 4, 8, D, dtype=torch.bfloat16, device=dev)
+    assert ops.attn_prefill_scored(none, one, one, torch.zeros(1, 4, 8, device=dev), 1, 0).shape == (0, 32 * D)
+    ops.kv_evict(k, k, sc, sp, n, 4)
+    g = _gen(dev, 9)
+    q = bf16_randn((3, 32, D), g, dev)
+    k, v = bf16_randn((3, 4, 300, D), g, dev), bf16_randn((3, 4, 300, D), g, dev)
+    n, sc = _i32([300, 2, 150], dev), torch.zeros(3, 4, 300, device=dev)
+    pos = torch.arange(300, dtype=torch.int32, device=dev).repeat(3, 4, 1)
+    a = ops.attn_decode_scored(q, k, v, n, sc)
+    sc2 = torch.zeros_like(sc)
+    b = ops.attn_decode_scored(q, k, v, n, sc2, workspace=ops.attn_decode_scored_workspace(3, 32, D, 300, dev))
+    assert torch.equal(a, b) and torch.equal(sc, sc2)
+    a = ops.attn_shared(q, k[0], v[0], k, v, n, 3, 1)
+    b = ops.attn_shared(q, k[0], v[0], k, v, n, 3, 1, workspace=ops.attn_shared_workspace(3, 1, 32, 4, D, 300, 300, dev))
+    assert torch.equal(a, b)
+    a = ops.attn_prefill_scored(q, k[:1], v[:1], sc[:1], 1, 3)
+    b = ops.attn_prefill_scored(q, k[:1], v[:1], sc2[:1], 1, 3,
+                                workspace=ops.attn_prefill_scored_workspace(1, 3, 32, 4, D, 0, dev))
+    assert torch.equal(a, b) and torch.equal(sc, sc2)
+    x, y = [t.clone() for t in (k, v, sc, pos)], [t.clone() for t in (k, v, sc, pos)]
+    ops.kv_evict(*x, n, 100, 5, 2)
+    ops.kv_evict(*y, n, 100, 5, 2, workspace=ops.kv_evict_workspace(3, 4, 300, 100, dev))
+    assert all(torch.equal(s, t) for s, t in zip(x, y))
