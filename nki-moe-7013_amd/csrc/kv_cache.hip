@@ -72,8 +72,8 @@ __global__ __launch_bounds__(64) void kv_append_kernel(
 
 // ====================================================================== scored decode
 constexpr int SD_KEYS = 64;       // keys of a wave
-constexpr int SD_WAVES = 4;       // waves of a workgroup, whose runs are joined in LDS
-constexpr int SD_SPLIT = SD_KEYS * SD_WAVES;
+constexpr int SD_WAVES = 4;       // waves of a workgroup, at most; their runs are joined in LDS
+constexpr int SD_SLICE = 256;     // keys whose scores a workgroup of the finish adds to
 constexpr int SD_REC = HD + 4;    // record: m, l, 2 pad, O[HD]
 constexpr int SD_MAX_G = 16;
 constexpr int SD_VCH = SD_KEYS * HD / 8 / 64;  // 16-byte V chunks of a lane
@@ -81,7 +81,7 @@ constexpr int SD_VCH = SD_KEYS * HD / 8 / 64;  // 16-byte V chunks of a lane
 struct SdArgs {
   const uint16_t *q, *k, *v;
   const int32_t* ctx_len;
-  int B, Hq, Hkv, S_max, max_ctx, nsplit, ldl;  // ldl: logits of a row, nsplit * SD_SPLIT
+  int B, Hq, Hkv, S_max, max_ctx, split, nsplit, ldl;  // split: keys of a workgroup; ldl: logits of a row
   float scale_log2;
   float* part;    // [B][Hq][nsplit][SD_REC]
   float* logits;  // [B][Hq][ldl], in log2 units
@@ -92,19 +92,24 @@ struct SdArgs {
 
 __device__ __forceinline__ int sd_ctx(const SdArgs& a, int b) { return min(max(a.ctx_len[b], 0), a.max_ctx); }
 
-// Workgroup = (split of 4 x 64 keys, kv head, row), wave = 64 of its keys with
+// Workgroup = (split of WAVES x 64 keys, kv head, row), wave = 64 of its keys with
 // the G q heads in the columns of S^T = K . Q^T and O^T = V^T . P^T.  K rows go
 // from the cache straight into A-operand registers, V through the wave's own
 // LDS tile; every load of a wave is in flight at once, so a wave costs one
 // round trip to memory.  The logits leave as four consecutive keys a lane.
-__global__ __launch_bounds__(SD_WAVES * 64) void attn_scored_kernel(const SdArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t vs[SD_WAVES][AP_TILE];
+// WAVES = 1 (few keys in all): the join of four waves is two barriers and a
+// round through LDS longer, and the finish has no more records than it can take
+// at once.
+template <int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void attn_scored_kernel(const SdArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t vs[WAVES][AP_TILE];
+  constexpr int SPLIT = WAVES * SD_KEYS;
   const int lane = threadIdx.x & 63, col = lane & 31, hi = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6));
+  const int wave = WAVES > 1 ? __builtin_amdgcn_readfirstlane(int(threadIdx.x >> 6)) : 0;
   const int split = blockIdx.x, kvh = blockIdx.y, b = blockIdx.z, G = a.Hq / a.Hkv;
   const int ctx = sd_ctx(a, b);
-  if (split * SD_SPLIT >= ctx) return;  // the finish knows which splits hold keys
-  const int kw0 = split * SD_SPLIT + wave * SD_KEYS, nk = min(SD_KEYS, ctx - kw0);
+  if (split * SPLIT >= ctx) return;  // the finish knows which splits hold keys
+  const int kw0 = split * SPLIT + wave * SD_KEYS, nk = min(SD_KEYS, ctx - kw0);
   float m = -INFINITY, l = 0.0f;
   f32x16 oacc[4];
 #pragma unroll
@@ -189,9 +194,23 @@ __global__ __launch_bounds__(SD_WAVES * 64) void attn_scored_kernel(const SdArgs
       }
     }
   }
+  float* pbase = a.part + ((int64_t(b) * a.Hq + kvh * G) * a.nsplit + split) * SD_REC;
+  if constexpr (WAVES == 1) {
+    if (col < G) {
+      float* pg = pbase + int64_t(col) * a.nsplit * SD_REC;
+      if (hi == 0) *reinterpret_cast<float2*>(pg) = make_float2(m, l);
+#pragma unroll
+      for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int e4 = 0; e4 < 4; ++e4)
+          *reinterpret_cast<float4*>(pg + 4 + db * 32 + e4 * 8 + hi * 4) =
+              make_float4(oacc[db][e4 * 4], oacc[db][e4 * 4 + 1], oacc[db][e4 * 4 + 2], oacc[db][e4 * 4 + 3]);
+    }
+    return;
+  }
   // the waves' (m, l, O) joined in LDS (the V tiles are free)
   float* rec = reinterpret_cast<float*>(&vs[0][0]);
-  static_assert(SD_WAVES * SD_MAX_G * SD_REC * 4 <= SD_WAVES * AP_TILE, "records fit the V tiles");
+  static_assert(WAVES * SD_MAX_G * SD_REC * 4 <= WAVES * AP_TILE, "records fit the V tiles");
   __syncthreads();
   if (col < G) {
     float* pg = rec + (wave * SD_MAX_G + col) * SD_REC;
@@ -207,14 +226,13 @@ __global__ __launch_bounds__(SD_WAVES * 64) void attn_scored_kernel(const SdArgs
             make_float4(oacc[db][e4 * 4], oacc[db][e4 * 4 + 1], oacc[db][e4 * 4 + 2], oacc[db][e4 * 4 + 3]);
   }
   __syncthreads();
-  float* pbase = a.part + ((int64_t(b) * a.Hq + kvh * G) * a.nsplit + split) * SD_REC;
-  for (int i = int(threadIdx.x); i < G * HD; i += SD_WAVES * 64) {
+  for (int i = int(threadIdx.x); i < G * HD; i += WAVES * 64) {
     const int c = i / HD, d = i % HD;
     float M = -INFINITY, L = 0.0f, O = 0.0f;
 #pragma unroll
-    for (int w = 0; w < SD_WAVES; ++w) M = fmaxf(M, rec[(w * SD_MAX_G + c) * SD_REC]);
+    for (int w = 0; w < WAVES; ++w) M = fmaxf(M, rec[(w * SD_MAX_G + c) * SD_REC]);
 #pragma unroll
-    for (int w = 0; w < SD_WAVES; ++w) {
+    for (int w = 0; w < WAVES; ++w) {
       const float* r = rec + (w * SD_MAX_G + c) * SD_REC;
       const float wt = r[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(r[0] - M);
       L = fmaf(wt, r[1], L);
@@ -247,7 +265,7 @@ __global__ __launch_bounds__(256) void attn_scored_finish_kernel(const SdArgs a)
   if (int(blockIdx.x) < a.n_merge) {
     const int row = int(blockIdx.x) * 4 + wave;
     if (row >= a.B * a.Hq) return;
-    const int live = (sd_ctx(a, row / a.Hq) + SD_SPLIT - 1) / SD_SPLIT;
+    const int live = (sd_ctx(a, row / a.Hq) + a.split - 1) / a.split;
     const float* p = a.part + int64_t(row) * a.nsplit * SD_REC;
     float M, L;
     sd_row(p, live, lane, M, L);
@@ -273,10 +291,10 @@ __global__ __launch_bounds__(256) void attn_scored_finish_kernel(const SdArgs a)
     return;
   }
   __shared__ float sm[SD_MAX_G], si[SD_MAX_G];
-  const int x = int(blockIdx.x) - a.n_merge, bh = x / a.nsplit, b = bh / a.Hkv;
-  const int key = x % a.nsplit * SD_SPLIT + int(threadIdx.x), ctx = sd_ctx(a, b);
+  const int slices = (a.ldl + SD_SLICE - 1) / SD_SLICE, x = int(blockIdx.x) - a.n_merge, bh = x / slices, b = bh / a.Hkv;
+  const int key = x % slices * SD_SLICE + int(threadIdx.x), ctx = sd_ctx(a, b);
   if (key - int(threadIdx.x) >= ctx) return;
-  const int live = (ctx + SD_SPLIT - 1) / SD_SPLIT;
+  const int live = (ctx + a.split - 1) / a.split;
   const int row0 = b * a.Hq + bh % a.Hkv * G;
   for (int g = wave; g < G; g += 4) {
     float M, L;
@@ -540,11 +558,22 @@ extern "C" int qmoe_kv_append(const float* qkv, const qmoe_bf16* q_norm_w, const
   return hip_status(fn);
 }
 
-static int64_t sd_splits(int64_t max_ctx) { return (max_ctx + SD_SPLIT - 1) / SD_SPLIT; }
+// Keys of a workgroup: 64, while that makes at most two of them a CU and 64
+// records a row (1 x 1100: 10.6 -> 8.3 us), else 256.
+static int64_t sd_split(int64_t B, int64_t Hkv, int64_t max_ctx) {
+  const int64_t n = (max_ctx + SD_KEYS - 1) / SD_KEYS;
+  return n <= 64 && n * B * Hkv <= 512 ? SD_KEYS : SD_KEYS * SD_WAVES;
+}
+static int64_t sd_bytes(int64_t B, int64_t Hq, int64_t max_ctx, int64_t split) {
+  const int64_t n = (max_ctx + split - 1) / split;
+  return B * Hq * n * (SD_REC + split) * int64_t(sizeof(float));
+}
 
+// (for the split that takes more, so that the size does not hang on Hkv)
 extern "C" int64_t qmoe_attn_decode_scored_workspace(int64_t B, int64_t Hq, int64_t D, int64_t max_ctx) {
   if (B < 0 || Hq < 0 || D != HD || max_ctx < 0 || max_ctx >= (1ll << 30)) return -1;
-  return B * Hq * sd_splits(max_ctx) * (SD_REC + SD_SPLIT) * int64_t(sizeof(float));
+  const int64_t few = (max_ctx + SD_KEYS - 1) / SD_KEYS <= 64 && B <= 512 ? sd_bytes(B, Hq, max_ctx, SD_KEYS) : 0;
+  return std::max(few, sd_bytes(B, Hq, max_ctx, SD_KEYS * SD_WAVES));
 }
 
 extern "C" int qmoe_attn_decode_scored(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
@@ -562,18 +591,22 @@ extern "C" int qmoe_attn_decode_scored(const qmoe_bf16* q, const qmoe_bf16* k_ca
   QMOE_REQUIRE(max_ctx > 0 && max_ctx <= S_max, "%s: need 0 < max_ctx <= S_max", fn);
   QMOE_REQUIRE(scale > 0.0f && std::isfinite(scale), "%s: scale must be positive and finite", fn);
   if (B == 0) return QMOE_OK;
-  const int64_t ns = sd_splits(max_ctx), need = B * Hq * ns * (SD_REC + SD_SPLIT) * int64_t(sizeof(float));
+  const int64_t split = sd_split(B, Hkv, max_ctx), ns = (max_ctx + split - 1) / split;
+  const int64_t need = sd_bytes(B, Hq, max_ctx, split);
   QMOE_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %lld bytes, need %lld", fn,
                (long long)workspace_bytes, (long long)need);
-  const int64_t n_merge = (B * Hq + 3) / 4;
-  QMOE_REQUIRE(n_merge + B * Hkv * ns < (1ll << 31), "%s: grid too large", fn);
-  SdArgs a{q, k_cache, v_cache, ctx_len, int(B), int(Hq), int(Hkv), int(S_max), int(max_ctx), int(ns),
-           int(ns * SD_SPLIT), scale * 1.4426950408889634f, static_cast<float*>(workspace),
+  const int64_t n_merge = (B * Hq + 3) / 4, slices = (ns * split + SD_SLICE - 1) / SD_SLICE;
+  QMOE_REQUIRE(n_merge + B * Hkv * slices < (1ll << 31), "%s: grid too large", fn);
+  SdArgs a{q, k_cache, v_cache, ctx_len, int(B), int(Hq), int(Hkv), int(S_max), int(max_ctx), int(split), int(ns),
+           int(ns * split), scale * 1.4426950408889634f, static_cast<float*>(workspace),
            static_cast<float*>(workspace) + B * Hq * ns * SD_REC, scores, out, int(n_merge)};
-  hipLaunchKernelGGL(attn_scored_kernel, dim3(unsigned(ns), unsigned(Hkv), unsigned(B)), dim3(SD_WAVES * 64), 0,
-                     as_stream(stream), a);
+  const dim3 grid{unsigned(ns), unsigned(Hkv), unsigned(B)};
+  if (split == SD_KEYS)
+    hipLaunchKernelGGL(attn_scored_kernel<1>, grid, dim3(64), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(attn_scored_kernel<SD_WAVES>, grid, dim3(SD_WAVES * 64), 0, as_stream(stream), a);
   if (int rc = hip_status(fn)) return rc;
-  hipLaunchKernelGGL(attn_scored_finish_kernel, dim3(unsigned(n_merge + B * Hkv * ns)), dim3(256), 0,
+  hipLaunchKernelGGL(attn_scored_finish_kernel, dim3(unsigned(n_merge + B * Hkv * slices)), dim3(256), 0,
                      as_stream(stream), a);
   return hip_status(fn);
 }
