@@ -39,8 +39,12 @@ constexpr int64_t AR_MAX_KEYS = 1ll << 22;  // keys of one run are addressed wit
 // Tiles (128 rows, 64 keys: flash_segment) share each key among four waves'
 // rows; streams (32 rows, 256 keys: stream_segment) share each row among four
 // waves' keys.
+// `split` streams of one step keep their waves' 64 keys apart, as records of their
+// own, where the join of the waves (five barriers) is longer than four records
+// are for the merge.
 struct ArKind {
-  int stream, rts, runs, run;
+  int stream, rts, runs, run, split;
+  __host__ __device__ int records() const { return split ? 4 * runs : runs; }
   __host__ __device__ int rows() const { return stream ? 32 : 128; }
   __host__ __device__ int keys() const { return stream ? 4 * AP_KT : AP_KT; }
 };
@@ -57,7 +61,7 @@ struct ArArgs {
   float* lse;   // [B][Hkv][S * G] or nullptr
   // n_pre prefix items (pre.rts row tiles over all B * S * G rows x pre.runs x
   // Hkv), then items of (own.rts row tiles x own.runs x B x Hkv), whose steps
-  // start with the prefix when joint.  NS = pre.runs + own.runs records a row.
+  // start with the prefix when joint.  NS = pre.records() + own.records() a row.
   int NS, n_pre, joint, nb_pre, nb_own;  // nb: blocks of 32 rows
   ArKind pre, own;
 };
@@ -147,16 +151,17 @@ __device__ __forceinline__ void ar_item(const ArArgs& a, const ArKind kd, const 
       flash_segment(smem, kk + base, vv + base, n, lim, __builtin_amdgcn_readfirstlane(first),
                     __builtin_amdgcn_readfirstlane(last), a.scale_log2, st);
   }
-  if constexpr (stream) {
+  if (stream && !kd.split) {
     flash_join(smem, st);
     if (wave) return;
   }
+  const int rec_run = stream && kd.split ? run * 4 + wave : run;
   const float l = st.row_sum();
   if (!live) return;
   if (a.NS > 1) {
-    const int64_t blk = pre ? (int64_t(run) * a.Hkv + kvh) * a.nb_pre + rw / 32
-                            : int64_t(a.pre.runs) * a.Hkv * a.nb_pre +
-                                  ((int64_t(run) * a.B + b) * a.Hkv + kvh) * a.nb_own + rw / 32;
+    const int64_t blk = pre ? (int64_t(rec_run) * a.Hkv + kvh) * a.nb_pre + rw / 32
+                            : int64_t(a.pre.records()) * a.Hkv * a.nb_pre +
+                                  ((int64_t(rec_run) * a.B + b) * a.Hkv + kvh) * a.nb_own + rw / 32;
     float* rec = a.part + blk * AR_REC;
     if (hl == 0) *reinterpret_cast<float2*>(rec + (lane & 31) * 2) = make_float2(st.m, l);
 #pragma unroll
@@ -219,7 +224,7 @@ __global__ __launch_bounds__(256) void attn_rows_merge_kernel(const ArArgs a) {
   const int sq = ar_div(r, a.g_magic), b = sq / a.S, rib = r - b * per;
   const int64_t pre_next = int64_t(a.Hkv) * a.nb_pre * AR_REC, own_next = int64_t(a.B) * a.Hkv * a.nb_own * AR_REC;
   const float* pp = a.part + (int64_t(kvh) * a.nb_pre + rb) * AR_REC;
-  const float* po = a.part + a.pre.runs * pre_next + ((int64_t(b) * a.Hkv + kvh) * a.nb_own + rib / 32) * AR_REC;
+  const float* po = a.part + a.pre.records() * pre_next + ((int64_t(b) * a.Hkv + kvh) * a.nb_own + rib / 32) * AR_REC;
   const int own_lane = rib % 32 + hl * 32;
   float M = -INFINITY, L = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -230,8 +235,8 @@ __global__ __launch_bounds__(256) void attn_rows_merge_kernel(const ArArgs a) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int i = i0 + u * WAVES_A_CHUNK, j = min(i, a.NS - 1);
-      const bool pre = j < a.pre.runs;
-      const float* p = pre ? pp + j * pre_next : po + (j - a.pre.runs) * own_next;
+      const bool pre = j < a.pre.records();
+      const float* p = pre ? pp + j * pre_next : po + (j - a.pre.records()) * own_next;
       const int ln = pre ? lane : own_lane;
       ml[u] = *reinterpret_cast<const float2*>(p + (ln & 31) * 2);
       v[u] = *reinterpret_cast<const f32x4*>(p + 64 + (chunk * 64 + ln) * 4);
@@ -547,7 +552,12 @@ static void ar_plan(ArArgs& a, int64_t own_keys, int64_t* grid) {
   ar_cut(a.own, own_steps,
          a.joint ? ar_joint_runs(own_items, own_steps, int64_t(a.B) * a.S * a.Hq, cus) : cus / own_items);
   if (a.pre.runs + a.own.runs == 0) a.own.runs = 1;  // nothing to see: items that write zeros
-  a.NS = a.pre.runs + a.own.runs;
+  // us without and with: 4 rows on 300 + 24 keys 10.7 / 9.6, 8 rows on 300 + 250 10.7 /
+  // 9.8; but 1 row on 4096 + 200 (17 runs) 11.1 / 12.1, 64 rows on 1000 + 1000 26.1 / 30.8
+  const bool few = a.pre.runs + a.own.runs <= 4 && pre_items * a.pre.runs + own_items * a.own.runs <= 128;
+  a.pre.split = few && a.pre.stream && a.pre.run == 1;
+  a.own.split = few && a.own.stream && a.own.run == 1;
+  a.NS = a.pre.records() + a.own.records();
   a.n_pre = int(pre_items * a.pre.runs);
   a.nb_pre = a.pre.runs ? int(ar_ceil(all, 32)) : 0;
   a.nb_own = a.own.runs ? int(ar_ceil(rows, 32)) : 0;
@@ -557,7 +567,8 @@ static void ar_plan(ArArgs& a, int64_t own_keys, int64_t* grid) {
 
 static int64_t ar_part_bytes(const ArArgs& a) {
   if (a.NS <= 1) return 0;
-  const int64_t blocks = int64_t(a.pre.runs) * a.Hkv * a.nb_pre + int64_t(a.own.runs) * a.B * a.Hkv * a.nb_own;
+  const int64_t blocks =
+      int64_t(a.pre.records()) * a.Hkv * a.nb_pre + int64_t(a.own.records()) * a.B * a.Hkv * a.nb_own;
   return blocks * AR_REC * int64_t(sizeof(float));
 }
 

@@ -339,10 +339,250 @@ __device__ __forceinline__ uint32_t ev_rank(float f) {
 // One workgroup a (row, kv head).  The budget-th largest rank by radix select
 // (11 + 11 + 10 bits, a histogram in LDS each), where protected entries (the
 // first `sink` positions and the `recent` last ones) rank above all; of the
-// entries at the threshold the lowest slots stay.  Each wave then owns a run of
-// slots and numbers its holes (free slots below the budget) and movers (kept
-// slots past it) with ballots.
-__global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const EvArgs a) {
+// entries at the threshold the lowest slots stay.  Each wave owns a run of slots
+// and numbers its holes (free slots below the budget) and movers (kept slots past
+// it) with ballots; the hole of each rank takes the mover of that rank.
+//
+// Caches of up to 1024 R slots: what bounds it is its chain of round trips and
+// barriers (8 rows of 4096 slots, 0.3 MB: 9.6 us), so every thread reads its R
+// slots at once, before the length is known, and keeps them in registers; a
+// histogram of its own for each pass needs no clearing between them; one wave
+// looks for the bin while the others wait; movers leave their score and position
+// in LDS, not only their slot.  `moves`: of a cache cut down in place by few
+// entries the rows move here as well (64 rows of 1088 slots, 64 moves: 6.7 us; with a
+// launch of their own, and the ranks in LDS, 11.3 + 4).
+struct EvMove {
+  uint16_t *k, *v;  // nullptr: kv_move_kernel does it
+};
+
+// Inclusive sums and the maximum over a wave's lanes by DPP (as wave_sum).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_SHR(1), 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_SHR(2), 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_SHR(4), 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_SHR(8), 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_BCAST15, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_BCAST31, 0xc, 0xf, false);
+  return v;
+}
+__device__ __forceinline__ int wave_max_int(int v) {
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, QMOE_DPP_ROW_SHR(1), 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, QMOE_DPP_ROW_SHR(2), 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, QMOE_DPP_ROW_SHR(4), 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, QMOE_DPP_ROW_SHR(8), 0xf, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, QMOE_DPP_ROW_BCAST15, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(v, v, QMOE_DPP_ROW_BCAST31, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+// The waves' values of red[EV_WAVES], by four wide reads, summed over the waves
+// before `wave` (total: over all).
+__device__ __forceinline__ int waves_before(const int* red, int wave, int& total) {
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int i = 0; i < EV_WAVES / 4; ++i) {
+    const int4 v = *reinterpret_cast<const int4*>(red + 4 * i);
+    const int q[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      total += q[j];
+      before += 4 * i + j < wave ? q[j] : 0;
+    }
+  }
+  return before;
+}
+
+template <int R>
+__global__ __launch_bounds__(EV_THREADS) void kv_select_kernel(const EvArgs a, const EvMove mvd) {
+  constexpr int MOVERS = R * 512;  // at most half of the slots move
+  extern __shared__ __attribute__((aligned(16))) uint32_t ev_smem[];
+  uint32_t* hist = ev_smem;                                // [3][EV_BINS], a lane's 32 (16) bins 64 apart, from the top
+  int* red = reinterpret_cast<int*>(hist + 3 * EV_BINS);   // [3][EV_WAVES]
+  int* sel = red + 3 * EV_WAVES;                           // [3][4]: bin, entries above it, entries in it
+  int* m_slot = sel + 16;                                  // [MOVERS] by rank
+  float* m_score = reinterpret_cast<float*>(m_slot + MOVERS);
+  int* m_pos = reinterpret_cast<int*>(m_score + MOVERS);
+  int* h_slot = m_pos + MOVERS;
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int bh = blockIdx.x;
+  const float* sc = a.scores + int64_t(bh) * a.S_max;
+  const int32_t* sp = a.slot_pos + int64_t(bh) * a.S_max;
+  float* so = a.scores_out + int64_t(bh) * a.S_out;
+  int32_t* po = a.pos_out + int64_t(bh) * a.S_out;
+  int32_t* src = a.src + int64_t(bh) * a.budget;
+  const bool same = a.scores_out == a.scores;
+  const int first = wave * R * 64 + lane;  // this thread's slots: first + 64 j
+  float score[R];
+  int pos[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int i = min(first + 64 * j, a.S_max - 1);
+    score[j] = sc[i];
+    pos[j] = sp[i];
+  }
+  const int n = min(max(a.ctx_len[bh / a.Hkv], 0), a.S_max), kept = min(n, a.budget);
+  for (int i = t; i < 3 * EV_BINS; i += EV_THREADS) hist[i] = 0;
+  if (n <= a.budget) {  // nothing to evict (workgroup-uniform)
+    for (int i = t; i < kept; i += EV_THREADS) src[i] = i;
+#pragma unroll
+    for (int j = 0; j < R; ++j)
+      if (!same && first + 64 * j < kept) {
+        so[first + 64 * j] = score[j];
+        po[first + 64 * j] = pos[j];
+      }
+    for (int i = kept + t; i < a.S_out; i += EV_THREADS) {
+      so[i] = 0.0f;
+      po[i] = -1;
+    }
+    return;
+  }
+  int newest = INT32_MIN;
+#pragma unroll
+  for (int j = 0; j < R; ++j)
+    if (first + 64 * j < n) newest = max(newest, pos[j]);
+  newest = wave_max_int(newest);
+  if (lane == 0) red[wave] = newest;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < EV_WAVES / 4; ++i) {
+    const int4 v = *reinterpret_cast<const int4*>(red + 4 * i);
+    newest = max(max(newest, max(v.x, v.y)), max(v.z, v.w));
+  }
+  uint32_t key[R];
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const bool held = int64_t(pos[j]) > int64_t(newest) - a.recent || pos[j] < a.sink;
+    key[j] = held ? 0xffffffffu : ev_rank(score[j]);
+  }
+  // prefix: the threshold's leading bits; need: its place among the entries that
+  // share them
+  uint32_t prefix = 0, thr = 0;
+  int need = a.budget;
+  bool found = false;
+#pragma unroll
+  for (int pass = 0; pass < 3; ++pass) {
+    if (found) continue;  // workgroup-uniform
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11, per = (1 << bits) / 64;
+    uint32_t* h = hist + pass * EV_BINS;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const bool in = first + 64 * j < n && (pass == 0 || (key[j] >> (shift + bits)) == prefix);
+      const uint64_t m = __ballot(in);
+      if (m == 0) continue;
+      const int bin = (1 << bits) - 1 - int((key[j] >> shift) & ((1u << bits) - 1));  // from the top
+      const int lead = __shfl(bin, __ffsll((unsigned long long)m) - 1, 64);
+      uint32_t* p = h + (bin % per) * 64 + bin / per;
+      if (__ballot(in && bin == lead) == m) {  // a run of equal scores: one addition
+        if (lane == __ffsll((unsigned long long)m) - 1) atomicAdd(p, uint32_t(__popcll(m)));
+      } else if (in) {
+        atomicAdd(p, 1u);
+      }
+    }
+    __syncthreads();
+    if (wave == 0) {  // lane l holds bins [per l, per l + per); first the lane, then the bin
+      int sum = 0;
+#pragma unroll
+      for (int i = 0; i < per; ++i) sum += int(h[i * 64 + lane]);
+      const int upto = wave_scan(sum);
+      const int at = __ffsll((unsigned long long)__ballot(upto >= need)) - 1;
+      const int above = __builtin_amdgcn_readlane(upto - sum, at);
+      const int c = lane < per ? int(h[lane * 64 + at]) : 0, incl = above + wave_scan(c);
+      const int i = __ffsll((unsigned long long)__ballot(incl >= need)) - 1;
+      if (lane == i) {
+        sel[pass * 4] = (1 << bits) - 1 - (at * per + i);
+        sel[pass * 4 + 1] = incl - c;
+        sel[pass * 4 + 2] = c;
+      }
+    }
+    __syncthreads();
+    prefix = (prefix << bits) | uint32_t(sel[pass * 4]);
+    need -= sel[pass * 4 + 1];
+    thr = prefix << shift;
+    if (sel[pass * 4 + 2] == need && thr > 0) {  // the whole bin stays
+      --thr;
+      need = 0;
+      found = true;
+    }
+  }
+  // key > thr stays, and of those at thr the first `need` slots
+  int eq = 0;
+#pragma unroll
+  for (int j = 0; j < R; ++j) eq += __popcll(__ballot(first + 64 * j < n && key[j] == thr));
+  if (lane == 0) red[EV_WAVES + wave] = eq;
+  __syncthreads();
+  int all, e = waves_before(red + EV_WAVES, wave, all);
+  const uint64_t below = (1ull << lane) - 1;
+  uint32_t keep = 0;  // bit j
+  int holes = 0, movers = 0;
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int i = first + 64 * j;
+    const bool at = i < n && key[j] == thr;
+    const uint64_t m = __ballot(at);
+    const bool k = i < n && (key[j] > thr || (at && e + int(__popcll(m & below)) < need));
+    e += __popcll(m);
+    keep |= uint32_t(k) << j;
+    holes += __popcll(__ballot(!k && i < a.budget));
+    movers += __popcll(__ballot(k && i >= a.budget));
+  }
+  if (lane == 0) {
+    red[wave] = holes;  // (the positions there were read two barriers ago)
+    red[2 * EV_WAVES + wave] = movers;
+  }
+  __syncthreads();
+  int total, h0 = waves_before(red, wave, total), m0 = waves_before(red + 2 * EV_WAVES, wave, all);
+  int rank[R];  // of a hole
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int i = first + 64 * j;
+    const bool k = (keep >> j) & 1u, hole = !k && i < a.budget, mover = k && i >= a.budget;
+    const uint64_t hm = __ballot(hole), mm = __ballot(mover);
+    rank[j] = hole ? h0 + int(__popcll(hm & below)) : -1;
+    if (hole) h_slot[rank[j]] = i;
+    if (mover) {
+      const int r = m0 + int(__popcll(mm & below));
+      m_slot[r] = i;
+      m_score[r] = score[j];
+      m_pos[r] = pos[j];
+    }
+    h0 += __popcll(hm);
+    m0 += __popcll(mm);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const int i = first + 64 * j;
+    if (i < a.budget) {  // (budget < n: a slot of the cache)
+      const int r = rank[j];
+      src[i] = r < 0 ? i : m_slot[r];
+      if (r >= 0 || !same) {
+        so[i] = r < 0 ? score[j] : m_score[r];
+        po[i] = r < 0 ? pos[j] : m_pos[r];
+      }
+    }
+  }
+  for (int i = a.budget + t; i < a.S_out; i += EV_THREADS) {
+    so[i] = 0.0f;
+    po[i] = -1;
+  }
+  if (mvd.k == nullptr) return;
+  for (int m = t >> 4; m < total; m += EV_THREADS / 16) {  // 16 lanes a row
+    const int64_t base = int64_t(bh) * a.S_max * HD + (t & 15) * 8;
+    const int64_t from = base + int64_t(m_slot[m]) * HD, to = base + int64_t(h_slot[m]) * HD;
+    const u32x4 kr = ld16(mvd.k + from), vr = ld16(mvd.v + from);
+    *reinterpret_cast<u32x4*>(mvd.k + to) = kr;
+    *reinterpret_cast<u32x4*>(mvd.v + to) = vr;
+  }
+}
+template <int R>
+constexpr int ev_lds() {
+  return (3 * EV_BINS + 3 * EV_WAVES + 16 + 4 * R * 512) * 4;
+}
+static_assert(ev_lds<16>() <= 160 * 1024, "LDS");
+
+// The same for longer caches: the ranks are read again from LDS or memory for
+// every pass, the movers' slots go through the workspace.
+__global__ __launch_bounds__(EV_THREADS) void kv_select_long_kernel(const EvArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t ev_smem[];
   uint32_t* hist = ev_smem;                                    // [EV_BINS]
   int* red = reinterpret_cast<int*>(ev_smem + EV_BINS);        // [EV_WAVES]
@@ -611,6 +851,19 @@ extern "C" int qmoe_attn_decode_scored(const qmoe_bf16* q, const qmoe_bf16* k_ca
   return hip_status(fn);
 }
 
+constexpr int64_t EV_HERE = 256;  // rows that the selection moves itself, at most
+
+template <int R>
+static void ev_launch(dim3 grid, const EvArgs& e, const EvMove& mv, hipStream_t s) {
+  static const bool attr = [] {
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kv_select_kernel<R>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, ev_lds<R>());
+    return true;
+  }();
+  (void)attr;
+  hipLaunchKernelGGL(kv_select_kernel<R>, grid, dim3(EV_THREADS), ev_lds<R>(), s, e, mv);
+}
+
 extern "C" int64_t qmoe_kv_evict_workspace(int64_t B, int64_t Hkv, int64_t S_max, int64_t budget) {
   if (B < 0 || Hkv < 0 || S_max < 0 || budget < 0) return -1;
   return 2 * B * Hkv * std::min(budget, S_max) * int64_t(sizeof(int32_t));
@@ -641,21 +894,38 @@ extern "C" int qmoe_kv_evict(const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
   const int64_t need = qmoe_kv_evict_workspace(B, Hkv, S_max, budget);
   QMOE_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %lld bytes, need %lld", fn,
                (long long)workspace_bytes, (long long)need);
-  const int lds_keys = int(std::min<int64_t>(S_max, EV_LDS_KEYS));
-  const int lds = (EV_BINS + 2 * EV_WAVES + 16 + lds_keys) * 4;
-  static const bool attr = [] {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kv_select_kernel),
-                              hipFuncAttributeMaxDynamicSharedMemorySize,
-                              (EV_BINS + 2 * EV_WAVES + 16 + EV_LDS_KEYS) * 4);
-    return true;
-  }();
-  (void)attr;
   int32_t* src = static_cast<int32_t*>(workspace);
+  const int lds_keys = int(std::min<int64_t>(S_max, EV_LDS_KEYS));
   EvArgs e{scores, slot_pos, ctx_len, int(B), int(Hkv), int(S_max), int(budget),
            int(std::min<int64_t>(recent, 1 << 30)), int(std::min<int64_t>(sink, 1 << 30)), int(S_out), lds_keys,
            scores_out, slot_pos_out, src, src + B * Hkv * budget};
-  hipLaunchKernelGGL(kv_select_kernel, dim3(unsigned(B * Hkv)), dim3(EV_THREADS), lds, as_stream(stream), e);
+  // in place, with few entries past the budget: 64 rows move at a time
+  const bool here = same && S_max <= 16 * EV_THREADS && std::min(budget, S_max - budget) <= EV_HERE;
+  const EvMove mv{here ? k_out : nullptr, here ? v_out : nullptr};
+  const dim3 grid{unsigned(B * Hkv)};
+  if (S_max <= EV_THREADS)
+    ev_launch<1>(grid, e, mv, as_stream(stream));
+  else if (S_max <= 2 * EV_THREADS)
+    ev_launch<2>(grid, e, mv, as_stream(stream));
+  else if (S_max <= 4 * EV_THREADS)
+    ev_launch<4>(grid, e, mv, as_stream(stream));
+  else if (S_max <= 8 * EV_THREADS)
+    ev_launch<8>(grid, e, mv, as_stream(stream));
+  else if (S_max <= 16 * EV_THREADS)
+    ev_launch<16>(grid, e, mv, as_stream(stream));
+  else {
+    static const bool attr = [] {
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kv_select_long_kernel),
+                                hipFuncAttributeMaxDynamicSharedMemorySize,
+                                (EV_BINS + 2 * EV_WAVES + 16 + EV_LDS_KEYS) * 4);
+      return true;
+    }();
+    (void)attr;
+    hipLaunchKernelGGL(kv_select_long_kernel, grid, dim3(EV_THREADS), (EV_BINS + 2 * EV_WAVES + 16 + lds_keys) * 4,
+                       as_stream(stream), e);
+  }
   if (int rc = hip_status(fn)) return rc;
+  if (here) return QMOE_OK;
   EmArgs m{k_cache, v_cache, k_out, v_out, src, ctx_len, int(Hkv), int(S_max), int(S_out), int(budget)};
   hipLaunchKernelGGL(kv_move_kernel, dim3(unsigned((budget + EM_SLOTS - 1) / EM_SLOTS), unsigned(B * Hkv)), dim3(256),
                      0, as_stream(stream), m);
