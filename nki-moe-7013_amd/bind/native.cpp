@@ -162,14 +162,25 @@ void heads(int64_t Hq, int64_t Hkv) {
 }
 
 float scale_of(py::handle h, int64_t D) {
-  const double s = h.is_none() ? 1.0 / std::sqrt(double(D)) : py::cast<double>(h);
+  const double s = h.is_none() ? 1.0 / std::sqrt(double(D)) : PyFloat_AsDouble(h.ptr());
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    refuse("scale must be a number");
+  }
   if (!(s > 0.0) || !std::isfinite(s)) refuse("scale must be positive and finite");
   return float(s);
 }
 
 // An integer within [lo, hi], or `none` where None was given.
 int64_t within(py::handle h, const char* name, int64_t lo, int64_t hi, int64_t none) {
-  const int64_t n = h.is_none() ? none : py::cast<int64_t>(h);
+  int64_t n = none;
+  if (!h.is_none()) {
+    n = PyLong_AsLongLong(h.ptr());  // any integer (an __index__ of its own included)
+    if (n == -1 && PyErr_Occurred()) {
+      PyErr_Clear();
+      refuse(std::string(name) + " must be an integer");
+    }
+  }
   if (n < lo || n > hi)
     refuse(std::string(name) + " must be in [" + std::to_string(lo) + ", " + std::to_string(hi) + "] (got " +
            std::to_string(n) + ")");

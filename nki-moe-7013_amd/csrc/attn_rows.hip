@@ -466,7 +466,8 @@ __global__ __launch_bounds__(256, 2) void attn_colsum_kernel(const CsArgs a) {
 __global__ __launch_bounds__(256) void attn_colsum_add_kernel(const CsArgs a) {
   __shared__ float red[4][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int grp = a.B * a.Hkv, bh = blockIdx.y, key = int(blockIdx.x) * 64 + lane;
+  const int slices = a.nkt * (CS_KEYS / 64), grp = a.B * a.Hkv;
+  const int bh = int(blockIdx.x) / slices, key = int(blockIdx.x) % slices * 64 + lane;
   const int c1 = (cs_tiles(a, key / CS_KEYS, a.Hq / a.Hkv, cs_len(a, bh / a.Hkv)) + a.run - 1) / a.run;
   if (c1 == 0) return;
   const float* p = a.part + int64_t(bh) * a.nkt * CS_KEYS + key;
@@ -744,7 +745,8 @@ extern "C" int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_c
   QMOE_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %lld bytes, need %lld", fn,
                (long long)workspace_bytes, (long long)need);
   const int64_t cgrid = int64_t(B) * Hkv * c.nkt * c.n_chunk;
-  QMOE_REQUIRE(grid < (1ll << 31) && cgrid < (1ll << 31), "%s: grid too large", fn);
+  QMOE_REQUIRE(grid < (1ll << 31) && cgrid < (1ll << 31) && int64_t(B) * Hkv * c.nkt * (CS_KEYS / 64) < (1ll << 31),
+               "%s: grid too large", fn);
   a.q = c.q = q;
   a.k = c.k = k_cache;
   a.v = v_cache;
@@ -757,7 +759,7 @@ extern "C" int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_c
   if (int rc = ar_launch(fn, a, grid, as_stream(stream))) return rc;
   hipLaunchKernelGGL(attn_colsum_kernel, dim3(unsigned(cgrid)), dim3(256), 0, as_stream(stream), c);
   if (int rc = hip_status(fn)) return rc;
-  hipLaunchKernelGGL(attn_colsum_add_kernel, dim3(unsigned(c.nkt * (CS_KEYS / 64)), unsigned(B * Hkv)), dim3(256),
-                     0, as_stream(stream), c);
+  hipLaunchKernelGGL(attn_colsum_add_kernel, dim3(unsigned(int64_t(B) * Hkv * c.nkt * (CS_KEYS / 64))),
+                     dim3(256), 0, as_stream(stream), c);
   return hip_status(fn);
 }

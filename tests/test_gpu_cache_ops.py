@@ -89,6 +89,11 @@ SHARED = [
     (2, 43, 130, 130, 60, 12, 4, [3, 17], None),
     (1, 130, 70, 70, 140, 8, 8, [5], None),
     (2, 9, 300, 300, 20, 64, 4, [1, 12], None),
+    # a prefix that is attended in tiles (more than 65536 keys over the blocks of 32 rows)
+    (70, 1, 2001, 2100, 40, 16, 1, [(3 * i) % 41 for i in range(70)], None),
+    (20, 3, 4511, 4511, 50, 32, 4, [1 + 2 * i for i in range(20)], None),
+    (9, 15, 2003, 2003, 30, 8, 1, [1 + (5 * i) % 16 for i in range(9)], None),   # and own keys in tiles
+    (1, 60, 1111, 1111, 300, 2, 2, [200], None),                                # one head, 60 queries
 ]
 
 
@@ -188,6 +193,11 @@ SCORED = [
     (5, 200, 8, 8, [200, 1, 0, 64, 65], None),
     (5, 200, 12, 4, [200, 1, 0, 64, 65], None),
     (40, 130, 16, 4, [(9 * i) % 131 for i in range(40)], None),
+    # four waves a workgroup (more than 512 waves' keys in all)
+    (33, 300, 32, 4, [(29 * i) % 301 for i in range(33)], None),
+    (9, 1000, 64, 4, [0, 1000, 257, 256, 64, 1, 999, 512, 300], None),
+    (20, 500, 8, 8, [(53 * i) % 501 for i in range(20)], 480),
+    (15, 800, 12, 4, [(97 * i) % 801 for i in range(15)], None),
 ]
 
 
@@ -292,6 +302,9 @@ EVICT = [
     (1, 2, 5000, [4999], 3000, 64, 4, "special"),        # infinities, NaN, zeros of both signs, negatives
     (3, 4, 90, [-4, 2_000_000_000, 90], 40, 5, 2, "spread"),
     (1, 8, 128, [128], 1000, 10, 4, "spread"),           # a budget past the capacity
+    (1, 2, 9000, [8765], 300, 64, 4, "special"),         # 16 slots a thread
+    (1, 2, 2000, [1999], 1700, 0, 0, "equal"),           # in place: 299 rows move in a launch of their own
+    (2, 2, 1500, [1500, 1300], 1250, 40, 4, "few"),      # in place: the selection moves them
 ]
 
 
@@ -346,9 +359,11 @@ def test_kv_evict(dev, case, place):
             assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
-def test_kv_evict_past_the_ranks_in_lds(dev):
-    """More entries than the selection holds in LDS: sorted by torch instead of by lists."""
-    B, Hkv, n, budget, recent, sink = 1, 2, 40_001, 20_000, 100, 4
+@pytest.mark.parametrize("n,budget", [(16_384, 5000), (20_001, 19_000), (40_001, 20_000)])
+def test_kv_evict_of_long_caches(dev, n, budget):
+    """As many entries as threads hold in registers, more (ranks in LDS), and more
+    than that holds: sorted by torch instead of by lists."""
+    B, Hkv, recent, sink = 1, 2, 100, 4
     announce(f"kv_evict n={n}")
     g = _gen(dev, 5)
     k, v = bf16_randn((B, Hkv, n, D), g, dev), bf16_randn((B, Hkv, n, D), g, dev)
