@@ -94,6 +94,17 @@ class KVCache:
         return (self.k, self.v)[i]
 
 
+def check_budget(budget: int, recent: int, sink: int, slack: int = 1) -> None:
+    if budget <= 0 or recent < 0 or sink < 0 or recent + sink > budget or slack < 1:
+        raise ValueError(f"need 0 <= recent + sink <= budget and at least one slot past it (budget={budget}, "
+                         f"recent={recent}, sink={sink}, slack={slack})")
+
+
+def default_recent(budget: int, sink: int) -> int:
+    """A quarter of the budget, and no more than the sinks leave of it."""
+    return max(0, min(budget // 4, budget - sink))
+
+
 class CacheBudget:
     """What the bounded caches of all layers have in common: how many entries a
     row keeps (``budget``: the first ``sink`` positions, the ``recent`` last
@@ -105,9 +116,7 @@ class CacheBudget:
     so no step has to ask the device.  ``lengths`` are a prompt's real tokens."""
 
     def __init__(self, B: int, budget: int, recent: int, sink: int, slack: int, device):
-        if budget <= 0 or recent < 0 or sink < 0 or recent + sink > budget or slack < 1:
-            raise ValueError(f"need 0 <= recent + sink <= budget and at least one slot past it (budget={budget}, "
-                             f"recent={recent}, sink={sink}, slack={slack})")
+        check_budget(budget, recent, sink, slack)
         self.budget, self.recent, self.sink, self.capacity = budget, recent, sink, budget + slack
         self.slots = torch.zeros(B, dtype=torch.int32, device=device)
         self.ctx = torch.ones(B, dtype=torch.int32, device=device)

@@ -33,7 +33,8 @@ from typing import Any, Callable, Dict, List, Optional
 import torch
 
 from . import _lib, ops, weights
-from .attention import Attention, BoundedKVCache, CacheBudget, KVCache, SharedPrefix, rope_tables
+from .attention import (Attention, BoundedKVCache, CacheBudget, KVCache, SharedPrefix, check_budget, default_recent,
+                        rope_tables)
 from .config import Qwen3MoeShape
 from .moe import MoEBlock
 
@@ -71,8 +72,9 @@ class MoENeuronConfig:
         # the most accumulated attention weight; kv_cache_slack decode steps run
         # between evictions
         self.kv_cache_budget = int(kwargs.pop("kv_cache_budget", 0))
-        self.kv_cache_recent = int(kwargs.pop("kv_cache_recent", self.kv_cache_budget // 4))
         self.kv_cache_sink = int(kwargs.pop("kv_cache_sink", min(4, self.kv_cache_budget)))
+        self.kv_cache_recent = int(kwargs.pop("kv_cache_recent", default_recent(self.kv_cache_budget,
+                                                                                self.kv_cache_sink)))
         self.kv_cache_slack = int(kwargs.pop("kv_cache_slack", 64))
         if self.kv_cache_budget < 0:
             raise ValueError("kv_cache_budget must be >= 0")
@@ -362,14 +364,16 @@ class NeuronQwen3MoeModel:
         ``budget`` entries a kv head, if that is fewer) the prefix of every
         row's cache; an empty ``input_ids`` takes the prefix away."""
         P, dev, c = input_ids.shape[1], self.embed_tokens.device, self.config
+        if P >= self.rope_full[0].shape[0]:
+            raise ValueError(f"a prefix of {P} tokens leaves no position of {self.rope_full[0].shape[0]} to continue at")
+        if budget:
+            check_budget(budget, recent, sink)
         own = self.caches()
         for cache in own:
             cache.prefix = None
         self.base, self.rope = 0, self.rope_full
         if P == 0:
             return
-        if P >= self.rope_full[0].shape[0]:
-            raise ValueError(f"a prefix of {P} tokens leaves no position of {self.rope_full[0].shape[0]} to continue at")
         n = P
         if 0 < budget < P:
             state = CacheBudget(1, budget, recent, sink, 1, dev)
@@ -382,6 +386,7 @@ class NeuronQwen3MoeModel:
             for l, cache in zip(self.layers, made):
                 l.cache = cache
             self.hidden(input_ids.to(dev), torch.arange(P, dtype=torch.int32, device=dev), 1, P, 0)
+            self.check_embed()
         finally:
             for l, cache in zip(self.layers, own):
                 l.cache = cache
@@ -645,7 +650,8 @@ class NeuronQwen3MoeForCausalLM:
         ``sink``, the ``recent`` last ones (default a quarter of the budget)
         and those that got the most attention weight within the prefix.  The
         embedding and the layers run as for any prompt; :meth:`drop_prefix`
-        takes the prefix away."""
+        takes the prefix away.  Sizes that do not fit are refused and change
+        nothing; a token outside the vocabulary leaves no prefix at all."""
         if self.model is None:
             raise RuntimeError("load() the model first")
         if self.model.budget is not None:
@@ -654,10 +660,12 @@ class NeuronQwen3MoeForCausalLM:
         ids = prefix_ids.reshape(1, -1)
         if prefix_ids.dim() > 2 or (prefix_ids.dim() == 2 and prefix_ids.shape[0] != 1) or ids.shape[1] == 0:
             raise ValueError("prefix_ids must be [P] or [1, P] with P > 0")
-        self._graphs.clear()  # captured steps hold the old prefix's addresses
-        self.model.set_prefix(ids, int(budget), int(budget) // 4 if recent is None else int(recent),
-                              min(int(sink), int(budget)))
-        self.model.check_embed()
+        budget, sink = int(budget), min(int(sink), int(budget))
+        recent = default_recent(budget, sink) if recent is None else int(recent)
+        try:
+            self.model.set_prefix(ids, budget, recent, sink)
+        finally:
+            self._graphs.clear()  # captured steps hold the old prefix's addresses
         self.reset()
 
     def drop_prefix(self) -> None:

@@ -182,3 +182,12 @@ def test_config_of_the_budget():
     assert (c.kv_cache_budget, c.kv_cache_recent, c.kv_cache_sink) == (0, 0, 0)
     with pytest.raises(ValueError, match="kv_cache_budget"):
         MoENeuronConfig(kv_cache_budget=-1)
+
+
+def test_default_split_of_small_budgets():
+    from qmoe.attention import check_budget
+    from qmoe.model import MoENeuronConfig
+
+    for budget in range(1, 40):
+        c = MoENeuronConfig(kv_cache_budget=budget)
+        check_budget(budget, c.kv_cache_recent, c.kv_cache_sink)

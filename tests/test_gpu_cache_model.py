@@ -415,3 +415,29 @@ def test_model_bounded_cache_one_token_prompt(dev):
     assert b.model.budget.used == [2, 2] and b.model.caches()[0].slot_pos[:, :, :2].tolist() == [[[0, 1]] * HKV] * 2
     with pytest.raises(ValueError, match="hold 2 rows"):
         b.prefill(_tokens(1, 3, 4))
+
+
+def test_model_prefix_refused_changes_nothing(dev):
+    """Sizes that do not fit leave the old prefix as it was; tokens outside the
+    vocabulary leave none; the smallest budgets work with the default split."""
+    announce("refused prefixes")
+    m = _model(2, 60)
+    prefix, prompts = _tokens(1, 20), _tokens(2, 2, 6)
+    m.share_prefix(prefix)
+    want = m.prefill(prompts)
+    for bad in (dict(budget=-3), dict(budget=10, recent=-1), dict(budget=10, recent=8, sink=3),
+                dict(budget=30, recent=28, sink=3)):
+        with pytest.raises(ValueError, match="recent \\+ sink"):
+            m.share_prefix(_tokens(3, 20), **bad)
+    with pytest.raises(ValueError, match="no position"):
+        m.share_prefix(_tokens(3, 61))
+    assert m.model.base == 20 and torch.equal(m.prefill(prompts), want)
+    for budget in (1, 4, 5):
+        m.share_prefix(prefix, budget=budget)
+        assert m.model.caches()[0].prefix.length == budget
+    m.drop_prefix()
+    plain = m.prefill(prompts)
+    m.share_prefix(prefix)
+    with pytest.raises(ValueError, match="token id"):
+        m.share_prefix(torch.full((8,), 5000))
+    assert m.model.base == 0 and torch.equal(m.prefill(prompts), plain)
