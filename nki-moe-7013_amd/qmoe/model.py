@@ -635,9 +635,11 @@ class NeuronQwen3MoeForCausalLM:
         return random_params(self.config, self.device, seed=self.neuron_config.seed)
 
     def reset(self):
-        """Start a new sequence (the KV cache is overwritten from position 0; a
-        shared prefix stays)."""
+        """Start a new sequence (the KV cache is overwritten from position 0,
+        bounded ones are empty again; a shared prefix stays)."""
         self.position = 0
+        if self.model is not None and self.model.budget is not None:
+            self.model.budget.begin([0] * len(self.model.budget.used))
 
     # -- shared prefix -----------------------------------------------------------
     def share_prefix(self, prefix_ids: torch.Tensor, budget: int = 0, recent: Optional[int] = None,
@@ -675,6 +677,13 @@ class NeuronQwen3MoeForCausalLM:
             self.model.set_prefix(torch.empty(1, 0, dtype=torch.long))
             self.reset()
 
+    def _budget_of(self, B: int) -> Optional[CacheBudget]:
+        """The bounded caches' state, if there are any (they hold a fixed number of rows)."""
+        budget = self.model.budget
+        if budget is not None and B != len(budget.used):
+            raise ValueError(f"the bounded caches hold {len(budget.used)} rows (got {B})")
+        return budget
+
     def _contiguous(self) -> bool:
         return self.model.budget is None and not self.model.base
 
@@ -687,10 +696,8 @@ class NeuronQwen3MoeForCausalLM:
         B, S = input_ids.shape
         dev = self.device
         pos = torch.arange(S, device=dev, dtype=torch.int32).repeat(B)
-        budget = self.model.budget
+        budget = self._budget_of(B)
         if budget is not None:
-            if B != len(budget.used):
-                raise ValueError(f"the bounded caches hold {len(budget.used)} rows (got {B})")
             # a single token is a decode step into empty caches
             budget.begin([S] * B if lengths is None else [int(n) for n in lengths]) if S > 1 else budget.begin([0] * B)
         h = self.model.hidden(input_ids.to(dev), pos, B, S, 0)
@@ -709,13 +716,13 @@ class NeuronQwen3MoeForCausalLM:
         position for every row); returns ``[B, V]`` logits."""
         B = token_ids.shape[0]
         dev = self.device
+        budget = self._budget_of(B)
         if positions is None:
             pos = torch.full((B,), self.position, device=dev, dtype=torch.int32)
             self.position += 1
         else:
             pos = positions.to(device=dev, dtype=torch.int32).contiguous()
             self.position = int(pos.max()) + 1
-        budget = self.model.budget
         if budget is not None:
             budget.make_room(self.model.caches())
         h = self.model.hidden(token_ids.to(dev).view(B, 1), pos, B, 1, 0)
@@ -741,6 +748,7 @@ class NeuronQwen3MoeForCausalLM:
         position += 1) is one replay.  Returns ``[B, n_steps]`` token ids."""
         use_graph = self.neuron_config.use_hip_graphs if use_graph is None else use_graph
         B = first_token.shape[0]
+        budget = self._budget_of(B)
         if positions is None:
             positions = torch.full((B,), self.position, dtype=torch.int32)
         pos0 = positions.to(device=self.device, dtype=torch.int32).view(B)
@@ -757,7 +765,6 @@ class NeuronQwen3MoeForCausalLM:
         st["tok"].copy_(first_token.to(self.device).view(B).long())
         st["pos"].copy_(pos0)
         out = torch.empty(B, n_steps, dtype=torch.long, device=self.device)
-        budget = self.model.budget
         for i in range(n_steps):
             ctx = top + i + 1
             if budget is not None:

@@ -441,3 +441,23 @@ def test_model_prefix_refused_changes_nothing(dev):
     with pytest.raises(ValueError, match="token id"):
         m.share_prefix(torch.full((8,), 5000))
     assert m.model.base == 0 and torch.equal(m.prefill(prompts), plain)
+
+
+def test_model_bounded_cache_starts_over(dev):
+    """Steps after reset() see nothing of the sequence before, and another number
+    of rows is refused before anything changes, for eager and captured steps."""
+    announce("bounded caches start over")
+    m = _model(2, 40, kv_cache_budget=16, kv_cache_slack=3)
+    a, b = _tokens(1, 2), _tokens(2, 2)
+    first = [m.decode_step(a), m.decode_step(b)]
+    m.prefill(_tokens(3, 2, 12))
+    m.decode_step(a)
+    m.reset()
+    assert m.model.budget.used == [0, 0]
+    assert torch.equal(m.decode_step(a), first[0]) and torch.equal(m.decode_step(b), first[1])
+    for call in (lambda: m.decode_step(_tokens(4, 3)), lambda: m.greedy_decode(_tokens(4, 3), 2),
+                 lambda: m.greedy_decode(_tokens(4, 1), 2, use_graph=False)):
+        with pytest.raises(ValueError, match="hold 2 rows"):
+            call()
+    st = m.model.budget
+    assert st.used == [2, 2] and st.slots.tolist() == [2, 2] and st.ctx.tolist() == [3, 3] and m.position == 2
