@@ -87,7 +87,8 @@ typedef void* qmoe_stream_t;
  * qmoe_attn_prefill_ws / qmoe_attn_prefill_workspace are new.  Entry points
  * added since leave the earlier ones as they were: qmoe_attn_shared,
  * qmoe_attn_prefill_scored, qmoe_attn_decode_scored, qmoe_kv_append,
- * qmoe_kv_evict and their workspace queries. */
+ * qmoe_kv_evict and their workspace queries.  All but qmoe_kv_append
+ * refuse bf16 tensors and attention workspaces that are not 16-byte aligned. */
 #define QMOE_VERSION 3
 
 int qmoe_version(void);

@@ -689,6 +689,8 @@ extern "C" int qmoe_attn_shared(const qmoe_bf16* q, const qmoe_bf16* k_prefix, c
   const int64_t need = ar_part_bytes(a);
   QMOE_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: workspace of %lld bytes, need %lld", fn,
                (long long)workspace_bytes, (long long)need);
+  QMOE_REQUIRE(aligned16(q, k_prefix, v_prefix, k_cache, v_cache, a.part, out), "%s: operands must be 16-byte aligned",
+               fn);
   return ar_launch(fn, a, grid, as_stream(stream));
 }
 
@@ -747,6 +749,8 @@ extern "C" int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_c
   const int64_t cgrid = int64_t(B) * Hkv * c.nkt * c.n_chunk;
   QMOE_REQUIRE(grid < (1ll << 31) && cgrid < (1ll << 31) && int64_t(B) * Hkv * c.nkt * (CS_KEYS / 64) < (1ll << 31),
                "%s: grid too large", fn);
+  QMOE_REQUIRE(aligned16(q, k_cache, v_cache, static_cast<uint8_t*>(workspace), out),
+               "%s: operands must be 16-byte aligned", fn);
   a.q = c.q = q;
   a.k = c.k = k_cache;
   a.v = v_cache;

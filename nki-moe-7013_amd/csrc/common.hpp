@@ -30,6 +30,12 @@ inline int hip_status(const char* where) {
     if (!(cond)) return ::qmoe::fail(QMOE_ERR_INVALID, __VA_ARGS__); \
   } while (0)
 
+// 16-byte loads, stores and LDS-DMA need it (nullptr counts as aligned).
+template <class... P>
+inline bool aligned16(const P*... p) {
+  return (((reinterpret_cast<uintptr_t>(p) & 15) == 0) && ...);
+}
+
 inline hipStream_t as_stream(qmoe_stream_t s) { return reinterpret_cast<hipStream_t>(s); }
 
 // ---------------------------------------------------------------- types

@@ -837,6 +837,8 @@ extern "C" int qmoe_attn_decode_scored(const qmoe_bf16* q, const qmoe_bf16* k_ca
                (long long)workspace_bytes, (long long)need);
   const int64_t n_merge = (B * Hq + 3) / 4, slices = (ns * split + SD_SLICE - 1) / SD_SLICE;
   QMOE_REQUIRE(n_merge + B * Hkv * slices < (1ll << 31), "%s: grid too large", fn);
+  QMOE_REQUIRE(aligned16(q, k_cache, v_cache, static_cast<uint8_t*>(workspace), out),
+               "%s: operands must be 16-byte aligned", fn);
   SdArgs a{q, k_cache, v_cache, ctx_len, int(B), int(Hq), int(Hkv), int(S_max), int(max_ctx), int(split), int(ns),
            int(ns * split), scale * 1.4426950408889634f, static_cast<float*>(workspace),
            static_cast<float*>(workspace) + B * Hq * ns * SD_REC, scores, out, int(n_merge)};
@@ -894,6 +896,7 @@ extern "C" int qmoe_kv_evict(const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
   const int64_t need = qmoe_kv_evict_workspace(B, Hkv, S_max, budget);
   QMOE_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %lld bytes, need %lld", fn,
                (long long)workspace_bytes, (long long)need);
+  QMOE_REQUIRE(aligned16(k_cache, v_cache, k_out, v_out), "%s: the caches must be 16-byte aligned", fn);
   int32_t* src = static_cast<int32_t*>(workspace);
   const int lds_keys = int(std::min<int64_t>(S_max, EV_LDS_KEYS));
   EvArgs e{scores, slot_pos, ctx_len, int(B), int(Hkv), int(S_max), int(budget),

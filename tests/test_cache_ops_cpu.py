@@ -67,6 +67,15 @@ REFUSED = [
     (evict, dict(S_out=63), "exactly this one"), (evict, dict(v2=8), "exactly this one"),
     (evict, dict(sp2=8), "exactly this one"), (evict, dict(n=1000), "workspace"), (evict, dict(ws=NONE), "workspace"),
 ]
+# addresses that no load of 16 bytes may take, everything else in order
+A = 1 << 20
+for _fn, _names, _rest in (
+        (shared, ("q", "kp", "vp", "k", "v", "out", "ws"), dict(n=A)),
+        (prompt, ("q", "k", "v", "out", "ws"), dict(n=A)),
+        (scored, ("q", "k", "v", "out", "ws"), dict(n=A)),
+        (evict, ("k", "v", "k2", "v2"), dict(sc2=9, sp2=10))):
+    _good = {name: (i + 1) * A for i, name in enumerate(_names)}
+    REFUSED += [(_fn, {**_good, **_rest, name: _good[name] + 8}, "16-byte aligned") for name in _names]
 
 
 @pytest.mark.parametrize("fn,change,msg", REFUSED, ids=lambda x: getattr(x, "__name__", None) or str(x)[:40])
