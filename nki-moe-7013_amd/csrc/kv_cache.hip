@@ -74,7 +74,7 @@ __global__ __launch_bounds__(64) void kv_append_kernel(
 constexpr int SD_KEYS = 64;       // keys of a wave
 constexpr int SD_WAVES = 4;       // waves of a workgroup, at most; their runs are joined in LDS
 constexpr int SD_SLICE = 256;     // keys whose scores a workgroup of the finish adds to
-constexpr int SD_REC = HD + 4;    // record: m, l, 2 pad, O[HD]
+constexpr int SD_REC = HD + 4;    // LDS record of a wave: m, l, 2 pad, O[HD]
 constexpr int SD_MAX_G = 16;
 constexpr int SD_VCH = SD_KEYS * HD / 8 / 64;  // 16-byte V chunks of a lane
 
@@ -83,7 +83,8 @@ struct SdArgs {
   const int32_t* ctx_len;
   int B, Hq, Hkv, S_max, max_ctx, split, nsplit, ldl;  // split: keys of a workgroup; ldl: logits of a row
   float scale_log2;
-  float* part;    // [B][Hq][nsplit][SD_REC]
+  float* ml;      // [B][Hq][nsplit][2]: a split's maximum and sum
+  float* part;    // [B][Hq][nsplit][HD]: its unnormalised output
   float* logits;  // [B][Hq][ldl], in log2 units
   float* scores;  // [B][Hkv][S_max]
   uint16_t* out;
@@ -116,20 +117,44 @@ __global__ __launch_bounds__(WAVES * 64) void attn_scored_kernel(const SdArgs a)
   for (int db = 0; db < 4; ++db) oacc[db] = f32x16{};
   if (nk > 0) {  // wave-uniform
     const int64_t base = (int64_t(b) * a.Hkv + kvh) * a.S_max + kw0;
+    // ka[mb][ks]: one wave, the A operand itself; four waves, chunk lane + 64 (8 mb + ks) of
+    // the tile, as V's (rows past nk repeat the last one, their p is 0)
     u32x4 ka[2][HD / 16], vr[SD_VCH], qb[HD / 16];
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb) {
       const uint16_t* kp = a.k + (base + min(mb * 32 + col, nk - 1)) * HD + hi * 8;
 #pragma unroll
-      for (int ks = 0; ks < HD / 16; ++ks) ka[mb][ks] = ld16(kp + ks * 16);
+      for (int ks = 0; ks < HD / 16; ++ks) {
+        if constexpr (WAVES == 1) {
+          ka[mb][ks] = ld16(kp + ks * 16);
+        } else {
+          const int c = lane + 64 * (8 * mb + ks);
+          ka[mb][ks] = ld16(a.k + (base + min(c >> 4, nk - 1)) * HD + (c & 15) * 8);
+        }
+      }
     }
     const uint16_t* qp = a.q + (int64_t(b) * a.Hq + kvh * G + min(col, G - 1)) * HD + hi * 8;
 #pragma unroll
     for (int ks = 0; ks < HD / 16; ++ks) qb[ks] = ld16(qp + ks * 16);
 #pragma unroll
-    for (int i = 0; i < SD_VCH; ++i) {  // rows past nk repeat the last one (their p is 0)
+    for (int i = 0; i < SD_VCH; ++i) {
       const int c = lane + 64 * i;
       vr[i] = ld16(a.v + (base + min(c >> 4, nk - 1)) * HD + (c & 15) * 8);
+    }
+    uint8_t* vb = vs[wave];
+    if constexpr (WAVES > 1) {
+#pragma unroll
+      for (int i = 0; i < SD_VCH; ++i) {
+        const int c = lane + 64 * i, r = c >> 4;
+        *reinterpret_cast<u32x4*>(vb + r * AP_ROWB + ap_kslot(r, c & 15) * 16) = ka[i >> 3][i & 7];
+      }
+      wave_lds_sync();
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int ks = 0; ks < HD / 16; ++ks)
+          ka[mb][ks] = *reinterpret_cast<const u32x4*>(vb + (mb * 32 + col) * AP_ROWB + ap_kslot(col, 2 * ks + hi) * 16);
+      wave_lds_sync();
     }
     f32x16 sc[2];
 #pragma unroll
@@ -169,7 +194,6 @@ __global__ __launch_bounds__(WAVES * 64) void attn_scored_kernel(const SdArgs a)
         pk[mb][i] = __builtin_bit_cast(uint32_t, pp);
       }
     l += __shfl_xor(l, 32, 64);
-    uint8_t* vb = vs[wave];
 #pragma unroll
     for (int i = 0; i < SD_VCH; ++i) {
       const int c = lane + 64 * i, r = c >> 4;
@@ -194,16 +218,17 @@ __global__ __launch_bounds__(WAVES * 64) void attn_scored_kernel(const SdArgs a)
       }
     }
   }
-  float* pbase = a.part + ((int64_t(b) * a.Hq + kvh * G) * a.nsplit + split) * SD_REC;
+  const int64_t rec0 = (int64_t(b) * a.Hq + kvh * G) * a.nsplit + split;  // q head c's: c * nsplit further
   if constexpr (WAVES == 1) {
     if (col < G) {
-      float* pg = pbase + int64_t(col) * a.nsplit * SD_REC;
-      if (hi == 0) *reinterpret_cast<float2*>(pg) = make_float2(m, l);
+      const int64_t at = rec0 + int64_t(col) * a.nsplit;
+      float* pg = a.part + at * HD;
+      if (hi == 0) *reinterpret_cast<float2*>(a.ml + at * 2) = make_float2(m, l);
 #pragma unroll
       for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int e4 = 0; e4 < 4; ++e4)
-          *reinterpret_cast<float4*>(pg + 4 + db * 32 + e4 * 8 + hi * 4) =
+          *reinterpret_cast<float4*>(pg + db * 32 + e4 * 8 + hi * 4) =
               make_float4(oacc[db][e4 * 4], oacc[db][e4 * 4 + 1], oacc[db][e4 * 4 + 2], oacc[db][e4 * 4 + 3]);
     }
     return;
@@ -238,19 +263,19 @@ __global__ __launch_bounds__(WAVES * 64) void attn_scored_kernel(const SdArgs a)
       L = fmaf(wt, r[1], L);
       O = fmaf(wt, r[4 + d], O);
     }
-    float* pg = pbase + int64_t(c) * a.nsplit * SD_REC;
-    if (d == 0) *reinterpret_cast<float2*>(pg) = make_float2(M, L);
-    pg[4 + d] = O;
+    const int64_t at = rec0 + int64_t(c) * a.nsplit;
+    if (d == 0) *reinterpret_cast<float2*>(a.ml + at * 2) = make_float2(M, L);
+    a.part[at * HD + d] = O;
   }
 }
 
 // Maximum and sum of a row's splits: lane i takes split i, i + 64, ...
-__device__ __forceinline__ void sd_row(const float* p, int live, int lane, float& M, float& L) {
+__device__ __forceinline__ void sd_row(const float* rec, int live, int lane, float& M, float& L) {
   M = -INFINITY;
   L = 0.0f;
   for (int c = 0; c < live; c += 64) {
     float2 ml = make_float2(-INFINITY, 0.0f);
-    if (c + lane < live) ml = *reinterpret_cast<const float2*>(p + int64_t(c + lane) * SD_REC);
+    if (c + lane < live) ml = *reinterpret_cast<const float2*>(rec + int64_t(c + lane) * 2);
     const float m = fmaxf(M, wave_max(ml.x));
     const float mz = m == -INFINITY ? 0.0f : m;
     L = L * __builtin_amdgcn_exp2f(M - mz) + wave_sum(ml.y * __builtin_amdgcn_exp2f(ml.x - mz));
@@ -266,18 +291,19 @@ __global__ __launch_bounds__(256) void attn_scored_finish_kernel(const SdArgs a)
     const int row = int(blockIdx.x) * 4 + wave;
     if (row >= a.B * a.Hq) return;
     const int live = (sd_ctx(a, row / a.Hq) + a.split - 1) / a.split;
-    const float* p = a.part + int64_t(row) * a.nsplit * SD_REC;
+    const float* p = a.part + int64_t(row) * a.nsplit * HD;
+    const float* rec = a.ml + int64_t(row) * a.nsplit * 2;
     float M, L;
-    sd_row(p, live, lane, M, L);
+    sd_row(rec, live, lane, M, L);
     float o0 = 0.0f, o1 = 0.0f;
     for (int i0 = 0; i0 < live; i0 += 8) {
       float2 v[8];
       float w[8];
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        const float* r = p + int64_t(min(i0 + u, live - 1)) * SD_REC;
-        v[u] = *reinterpret_cast<const float2*>(r + 4 + lane * 2);
-        w[u] = i0 + u < live ? r[0] : -INFINITY;
+        const int i = min(i0 + u, live - 1);
+        v[u] = *reinterpret_cast<const float2*>(p + int64_t(i) * HD + lane * 2);
+        w[u] = i0 + u < live ? rec[2 * i] : -INFINITY;
       }
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
@@ -298,7 +324,7 @@ __global__ __launch_bounds__(256) void attn_scored_finish_kernel(const SdArgs a)
   const int row0 = b * a.Hq + bh % a.Hkv * G;
   for (int g = wave; g < G; g += 4) {
     float M, L;
-    sd_row(a.part + int64_t(row0 + g) * a.nsplit * SD_REC, live, lane, M, L);
+    sd_row(a.ml + int64_t(row0 + g) * a.nsplit * 2, live, lane, M, L);
     if (lane == 0) {
       sm[g] = M;
       si[g] = L > 0.0f ? 1.0f / L : 0.0f;
@@ -806,7 +832,7 @@ static int64_t sd_split(int64_t B, int64_t Hkv, int64_t max_ctx) {
 }
 static int64_t sd_bytes(int64_t B, int64_t Hq, int64_t max_ctx, int64_t split) {
   const int64_t n = (max_ctx + split - 1) / split;
-  return B * Hq * n * (SD_REC + split) * int64_t(sizeof(float));
+  return B * Hq * n * (2 + HD + split) * int64_t(sizeof(float));
 }
 
 // (for the split that takes more, so that the size does not hang on Hkv)
@@ -839,9 +865,11 @@ extern "C" int qmoe_attn_decode_scored(const qmoe_bf16* q, const qmoe_bf16* k_ca
   QMOE_REQUIRE(n_merge + B * Hkv * slices < (1ll << 31), "%s: grid too large", fn);
   QMOE_REQUIRE(aligned16(q, k_cache, v_cache, static_cast<uint8_t*>(workspace), out),
                "%s: operands must be 16-byte aligned", fn);
+  const int64_t recs = B * Hq * ns;  // 16-byte pieces first: outputs, logits, then (m, l)
+  float* f = static_cast<float*>(workspace);
   SdArgs a{q, k_cache, v_cache, ctx_len, int(B), int(Hq), int(Hkv), int(S_max), int(max_ctx), int(split), int(ns),
-           int(ns * split), scale * 1.4426950408889634f, static_cast<float*>(workspace),
-           static_cast<float*>(workspace) + B * Hq * ns * SD_REC, scores, out, int(n_merge)};
+           int(ns * split), scale * 1.4426950408889634f, f + recs * (HD + split), f, f + recs * HD, scores, out,
+           int(n_merge)};
   const dim3 grid{unsigned(ns), unsigned(Hkv), unsigned(B)};
   if (split == SD_KEYS)
     hipLaunchKernelGGL(attn_scored_kernel<1>, grid, dim3(64), 0, as_stream(stream), a);
