@@ -29,6 +29,7 @@ namespace qmoe {
 // ====================================================================== append
 // One wave a (head, token): lane l holds elements l and l + 64, which RoPE pairs.
 // v / sqrt(mean(v^2) + eps) * w, then the rotation by the position's (cos, sin).
+// Bound by its one chain of memory round trips (1 row 2.5 us, 64 rows 2.9).
 __global__ __launch_bounds__(64) void kv_append_kernel(
     const float* __restrict__ raw, const uint16_t* __restrict__ qn_w, const uint16_t* __restrict__ kn_w,
     const float* __restrict__ rope_cos, const float* __restrict__ rope_sin, const int32_t* __restrict__ positions,
@@ -94,13 +95,16 @@ struct SdArgs {
 __device__ __forceinline__ int sd_ctx(const SdArgs& a, int b) { return min(max(a.ctx_len[b], 0), a.max_ctx); }
 
 // Workgroup = (split of WAVES x 64 keys, kv head, row), wave = 64 of its keys with
-// the G q heads in the columns of S^T = K . Q^T and O^T = V^T . P^T.  K rows go
-// from the cache straight into A-operand registers, V through the wave's own
-// LDS tile; every load of a wave is in flight at once, so a wave costs one
-// round trip to memory.  The logits leave as four consecutive keys a lane.
-// WAVES = 1 (few keys in all): the join of four waves is two barriers and a
-// round through LDS longer, and the finish has no more records than it can take
-// at once.
+// the G q heads in the columns of S^T = K . Q^T and O^T = V^T . P^T.  Every load of
+// a wave is in flight at once, so a wave costs one round trip to memory; K and
+// V take turns in the wave's own LDS tile.  The logits leave as four
+// consecutive keys a lane.  Bound by memory: 32 rows of up to 4160 entries, 171 MB,
+// in 39 us (4.4 TB/s); 44 us with K's A operands loaded straight from the cache, 32
+// bytes of each of 32 rows an instruction.
+// WAVES = 1 (few keys in all): K does go straight into its operands, since the
+// round through LDS is longer than what whole rows save (one row of 1100: 8.4 us, 8.7
+// with it), there is no join of four waves, which is two barriers longer, and the
+// finish has no more records than it can take at once.
 template <int WAVES>
 __global__ __launch_bounds__(WAVES * 64) void attn_scored_kernel(const SdArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t vs[WAVES][AP_TILE];
@@ -269,7 +273,9 @@ __global__ __launch_bounds__(WAVES * 64) void attn_scored_kernel(const SdArgs a)
   }
 }
 
-// Maximum and sum of a row's splits: lane i takes split i, i + 64, ...
+// Maximum and sum of a row's splits: lane i takes split i, i + 64, ...  Every
+// workgroup of the finish reads them, so they lie apart from the outputs (one row
+// of 131072: 106 us, 129 with each pair in front of its output).
 __device__ __forceinline__ void sd_row(const float* rec, int live, int lane, float& M, float& L) {
   M = -INFINITY;
   L = 0.0f;
@@ -285,6 +291,8 @@ __device__ __forceinline__ void sd_row(const float* rec, int live, int lane, flo
 
 // Workgroups [0, n_merge): a wave joins one (row, q head).  The rest: 256 keys of
 // a (row, kv head), a thread a key, scores += sum over the group of 2^(s - m) / l.
+// 32 rows of up to 4160: 7.5 us, of which the logits' 11 MB are about 3; one row of
+// 1100, two round trips: 4.4.
 __global__ __launch_bounds__(256) void attn_scored_finish_kernel(const SdArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, G = a.Hq / a.Hkv;
   if (int(blockIdx.x) < a.n_merge) {

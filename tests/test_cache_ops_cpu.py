@@ -106,9 +106,9 @@ def test_workspace_queries():
     assert l.qmoe_attn_prefill_scored_workspace(1, 5, 32, 4, 128, 0) >= 5 * 32 * 4
     for bad in [(1, 5, 32, 4, 128, -1), (1, -5, 32, 4, 128, 0), (1, 5, 32, 4, 128, 1 << 22), (1, 5, 32, 3, 128, 0)]:
         assert l.qmoe_attn_prefill_scored_workspace(*bad) == -1, bad
-    # a record of 132 floats and its logits for each split: five of 64 keys, or 17 of 256
-    assert l.qmoe_attn_decode_scored_workspace(3, 32, 128, 257) == 3 * 32 * 5 * (132 + 64) * 4
-    assert l.qmoe_attn_decode_scored_workspace(3, 32, 128, 4200) == 3 * 32 * 17 * (132 + 256) * 4
+    # 128 outputs, a maximum, a sum and the logits of each split: five of 64 keys, or 17 of 256
+    assert l.qmoe_attn_decode_scored_workspace(3, 32, 128, 257) == 3 * 32 * 5 * (130 + 64) * 4
+    assert l.qmoe_attn_decode_scored_workspace(3, 32, 128, 4200) == 3 * 32 * 17 * (130 + 256) * 4
     assert l.qmoe_attn_decode_scored_workspace(3, 32, 64, 257) == -1
     assert l.qmoe_attn_decode_scored_workspace(3, 32, 128, -1) == -1
     assert l.qmoe_kv_evict_workspace(2, 4, 100, 50) == 2 * 2 * 4 * 50 * 4
