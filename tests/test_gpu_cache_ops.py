@@ -493,3 +493,81 @@ def test_empty_batches_and_given_workspaces(dev):
     ops.kv_evict(*x, n, 100, 5, 2)
     ops.kv_evict(*y, n, 100, 5, 2, workspace=ops.kv_evict_workspace(3, 4, 300, 100, dev))
     assert all(torch.equal(s, t) for s, t in zip(x, y))
+
+
+def test_offsets_past_32_bits(dev):
+    """Caches of 2^32 elements (8.6 GB): the last row's last head sits behind
+    2^31 elements, and the longest run of keys that a call takes is 2^30 bytes.
+    The keys of the last group's heads are planted at the far end: a logit of 2
+    |q|^2 / sqrt(D) >= 60 against 4 million others of standard deviation 2 (at
+    most 14 in all likelihood, together below e^(14 + 16)), so the output is that entry's
+    value but for e^-30 and the rounding of its weight and its own."""
+    announce("caches past 32-bit offsets")
+    B, Hq, Hkv, n = 2, 32, 4, 1 << 22
+    if torch.cuda.get_device_properties(dev).total_memory < 64 << 30:
+        pytest.skip("needs 40 GB")
+    g = _gen(dev, 77)
+    k, v = [torch.empty(B, Hkv, n, D, dtype=torch.bfloat16, device=dev).normal_(generator=g) for _ in range(2)]
+    q = bf16_randn((1, Hq, D), g, dev, 2.0).expand(B, Hq, D).contiguous()
+    assert float((q[0].double() ** 2).sum(1).min()) * 2 * SCALE >= 60
+    heads, far = range(Hq - 8, Hq), [n - 40 - 3 * i for i in range(8)]
+    for b in range(B):
+        k[b, 3, far] = 2 * q[b, Hq - 8:]
+    sc = torch.zeros(B, Hkv, n, device=dev)
+
+    def at_far(got, b, what):  # got [8, D]
+        want = v[b, 3, far].double()
+        _within(got, want, want.abs() * 2 * ref.HALF_BF16 + 1e-9, what)
+
+    out = ops.attn_decode_scored(q, k, v, _i32([n, n - 1], dev), sc).view(B, Hq, D)
+    for b in range(B):
+        at_far(out[b, heads[0]:], b, f"scored, row {b}")
+        assert bool(((sc[b, 3, far].double() - 1).abs() <= 1e-5).all())
+    sc.zero_()
+    ctx = [300, 257]
+    out = ops.attn_decode_scored(q, k, v, _i32(ctx, dev), sc, max_ctx=300).view(B, Hq, D)
+    for b, c in enumerate(ctx):
+        sees = torch.ones(1, c, dtype=torch.bool, device=dev)
+        add, off = 0, 0
+        for h in heads:
+            o, e, w, rel = ref.attend(q[b, h:h + 1], k[b, 3, :c], v[b, 3, :c], sees, SCALE)
+            _within(out[b, h:h + 1], o, e, f"scored {c}, head {h}")
+            add, off = add + w[0], off + w[0] * (rel + 64 * ref.F32)
+        _within(sc[b, 3, :c], add, off + 1e-30, "scores")
+        assert not bool(sc[b, 3, c:].any())
+    out = ops.attn_shared(q, k[1], v[1], k, v, _i32([100, 7], dev), B, 1, max_ctx=100).view(B, Hq, D)
+    for b in range(B):
+        at_far(out[b, heads[0]:], 1, f"prefix, row {b}")
+    out = ops.attn_shared(q, k[0, :, :50].contiguous(), v[0, :, :50].contiguous(), k, v, _i32([n, n], dev), B,
+                          1).view(B, Hq, D)
+    for b in range(B):
+        at_far(out[b, heads[0]:], b, f"own entries, row {b}")
+    S = 20
+    sc.zero_()
+    qc = bf16_randn((B * S, Hq, D), g, dev, 2.0).view(B, S, Hq, D)
+    qc[:, 7] = q
+    out = ops.attn_prefill_scored(qc.view(B * S, Hq, D), k, v, sc, B, S, n - S).view(B, S, Hq, D)
+    for b in range(B):
+        at_far(out[b, 7, heads[0]:], b, f"chunk, row {b}")
+        assert bool((sc[b, 3, far] >= 1 - 1e-5).all())  # and what the other queries gave them
+    # append to the last slot, then cut down to the best 1000
+    pos = torch.arange(n, dtype=torch.int32, device=dev).repeat(B, Hkv, 1)
+    raw = torch.randn(B, (Hq + 2 * Hkv) * D, generator=g, device=dev)
+    w, cos = torch.ones(D, dtype=torch.bfloat16, device=dev), torch.ones(8, D // 2, device=dev)
+    guard = k[1, 3, n - 2].clone()
+    ops.kv_append(raw, w, w, cos, torch.zeros_like(cos), _i32([3, 5], dev), _i32([n - 1, n - 1], dev), Hq, Hkv, k, v,
+                  1e-6, scores=sc, slot_pos=pos)
+    assert torch.equal(v[:, :, n - 1].reshape(B, -1), raw[:, (Hq + Hkv) * D:].bfloat16())
+    assert torch.equal(k[1, 3, n - 2], guard) and pos[:, :, n - 1].tolist() == [[3] * 4, [5] * 4]
+    assert not bool(sc[:, :, n - 1].any())
+    sc.copy_(torch.rand(B, Hkv, n, generator=g, device=dev))
+    keep = sc[1, 3].sort(descending=True, stable=True).indices[:1000].sort().values
+    rows = k[1, 3, keep].clone()
+    ops.kv_evict(k, v, sc, pos, _i32([n, n], dev), 1000)
+    stay = keep < 1000
+    order = torch.empty(1000, dtype=torch.long, device=dev)
+    hole = torch.ones(1000, dtype=torch.bool, device=dev)
+    hole[keep[stay]] = False
+    order[keep[stay]] = stay.nonzero()[:, 0]
+    order[hole] = (~stay).nonzero()[:, 0]
+    assert torch.equal(k[1, 3, :1000], rows[order]) and torch.equal(pos[1, 3, :1000].long(), keep[order])
