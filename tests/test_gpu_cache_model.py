@@ -461,3 +461,19 @@ def test_model_bounded_cache_starts_over(dev):
             call()
     st = m.model.budget
     assert st.used == [2, 2] and st.slots.tolist() == [2, 2] and st.ctx.tolist() == [3, 3] and m.position == 2
+
+
+@pytest.mark.parametrize("P", [1, 2, 17])
+def test_model_on_a_short_prefix(dev, P):
+    """A prefix of one token runs as a decode step, of two as a chunk, and prompts of
+    one token continue it as steps."""
+    announce(f"model on a prefix of {P}")
+    m = _model(2, 40)
+    prefix, steps = _tokens(1, P), [_tokens(3 + i, 2) for i in range(3)]
+    want = [m.prefill(torch.cat([prefix.expand(2, P), steps[0][:, None]], 1))]
+    want += [m.decode_step(t) for t in steps[1:]]
+    m.share_prefix(prefix)
+    got = [m.prefill(steps[0][:, None])] + [m.decode_step(t) for t in steps[1:]]
+    for i, (a, b) in enumerate(zip(got, want)):
+        _close(a, b, f"step {i}")
+    assert m.position == 3
