@@ -296,6 +296,10 @@ class Attention:
                 raise ValueError("the fused input norm takes one fp32 row on the GEMV path")
             if bounded and start != 0:
                 raise ValueError("a bounded cache takes a prompt from its first token on")
+            # past it qkv_norm_rope writes neither queries nor entries
+            limit = rope_cos.shape[0] if bounded else min(rope_cos.shape[0], cache.capacity)
+            if start < 0 or start + S > limit:
+                raise ValueError(f"need 0 <= start and start + S <= {limit} (start={start}, S={S})")
             n = ops.qkv_norm_rope_workspace(B * S, x.shape[1], self.n_q, self.n_kv, self.head_dim)
             ws = torch.empty(n // 4, dtype=torch.float32, device=x.device) if n > 0 else None
             own, scores, pos = cache.state.prompt_cache(self.n_kv, S, self.head_dim) if bounded else (cache, None, None)

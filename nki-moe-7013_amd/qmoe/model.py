@@ -684,6 +684,10 @@ class NeuronQwen3MoeForCausalLM:
             raise ValueError(f"the bounded caches hold {len(budget.used)} rows (got {B})")
         return budget
 
+    def _positions(self) -> int:
+        """Positions a sequence has (after a shared prefix): the rows of the RoPE tables."""
+        return self.model.rope[0].shape[0]
+
     def _contiguous(self) -> bool:
         return self.model.budget is None and not self.model.base
 
@@ -695,6 +699,11 @@ class NeuronQwen3MoeForCausalLM:
         end, so causal attention keeps them out of its real positions)."""
         B, S = input_ids.shape
         dev = self.device
+        # a bounded cache's scratch holds any prompt and a row's own cache is not
+        # shorter for a prefix in front of it, so no operator sees the limit
+        if S > self._positions():
+            raise ValueError(f"a prompt of {S} tokens does not fit the {self._positions()} positions there are"
+                             + (f" after a prefix of {self.model.base}" if self.model.base else ""))
         pos = torch.arange(S, device=dev, dtype=torch.int32).repeat(B)
         budget = self._budget_of(B)
         if budget is not None:

@@ -1,0 +1,86 @@
+"""Host logic of the model on a shared prefix and on bounded caches: what prefill and
+the decode steps refuse, what a refusal leaves as it was, and what the caches'
+state says.  The layers are replaced by a recorder, so no GPU is touched."""
+
+import pytest
+import torch
+
+from qmoe import model as qm
+from qmoe import ops
+from qmoe.attention import Attention, BoundedKVCache, CacheBudget, KVCache, SharedPrefix
+
+H, E, D, V, HKV = 64, 4, 16, 50, 1
+
+
+class _Causal(qm.NeuronQwen3MoeForCausalLM):
+    """The real host class over a real model object on the CPU whose layers do nothing but note the call."""
+
+    def __init__(self, batch=2, max_length=20, **kw):
+        nc = qm.MoENeuronConfig(batch_size=batch, max_batch_size=batch, seq_len=max_length, max_length=max_length,
+                                **kw)
+        config = qm.Qwen3MoeInferenceConfig(
+            nc, num_hidden_layers=2, hidden_size=H, num_experts=E, moe_intermediate_size=32, num_attention_heads=2,
+            num_key_value_heads=HKV, head_dim=D, vocab_size=V, num_experts_per_tok=2, tie_word_embeddings=False)
+        super().__init__(None, config)
+        self.device = torch.device("cpu")
+        params = qm.random_params(config, "cpu", seed=1)
+        self.model = qm.NeuronQwen3MoeModel(config, params)
+        self.calls = []
+        self.model.hidden = self._hidden
+        self.model.logits = lambda h, out=None: torch.zeros(h.shape[0], V)
+        self.model.allocate_cache(batch, max_length + 1)
+        self.reset()
+
+    def _hidden(self, ids, positions, B, S, start, h_buf=None, max_ctx=None):
+        self.calls.append((positions.tolist(), B, S, max_ctx))
+        return torch.zeros(B * S, H)
+
+
+def _tokens(*shape):
+    return torch.zeros(*shape, dtype=torch.long)
+
+
+def _stand(m):
+    b = m.model.budget
+    return None if b is None else (list(b.used), b.slots.tolist(), b.ctx.tolist(), b.lengths.tolist())
+
+
+# ------------------------------------------------------------------ prompts past the last position
+@pytest.mark.parametrize("kind", ["plain", "prefix", "bounded"])
+def test_prefill_refuses_a_prompt_past_the_last_position(kind):
+    m = _Causal(**(dict(kv_cache_budget=8, kv_cache_slack=3) if kind == "bounded" else {}))
+    P = 6 if kind == "prefix" else 0
+    if P:
+        m.share_prefix(_tokens(P))
+    m.prefill(_tokens(2, 21 - P))  # as many as there are positions
+    assert m.calls[-1][2] == 21 - P
+    m.reset()
+    if kind == "bounded":
+        m.decode_step(_tokens(2))
+    before, n, position = _stand(m), len(m.calls), m.position
+    for call in (lambda: m.prefill(_tokens(2, 22 - P)), lambda: m.prefill(_tokens(2, 40), torch.tensor([3, 4])),
+                 lambda: m.forward(_tokens(2, 22 - P))):
+        with pytest.raises(ValueError, match="positions"):
+            call()
+    assert (_stand(m), len(m.calls), m.position) == (before, n, position)
+
+
+@pytest.mark.parametrize("bounded", [False, True])
+def test_attention_refuses_chunks_past_the_tables_or_the_cache(monkeypatch, bounded):
+    """The layer itself: the projection would write neither queries nor entries there."""
+    d, hq, hkv, h = 128, 4, 2, 512
+    w = torch.ones(d, dtype=torch.bfloat16)
+    a = Attention(torch.zeros((hq + 2 * hkv) * d, h, dtype=torch.bfloat16), w, w,
+                  torch.zeros(h, hq * d, dtype=torch.bfloat16), hq, hkv, d, 1e-6)
+    for name in ("gemm", "qkv_norm_rope", "attn_shared", "attn_prefill_scored", "kv_evict"):
+        monkeypatch.setattr(ops, name, lambda *args, **kw: pytest.fail("launched"))
+    if bounded:
+        cache, chunks = BoundedKVCache(CacheBudget(1, 8, 2, 1, 3, "cpu"), hkv, d), [(0, 11), (0, 400)]
+    else:
+        cache, chunks = KVCache(1, hkv, 8, d, "cpu"), [(0, 9), (5, 4), (9, 2), (-1, 4)]
+        cache.prefix = SharedPrefix(cache.k[0], cache.v[0], 4)
+    rope = torch.zeros(10, d // 2)
+    for start, S in chunks:
+        x, pos = torch.zeros(S, h, dtype=torch.bfloat16), torch.arange(S, dtype=torch.int32) + start
+        with pytest.raises(ValueError, match="start \\+ S <= "):
+            a.forward(x, torch.zeros(S, h), pos, 1, S, cache, rope, rope, start)
