@@ -688,6 +688,23 @@ class NeuronQwen3MoeForCausalLM:
         """Positions a sequence has (after a shared prefix): the rows of the RoPE tables."""
         return self.model.rope[0].shape[0]
 
+    def _check_steps(self, first: int, end: int) -> None:
+        """Refuses steps at positions outside ``[0, _positions())`` on caches with a
+        prefix or a budget: there the step's entry is rejected, its zero query
+        gives every entry the same weight, and a bounded row moves on to a slot
+        that holds nothing.  (A plain cache's step is a zero row.)"""
+        if not self._contiguous() and (first < 0 or end > self._positions()):
+            raise ValueError(f"steps at positions {first} to {end - 1}: there are {self._positions()}"
+                             + (f" after a prefix of {self.model.base}" if self.model.base else ""))
+
+    def _top(self, pos: torch.Tensor, n_steps: int) -> int:
+        """The largest of a batch's positions, from which ``n_steps`` steps may go on."""
+        if self._contiguous():
+            return int(pos.max())
+        low, top = torch.stack(torch.aminmax(pos)).tolist()
+        self._check_steps(low, top + n_steps)
+        return top
+
     def _contiguous(self) -> bool:
         return self.model.budget is None and not self.model.base
 
@@ -727,11 +744,12 @@ class NeuronQwen3MoeForCausalLM:
         dev = self.device
         budget = self._budget_of(B)
         if positions is None:
-            pos = torch.full((B,), self.position, device=dev, dtype=torch.int32)
-            self.position += 1
+            pos, top = torch.full((B,), self.position, device=dev, dtype=torch.int32), self.position
+            self._check_steps(top, top + 1)
         else:
             pos = positions.to(device=dev, dtype=torch.int32).contiguous()
-            self.position = int(pos.max()) + 1
+            top = self._top(pos, 1)
+        self.position = top + 1
         if budget is not None:
             budget.make_room(self.model.caches())
         h = self.model.hidden(token_ids.to(dev).view(B, 1), pos, B, 1, 0)
@@ -761,7 +779,7 @@ class NeuronQwen3MoeForCausalLM:
         if positions is None:
             positions = torch.full((B,), self.position, dtype=torch.int32)
         pos0 = positions.to(device=self.device, dtype=torch.int32).view(B)
-        top = int(pos0.max())
+        top = self._top(pos0, n_steps)
         if not use_graph:
             toks, cur = [], first_token.to(self.device)
             for i in range(n_steps):

@@ -84,3 +84,38 @@ def test_attention_refuses_chunks_past_the_tables_or_the_cache(monkeypatch, boun
         x, pos = torch.zeros(S, h, dtype=torch.bfloat16), torch.arange(S, dtype=torch.int32) + start
         with pytest.raises(ValueError, match="start \\+ S <= "):
             a.forward(x, torch.zeros(S, h), pos, 1, S, cache, rope, rope, start)
+
+
+# ------------------------------------------------------------------ steps past the last position
+@pytest.mark.parametrize("kind", ["prefix", "bounded"])
+def test_steps_past_the_last_position_are_refused(kind):
+    m = _Causal(**(dict(kv_cache_budget=8, kv_cache_slack=30) if kind == "bounded" else {}))
+    P = 6 if kind == "prefix" else 0
+    if P:
+        m.share_prefix(_tokens(P))
+    end = 21 - P  # positions 0 to end - 1
+    m.prefill(_tokens(2, end - 2))
+    m.decode_step(_tokens(2), torch.tensor([0, end - 2]))
+    m.decode_step(_tokens(2))
+    assert m.calls[-1][0] == [end - 1] * 2 and m.position == end
+    before, n = _stand(m), len(m.calls)
+    for call in (lambda: m.decode_step(_tokens(2)), lambda: m.forward(_tokens(2, 1)),
+                 lambda: m.decode_step(_tokens(2), torch.tensor([0, end])),
+                 lambda: m.decode_step(_tokens(2), torch.tensor([-1, 0])),
+                 lambda: m.greedy_decode(_tokens(2), 1, use_graph=False),
+                 lambda: m.greedy_decode(_tokens(2), 1, use_graph=True),
+                 lambda: m.greedy_decode(_tokens(2), 4, False, torch.tensor([0, end - 3])),
+                 lambda: m.greedy_decode(_tokens(2), 4, True, torch.tensor([0, end - 3])),
+                 lambda: m.greedy_decode(_tokens(2), 1, True, torch.tensor([-1, 3]))):
+        with pytest.raises(ValueError, match="positions"):
+            call()
+        assert (_stand(m), len(m.calls), m.position) == (before, n, end)
+
+
+def test_steps_past_the_last_position_of_plain_caches():
+    """They write nothing and get zeros, as the fused decode says: not refused."""
+    m = _Causal()
+    m.prefill(_tokens(2, 21))
+    m.decode_step(_tokens(2))
+    m.decode_step(_tokens(2), torch.tensor([3, 30]))
+    assert m.position == 31

@@ -50,3 +50,33 @@ def test_prompt_past_the_last_position(dev):
     with pytest.raises(ValueError, match="positions"):
         b.prefill(_tokens(2, 2, 32))
     assert b.model.budget.used == used and all(torch.equal(x, y) for x, y in zip(_cache_bits(b), bits))
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+def test_steps_past_the_last_position(dev, graphs):
+    """One step past the end: refused, with every slot, score and position as it was."""
+    announce(f"steps past the last position, graphs {graphs}")
+    b = _model(2, 30, kv_cache_budget=12, kv_cache_slack=3, use_hip_graphs=graphs)
+    first = b.prefill(_tokens(1, 2, 20)).argmax(-1)
+    b.greedy_decode(first, 10)  # positions 20 to 29 of 31
+    bits, budget = _cache_bits(b), b.model.budget
+    state = [list(budget.used), budget.slots.tolist(), budget.ctx.tolist()]
+    for call in (lambda: b.greedy_decode(first, 2), lambda: b.decode_step(first, torch.tensor([3, 31])),
+                 lambda: b.decode_step(first, torch.tensor([-1, 3]))):
+        with pytest.raises(ValueError, match="positions"):
+            call()
+    assert [list(budget.used), budget.slots.tolist(), budget.ctx.tolist()] == state and b.position == 30
+    assert all(torch.equal(x, y) for x, y in zip(_cache_bits(b), bits))
+    assert b.greedy_decode(first, 1).shape == (2, 1) and b.position == 31
+    for c in b.model.caches():  # every live slot holds a position
+        assert all(bool((c.slot_pos[r, :, :n] >= 0).all()) for r, n in enumerate(budget.used))
+    m = _model(2, 30, use_hip_graphs=graphs)
+    m.share_prefix(_tokens(1, 12))
+    first = m.prefill(_tokens(2, 2, 10)).argmax(-1)
+    m.greedy_decode(first, 9)  # the last of 19 positions
+    bits = [t.clone() for c in m.model.caches() for t in (c.k, c.v)]
+    for call in (lambda: m.greedy_decode(first, 1), lambda: m.decode_step(first)):
+        with pytest.raises(ValueError, match="after a prefix of 12"):
+            call()
+    assert m.position == 19
+    assert all(torch.equal(x, y) for x, y in zip([t for c in m.model.caches() for t in (c.k, c.v)], bits))
