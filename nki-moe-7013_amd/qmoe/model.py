@@ -334,8 +334,10 @@ class NeuronQwen3MoeModel:
 
     def allocate_cache(self, B: int, S_max: int):
         """A contiguous cache of ``S_max`` entries a row in every layer, or, with
-        ``neuron_config.kv_cache_budget``, a bounded one."""
+        ``neuron_config.kv_cache_budget``, a bounded one.  A shared prefix goes
+        with the caches that had it."""
         c, n = self.config, self.config.neuron_config
+        self.base, self.rope, self.budget = 0, self.rope_full, None
         if n.kv_cache_budget > 0:
             self.budget = CacheBudget(B, n.kv_cache_budget, n.kv_cache_recent, n.kv_cache_sink, n.kv_cache_slack,
                                       self.embed_tokens.device)

@@ -119,3 +119,20 @@ def test_steps_past_the_last_position_of_plain_caches():
     m.decode_step(_tokens(2))
     m.decode_step(_tokens(2), torch.tensor([3, 30]))
     assert m.position == 31
+
+
+# ------------------------------------------------------------------ new caches
+def test_new_caches_have_no_prefix():
+    m = _Causal()
+    m.share_prefix(_tokens(6))
+    assert m.model.base == 6 and m._positions() == 15 and not m._contiguous()
+    m.model.allocate_cache(3, 21)
+    assert m.model.base == 0 and m._positions() == 21 and m._contiguous()
+    assert all(c.prefix is None and c.k.shape[0] == 3 for c in m.model.caches())
+    m.prefill(_tokens(3, 21))
+    m.model.config.neuron_config.kv_cache_budget = 8
+    m.model.allocate_cache(3, 21)
+    assert m._budget_of(3) is m.model.budget and m.model.caches()[0].state is m.model.budget
+    m.model.config.neuron_config.kv_cache_budget = 0  # and no state of bounded caches on plain ones
+    m.model.allocate_cache(2, 21)
+    assert m.model.budget is None and m._contiguous()
