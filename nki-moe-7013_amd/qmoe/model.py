@@ -329,6 +329,7 @@ class NeuronQwen3MoeModel:
         self.rope = self.rope_full = rope_tables(config.head_dim, max_pos, float(config.rope_theta), dev)
         self.base = 0  # tokens of a shared prefix: the position of cache index 0, where ``rope`` starts
         self.budget: Optional[CacheBudget] = None
+        self.allocations = 0  # of caches: a captured step is good for those it was captured with
         # set by the embedding gather when a token id is outside the vocabulary
         self.embed_err = torch.zeros(1, dtype=torch.int32, device=dev)
 
@@ -338,6 +339,7 @@ class NeuronQwen3MoeModel:
         with the caches that had it."""
         c, n = self.config, self.config.neuron_config
         self.base, self.rope, self.budget = 0, self.rope_full, None
+        self.allocations += 1
         if n.kv_cache_budget > 0:
             self.budget = CacheBudget(B, n.kv_cache_budget, n.kv_cache_recent, n.kv_cache_sink, n.kv_cache_slack,
                                       self.embed_tokens.device)
@@ -587,6 +589,7 @@ class NeuronQwen3MoeForCausalLM:
         self.model: Optional[NeuronQwen3MoeModel] = None
         self.device = torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else None
         self._graphs: Dict[Any, Any] = {}
+        self._graphs_of = 0  # the model's allocation of caches that they were captured with
         self.position = 0
 
     # -- class surface --------------------------------------------------------
@@ -626,6 +629,7 @@ class NeuronQwen3MoeForCausalLM:
             raise RuntimeError("no GPU visible: this model runs only on an MI355X")
         if params is None:
             params = self._load_params()
+        self._graphs.clear()  # captured steps hold the addresses of an earlier load's weights
         self.model = self._model_cls(self.config, params)
         self.model.allocate_cache(self.neuron_config.max_batch_size, int(self.neuron_config.max_length) + 1)
         self.reset()
@@ -819,8 +823,16 @@ class NeuronQwen3MoeForCausalLM:
             b *= 2
         return min(b, cap)
 
+    def _fresh_graphs(self) -> None:
+        """Drops captured steps that hold the addresses of caches that the model no
+        longer has."""
+        if self._graphs_of != self.model.allocations:
+            self._graphs.clear()
+            self._graphs_of = self.model.allocations
+
     def _decode_state(self, B: int):
         """Step buffers shared by every bucket's graph of batch ``B``."""
+        self._fresh_graphs()
         st = self._graphs.get(("state", B))
         if st is None:
             dev = self.device
@@ -833,6 +845,7 @@ class NeuronQwen3MoeForCausalLM:
         return st
 
     def _decode_graph(self, B: int, bucket: int):
+        self._fresh_graphs()
         key = ("decode", B, bucket)
         g = self._graphs.get(key)
         if g is not None:
@@ -940,6 +953,7 @@ class NeuronQwen3MoeForCausalLM:
         """Captured ``S``-token pass at a device-resident position (batch 1):
         embedding, 48 layers (attention over the cache with the chunk start read
         on the device), final norm + lm_head for all S rows, per-row argmax."""
+        self._fresh_graphs()
         key = ("verify", S)
         st = self._graphs.get(key)
         if st is not None:

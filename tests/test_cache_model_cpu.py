@@ -136,3 +136,22 @@ def test_new_caches_have_no_prefix():
     m.model.config.neuron_config.kv_cache_budget = 0  # and no state of bounded caches on plain ones
     m.model.allocate_cache(2, 21)
     assert m.model.budget is None and m._contiguous()
+
+
+def test_captured_steps_go_with_the_caches(monkeypatch):
+    """A step that was captured with caches that are gone would write into memory
+    that something else has by now (the capture itself needs a GPU: its place in
+    the table is what is looked at)."""
+    monkeypatch.setattr(ops, "argmax_workspace", lambda *args: None)
+    m = _Causal()
+    state = m._decode_state(2)
+    m._graphs[("decode", 2, 21)] = captured = object()
+    m._graphs[("verify", 4)] = captured
+    assert m._decode_graph(2, 21) is captured and m._verify_graph(4) is captured and m._decode_state(2) is state
+    m.model.allocate_cache(2, 21)
+    again = m._decode_state(2)
+    assert again is not state and list(m._graphs) == [("state", 2)]
+    assert m._decode_state(2) is again
+    m._graphs[("decode", 2, 21)] = captured
+    m.load(params=qm.random_params(m.config, "cpu", seed=2))
+    assert not m._graphs

@@ -80,3 +80,17 @@ def test_steps_past_the_last_position(dev, graphs):
             call()
     assert m.position == 19
     assert all(torch.equal(x, y) for x, y in zip([t for c in m.model.caches() for t in (c.k, c.v)], bits))
+
+
+def test_captured_steps_on_new_caches(dev):
+    """Steps captured before the caches were replaced are not replayed on them."""
+    announce("captured steps on new caches")
+    m, prompt = _model(2, 40), _tokens(1, 2, 9)
+    ad = qn.HuggingFaceGenerationAdapter(m)
+    want = ad.generate(prompt, max_new_tokens=12)
+    old = [c.k for c in m.model.caches()]  # kept, so that a replay into them would show
+    m.model.allocate_cache(2, 41)
+    before = [t.clone() for t in old]
+    assert torch.equal(ad.generate(prompt, max_new_tokens=12), want)
+    assert all(torch.equal(x, y) for x, y in zip(old, before))
+    assert all(bool(c.k[:, :, 20 - 1].any()) for c in m.model.caches())
