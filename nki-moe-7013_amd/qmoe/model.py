@@ -874,20 +874,25 @@ class NeuronQwen3MoeForCausalLM:
             stand = (m.budget.slots.clone(), m.budget.ctx.clone())
             m.budget.slots.fill_(-1)
             m.budget.ctx.fill_(0)
-        s = torch.cuda.Stream()
-        s.wait_stream(torch.cuda.current_stream())
-        with torch.cuda.stream(s):
-            step()
-        torch.cuda.current_stream().wait_stream(s)
-        torch.cuda.synchronize()
-        g = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(g):
-            step()
-        st["tok"].copy_(saved[0])
-        st["pos"].copy_(saved[1])
-        if m.budget is not None:
-            m.budget.slots.copy_(stand[0])
-            m.budget.ctx.copy_(stand[1])
+        s = None
+        try:
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                step()
+            torch.cuda.current_stream().wait_stream(s)
+            torch.cuda.synchronize()
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                step()
+        finally:  # a step that fails leaves the rows where they stand
+            if s is not None:  # what it launched reads them
+                torch.cuda.current_stream().wait_stream(s)
+            st["tok"].copy_(saved[0])
+            st["pos"].copy_(saved[1])
+            if m.budget is not None:
+                m.budget.slots.copy_(stand[0])
+                m.budget.ctx.copy_(stand[1])
         torch.cuda.synchronize()
         self._graphs[key] = g
         return g

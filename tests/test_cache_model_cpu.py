@@ -155,3 +155,18 @@ def test_captured_steps_go_with_the_caches(monkeypatch):
     m._graphs[("decode", 2, 21)] = captured
     m.load(params=qm.random_params(m.config, "cpu", seed=2))
     assert not m._graphs
+
+
+def test_a_failed_capture_leaves_the_rows_where_they_stand(monkeypatch):
+    def fail(*args, **kw):
+        raise RuntimeError("no memory")
+
+    monkeypatch.setattr(ops, "argmax_workspace", lambda *args: None)
+    m = _Causal(kv_cache_budget=8, kv_cache_slack=3)
+    m.prefill(_tokens(2, 7), torch.tensor([7, 4]))
+    before = _stand(m)
+    assert before[1:3] == ([7, 4], [8, 5])
+    monkeypatch.setattr(torch.cuda, "Stream", fail)
+    with pytest.raises(RuntimeError, match="no memory"):
+        m._decode_graph(2, 11)
+    assert _stand(m) == before and ("decode", 2, 11) not in m._graphs

@@ -94,3 +94,21 @@ def test_captured_steps_on_new_caches(dev):
     assert torch.equal(ad.generate(prompt, max_new_tokens=12), want)
     assert all(torch.equal(x, y) for x, y in zip(old, before))
     assert all(bool(c.k[:, :, 20 - 1].any()) for c in m.model.caches())
+
+
+def test_a_failed_capture_leaves_the_rows_where_they_stand(dev, monkeypatch):
+    announce("a capture that fails in its warm-up")
+    outs = []
+    for fails in (False, True):
+        m = _model(2, 60, kv_cache_budget=16, kv_cache_slack=3)
+        first = m.prefill(_tokens(1, 2, 20)).argmax(-1)
+        if fails:
+            bits, stand = _cache_bits(m), [m.model.budget.slots.tolist(), m.model.budget.ctx.tolist()]
+            with monkeypatch.context() as mp:
+                mp.setattr(m.model, "logits", lambda h, out=None: (_ for _ in ()).throw(RuntimeError("no memory")))
+                with pytest.raises(RuntimeError, match="no memory"):
+                    m.greedy_decode(first, 12)
+            assert [m.model.budget.slots.tolist(), m.model.budget.ctx.tolist()] == stand
+            assert all(torch.equal(x, y) for x, y in zip(_cache_bits(m), bits))
+        outs.append(m.greedy_decode(first, 12))
+    assert torch.equal(*outs)
