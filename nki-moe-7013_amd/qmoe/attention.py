@@ -314,16 +314,39 @@ class Attention:
             ops.kv_evict(own.k, own.v, scores, pos, st.lengths, st.budget, st.recent, st.sink,
                          out=(cache.k, cache.v, cache.scores, cache.slot_pos))
             return o
+        gemv = ops.qkv_norm_rope_workspace(B, x.shape[1], self.n_q, self.n_kv, self.head_dim) > 0
         if norm is not None:
             raw = ops.gemv_rmsnorm(x, norm[0], norm[1], self.wqkv, _lib.GEMM_STORE_F32)
-        else:
+        elif gemv or self._skinny_decode(x, B):
             raw = ops.gemm(x, self.wqkv, _lib.GEMM_STORE_F32)
+        else:
+            raw = self._raw_of_any(x) if bounded else None
         if not bounded:
-            q = ops.kv_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, positions, self.n_q,
-                              self.n_kv, cache.k, cache.v, self.eps)
+            if raw is None:
+                q = ops.qkv_norm_rope(x, self.wqkv, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, B, 1,
+                                      self.n_q, self.n_kv, cache.k, cache.v, self.eps)
+            else:
+                q = ops.kv_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, positions, self.n_q,
+                                  self.n_kv, cache.k, cache.v, self.eps)
             return ops.attn_shared(q, cache.prefix.k, cache.prefix.v, cache.k, cache.v, positions + 1, B, 1,
                                    cache.prefix.length, self.scale, max_ctx=max_ctx)
         st = cache.state
         q = ops.kv_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, st.slots, self.n_q, self.n_kv,
                           cache.k, cache.v, self.eps, scores=cache.scores, slot_pos=cache.slot_pos)
         return ops.attn_decode_scored(q, cache.k, cache.v, st.ctx, cache.scores, self.scale, max_ctx=max_ctx)
+
+    def _raw_of_any(self, x: torch.Tensor) -> torch.Tensor:
+        """The raw projection of rows that ``_skinny_decode`` leaves to
+        ``qkv_norm_rope``, whose cache row is the position and so no slot of a
+        bounded cache.  ``ops.gemm`` takes them with operands on its alignment
+        (copies of those that are not), ``wqkv`` in pieces below 2 GiB, and no
+        fewer rows than its tiles have where the GEMV does not take the hidden
+        size."""
+        rows, H = x.shape
+        if rows < 17 and H % 512:
+            x = torch.nn.functional.pad(x, (0, 0, 0, 17 - rows))
+        elif x.data_ptr() % 16:
+            x = x.clone()
+        pieces = self.wqkv.chunk(1 + self.wqkv.numel() * self.wqkv.element_size() // 2**31)
+        raw = [ops.gemm(x, w.clone() if w.data_ptr() % 16 else w, _lib.GEMM_STORE_F32) for w in pieces]
+        return (raw[0] if len(raw) == 1 else torch.cat(raw, 1))[:rows]

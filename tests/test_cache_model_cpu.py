@@ -170,3 +170,82 @@ def test_a_failed_capture_leaves_the_rows_where_they_stand(monkeypatch):
     with pytest.raises(RuntimeError, match="no memory"):
         m._decode_graph(2, 11)
     assert _stand(m) == before and ("decode", 2, 11) not in m._graphs
+
+
+# ------------------------------------------------------------------ a step's projection, by its operands
+def _off(offset, *shape):
+    """bf16 zeros, ``offset`` bytes past a 16-byte boundary."""
+    n = 1
+    for k in shape:
+        n *= k
+    t = torch.zeros(n + 16, dtype=torch.bfloat16)
+    first = (-t.data_ptr() % 16 + offset) // 2
+    return t[first:first + n].view(shape)
+
+
+def _step(monkeypatch, kind, B, h, w_off=0, x_off=0, hq=4, hkv=2):
+    """The names of a step's calls up to its attention, and the operands of its GEMMs."""
+    d, names, gemms = 128, [], []
+
+    def record(name, result):
+        def fn(*args, **kw):
+            names.append(name)
+            if name == "gemm":
+                gemms.append(args[:2])
+            return result(*args)
+        monkeypatch.setattr(ops, name, fn)
+
+    rows = torch.zeros(B, hq * d, dtype=torch.bfloat16)
+    record("gemm", lambda a, b, *_: torch.empty(a.shape[0], b.shape[0]))
+    record("qkv_norm_rope", lambda *_: rows.view(B, hq, d))
+    record("kv_append", lambda raw, *_: rows.view(B, hq, d) if raw.shape == (B, (hq + 2 * hkv) * d)
+           and raw.is_contiguous() else pytest.fail(str(raw.shape)))
+    record("attn_shared", lambda *_: rows)
+    record("attn_decode_scored", lambda *_: rows)
+    monkeypatch.setattr(ops, "gemm_workspace", lambda *_: None)
+    w = torch.ones(d, dtype=torch.bfloat16)
+    a = Attention(_off(w_off, (hq + 2 * hkv) * d, h), w, w, torch.zeros(h, hq * d, dtype=torch.bfloat16), hq, hkv, d,
+                  1e-6)
+    if kind == "bounded":
+        cache = BoundedKVCache(CacheBudget(B, 8, 2, 1, 3, "cpu"), hkv, d)
+    else:
+        cache = KVCache(B, hkv, 8, d, "cpu")
+        cache.prefix = SharedPrefix(cache.k[0], cache.v[0], 4)
+    rope = torch.zeros(10, d // 2)
+    a.forward(_off(x_off, B, h), torch.zeros(B, h), torch.zeros(B, dtype=torch.int32), B, 1, cache, rope, rope)
+    return names[:-1], gemms[:-1]  # (the last one is the output projection)
+
+
+ATTN = {"prefix": "attn_shared", "bounded": "attn_decode_scored"}
+
+
+@pytest.mark.parametrize("kind", ["prefix", "bounded"])
+@pytest.mark.parametrize("B,h", [(1, 2048), (16, 2048), (17, 2048), (20, 512), (64, 1024), (9, 4096)])
+def test_steps_on_the_alignment_take_the_raw_projection(monkeypatch, kind, B, h):
+    names, gemms = _step(monkeypatch, kind, B, h)
+    assert names == ["gemm", "kv_append", ATTN[kind]] and len(gemms) == 1
+
+
+@pytest.mark.parametrize("kind", ["prefix", "bounded"])
+@pytest.mark.parametrize("B,h", [(17, 2048), (20, 512), (64, 1024), (9, 4096), (33, 4096), (70, 2048)])
+@pytest.mark.parametrize("w_off,x_off", [(4, 0), (0, 8), (12, 2)])
+def test_steps_off_the_alignment(monkeypatch, kind, B, h, w_off, x_off):
+    """As on plain caches: no GEMM gets operands that its LDS-DMA kernels do not take."""
+    names, gemms = _step(monkeypatch, kind, B, h, w_off, x_off)
+    if kind == "prefix":
+        assert names == ["qkv_norm_rope", "attn_shared"]
+    else:
+        assert names == ["gemm", "kv_append", "attn_decode_scored"]
+    assert all(t.data_ptr() % 16 == 0 for operands in gemms for t in operands)
+
+
+@pytest.mark.parametrize("kind", ["prefix", "bounded"])
+def test_steps_whose_weights_the_gemm_refuses(monkeypatch, kind):
+    # 2 GiB of weights (never touched), and a hidden size that the GEMV does not take
+    names, gemms = _step(monkeypatch, kind, 9, 4096, hq=1792, hkv=128)
+    assert names[0] == ("qkv_norm_rope" if kind == "prefix" else "gemm")
+    assert all(b.numel() * 2 < 2**31 for _, b in gemms)
+    assert kind == "prefix" or sum(b.shape[0] for _, b in gemms) == 2048 * 128
+    names, gemms = _step(monkeypatch, kind, 3, 576)
+    assert names[0] == ("qkv_norm_rope" if kind == "prefix" else "gemm")
+    assert all(a.shape[0] > 16 for a, _ in gemms)

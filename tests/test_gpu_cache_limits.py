@@ -1,15 +1,19 @@
 """The model and its layers on shared prefixes and bounded caches at their limits:
-prompts and steps past the last position."""
+prompts and steps past the last position, captured steps, operands off the
+alignment."""
 
 import pytest
 import torch
 
-from gpu_util import announce
+from gpu_util import announce, bf16_randn, mean_rel
 from qmoe import model as qm
+from qmoe.attention import Attention, BoundedKVCache, CacheBudget, KVCache, SharedPrefix, rope_tables
 
 import qwen_with_nki as qn
 
 pytestmark = pytest.mark.gpu
+
+HQ, HKV, D, H = 32, 4, 128, 2048
 
 
 def _model(batch, max_length, **kw):
@@ -112,3 +116,71 @@ def test_a_failed_capture_leaves_the_rows_where_they_stand(dev, monkeypatch):
             assert all(torch.equal(x, y) for x, y in zip(_cache_bits(m), bits))
         outs.append(m.greedy_decode(first, 12))
     assert torch.equal(*outs)
+
+
+def _off(t, offset):
+    """A copy of ``t`` that starts ``offset`` bytes past a 16-byte boundary."""
+    buf = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)
+    out = buf[offset // 2:offset // 2 + t.numel()].view(t.shape)
+    assert out.data_ptr() % 16 == offset
+    return out.copy_(t)
+
+
+@pytest.mark.parametrize("w_off,x_off", [(8, 0), (0, 4), (12, 2)])
+@pytest.mark.parametrize("B", [17, 70])
+def test_steps_off_the_alignment(dev, B, w_off, x_off):
+    """A step whose operands are off the alignment: on bounded caches the bits of
+    the aligned step (the same products on copies); on a shared prefix close to
+    the layer whose rows hold the prefix themselves and off the alignment
+    too, whose entries come from the same kernel."""
+    announce(f"steps off the alignment, B={B} {w_off} {x_off}")
+    g = torch.Generator(device=dev).manual_seed(B)
+    w, wo = bf16_randn(((HQ + 2 * HKV) * D, H), g, dev, 0.03), bf16_randn((H, HQ * D), g, dev, 0.03)
+    nw = torch.ones(D, dtype=torch.bfloat16, device=dev)
+    x, P = bf16_randn((B, H), g, dev), 40
+    cos, sin = rope_tables(D, P + 4, 1e6, dev)
+    at, off = [Attention(t, nw, nw, wo, HQ, HKV, D, 1e-6) for t in (w, _off(w, w_off))]
+    pos = torch.arange(B, dtype=torch.int32, device=dev) % 4
+    outs = []
+    for a, y in ((at, x), (off, _off(x, x_off))):
+        state = CacheBudget(B, 8, 2, 1, 3, dev)
+        state.slots.copy_(pos)
+        state.ctx.copy_(pos + 1)
+        cache, res = BoundedKVCache(state, HKV, D), torch.zeros(B, H, device=dev)
+        a.forward(y, res, pos, B, 1, cache, cos, sin)
+        outs.append((res, cache.k, cache.v, cache.scores, cache.slot_pos))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    pre = bf16_randn((2, HKV, P, D), g, dev)
+    full, own = KVCache(B, HKV, P + 4, D, dev), KVCache(B, HKV, 4, D, dev)
+    for t, e in ((full.k, pre[0]), (full.v, pre[1])):
+        t.normal_(generator=g)
+        t[:, :, :P] = e
+    own.k.copy_(full.k[:, :, P:])
+    own.v.copy_(full.v[:, :, P:])
+    own.prefix = SharedPrefix(pre[0], pre[1], P)
+    a, b = torch.zeros(B, H, device=dev), torch.zeros(B, H, device=dev)
+    off.forward(_off(x, x_off), a, pos + P, B, 1, full, cos, sin)
+    off.forward(_off(x, x_off), b, pos, B, 1, own, cos[P:], sin[P:])
+    rel = mean_rel(b, a)
+    print(f"  mean rel {rel:.2e}", flush=True)
+    # two roundings to bf16 on either side of the attention (its weights, its output)
+    assert rel <= 4 * 2.0 ** -9
+    assert torch.equal(own.k, full.k[:, :, P:]) and torch.equal(own.v, full.v[:, :, P:])
+
+
+@pytest.mark.parametrize("B,h,heads", [(3, 576, 40), (16, 64, 8), (9, 4096, 2049)])
+def test_raw_projection_of_any_operands(dev, B, h, heads):
+    """Hidden sizes that the GEMV does not take, and 2 GiB of weights, in the raw
+    projection of a bounded cache's step.  Bound: a sum of h products in 32 bits."""
+    announce(f"raw projection, B={B} h={h} heads={heads}")
+    g = torch.Generator(device=dev).manual_seed(h)
+    w, x = bf16_randn((heads * D, h), g, dev, 0.1), bf16_randn((B, h), g, dev)
+    a = Attention(w, None, None, None, heads - 2, 1, D, 1e-6)
+    got = a._raw_of_any(x)
+    assert got.shape == (B, heads * D) and got.is_contiguous()
+    for c in {0, heads * D // 2 - 256, heads * D // 2, heads * D - 512}:  # (the middle: where the pieces meet)
+        c = max(0, c)
+        part = w[c:c + 512].double()
+        want, size = x.double() @ part.t(), x.double().abs() @ part.abs().t()
+        assert bool(((got[:, c:c + 512].double() - want).abs() <= h * 2.0 ** -24 * size).all())
