@@ -262,19 +262,19 @@ class NeuronQwen3MoeDecoderLayer:
         starts = pos_cpu[:, 0]
         _check_causal_mask(attention_mask, pos_cpu)
         end = int(pos_cpu.max()) + 1
-        if past_key_value is not None:
-            self.cache = KVCache.wrap(past_key_value)
-        elif (self.cache is None or self.cache.k.shape[0] != B or self.cache.capacity < end) and int(starts.min()) == 0 \
-                and not _special(self.cache):
-            cap = max(end, int(self.config.neuron_config.max_length) + 1)
-            self.cache = KVCache(B, self.config.num_key_value_heads, cap, self.config.head_dim, dev)
-        if _special(self.cache):
+        cache = self.cache if past_key_value is None else KVCache.wrap(past_key_value)
+        if _special(cache):
             raise ValueError("a cache with a shared prefix or a budget is driven by the model (its indices are not "
                              "positions): pass a KVCache or a (K, V) pair")
-        if self.cache is None or self.cache.k.shape[0] != B:
+        if past_key_value is None and int(starts.min()) == 0 \
+                and (cache is None or cache.k.shape[0] != B or cache.capacity < end):
+            cap = max(end, int(self.config.neuron_config.max_length) + 1)
+            cache = KVCache(B, self.config.num_key_value_heads, cap, self.config.head_dim, dev)
+        if cache is None or cache.k.shape[0] != B:
             raise ValueError("no KV cache for this batch: start at position 0 or pass past_key_value")
-        if self.cache.capacity < end:
-            raise ValueError(f"position {end - 1} is beyond the KV cache capacity {self.cache.capacity}")
+        if cache.capacity < end:
+            raise ValueError(f"position {end - 1} is beyond the KV cache capacity {cache.capacity}")
+        self.cache = cache
         if rope is None:
             rope = self.rope_tables(end, dev)
         pos = position_ids.to(device=dev, dtype=torch.int32).reshape(-1).contiguous()

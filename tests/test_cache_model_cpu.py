@@ -249,3 +249,23 @@ def test_steps_whose_weights_the_gemm_refuses(monkeypatch, kind):
     names, gemms = _step(monkeypatch, kind, 3, 576)
     assert names[0] == ("qkv_norm_rope" if kind == "prefix" else "gemm")
     assert all(a.shape[0] > 16 for a, _ in gemms)
+
+
+# ------------------------------------------------------------------ the layer's own cache
+class _OnGpu(torch.Tensor):
+    is_cuda = True  # as far as the layer's first check goes
+
+
+def test_a_refused_cache_is_not_the_layers(monkeypatch):
+    m = _Causal()
+    layer, own = m.model.layers[0], m.model.caches()[0]
+    monkeypatch.setattr(layer, "run", lambda *args, **kw: pytest.fail("ran"))
+    x = torch.zeros(2, 3, H).as_subclass(_OnGpu)
+    prefixed, small = KVCache(2, HKV, 30, D, "cpu"), KVCache(2, HKV, 2, D, "cpu")
+    prefixed.prefix = SharedPrefix(prefixed.k[0], prefixed.v[0], 4)
+    bounded = BoundedKVCache(CacheBudget(2, 8, 2, 1, 3, "cpu"), HKV, D)
+    for cache, why in ((prefixed, "driven by the model"), (bounded, "driven by the model"),
+                       (KVCache(3, HKV, 30, D, "cpu"), "no KV cache"), (small, "beyond the KV cache")):
+        with pytest.raises(ValueError, match=why):
+            layer.forward(x, past_key_value=cache)
+        assert layer.cache is own
