@@ -541,7 +541,9 @@ int qmoe_attn_decode(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf
  *   overlap.  out: bf16 [B*S, Hq*D].
  *   The entries that some query of a chunk sees have to be finite (a NaN value
  *   reaches the queries that do not see it); entries past them are not read.
- *   Deterministic.  Limits: D == 128, Hq / Hkv <= 16, P_max and S_max <= 2^22,
+ *   Deterministic; P and max_ctx decide how the keys are cut, so calls of
+ *   another max_ctx may differ in the last bits (qmoe_attn_decode_bucket's do
+ *   not).  Limits: D == 128, Hq / Hkv <= 16, P_max and S_max <= 2^22,
  *   B * S * Hq < 2^27.
  * Replaces: the token-generation and context-encoding attention of
  *   NeuronQwen3MoEAttention (qwen_with_nki.py:9943-9946, 10081-10109) for a
@@ -588,7 +590,10 @@ int64_t qmoe_attn_prefill_scored_workspace(int64_t B, int64_t S, int64_t Hq, int
  * scores[b, kvh, slot].  Slots past ctx_len are neither read nor scored.
  *   scores: f32 [B, Hkv, S_max]; workspace:
  *   qmoe_attn_decode_scored_workspace(B, Hq, D, max_ctx) bytes, holding nothing
- *   between calls; calls that share one must not overlap.  Deterministic.
+ *   between calls; calls that share one must not overlap.  Deterministic;
+ *   max_ctx decides how the keys are cut, so calls of another max_ctx may
+ *   differ in the last bits, outputs and scores (qmoe_attn_decode_bucket's do
+ *   not): use the same one wherever a run is to be repeated.
  *   Limits: D == 128, Hq / Hkv <= 16, 0 < max_ctx <= S_max, scale > 0.
  * Replaces: the token-generation attention (qwen_with_nki.py:9943-9946) over a
  *   bounded cache; the scores have no counterpart in the reference. */

@@ -756,9 +756,14 @@ class NeuronQwen3MoeForCausalLM:
             pos = positions.to(device=dev, dtype=torch.int32).contiguous()
             top = self._top(pos, 1)
         self.position = top + 1
+        ctx = top + 1
         if budget is not None:
             budget.make_room(self.model.caches())
-        h = self.model.hidden(token_ids.to(dev).view(B, 1), pos, B, 1, 0)
+            ctx = max(budget.used) + 1
+        # the bucket of the captured step: the operators on a prefix or a bounded
+        # cache cut their work by it, so eager and captured steps give the same bits
+        bucket = None if self._contiguous() else self._bucket(ctx)
+        h = self.model.hidden(token_ids.to(dev).view(B, 1), pos, B, 1, 0, max_ctx=bucket)
         if budget is not None:
             budget.slots.add_(1)
             budget.ctx.add_(1)

@@ -813,7 +813,7 @@ def attn_shared(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor,
     ``k_prefix/v_prefix[Hkv, P_max, D]``, which the batch reads once, and the
     first ``ctx_len[b] + s`` entries of its own ``k_cache/v_cache[B, Hkv, S_max,
     D]``, at most ``max_ctx`` of them (default ``S_max``; a context bucket sizes
-    the launch).  Decode: S = 1 and ``ctx_len`` (i32 ``[B]``, on the device)
+    the launch, and its last bits go with it).  Decode: S = 1 and ``ctx_len`` (i32 ``[B]``, on the device)
     counts the new entry; a chunk of S tokens whose first one is own entry e:
     ``ctx_len = e + 1``.  A query that sees nothing gets zeros.  Returns
     ``[B*S, Hq*D]``."""
@@ -850,7 +850,8 @@ def attn_decode_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Te
                        max_ctx: Optional[int] = None) -> torch.Tensor:
     """:func:`attn_decode` that also adds each slot's attention weight, summed
     over the q heads of its group, to ``scores[B, Hkv, S_max]`` (f32, in place).
-    A row with ``ctx_len`` of zero gets zeros.  Returns ``[B, Hq*D]``."""
+    A row with ``ctx_len`` of zero gets zeros.  The last bits go with ``max_ctx``,
+    by which the keys are cut.  Returns ``[B, Hq*D]``."""
     return _native().attn_decode_scored(q, k_cache, v_cache, ctx_len, scores, scale, workspace, out, max_ctx)
 
 

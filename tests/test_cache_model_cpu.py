@@ -269,3 +269,26 @@ def test_a_refused_cache_is_not_the_layers(monkeypatch):
         with pytest.raises(ValueError, match=why):
             layer.forward(x, past_key_value=cache)
         assert layer.cache is own
+
+
+# ------------------------------------------------------------------ eager steps run in the captured step's bucket
+def test_eager_steps_take_the_bucket(monkeypatch):
+    m = _Causal(max_length=700)
+    m.prefill(_tokens(2, 250))
+    m.decode_step(_tokens(2))
+    assert m.calls[-1][3] is None  # plain caches split by their capacity
+    m.share_prefix(_tokens(90))
+    m.prefill(_tokens(2, 250))
+    for pos, bucket in ((250, 256), (255, 256), (256, 512), (512, 701)):
+        m.decode_step(_tokens(2), torch.tensor([3, pos]))
+        assert m.calls[-1][3] == bucket
+    monkeypatch.setattr(ops, "kv_evict", lambda *args: None)
+    m = _Causal(max_length=900, kv_cache_budget=400, kv_cache_slack=112)
+    m.prefill(_tokens(2, 255))
+    for used, bucket in ((256, 256), (257, 512)):
+        m.decode_step(_tokens(2))
+        assert m.calls[-1][3] == bucket and m.model.budget.used == [used, used]
+    m.prefill(_tokens(2, 600))
+    for _ in range(113):  # the last one evicts first
+        m.decode_step(_tokens(2))
+    assert m.calls[-1][3] == 512 and m.model.budget.used == [401, 401]

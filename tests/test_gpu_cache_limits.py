@@ -184,3 +184,30 @@ def test_raw_projection_of_any_operands(dev, B, h, heads):
         part = w[c:c + 512].double()
         want, size = x.double() @ part.t(), x.double().abs() @ part.abs().t()
         assert bool(((got[:, c:c + 512].double() - want).abs() <= h * 2.0 ** -24 * size).all())
+
+
+def test_captured_and_eager_steps_give_the_same_bits(dev):
+    """Caches of more slots than the first context bucket, which the rows do not
+    leave at first: entries, scores and positions after eager steps are those
+    after captured ones, and so is what an eviction keeps."""
+    announce("captured and eager steps, caches past a bucket")
+    prompts, runs = _tokens(1, 16, 200), []
+    for graphs in (True, False):
+        m = _model(16, 700, kv_cache_budget=560, kv_cache_slack=40, use_hip_graphs=graphs)
+        first, stages = m.prefill(prompts).argmax(-1), []
+        for n in (30, 60, 320):  # in the buckets of 256 and 512, then past an eviction
+            first = m.greedy_decode(first, n)[:, -1]
+            stages += [first.clone(), *_cache_bits(m)]
+        runs.append(stages)
+    assert m.model.caches()[0].capacity == 600
+    for i, (a, b) in enumerate(zip(*runs)):
+        assert torch.equal(a, b), i
+    runs = []
+    for graphs in (True, False):
+        m = _model(5, 700, use_hip_graphs=graphs)
+        m.share_prefix(_tokens(2, 100))
+        first = m.prefill(_tokens(3, 5, 230)).argmax(-1)
+        toks = m.greedy_decode(first, 60)
+        runs.append([toks] + [t[:, :, :290].clone() for c in m.model.caches() for t in (c.k, c.v)])
+    for i, (a, b) in enumerate(zip(*runs)):
+        assert torch.equal(a, b), i
