@@ -719,7 +719,8 @@ class NeuronQwen3MoeForCausalLM:
         """Context encoding of ``input_ids[B,S]`` at positions 0..S-1; returns
         the logits ``[B, V]`` (fp32) of each row's last token: position S-1, or
         ``lengths[b] - 1`` for right-padded rows (pad tokens sit after a row's
-        end, so causal attention keeps them out of its real positions)."""
+        end, so causal attention keeps them out of its real positions).  Every
+        row has a real token."""
         B, S = input_ids.shape
         dev = self.device
         # a bounded cache's scratch holds any prompt and a row's own cache is not
@@ -727,11 +728,14 @@ class NeuronQwen3MoeForCausalLM:
         if S > self._positions():
             raise ValueError(f"a prompt of {S} tokens does not fit the {self._positions()} positions there are"
                              + (f" after a prefix of {self.model.base}" if self.model.base else ""))
+        real = [S] * B if lengths is None else [int(n) for n in lengths]
+        if len(real) != B or any(not 1 <= n <= S for n in real):
+            raise ValueError(f"lengths must be {B} numbers from 1 to {S} (got {real})")
         pos = torch.arange(S, device=dev, dtype=torch.int32).repeat(B)
         budget = self._budget_of(B)
         if budget is not None:
             # a single token is a decode step into empty caches
-            budget.begin([S] * B if lengths is None else [int(n) for n in lengths]) if S > 1 else budget.begin([0] * B)
+            budget.begin(real if S > 1 else [0] * B)
         h = self.model.hidden(input_ids.to(dev), pos, B, S, 0)
         if budget is not None and S == 1:
             budget.begin([1] * B)

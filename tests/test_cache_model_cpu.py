@@ -292,3 +292,20 @@ def test_eager_steps_take_the_bucket(monkeypatch):
     for _ in range(113):  # the last one evicts first
         m.decode_step(_tokens(2))
     assert m.calls[-1][3] == 512 and m.model.budget.used == [401, 401]
+
+
+# ------------------------------------------------------------------ lengths of padded prompts
+@pytest.mark.parametrize("kind", ["plain", "prefix", "bounded"])
+def test_prefill_refuses_lengths_outside_the_prompt(kind):
+    """A row's last token is looked up behind them, and a bounded row stands at them."""
+    m = _Causal(**(dict(kv_cache_budget=8, kv_cache_slack=3) if kind == "bounded" else {}))
+    if kind == "prefix":
+        m.share_prefix(_tokens(6))
+    m.prefill(_tokens(2, 5), torch.tensor([5, 1]))
+    before, n = _stand(m), len(m.calls)
+    for bad in ([6, 1], [5, 0], [-1, 5], [5], [5, 5, 5]):
+        with pytest.raises(ValueError, match="lengths"):
+            m.prefill(_tokens(2, 5), torch.tensor(bad))
+    with pytest.raises(ValueError, match="lengths"):
+        m.prefill(_tokens(2, 1), torch.tensor([1, 2]))
+    assert (_stand(m), len(m.calls), m.position) == (before, n, 5)
