@@ -51,8 +51,14 @@ int gpu_of(const at::Tensor& t, const char* name, const char* dims, int64_t n) {
   return t.get_device();
 }
 
-// Address of a contiguous, 16-byte aligned tensor of this dtype and shape on GPU ix.
-void* address(const at::Tensor& t, const char* name, at::ScalarType dtype, at::IntArrayRef shape, int ix) {
+// The kernels load and store bf16 rows 16 bytes at a time (kv_append's one element at a
+// time), and everything else, lengths and scores, in single words.
+constexpr uintptr_t any_alignment = 1;
+constexpr uintptr_t alignment_of(at::ScalarType dtype) { return dtype == BF16 ? 16 : any_alignment; }
+
+// Address of a contiguous tensor of this dtype, shape and alignment on GPU ix.
+void* address(const at::Tensor& t, const char* name, at::ScalarType dtype, at::IntArrayRef shape, int ix,
+              uintptr_t align) {
   if (!t.is_cuda()) refuse(std::string(name) + ": must be on a GPU (got " + t.device().str() + ")");
   if (t.scalar_type() != dtype)
     refuse(std::string(name) + ": dtype must be " + c10::toString(dtype) + " (got " + c10::toString(t.scalar_type()) +
@@ -64,17 +70,23 @@ void* address(const at::Tensor& t, const char* name, at::ScalarType dtype, at::I
     refuse("tensors are on different devices: " + std::string(name) + " is on " + t.device().str() +
            ", expected cuda:" + std::to_string(ix));
   void* p = t.data_ptr();
-  if (reinterpret_cast<uintptr_t>(p) % 16) refuse(std::string(name) + ": must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(p) % align)
+    refuse(std::string(name) + ": must be " + std::to_string(align) + "-byte aligned");
   return p;
 }
 
-void* address(py::handle h, const char* name, at::ScalarType dtype, at::IntArrayRef shape, int ix) {
-  return address(tensor(h, name), name, dtype, shape, ix);
+void* address(const at::Tensor& t, const char* name, at::ScalarType dtype, at::IntArrayRef shape, int ix) {
+  return address(t, name, dtype, shape, ix, alignment_of(dtype));
+}
+
+template <class T>
+T* arg(py::handle h, const char* name, at::ScalarType dtype, Shape shape, int ix, uintptr_t align) {
+  return static_cast<T*>(address(tensor(h, name), name, dtype, at::IntArrayRef(shape), ix, align));
 }
 
 template <class T>
 T* arg(py::handle h, const char* name, at::ScalarType dtype, Shape shape, int ix) {
-  return static_cast<T*>(address(h, name, dtype, at::IntArrayRef(shape), ix));
+  return arg<T>(h, name, dtype, shape, ix, alignment_of(dtype));
 }
 
 template <class T>
@@ -90,13 +102,13 @@ at::Tensor empty(at::IntArrayRef shape, at::ScalarType dtype, int ix) {
 struct Output {
   py::object obj;
   void* p;
-  Output(py::handle h, const char* name, at::ScalarType dtype, Shape shape, int ix) {
+  Output(py::handle h, const char* name, at::ScalarType dtype, Shape shape, int ix, uintptr_t align) {
     if (h.is_none()) {
       at::Tensor t = empty(at::IntArrayRef(shape), dtype, ix);
       p = t.data_ptr();
       obj = py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(t)));
     } else {
-      p = address(h, name, dtype, at::IntArrayRef(shape), ix);
+      p = address(tensor(h, name), name, dtype, at::IntArrayRef(shape), ix, align);
       obj = py::reinterpret_borrow<py::object>(h);
     }
   }
@@ -107,7 +119,7 @@ struct Scratch {
   at::Tensor t;
   void* p = nullptr;
   int64_t bytes = 0;
-  Scratch(py::handle h, int64_t need, int ix) {
+  Scratch(py::handle h, int64_t need, int ix, uintptr_t align) {
     if (h.is_none()) {
       if (need <= 0) return;
       t = empty({need}, U8, ix);
@@ -122,7 +134,8 @@ struct Scratch {
     if (bytes < need)
       refuse("workspace: needs " + std::to_string(need) + " bytes (got " + std::to_string(bytes) + ")");
     p = t.data_ptr();
-    if (reinterpret_cast<uintptr_t>(p) % 16) refuse("workspace: must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(p) % align)
+      refuse("workspace: must be " + std::to_string(align) + "-byte aligned");
   }
 };
 
@@ -225,9 +238,9 @@ py::object attn_shared(py::handle q, py::handle k_prefix, py::handle v_prefix, p
   const Bf* pv = arg<Bf>(v_cache, "v_cache", BF16, {B, Hkv, S_max, x.D}, x.ix);
   const int32_t* pc = arg<int32_t>(ctx_len, "ctx_len", I32, {B}, x.ix);
   const On on(x.ix);
-  const Output o(out, "out", BF16, {x.T, x.Hq * x.D}, x.ix);
+  const Output o(out, "out", BF16, {x.T, x.Hq * x.D}, x.ix, 16);
   const Scratch ws(workspace, size(qmoe_attn_shared_workspace(B, S, x.Hq, Hkv, x.D, P, ctx), "qmoe_attn_shared"),
-                   x.ix);
+                   x.ix, 16);
   check(qmoe_attn_shared(x.p, pkp, pvp, P, P_max, pk, pv, pc, B, S, x.Hq, Hkv, x.D, S_max, ctx, sc, ws.p, ws.bytes,
                          static_cast<Bf*>(o.p), stream(x.ix)),
         "qmoe_attn_shared");
@@ -250,10 +263,10 @@ py::object attn_prefill_scored(py::handle q, py::handle k_cache, py::handle v_ca
   float* ps = arg<float>(scores, "scores", F32, {B, Hkv, S_max}, x.ix);
   const int32_t* pl = optional_arg<int32_t>(lengths, "lengths", I32, {B}, x.ix);
   const On on(x.ix);
-  const Output o(out, "out", BF16, {x.T, x.Hq * x.D}, x.ix);
+  const Output o(out, "out", BF16, {x.T, x.Hq * x.D}, x.ix, 16);
   const Scratch ws(
       workspace,
-      size(qmoe_attn_prefill_scored_workspace(B, S, x.Hq, Hkv, x.D, start), "qmoe_attn_prefill_scored"), x.ix);
+      size(qmoe_attn_prefill_scored_workspace(B, S, x.Hq, Hkv, x.D, start), "qmoe_attn_prefill_scored"), x.ix, 16);
   check(qmoe_attn_prefill_scored(x.p, pk, pv, B, S, x.Hq, Hkv, x.D, S_max, start, pl, sc, ws.p, ws.bytes, ps,
                                  static_cast<Bf*>(o.p), stream(x.ix)),
         "qmoe_attn_prefill_scored");
@@ -275,9 +288,10 @@ py::object attn_decode_scored(py::handle q, py::handle k_cache, py::handle v_cac
   float* ps = arg<float>(scores, "scores", F32, {B, Hkv, S_max}, x.ix);
   const int32_t* pc = arg<int32_t>(ctx_len, "ctx_len", I32, {B}, x.ix);
   const On on(x.ix);
-  const Output o(out, "out", BF16, {B, x.Hq * x.D}, x.ix);
+  const Output o(out, "out", BF16, {B, x.Hq * x.D}, x.ix, 16);
   const Scratch ws(workspace,
-                   size(qmoe_attn_decode_scored_workspace(B, x.Hq, x.D, ctx), "qmoe_attn_decode_scored"), x.ix);
+                   size(qmoe_attn_decode_scored_workspace(B, x.Hq, x.D, ctx), "qmoe_attn_decode_scored"), x.ix,
+                   16);
   check(qmoe_attn_decode_scored(x.p, pk, pv, pc, B, x.Hq, Hkv, x.D, S_max, ctx, sc, ws.p, ws.bytes, ps,
                                 static_cast<Bf*>(o.p), stream(x.ix)),
         "qmoe_attn_decode_scored");
@@ -299,18 +313,18 @@ py::object kv_append(py::handle qkv, py::handle q_norm_w, py::handle k_norm_w, p
   if (cos.dim() != 2) refuse("rope_cos must be [max_pos, D / 2]");
   const int64_t max_pos = cos.size(0);
   const float* praw = arg<float>(qkv, "qkv", F32, {B, (Hq + 2 * Hkv) * D}, ix);
-  const Bf* pqn = arg<Bf>(q_norm_w, "q_norm_w", BF16, {D}, ix);
-  const Bf* pkn = arg<Bf>(k_norm_w, "k_norm_w", BF16, {D}, ix);
+  const Bf* pqn = arg<Bf>(q_norm_w, "q_norm_w", BF16, {D}, ix, any_alignment);
+  const Bf* pkn = arg<Bf>(k_norm_w, "k_norm_w", BF16, {D}, ix, any_alignment);
   const float* pcos = arg<float>(rope_cos, "rope_cos", F32, {max_pos, D / 2}, ix);
   const float* psin = arg<float>(rope_sin, "rope_sin", F32, {max_pos, D / 2}, ix);
   const int32_t* pp = arg<int32_t>(positions, "positions", I32, {B}, ix);
   const int32_t* psl = arg<int32_t>(slots, "slots", I32, {B}, ix);
-  Bf* pk = arg<Bf>(k_cache, "k_cache", BF16, {B, Hkv, S_max, D}, ix);
-  Bf* pv = arg<Bf>(v_cache, "v_cache", BF16, {B, Hkv, S_max, D}, ix);
+  Bf* pk = arg<Bf>(k_cache, "k_cache", BF16, {B, Hkv, S_max, D}, ix, any_alignment);
+  Bf* pv = arg<Bf>(v_cache, "v_cache", BF16, {B, Hkv, S_max, D}, ix, any_alignment);
   float* ps = optional_arg<float>(scores, "scores", F32, {B, Hkv, S_max}, ix);
   int32_t* psp = optional_arg<int32_t>(slot_pos, "slot_pos", I32, {B, Hkv, S_max}, ix);
   const On on(ix);
-  const Output o(q_out, "q_out", BF16, {B, Hq, D}, ix);
+  const Output o(q_out, "q_out", BF16, {B, Hq, D}, ix, any_alignment);
   check(qmoe_kv_append(praw, pqn, pkn, pcos, psin, max_pos, pp, psl, B, Hq, Hkv, D, S_max, float(eps),
                        static_cast<Bf*>(o.p), pk, pv, ps, psp, stream(ix)),
         "qmoe_kv_append");
@@ -365,7 +379,8 @@ void kv_evict(py::handle k_cache, py::handle v_cache, py::handle scores, py::han
   }
   const Cache& to = other ? *other : from;
   const On on(ix);
-  const Scratch ws(workspace, size(qmoe_kv_evict_workspace(B, Hkv, S_max, budget), "qmoe_kv_evict"), ix);
+  const Scratch ws(workspace, size(qmoe_kv_evict_workspace(B, Hkv, S_max, budget), "qmoe_kv_evict"), ix,
+                   alignof(int32_t));
   check(qmoe_kv_evict(static_cast<Bf*>(from.p[0]), static_cast<Bf*>(from.p[1]), static_cast<float*>(from.p[2]),
                       static_cast<int32_t*>(from.p[3]), pc, B, Hkv, D, S_max, budget, recent, sink, ws.p, ws.bytes,
                       S_out, static_cast<Bf*>(to.p[0]), static_cast<Bf*>(to.p[1]), static_cast<float*>(to.p[2]),

@@ -1,12 +1,13 @@
 """The model and its layers on shared prefixes and bounded caches at their limits:
 prompts and steps past the last position, captured steps, operands off the
-alignment."""
+alignment; and the operators' arguments that need none."""
 
 import pytest
 import torch
 
 from gpu_util import announce, bf16_randn, mean_rel
 from qmoe import model as qm
+from qmoe import ops
 from qmoe.attention import Attention, BoundedKVCache, CacheBudget, KVCache, SharedPrefix, rope_tables
 
 import qwen_with_nki as qn
@@ -121,7 +122,8 @@ def test_a_failed_capture_leaves_the_rows_where_they_stand(dev, monkeypatch):
 def _off(t, offset):
     """A copy of ``t`` that starts ``offset`` bytes past a 16-byte boundary."""
     buf = torch.empty(t.numel() + 8, dtype=t.dtype, device=t.device)
-    out = buf[offset // 2:offset // 2 + t.numel()].view(t.shape)
+    first = offset // t.element_size()
+    out = buf[first:first + t.numel()].view(t.shape)
     assert out.data_ptr() % 16 == offset
     return out.copy_(t)
 
@@ -211,3 +213,47 @@ def test_captured_and_eager_steps_give_the_same_bits(dev):
         runs.append([toks] + [t[:, :, :290].clone() for c in m.model.caches() for t in (c.k, c.v)])
     for i, (a, b) in enumerate(zip(*runs)):
         assert torch.equal(a, b), i
+
+
+def test_arguments_that_need_no_alignment(dev):
+    """Lengths, positions, slots, scores and tables are read in single words, and
+    kv_append's rows too: a slice of a batch's lengths is as good as its start."""
+    announce("arguments off 16 bytes")
+    g = torch.Generator(device=dev).manual_seed(8)
+    B, S_max, cap = 3, 70, 5
+
+    def i32(*values):
+        return torch.tensor(values, dtype=torch.int32, device=dev)
+
+    def off(t):  # one element behind a boundary
+        return _off(t, t.element_size())
+
+    q, k, v = [bf16_randn(s, g, dev) for s in ((B, HQ, D), (B, HKV, S_max, D), (B, HKV, S_max, D))]
+    lens, many = i32(70, 3, 66), i32(9, 70, 3, 66)
+    assert many[1:].data_ptr() % 16
+    want = ops.attn_shared(q, k[0], v[0], k, v, lens, B, 1)
+    assert torch.equal(want, ops.attn_shared(q, k[0], v[0], k, v, many[1:], B, 1))
+    scores = torch.rand(B, HKV, S_max, generator=g, device=dev)
+    runs = []
+    for n, sc in ((lens, scores.clone()), (many[1:], off(scores))):
+        out = ops.attn_decode_scored(q, k, v, n, sc)
+        runs.append([out, ops.attn_prefill_scored(q, k, v, sc, B, 1, 5, lengths=off(i32(1, 0, 1))), sc])
+    raw = torch.randn(B, (HQ + 2 * HKV) * D, generator=g, device=dev)
+    w, (cos, sin) = bf16_randn((2, D), g, dev), rope_tables(D, 50, 1e6, dev)
+    k2, v2 = bf16_randn((B, HKV, cap, D), g, dev), bf16_randn((B, HKV, cap, D), g, dev)
+    pos, slots, at = i32(7, 49, 0), i32(4, 0, 2), torch.arange(S_max, dtype=torch.int32, device=dev).repeat(B, HKV, 1)
+    for same in (torch.clone, off):
+        cache = [same(t) for t in (k2, v2, scores[:, :, :cap].contiguous(), at[:, :, :cap].contiguous())]
+        got = ops.kv_append(same(raw), same(w[0]), same(w[1]), same(cos), same(sin), same(pos), same(slots), HQ, HKV,
+                            cache[0], cache[1], 1e-6, scores=cache[2], slot_pos=cache[3], q_out=same(q))
+        full = [k.clone(), v.clone(), same(scores), same(at)]
+        ops.kv_evict(*full, same(lens), 40, 5, 2,
+                     workspace=same(torch.zeros(2 * B * HKV * 40, dtype=torch.int32, device=dev)))
+        runs[same is off] += [got, *cache, *full]
+    for i, (a, b) in enumerate(zip(*runs)):
+        assert torch.equal(a, b), i
+    for bad in (dict(k=off(k)), dict(out=off(want)), dict(q=off(q))):  # and what does need it is still refused
+        args = dict(q=q, k=k, v=v, out=None)
+        args.update(bad)
+        with pytest.raises(ValueError, match="16-byte aligned"):
+            ops.attn_decode_scored(args["q"], args["k"], args["v"], lens, scores, out=args["out"])
