@@ -174,31 +174,48 @@ void heads(int64_t Hq, int64_t Hkv) {
     refuse("need Hq a multiple of Hkv, by at most 16 (Hq=" + std::to_string(Hq) + ", Hkv=" + std::to_string(Hkv) + ")");
 }
 
-float scale_of(py::handle h, int64_t D) {
-  const double s = h.is_none() ? 1.0 / std::sqrt(double(D)) : PyFloat_AsDouble(h.ptr());
-  if (PyErr_Occurred()) {
+double number(py::handle h, const char* name) {
+  const double x = PyFloat_AsDouble(h.ptr());
+  if (x == -1.0 && PyErr_Occurred()) {
     PyErr_Clear();
-    refuse("scale must be a number");
+    refuse(std::string(name) + " must be a number");
   }
+  return x;
+}
+
+float scale_of(py::handle h, int64_t D) {
+  const double s = h.is_none() ? 1.0 / std::sqrt(double(D)) : number(h, "scale");
   if (!(s > 0.0) || !std::isfinite(s)) refuse("scale must be positive and finite");
   return float(s);
 }
 
-// An integer within [lo, hi], or `none` where None was given.
-int64_t within(py::handle h, const char* name, int64_t lo, int64_t hi, int64_t none) {
-  int64_t n = none;
-  if (!h.is_none()) {
-    n = PyLong_AsLongLong(h.ptr());  // any integer (an __index__ of its own included)
-    if (n == -1 && PyErr_Occurred()) {
-      PyErr_Clear();
-      refuse(std::string(name) + " must be an integer");
-    }
+// Any integer (an __index__ of its own included).  Arguments come as handles, not as
+// typed parameters: pybind would answer another type with its own TypeError.
+int64_t integer(py::handle h, const char* name) {
+  const int64_t n = h.is_none() ? -1 : PyLong_AsLongLong(h.ptr());
+  if (h.is_none() || (n == -1 && PyErr_Occurred())) {
+    PyErr_Clear();
+    refuse(std::string(name) + " must be an integer");
   }
+  return n;
+}
+
+// An integer within [lo, hi].
+int64_t within(py::handle h, const char* name, int64_t lo, int64_t hi) {
+  const int64_t n = integer(h, name);
   if (n < lo || n > hi)
     refuse(std::string(name) + " must be in [" + std::to_string(lo) + ", " + std::to_string(hi) + "] (got " +
            std::to_string(n) + ")");
   return n;
 }
+
+// The same, or `none` where None was given.
+int64_t within(py::handle h, const char* name, int64_t lo, int64_t hi, int64_t none) {
+  return h.is_none() ? none : within(h, name, lo, hi);
+}
+
+// A number of rows, tokens or heads.
+int64_t count(py::handle h, const char* name) { return within(h, name, 0, INT32_MAX); }
 
 using Bf = qmoe_bf16;
 
@@ -219,8 +236,9 @@ struct Queries {
 };
 
 py::object attn_shared(py::handle q, py::handle k_prefix, py::handle v_prefix, py::handle k_cache, py::handle v_cache,
-                       py::handle ctx_len, int64_t B, int64_t S, py::handle prefix_len, py::handle scale,
-                       py::handle workspace, py::handle out, py::handle max_ctx) {
+                       py::handle ctx_len, py::handle batch, py::handle queries, py::handle prefix_len,
+                       py::handle scale, py::handle workspace, py::handle out, py::handle max_ctx) {
+  const int64_t B = count(batch, "B"), S = count(queries, "S");
   const Queries x(q, B * S, "[B*S, Hq, D]");
   int64_t Hkv, S_max;
   cache_sizes(tensor(k_cache, "k_cache"), B, x.D, Hkv, S_max);
@@ -247,14 +265,15 @@ py::object attn_shared(py::handle q, py::handle k_prefix, py::handle v_prefix, p
   return o.obj;
 }
 
-py::object attn_prefill_scored(py::handle q, py::handle k_cache, py::handle v_cache, py::handle scores, int64_t B,
-                               int64_t S, int64_t start, py::handle lengths, py::handle scale, py::handle workspace,
-                               py::handle out) {
+py::object attn_prefill_scored(py::handle q, py::handle k_cache, py::handle v_cache, py::handle scores,
+                               py::handle batch, py::handle queries, py::handle at, py::handle lengths,
+                               py::handle scale, py::handle workspace, py::handle out) {
+  const int64_t B = count(batch, "B"), S = count(queries, "S"), start = integer(at, "start");
   const Queries x(q, B * S, "[B*S, Hq, D]");
   int64_t Hkv, S_max;
   cache_sizes(tensor(k_cache, "k_cache"), B, x.D, Hkv, S_max);
   heads(x.Hq, Hkv);
-  if (start < 0 || S < 0 || start + S > S_max)
+  if (start < 0 || start > S_max - S)
     refuse("need 0 <= start and start + S <= S_max=" + std::to_string(S_max) + " (start=" + std::to_string(start) +
            ", S=" + std::to_string(S) + ")");
   const float sc = scale_of(scale, x.D);
@@ -299,9 +318,11 @@ py::object attn_decode_scored(py::handle q, py::handle k_cache, py::handle v_cac
 }
 
 py::object kv_append(py::handle qkv, py::handle q_norm_w, py::handle k_norm_w, py::handle rope_cos,
-                     py::handle rope_sin, py::handle positions, py::handle slots, int64_t Hq, int64_t Hkv,
-                     py::handle k_cache, py::handle v_cache, double eps, py::handle scores, py::handle slot_pos,
-                     py::handle q_out) {
+                     py::handle rope_sin, py::handle positions, py::handle slots, py::handle q_heads,
+                     py::handle kv_heads, py::handle k_cache, py::handle v_cache, py::handle epsilon,
+                     py::handle scores, py::handle slot_pos, py::handle q_out) {
+  const int64_t Hq = count(q_heads, "Hq"), Hkv = count(kv_heads, "Hkv");
+  const float eps = float(number(epsilon, "eps"));
   const at::Tensor& raw = tensor(qkv, "qkv");
   const int ix = gpu_of(raw, "qkv", "[B, (Hq + 2 Hkv) * D]", 2);
   const at::Tensor &k = tensor(k_cache, "k_cache"), &cos = tensor(rope_cos, "rope_cos");
@@ -325,7 +346,7 @@ py::object kv_append(py::handle qkv, py::handle q_norm_w, py::handle k_norm_w, p
   int32_t* psp = optional_arg<int32_t>(slot_pos, "slot_pos", I32, {B, Hkv, S_max}, ix);
   const On on(ix);
   const Output o(q_out, "q_out", BF16, {B, Hq, D}, ix, any_alignment);
-  check(qmoe_kv_append(praw, pqn, pkn, pcos, psin, max_pos, pp, psl, B, Hq, Hkv, D, S_max, float(eps),
+  check(qmoe_kv_append(praw, pqn, pkn, pcos, psin, max_pos, pp, psl, B, Hq, Hkv, D, S_max, eps,
                        static_cast<Bf*>(o.p), pk, pv, ps, psp, stream(ix)),
         "qmoe_kv_append");
   return o.obj;
@@ -353,7 +374,8 @@ struct Cache {
 };
 
 void kv_evict(py::handle k_cache, py::handle v_cache, py::handle scores, py::handle slot_pos, py::handle ctx_len,
-              int64_t budget, int64_t recent, int64_t sink, py::handle out, py::handle workspace) {
+              py::handle entries, py::handle last, py::handle first, py::handle out, py::handle workspace) {
+  const int64_t budget = integer(entries, "budget"), recent = integer(last, "recent"), sink = integer(first, "sink");
   const at::Tensor& k = tensor(k_cache, "k_cache");
   const int ix = gpu_of(k, "k_cache", "[B, Hkv, S_max, D]", 4);
   const int64_t B = k.size(0), Hkv = k.size(1), S_max = k.size(2), D = k.size(3);

@@ -200,3 +200,36 @@ def test_default_split_of_small_budgets():
     for budget in range(1, 40):
         c = MoENeuronConfig(kv_cache_budget=budget)
         check_budget(budget, c.kv_cache_recent, c.kv_cache_sink)
+
+
+@pytest.mark.parametrize("bad", ["2", 2.0, None, 2 ** 70, [2]], ids=str)
+def test_wrappers_refuse_what_is_no_integer(bad):
+    """As every wrapper does: a ValueError that names the argument."""
+    q, k, kp = _bf(2, 32, 128), _bf(2, 4, 8, 128), _bf(4, 9, 128)
+    sc, sp, n, t, w = torch.zeros(2, 4, 8), _i(2, 4, 8), _i(2), torch.zeros(4, 64), _bf(128)
+    raw = torch.zeros(2, 40 * 128)
+    calls = {
+        "B": [lambda: ops.attn_shared(q, kp, kp, k, k, n, bad, 1), lambda: ops.attn_prefill_scored(q, k, k, sc, bad, 1)],
+        "S": [lambda: ops.attn_shared(q, kp, kp, k, k, n, 2, bad), lambda: ops.attn_prefill_scored(q, k, k, sc, 2, bad)],
+        "start": [lambda: ops.attn_prefill_scored(q, k, k, sc, 2, 1, bad)],
+        "Hq": [lambda: ops.kv_append(raw, w, w, t, t, n, n, bad, 4, k, k, 1e-6)],
+        "Hkv": [lambda: ops.kv_append(raw, w, w, t, t, n, n, 32, bad, k, k, 1e-6)],
+        "budget": [lambda: ops.kv_evict(k, k, sc, sp, n, bad)],
+        "recent": [lambda: ops.kv_evict(k, k, sc, sp, n, 4, bad)],
+        "sink": [lambda: ops.kv_evict(k, k, sc, sp, n, 4, 1, bad)],
+    }
+    for name, fs in calls.items():
+        for f in fs:
+            with pytest.raises(ValueError, match=f"^{name} must be an integer"):
+                f()
+    if not isinstance(bad, (int, float)):
+        with pytest.raises(ValueError, match="^eps must be a number"):
+            ops.kv_append(raw, w, w, t, t, n, n, 32, 4, k, k, bad)
+
+
+def test_wrappers_refuse_negative_counts():
+    q, k, kp, sc, n = _bf(2, 32, 128), _bf(2, 4, 8, 128), _bf(4, 9, 128), torch.zeros(2, 4, 8), _i(2)
+    for f in (lambda: ops.attn_shared(q, kp, kp, k, k, n, -2, -1), lambda: ops.attn_shared(q, kp, kp, k, k, n, 2, -1),
+              lambda: ops.attn_shared(q, kp, kp, k, k, n, 2 ** 33, 1), lambda: ops.attn_prefill_scored(q, k, k, sc, -1, -2)):
+        with pytest.raises(ValueError, match="must be in"):
+            f()
