@@ -720,7 +720,7 @@ static int64_t ps_col_bytes(const CsArgs& c) {
 
 extern "C" int64_t qmoe_attn_prefill_scored_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
                                                       int64_t start) {
-  if (start < 0 || S < 0 || start + S > AR_MAX_KEYS ||
+  if (start < 0 || S < 0 || S > AR_MAX_KEYS || start > AR_MAX_KEYS - S ||
       ar_check("qmoe_attn_prefill_scored_workspace", B, S, Hq, Hkv, D, std::max<int64_t>(start + S, 1), 1.0f))
     return -1;
   if (B == 0 || S == 0) return 0;
@@ -739,7 +739,7 @@ extern "C" int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_c
   const char* fn = "qmoe_attn_prefill_scored";
   QMOE_REQUIRE(k_cache && v_cache && scores && (B == 0 || S == 0 || (q && out)), "%s: null pointer", fn);
   if (int rc = ar_check(fn, B, S, Hq, Hkv, D, S_max, scale)) return rc;
-  QMOE_REQUIRE(start >= 0 && start + S <= S_max, "%s: need 0 <= start and start + S <= S_max", fn);
+  QMOE_REQUIRE(start >= 0 && start <= S_max - S, "%s: need 0 <= start and start + S <= S_max", fn);
   // a row's queries are addressed with 32-bit byte offsets
   QMOE_REQUIRE(S * Hq * AP_ROWB < (1ll << 31), "%s: S * Hq must be below 2^23", fn);
   if (B == 0 || S == 0) return QMOE_OK;

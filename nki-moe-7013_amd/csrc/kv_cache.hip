@@ -823,7 +823,7 @@ extern "C" int qmoe_kv_append(const float* qkv, const qmoe_bf16* q_norm_w, const
                    (B == 0 || (qkv && positions && slots && q_out && k_cache && v_cache)),
                "%s: null pointer", fn);
   QMOE_REQUIRE(D == HD, "%s: head_dim must be 128 (D=%lld)", fn, (long long)D);
-  QMOE_REQUIRE(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq + 2 * Hkv < 65536, "%s: bad head counts", fn);
+  QMOE_REQUIRE(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq < 65536 && Hq + 2 * Hkv < 65536, "%s: bad head counts", fn);
   QMOE_REQUIRE(B >= 0 && B < 65536 && S_max > 0 && S_max < (1ll << 30) && max_pos > 0, "%s: bad B/S_max/max_pos", fn);
   if (B == 0) return QMOE_OK;
   hipLaunchKernelGGL(kv_append_kernel, dim3(unsigned(Hq + 2 * Hkv), unsigned(B)), dim3(64), 0, as_stream(stream),
@@ -845,7 +845,9 @@ static int64_t sd_bytes(int64_t B, int64_t Hq, int64_t max_ctx, int64_t split) {
 
 // (for the split that takes more, so that the size does not hang on Hkv)
 extern "C" int64_t qmoe_attn_decode_scored_workspace(int64_t B, int64_t Hq, int64_t D, int64_t max_ctx) {
-  if (B < 0 || Hq < 0 || D != HD || max_ctx < 0 || max_ctx >= (1ll << 30)) return -1;
+  if (B < 0 || B >= 65536 || Hq < 0 || Hq >= 65536 * SD_MAX_G || D != HD || max_ctx < 0 || max_ctx >= (1ll << 30))
+    return -1;
+  if (B * Hq >= (1ll << 31) || B * Hq * max_ctx >= (1ll << 58)) return -1;  // at most 12.2 bytes each, and 1.5 KB a head
   const int64_t few = (max_ctx + SD_KEYS - 1) / SD_KEYS <= 64 && B <= 512 ? sd_bytes(B, Hq, max_ctx, SD_KEYS) : 0;
   return std::max(few, sd_bytes(B, Hq, max_ctx, SD_KEYS * SD_WAVES));
 }
@@ -863,6 +865,7 @@ extern "C" int qmoe_attn_decode_scored(const qmoe_bf16* q, const qmoe_bf16* k_ca
   QMOE_REQUIRE(B >= 0 && B < 65536 && S_max > 0 && S_max < (1ll << 30) && B * Hq < (1ll << 31),
                "%s: bad B/S_max", fn);
   QMOE_REQUIRE(max_ctx > 0 && max_ctx <= S_max, "%s: need 0 < max_ctx <= S_max", fn);
+  QMOE_REQUIRE(qmoe_attn_decode_scored_workspace(B, Hq, D, max_ctx) >= 0, "%s: B * Hq * max_ctx too large", fn);
   QMOE_REQUIRE(scale > 0.0f && std::isfinite(scale), "%s: scale must be positive and finite", fn);
   if (B == 0) return QMOE_OK;
   const int64_t split = sd_split(B, Hkv, max_ctx), ns = (max_ctx + split - 1) / split;
@@ -903,7 +906,9 @@ static void ev_launch(dim3 grid, const EvArgs& e, const EvMove& mv, hipStream_t 
 }
 
 extern "C" int64_t qmoe_kv_evict_workspace(int64_t B, int64_t Hkv, int64_t S_max, int64_t budget) {
-  if (B < 0 || Hkv < 0 || S_max < 0 || budget < 0) return -1;
+  if (B < 0 || B >= 65536 || Hkv < 0 || Hkv >= 65536 || B * Hkv >= 65536 || S_max < 0 || S_max >= (1ll << 30) ||
+      budget < 0)
+    return -1;
   return 2 * B * Hkv * std::min(budget, S_max) * int64_t(sizeof(int32_t));
 }
 
@@ -917,7 +922,7 @@ extern "C" int qmoe_kv_evict(const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
                           slot_pos_out),
                "%s: null pointer", fn);
   QMOE_REQUIRE(D == HD, "%s: head_dim must be 128 (D=%lld)", fn, (long long)D);
-  QMOE_REQUIRE(B >= 0 && Hkv > 0 && B * Hkv < 65536, "%s: need 0 <= B * Hkv < 65536", fn);
+  QMOE_REQUIRE(B >= 0 && B < 65536 && Hkv > 0 && Hkv < 65536 && B * Hkv < 65536, "%s: need 0 <= B * Hkv < 65536", fn);
   QMOE_REQUIRE(S_max > 0 && S_max < (1ll << 30) && S_out < (1ll << 30), "%s: bad S_max/S_out", fn);
   QMOE_REQUIRE(budget > 0 && recent >= 0 && sink >= 0 && recent <= budget - sink,
                "%s: need budget > 0 and 0 <= recent + sink <= budget", fn);

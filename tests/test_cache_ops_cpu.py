@@ -233,3 +233,33 @@ def test_wrappers_refuse_negative_counts():
               lambda: ops.attn_shared(q, kp, kp, k, k, n, 2 ** 33, 1), lambda: ops.attn_prefill_scored(q, k, k, sc, -1, -2)):
         with pytest.raises(ValueError, match="must be in"):
             f()
+
+
+BIG = 2 ** 63 - 1
+
+
+@pytest.mark.parametrize("fn,change,msg", [
+    (prompt, dict(start=BIG, ws=NONE), "start + S"), (prompt, dict(start=BIG - 3, ws=NONE), "start + S"),
+    (append, dict(Hq=2 ** 62, Hkv=2 ** 62, raw=A, qn=A, kn=A), "head counts"),
+    (evict, dict(B=2 ** 33, Hkv=2 ** 31, ws=NONE), "B * Hkv"),
+    (scored, dict(B=65535, Hq=32767, Hkv=32767, S_max=2 ** 30 - 1, max_ctx=2 ** 30 - 1, ws=NONE), "too large"),
+], ids=["start", "start3", "heads", "rows", "entries"])
+def test_c_entries_refuse_sizes_whose_sum_or_product_wraps(fn, change, msg):
+    """(With the workspace missing, so that nothing could run if they were not.)"""
+    assert fn(_lib.lib(), **change) == ERR
+    assert msg in _lib.last_error(), _lib.last_error()
+
+
+def test_workspace_queries_of_sizes_that_wrap():
+    l = _lib.lib()
+    for start in (BIG, BIG - 3, (1 << 22) - 4):
+        assert l.qmoe_attn_prefill_scored_workspace(1, 5, 32, 4, 128, start) == -1
+    assert l.qmoe_attn_prefill_scored_workspace(1, BIG, 32, 4, 128, 0) == -1
+    assert l.qmoe_attn_decode_scored_workspace(65535, 32767, 128, 2 ** 30 - 1) == -1
+    assert l.qmoe_attn_decode_scored_workspace(2 ** 40, 2 ** 40, 128, 64) == -1
+    assert l.qmoe_kv_evict_workspace(2 ** 33, 2 ** 31, 64, 32) == -1
+    assert l.qmoe_kv_evict_workspace(1, 1, 2 ** 62, 2 ** 62) == -1
+    # as large as the calls take
+    assert l.qmoe_attn_prefill_scored_workspace(1, 5, 32, 4, 128, (1 << 22) - 5) > 0
+    assert l.qmoe_attn_decode_scored_workspace(64, 32, 128, 1 << 22) == 64 * 32 * (1 << 14) * (130 + 256) * 4
+    assert l.qmoe_kv_evict_workspace(8191, 8, 2 ** 30 - 1, 1000) == 2 * 8191 * 8 * 1000 * 4
