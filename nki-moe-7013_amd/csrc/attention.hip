@@ -1334,7 +1334,7 @@ static int ap_launch(const char* fn, const qmoe_bf16* q, const qmoe_bf16* k_cach
   QMOE_REQUIRE(k_cache && v_cache && (B == 0 || S == 0 || (q && out)), "%s: null pointer", fn);
   QMOE_REQUIRE(D == HD, "%s: head_dim must be 128", fn);
   QMOE_REQUIRE(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq < 65536, "%s: bad heads", fn);
-  QMOE_REQUIRE(B >= 0 && B < 65536 && S >= 0 && S <= S_max && start >= 0 && start + S <= S_max,
+  QMOE_REQUIRE(B >= 0 && B < 65536 && S >= 0 && S <= S_max && start >= 0 && start <= S_max - S,
                "%s: need 0 <= start and start + S <= S_max", fn);
   QMOE_REQUIRE(S_max <= AP_MAX_SMAX, "%s: S_max must be <= %d", fn, AP_MAX_SMAX);
   QMOE_REQUIRE(ws_bytes >= 0 && (ws != nullptr || ws_bytes == 0), "%s: bad workspace", fn);

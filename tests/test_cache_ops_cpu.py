@@ -263,3 +263,11 @@ def test_workspace_queries_of_sizes_that_wrap():
     assert l.qmoe_attn_prefill_scored_workspace(1, 5, 32, 4, 128, (1 << 22) - 5) > 0
     assert l.qmoe_attn_decode_scored_workspace(64, 32, 128, 1 << 22) == 64 * 32 * (1 << 14) * (130 + 256) * 4
     assert l.qmoe_kv_evict_workspace(8191, 8, 2 ** 30 - 1, 1000) == 2 * 8191 * 8 * 1000 * 4
+
+
+def test_plain_prefill_attention_refuses_a_start_that_wraps():
+    l = _lib.lib()
+    for start in (BIG, BIG - 3):
+        for call in (lambda: l.qmoe_attn_prefill(1, 1, 1, 1, 4, 32, 4, 128, 64, start, 0.1, 1, NONE),
+                     lambda: l.qmoe_attn_prefill_ws(1, 1, 1, 1, 4, 32, 4, 128, 64, start, 0.1, NONE, 0, 1, NONE)):
+            assert call() == ERR and "start + S" in _lib.last_error()
