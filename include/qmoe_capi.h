@@ -568,7 +568,8 @@ int64_t qmoe_attn_shared_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv
  *   scores: f32 [B, Hkv, S_max]; entries past start + S are not touched;
  *   workspace: qmoe_attn_prefill_scored_workspace(B, S, Hq, Hkv, D, start)
  *   bytes, holding nothing between calls; calls that share one must not
- *   overlap.  Other arguments as qmoe_attn_prefill.  The entries
+ *   overlap.  out does not overlap q (the scores read q once more: refused).
+ *   Other arguments as qmoe_attn_prefill.  The entries
  *   [0, start + S) have to be finite.  Deterministic (no atomics).
  *   Limits: D == 128, Hq / Hkv <= 16, S_max <= 2^22, S * Hq < 2^23,
  *   B * S * Hq < 2^27, scale > 0.

@@ -755,6 +755,9 @@ extern "C" int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_c
                "%s: grid too large", fn);
   QMOE_REQUIRE(aligned16(q, k_cache, v_cache, static_cast<uint8_t*>(workspace), out),
                "%s: operands must be 16-byte aligned", fn);
+  const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
+  QMOE_REQUIRE((q0 < o0 ? o0 - q0 : q0 - o0) >= uintptr_t(B * S * Hq * AP_ROWB),
+               "%s: out overlaps q, which the scores read once more", fn);
   a.q = c.q = q;
   a.k = c.k = k_cache;
   a.v = v_cache;

@@ -835,7 +835,7 @@ def attn_prefill_scored(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.T
     of every cache entry, summed over the queries and the q heads of each
     group, to ``scores[B, Hkv, S_max]`` (f32, in place).  ``lengths`` (i32
     ``[B]``): of a right-padded row only the first ``lengths[b]`` queries count.
-    Returns ``[B*S, Hq*D]``."""
+    ``out`` is not ``q``.  Returns ``[B*S, Hq*D]``."""
     return _native().attn_prefill_scored(q, k_cache, v_cache, scores, B, S, start, lengths, scale, workspace, out)
 
 

@@ -271,3 +271,14 @@ def test_plain_prefill_attention_refuses_a_start_that_wraps():
         for call in (lambda: l.qmoe_attn_prefill(1, 1, 1, 1, 4, 32, 4, 128, 64, start, 0.1, 1, NONE),
                      lambda: l.qmoe_attn_prefill_ws(1, 1, 1, 1, 4, 32, 4, 128, 64, start, 0.1, NONE, 0, 1, NONE)):
             assert call() == ERR and "start + S" in _lib.last_error()
+
+
+def test_scored_prompt_refuses_an_output_on_its_queries():
+    """The attention would write over the queries that the scores still need (2 * 4 * 32 rows of 256 bytes)."""
+    l, rows = _lib.lib(), 2 * 4 * 32 * 256
+    for out in (A, A + rows - 16, A - rows + 16):
+        assert prompt(l, q=A, k=4 * A, v=5 * A, ws=6 * A, n=A, out=out) == ERR
+        assert "out overlaps q" in _lib.last_error(), _lib.last_error()
+    for out in (A + rows, A - rows):
+        assert prompt(l, q=A, k=4 * A, v=5 * A, ws=6 * A, out=out) == ERR
+        assert "workspace of 0 bytes" in _lib.last_error()

@@ -257,3 +257,19 @@ def test_arguments_that_need_no_alignment(dev):
         args.update(bad)
         with pytest.raises(ValueError, match="16-byte aligned"):
             ops.attn_decode_scored(args["q"], args["k"], args["v"], lens, scores, out=args["out"])
+
+
+def test_scored_prompt_refuses_its_queries_as_output(dev):
+    announce("scored prompt onto its queries")
+    g = torch.Generator(device=dev).manual_seed(9)
+    q, k, v = [bf16_randn(s, g, dev) for s in ((30, HQ, D), (1, HKV, 30, D), (1, HKV, 30, D))]
+    scores, q0 = torch.zeros(1, HKV, 30, device=dev), q.clone()
+    with pytest.raises(ValueError, match="out overlaps q"):
+        ops.attn_prefill_scored(q, k, v, scores, 1, 30, out=q.view(30, HQ * D))
+    assert torch.equal(q, q0) and not bool(scores.any())
+    # the other two read their queries first: out may be q
+    want = ops.attn_shared(q, k[0], v[0], k, v, torch.ones(1, dtype=torch.int32, device=dev), 1, 30)
+    mine = q.clone()
+    ops.attn_shared(mine, k[0], v[0], k, v, torch.ones(1, dtype=torch.int32, device=dev), 1, 30,
+                    out=mine.view(30, HQ * D))
+    assert torch.equal(mine.view(30, HQ * D), want)
