@@ -8,7 +8,9 @@ then linked into qmoe/libqmoe.so next to the Python bindings; bind/native.cpp
 qmoe/_native.so, which links to it; probes/*.hip (measurement kernels that
 bench.py uses for measured peaks, not part of the C ABI) go into
 qmoe/libqmoe_probe.so.  Every HIP translation unit is built
-with packed-FP32 instruction selection disabled.
+with packed-FP32 instruction selection disabled.  The libraries need hipcc
+alone: without torch the extension module, which only qmoe/ops.py loads, is
+left out.
 """
 
 from __future__ import annotations
@@ -69,14 +71,20 @@ def _compile(src: str) -> str:
 
 def _build_native() -> None:
     """The extension module, with the host compiler: no device code in it."""
-    import torch
-    from torch.utils import cpp_extension
-
+    try:
+        import torch
+        from torch.utils import cpp_extension
+    except ImportError as e:
+        if os.path.exists(NATIVE):  # of an earlier library
+            os.remove(NATIVE)
+        print(f"qmoe/_native.so (the cache operators of qmoe/ops.py) is not built: {e}", file=sys.stderr)
+        return
     lib_dir = os.path.join(os.path.dirname(torch.__file__), "lib")
     rocm = os.path.dirname(os.path.dirname(hipcc()))
     includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], os.path.join(rocm, "include"),
                 os.path.join(ROOT, "include")]
-    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    cxx = shutil.which("g++") or shutil.which("c++") or os.path.join(rocm, "llvm", "bin", "clang++")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *[f"-I{i}" for i in includes], NATIVE_SRC, "-o", NATIVE + ".tmp", f"-L{lib_dir}", "-ltorch_python",
            "-ltorch_cpu", "-lc10", "-lc10_hip", f"-L{os.path.dirname(LIB)}", "-l:libqmoe.so", "-Wl,-rpath,$ORIGIN",
@@ -100,7 +108,6 @@ def build(jobs: int = 8) -> str:
     if r.returncode != 0:
         raise RuntimeError("link failed:\n" + r.stdout + r.stderr)
     os.replace(tmp, LIB)
-    _build_native()
     # measurement probes (bench.py's measured peaks): a library of their own
     psrcs = sorted(os.path.join(PROBES, f) for f in os.listdir(PROBES) if f.endswith(".hip"))
     pobjs = [_compile(p) for p in psrcs]
@@ -110,6 +117,7 @@ def build(jobs: int = 8) -> str:
         raise RuntimeError("probe link failed:\n" + r.stdout + r.stderr)
     os.replace(PROBE_LIB + ".tmp", PROBE_LIB)
     _write_build_info()
+    _build_native()
     return LIB
 
 
