@@ -590,7 +590,9 @@ int64_t qmoe_attn_prefill_scored_workspace(int64_t B, int64_t S, int64_t Hq, int
  * adds each slot's attention weight, summed over the group's q heads, to
  * scores[b, kvh, slot].  Slots past ctx_len are neither read nor scored.
  *   scores: f32 [B, Hkv, S_max]; workspace:
- *   qmoe_attn_decode_scored_workspace(B, Hq, D, max_ctx) bytes, holding nothing
+ *   qmoe_attn_decode_scored_workspace(B, Hq, D, max_ctx) bytes (the logits and
+ *   the splits' outputs: about 6 bytes an entry of each q head, 12 up to 4096
+ *   entries; 1.6 GB for 32 heads of 64 rows of 131072), holding nothing
  *   between calls; calls that share one must not overlap.  Deterministic;
  *   max_ctx decides how the keys are cut, so calls of another max_ctx may
  *   differ in the last bits, outputs and scores (qmoe_attn_decode_bucket's do
@@ -612,7 +614,8 @@ int64_t qmoe_attn_decode_scored_workspace(int64_t B, int64_t Hq, int64_t D, int6
  * to q_out, the K and V rows to slot slots[b] of row b, scores[b, :, slot] = 0
  * and slot_pos[b, :, slot] = positions[b].  A row whose position is outside
  * [0, max_pos) or slot outside [0, S_max) writes no cache entry and gets a zero
- * q.
+ * q; its slot is not to count in the ctx_len of what follows.  No operand has to
+ * be aligned beyond its elements.
  *   qkv: f32 [B, (Hq + 2*Hkv)*D]; positions, slots: i32 [B]; q_out: bf16
  *   [B, Hq, D]; scores: f32 and slot_pos: i32 [B, Hkv, S_max], each may be
  *   NULL.  Limits: D == 128.

@@ -189,8 +189,11 @@ __device__ __forceinline__ void ar_item(const ArArgs& a, const ArKind kd, const 
 
 // Both kinds of item in one launch: the prefix's tiles are bound by the matrix
 // pipe beside the softmax's VALU work (two causal prompts of 4096: 300 us, 0.92
-// PFLOP/s), the streams by the L2's round trips (32 rows on 8192 + up to 300 entries:
-// 20 us, 134 MB), and they share the CUs (64 rows on 32768 + up to 300: 60 us).
+// PFLOP/s), the streams by their waves' chains, a loaded round trip and then the
+// MFMAs and the softmax of each 64-key tile (32 rows on 8192 + up to 512 entries:
+// 20 us, four tiles a wave of the prefix and one of the own entries; the 134 MB come
+// at 6.6 TB/s, of the 37 that the L2s deliver), and they share the CUs (64 rows on
+// 32768 + up to 1024: 60 us).
 template <bool TILES, bool STREAMS>
 __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];

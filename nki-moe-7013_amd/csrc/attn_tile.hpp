@@ -86,6 +86,13 @@ constexpr int FL_SMEM = 4 * AP_TILE;  // K0, K1, V0, V1
 // requested.  The maximum is lazy: O and l are rescaled only when a row's
 // tile maximum exceeds it by more than AP_TAU, so p stays below 2^AP_TAU and
 // O / l is the same.  Every wave of the workgroup calls this alike.
+//
+// The weights are rounded to bf16 for the product with V, whose MFMA takes both
+// operands in the cache's type (half a step, 2^-9 to 2^-8 of each weight), and l
+// sums them in 32 bits before that.  With the lazy maximum a row's leading weight is
+// any value up to 2^8 rather than 1, so it is rounded too: relative error of a
+// chunk's outputs against 64 bits 0.0021-0.0023, of which the rounding of the
+// output itself is 0.0016-0.0017 (stream_segment, whose maximum is exact: 0.0018).
 __device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
                                               int lim, int first, int last, float scale_log2, FlashRows& st) {
   const int t = threadIdx.x, lane = t & 63, hl = lane >> 5;
@@ -251,7 +258,8 @@ __device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, 
 // w, w + 4, ... of keys [0, n_keys) of k / v.  K rows go from memory straight
 // into A-operand registers and V by DMA into the wave's own LDS tile, every load
 // of a tile in flight at once and no barrier between the waves; flash_join adds
-// up their states.  Lane's row sees keys [0, lim].
+// up their states.  Lane's row sees keys [0, lim].  Weights in bf16 for the MFMA with V
+// and l in 32 bits, as in flash_segment.
 __device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
                                                int lim, float scale_log2, FlashRows& st) {
   const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5;

@@ -98,7 +98,10 @@ __device__ __forceinline__ int sd_ctx(const SdArgs& a, int b) { return min(max(a
 // the G q heads in the columns of S^T = K . Q^T and O^T = V^T . P^T.  Every load of
 // a wave is in flight at once, so a wave costs one round trip to memory; K and
 // V take turns in the wave's own LDS tile.  The logits leave as four
-// consecutive keys a lane.  Bound by memory: 32 rows of up to 4160 entries, 171 MB,
+// consecutive keys a lane.  The weights are rounded to bf16 for the MFMA with V alone
+// (half a step each; relative error of the outputs 0.0017 against 64 bits, with
+// the output's own rounding); their sum l and what the scores get stay in 32 bits.
+// Bound by memory: 32 rows of up to 4160 entries, 171 MB,
 // in 39 us (4.4 TB/s); 44 us with K's A operands loaded straight from the cache, 32
 // bytes of each of 32 rows an instruction.
 // WAVES = 1 (few keys in all): K does go straight into its operands, since the
@@ -615,7 +618,10 @@ constexpr int ev_lds() {
 static_assert(ev_lds<16>() <= 160 * 1024, "LDS");
 
 // The same for longer caches: the ranks are read again from LDS or memory for
-// every pass, the movers' slots go through the workspace.
+// every pass, the movers' slots go through the workspace.  Bound by one workgroup's
+// passes over a (row, kv head), six or more of them (with the moves, into another
+// cache, 4 heads: 16,385 entries to 1024 36 us, 16,384 in registers 28; 32,768 to
+// 2048 60 us; past EV_LDS_KEYS from memory, 131,072 to 4096 358 us).
 __global__ __launch_bounds__(EV_THREADS) void kv_select_long_kernel(const EvArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint32_t ev_smem[];
   uint32_t* hist = ev_smem;                                    // [EV_BINS]
