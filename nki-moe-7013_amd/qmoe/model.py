@@ -723,14 +723,16 @@ class NeuronQwen3MoeForCausalLM:
         row has a real token."""
         B, S = input_ids.shape
         dev = self.device
-        # a bounded cache's scratch holds any prompt and a row's own cache is not
-        # shorter for a prefix in front of it, so no operator sees the limit
-        if S > self._positions():
-            raise ValueError(f"a prompt of {S} tokens does not fit the {self._positions()} positions there are"
-                             + (f" after a prefix of {self.model.base}" if self.model.base else ""))
-        real = [S] * B if lengths is None else [int(n) for n in lengths]
+        real = [S] * B if lengths is None else [int(n) for n in lengths.tolist()]
         if len(real) != B or any(not 1 <= n <= S for n in real):
             raise ValueError(f"lengths must be {B} numbers from 1 to {S} (got {real})")
+        # a bounded cache's scratch holds any prompt and a row's own cache is not
+        # shorter for a prefix in front of it, so no operator sees the limit; a plain
+        # cache's operators do, and its padding may lie past the tables
+        last = max(real, default=0) if self._contiguous() else S
+        if last > self._positions():
+            raise ValueError(f"a prompt of {last} tokens does not fit the {self._positions()} positions there are"
+                             + (f" after a prefix of {self.model.base}" if self.model.base else ""))
         pos = torch.arange(S, device=dev, dtype=torch.int32).repeat(B)
         budget = self._budget_of(B)
         if budget is not None:

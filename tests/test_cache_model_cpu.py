@@ -15,12 +15,13 @@ H, E, D, V, HKV = 64, 4, 16, 50, 1
 class _Causal(qm.NeuronQwen3MoeForCausalLM):
     """The real host class over a real model object on the CPU whose layers do nothing but note the call."""
 
-    def __init__(self, batch=2, max_length=20, **kw):
+    def __init__(self, batch=2, max_length=20, max_position_embeddings=40960, **kw):
         nc = qm.MoENeuronConfig(batch_size=batch, max_batch_size=batch, seq_len=max_length, max_length=max_length,
                                 **kw)
         config = qm.Qwen3MoeInferenceConfig(
             nc, num_hidden_layers=2, hidden_size=H, num_experts=E, moe_intermediate_size=32, num_attention_heads=2,
-            num_key_value_heads=HKV, head_dim=D, vocab_size=V, num_experts_per_tok=2, tie_word_embeddings=False)
+            num_key_value_heads=HKV, head_dim=D, vocab_size=V, num_experts_per_tok=2, tie_word_embeddings=False,
+            max_position_embeddings=max_position_embeddings)
         super().__init__(None, config)
         self.device = torch.device("cpu")
         params = qm.random_params(config, "cpu", seed=1)
@@ -58,11 +59,24 @@ def test_prefill_refuses_a_prompt_past_the_last_position(kind):
     if kind == "bounded":
         m.decode_step(_tokens(2))
     before, n, position = _stand(m), len(m.calls), m.position
-    for call in (lambda: m.prefill(_tokens(2, 22 - P)), lambda: m.prefill(_tokens(2, 40), torch.tensor([3, 4])),
-                 lambda: m.forward(_tokens(2, 22 - P))):
+    calls = [lambda: m.prefill(_tokens(2, 22 - P)), lambda: m.forward(_tokens(2, 22 - P))]
+    if kind != "plain":  # (there the operators refuse it)
+        calls.append(lambda: m.prefill(_tokens(2, 40), torch.tensor([3, 4])))
+    for call in calls:
         with pytest.raises(ValueError, match="positions"):
             call()
     assert (_stand(m), len(m.calls), m.position) == (before, n, position)
+
+
+def test_padding_past_the_tables_of_a_plain_cache():
+    """Positions that the model has no embedding for, in rows that end before them."""
+    m = _Causal(max_position_embeddings=10)
+    assert m._positions() == 10 and m.model.caches()[0].capacity == 21
+    m.prefill(_tokens(2, 15), torch.tensor([9, 10]))
+    assert m.calls[-1][2] == 15
+    for lengths in (torch.tensor([9, 11]), None):
+        with pytest.raises(ValueError, match="positions"):
+            m.prefill(_tokens(2, 15), lengths)
 
 
 @pytest.mark.parametrize("bounded", [False, True])
