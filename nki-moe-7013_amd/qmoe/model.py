@@ -329,7 +329,7 @@ class NeuronQwen3MoeModel:
         self.rope = self.rope_full = rope_tables(config.head_dim, max_pos, float(config.rope_theta), dev)
         self.base = 0  # tokens of a shared prefix: the position of cache index 0, where ``rope`` starts
         self.budget: Optional[CacheBudget] = None
-        self.allocations = 0  # of caches: a captured step is good for those it was captured with
+        self.allocations = 0  # of caches and prefixes: a captured step is good for those it was captured with
         # set by the embedding gather when a token id is outside the vocabulary
         self.embed_err = torch.zeros(1, dtype=torch.int32, device=dev)
 
@@ -368,6 +368,9 @@ class NeuronQwen3MoeModel:
         ``budget`` entries a kv head, if that is fewer) the prefix of every
         row's cache; an empty ``input_ids`` takes the prefix away."""
         P, dev, c = input_ids.shape[1], self.embed_tokens.device, self.config
+        if self.budget is not None:
+            raise ValueError("a prefix is shared by contiguous caches (kv_cache_budget is set); "
+                             "pass budget here to keep part of the prefix")
         if P >= self.rope_full[0].shape[0]:
             raise ValueError(f"a prefix of {P} tokens leaves no position of {self.rope_full[0].shape[0]} to continue at")
         if budget:
@@ -376,6 +379,7 @@ class NeuronQwen3MoeModel:
         for cache in own:
             cache.prefix = None
         self.base, self.rope = 0, self.rope_full
+        self.allocations += 1  # captured steps hold the old prefix's addresses
         if P == 0:
             return
         n = P
@@ -662,24 +666,17 @@ class NeuronQwen3MoeForCausalLM:
         nothing; a token outside the vocabulary leaves no prefix at all."""
         if self.model is None:
             raise RuntimeError("load() the model first")
-        if self.model.budget is not None:
-            raise ValueError("a prefix is shared by contiguous caches (kv_cache_budget is set); "
-                             "pass budget here to keep part of the prefix")
         ids = prefix_ids.reshape(1, -1)
         if prefix_ids.dim() > 2 or (prefix_ids.dim() == 2 and prefix_ids.shape[0] != 1) or ids.shape[1] == 0:
             raise ValueError("prefix_ids must be [P] or [1, P] with P > 0")
         budget, sink = int(budget), min(int(sink), int(budget))
         recent = default_recent(budget, sink) if recent is None else int(recent)
-        try:
-            self.model.set_prefix(ids, budget, recent, sink)
-        finally:
-            self._graphs.clear()  # captured steps hold the old prefix's addresses
+        self.model.set_prefix(ids, budget, recent, sink)
         self.reset()
 
     def drop_prefix(self) -> None:
         """Sequences start at position 0 again."""
         if self.model is not None and self.model.base:
-            self._graphs.clear()
             self.model.set_prefix(torch.empty(1, 0, dtype=torch.long))
             self.reset()
 
@@ -835,8 +832,8 @@ class NeuronQwen3MoeForCausalLM:
         return min(b, cap)
 
     def _fresh_graphs(self) -> None:
-        """Drops captured steps that hold the addresses of caches that the model no
-        longer has."""
+        """Drops captured steps that hold the addresses of caches or a prefix that
+        the model no longer has."""
         if self._graphs_of != self.model.allocations:
             self._graphs.clear()
             self._graphs_of = self.model.allocations

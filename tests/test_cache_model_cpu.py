@@ -323,3 +323,24 @@ def test_prefill_refuses_lengths_outside_the_prompt(kind):
     with pytest.raises(ValueError, match="lengths"):
         m.prefill(_tokens(2, 1), torch.tensor([1, 2]))
     assert (_stand(m), len(m.calls), m.position) == (before, n, 5)
+
+
+def test_a_prefix_set_on_the_model_itself(monkeypatch):
+    """As through share_prefix: captured steps go with the prefix that they saw, and
+    bounded caches, whose attention would not see it, take none."""
+    monkeypatch.setattr(ops, "argmax_workspace", lambda *args: None)
+    m = _Causal()
+    for P in (4, 6, 0):
+        state = m._decode_state(2)
+        m._graphs[("decode", 2, 21)] = object()
+        m.model.set_prefix(_tokens(1, P))
+        assert m._decode_state(2) is not state and list(m._graphs) == [("state", 2)]
+    state = m._decode_state(2)
+    with pytest.raises(ValueError, match="no position"):  # refused: nothing changes
+        m.model.set_prefix(_tokens(1, 21))
+    assert m._decode_state(2) is state
+    m = _Causal(kv_cache_budget=8)
+    for call in (lambda: m.model.set_prefix(_tokens(1, 4)), lambda: m.share_prefix(_tokens(4))):
+        with pytest.raises(ValueError, match="kv_cache_budget"):
+            call()
+    assert m.model.base == 0
