@@ -631,7 +631,9 @@ int qmoe_kv_append(const float* qkv, const qmoe_bf16* q_norm_w, const qmoe_bf16*
  * n = clamp(ctx_len[b], 0, S_max) entries, where n > budget, these stay, in this
  * order of precedence: entries with slot_pos < sink or slot_pos > newest -
  * recent (newest: the largest slot_pos of the n); then the largest scores (NaN
- * ranks highest, -0 as 0).  Ties go to the lowest slot.  Kept entries below slot
+ * ranks highest, -0 as 0).  Ties go to the lowest slot, and so it is among the
+ * protected entries where positions repeat and more than `budget` are (their
+ * scores do not count).  Kept entries below slot
  * `budget` stay where they are; the i-th kept entry past it moves to the i-th
  * freed slot (K, V, score and position).  Afterwards slots [0, min(n, budget))
  * hold the kept entries; the scores of all other slots are 0 and their

@@ -273,3 +273,27 @@ def test_scored_prompt_refuses_its_queries_as_output(dev):
     ops.attn_shared(mine, k[0], v[0], k, v, torch.ones(1, dtype=torch.int32, device=dev), 1, 30,
                     out=mine.view(30, HQ * D))
     assert torch.equal(mine.view(30, HQ * D), want)
+
+
+@pytest.mark.parametrize("n,budget,recent,sink", [(9, 3, 1, 2), (313, 6, 0, 6), (881, 84, 37, 4), (20_000, 90, 40, 9)])
+def test_eviction_with_more_protected_entries_than_the_budget(dev, n, budget, recent, sink):
+    """Positions that repeat: more entries are protected than stay.  They rank alike
+    whatever their scores, NaN among them, so the lowest slots stay."""
+    announce(f"eviction, {n} entries to {budget}, positions that repeat")
+    g = torch.Generator(device=dev).manual_seed(n)
+    k, v = [bf16_randn((1, 2, n, D), g, dev) for _ in range(2)]
+    sc = torch.randn(1, 2, n, generator=g, device=dev)
+    sc[torch.rand(1, 2, n, generator=g, device=dev) < 0.2] = float("nan")
+    pos = (torch.rand(1, 2, n, generator=g, device=dev).argsort(-1) // 3).int().contiguous()
+    k0, pos0 = k.clone(), pos.clone()
+    ops.kv_evict(k, v, sc, pos, torch.tensor([n], dtype=torch.int32, device=dev), budget, recent, sink)
+    for h in range(2):
+        held = ((pos0[0, h] < sink) | (pos0[0, h] > pos0[0, h].max() - recent)).nonzero()[:, 0]
+        assert len(held) > budget
+        keep = held[:budget]
+        stay, order = keep[keep < budget], torch.arange(budget, device=dev)
+        hole = torch.ones(budget, dtype=torch.bool, device=dev)
+        hole[stay] = False
+        order[hole] = keep[keep >= budget]
+        assert torch.equal(pos[0, h, :budget], pos0[0, h, order]) and torch.equal(k[0, h, :budget], k0[0, h, order])
+        assert bool((pos[0, h, budget:] == -1).all())
