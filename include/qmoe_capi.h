@@ -87,8 +87,10 @@ typedef void* qmoe_stream_t;
  * qmoe_attn_prefill_ws / qmoe_attn_prefill_workspace are new.  Entry points
  * added since leave the earlier ones as they were: qmoe_attn_shared,
  * qmoe_attn_prefill_scored, qmoe_attn_decode_scored, qmoe_kv_append,
- * qmoe_kv_evict and their workspace queries.  All but qmoe_kv_append
- * refuse bf16 tensors and attention workspaces that are not 16-byte aligned. */
+ * qmoe_kv_evict, qmoe_attn_window, qmoe_attn_kv4 and their workspace queries,
+ * qmoe_kv4_store, qmoe_kv4_load, qmoe_kv4_append.  All but the two that append
+ * refuse tensors read or written by rows and attention workspaces that are not
+ * 16-byte aligned. */
 #define QMOE_VERSION 3
 
 int qmoe_version(void);
@@ -655,6 +657,90 @@ int qmoe_kv_evict(const qmoe_bf16* k_cache, const qmoe_bf16* v_cache, const floa
 /* Workspace bytes of qmoe_kv_evict (-1 for bad sizes).
  * Replaces: nothing in the reference (a sizing helper of this library). */
 int64_t qmoe_kv_evict_workspace(int64_t B, int64_t Hkv, int64_t S_max, int64_t budget);
+
+/* Attention with a sliding window and a few first entries that stay visible.
+ * Query s of row b stands at index p = c - 1 + s, c = min(ctx_len[b], S_max)
+ * (decode: S = 1 and ctx_len counts the new token's entry; a chunk whose tokens
+ * start at entry e: ctx_len = e + 1), and sees the entries e <= p of its row's
+ * cache with e > p - window or e < sink, none of them from max_ctx on.  A query
+ * that sees nothing gets zeros.
+ *   q: bf16 [B*S, Hq, D]; k_cache, v_cache: bf16 [B, Hkv, S_max, D]; ctx_len:
+ *   i32 [B]; window > 0, sink >= 0; max_ctx <= S_max sizes the launch; scale > 0;
+ *   workspace: qmoe_attn_window_workspace(B, S, Hq, Hkv, D, window, sink,
+ *   max_ctx) bytes (NULL when that is 0), holding nothing between calls; calls
+ *   that share one must not overlap.  out: bf16 [B*S, Hq*D], not overlapping q.
+ *   The entries that some query of a chunk sees have to be finite (a NaN value
+ *   reaches the queries that do not see it); entries that no query sees are not
+ *   read.  Deterministic; calls of another max_ctx may differ in the last bits.
+ *   Limits: D == 128, Hq / Hkv <= 16, S_max <= 2^22, B * S * Hq < 2^27.
+ * Replaces: the attention of NeuronQwen3MoEAttention (qwen_with_nki.py:9943-9946,
+ *   10081-10109) for a checkpoint whose config sets use_sliding_window; the
+ *   first entries that stay have no counterpart in the reference. */
+int qmoe_attn_window(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache, const int32_t* ctx_len,
+                     int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max, int64_t max_ctx,
+                     int64_t window, int64_t sink, float scale, void* workspace, int64_t workspace_bytes,
+                     qmoe_bf16* out, qmoe_stream_t stream);
+
+/* Workspace bytes of qmoe_attn_window on the current device (-1 for bad sizes).
+ * Replaces: nothing in the reference (a sizing helper of this library). */
+int64_t qmoe_attn_window_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                                   int64_t sink, int64_t max_ctx);
+
+/* The cache in 4 bits: an entry is 128 e2m1 numbers (0, 0.5, 1, 1.5, 2, 3, 4, 6
+ * and their negatives, codes 0-7 and 8-15; two a byte, the even element in the
+ * low half) and a power of two for every 32 of them (a byte p for 2^(p - 127)).
+ * k_cache, v_cache: u8 [B, Hkv, S_max, 64]; k_scales, v_scales: u8 [B, Hkv,
+ * S_max, 4].  A block's power is the smallest in [7, 252] whose seventh multiple
+ * is above the block's largest magnitude; elements round to the nearest number,
+ * ties to the even code, and what is past 6 to 6.  A block with an infinity or a
+ * NaN has the power 255 and reads as NaN.  Bytes of 0 read as 0. */
+
+/* qmoe_attn_window over a cache in 4 bits; window 0: every entry up to the
+ * query's own.  Rules, limits and workspace as there.
+ * Replaces: the attention over the KV cache (qwen_with_nki.py:9943-9946); the
+ *   reference's cache is in bf16. */
+int qmoe_attn_kv4(const qmoe_bf16* q, const uint8_t* k_cache, const uint8_t* k_scales, const uint8_t* v_cache,
+                  const uint8_t* v_scales, const int32_t* ctx_len, int64_t B, int64_t S, int64_t Hq, int64_t Hkv,
+                  int64_t D, int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
+                  void* workspace, int64_t workspace_bytes, qmoe_bf16* out, qmoe_stream_t stream);
+
+/* Workspace bytes of qmoe_attn_kv4 on the current device (-1 for bad sizes).
+ * Replaces: nothing in the reference (a sizing helper of this library). */
+int64_t qmoe_attn_kv4_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                                int64_t sink, int64_t max_ctx);
+
+/* Rows of a bf16 cache into one in 4 bits: token s < min(n, lengths[b]) of row b
+ * becomes entry starts[b] + s, if that is in [0, S_max); every other entry stays
+ * as it was.
+ *   k, v: bf16 [B, Hkv, S_src, D], tokens [0, n) of which are read; starts,
+ *   lengths: i32 [B], each may be NULL (0 and n).  Limits: D == 128.
+ * Replaces: the KV-cache update (qwen_with_nki.py:9943-9946). */
+int qmoe_kv4_store(const qmoe_bf16* k, const qmoe_bf16* v, int64_t S_src, int64_t n, const int32_t* starts,
+                   const int32_t* lengths, int64_t B, int64_t Hkv, int64_t D, int64_t S_max, uint8_t* k_cache,
+                   uint8_t* k_scales, uint8_t* v_cache, uint8_t* v_scales, qmoe_stream_t stream);
+
+/* Entries [0, n) of a cache in 4 bits as bf16 rows k, v: [B, Hkv, n, D] (exact).
+ *   n <= S_max.  Limits: D == 128.
+ * Replaces: nothing in the reference, whose cache is in bf16. */
+int qmoe_kv4_load(const uint8_t* k_cache, const uint8_t* k_scales, const uint8_t* v_cache, const uint8_t* v_scales,
+                  int64_t B, int64_t Hkv, int64_t D, int64_t S_max, int64_t n, qmoe_bf16* k, qmoe_bf16* v,
+                  qmoe_stream_t stream);
+
+/* qmoe_kv_append into a cache in 4 bits, S tokens a row: token t = b * S + s at
+ * positions[t] into entry slots[t] of row b.  Queries have qmoe_kv_append's bits;
+ * keys are computed in 64 bits and rounded once, values are the projection's.  The
+ * slots of a row's tokens have to differ.  A token whose position is outside
+ * [0, max_pos) or slot outside [0, S_max) writes no entry and gets a zero q.
+ *   qkv: f32 [B*S, (Hq + 2*Hkv)*D]; positions, slots: i32 [B*S]; q_out: bf16
+ *   [B*S, Hq, D].  The caches' rows are 4-byte aligned, the rest as its elements.
+ *   Limits: D == 128, B * S < 65536.
+ * Replaces: q_layernorm/k_layernorm, RoPE and the KV-cache update of
+ *   NeuronQwen3MoEAttention (qwen_with_nki.py:10102-10103, 10083-10087,
+ *   9943-9946). */
+int qmoe_kv4_append(const float* qkv, const qmoe_bf16* q_norm_w, const qmoe_bf16* k_norm_w, const float* rope_cos,
+                    const float* rope_sin, int64_t max_pos, const int32_t* positions, const int32_t* slots, int64_t B,
+                    int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max, float eps, qmoe_bf16* q_out,
+                    uint8_t* k_cache, uint8_t* k_scales, uint8_t* v_cache, uint8_t* v_scales, qmoe_stream_t stream);
 
 /* Token embedding gather into the fp32 residual stream:
  *   out[i, :] = float(table[ids[i], :]);  table: bf16 [V, H]; ids: i64 [n];

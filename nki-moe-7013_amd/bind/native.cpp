@@ -410,6 +410,155 @@ void kv_evict(py::handle k_cache, py::handle v_cache, py::handle scores, py::han
         "qmoe_kv_evict");
 }
 
+// A cache in 4 bits: (k, k_scales, v, v_scales).
+struct Cache4 {
+  int ix;
+  int64_t B, Hkv, S_max, D;
+  uint8_t* p[4];
+  Cache4(py::handle cache, uintptr_t align, uintptr_t scales_align) {
+    static const char* const names[4] = {"cache k", "cache k_scales", "cache v", "cache v_scales"};
+    if (!PySequence_Check(cache.ptr()) || THPVariable_Check(cache.ptr()) || PySequence_Size(cache.ptr()) != 4)
+      refuse("cache must be (k, k_scales, v, v_scales)");
+    const py::sequence s = py::reinterpret_borrow<py::sequence>(cache);
+    const py::object o[4] = {s[0], s[1], s[2], s[3]};
+    const at::Tensor& k = tensor(o[0], names[0]);
+    ix = gpu_of(k, names[0], "[B, Hkv, S_max, D / 2]", 4);
+    B = k.size(0);
+    Hkv = k.size(1);
+    S_max = k.size(2);
+    const int64_t w = k.size(3);
+    for (int i = 0; i < 4; ++i) {
+      const int64_t shape[4] = {B, Hkv, S_max, i % 2 ? w / 16 : w};
+      p[i] = static_cast<uint8_t*>(
+          address(tensor(o[i], names[i]), names[i], U8, at::IntArrayRef(shape), ix, i % 2 ? scales_align : align));
+    }
+    D = 2 * w;
+  }
+  void holds(int64_t rows, int64_t head_dim) const {
+    if (B != rows || D != head_dim)
+      refuse("cache must hold B=" + std::to_string(rows) + " rows of D=" + std::to_string(head_dim) + " (got B=" +
+             std::to_string(B) + ", D=" + std::to_string(D) + ")");
+  }
+};
+
+void same(const Queries& x, int ix) {
+  if (x.ix != ix) refuse("tensors are on different devices: q is on cuda:" + std::to_string(x.ix) + ", the cache on cuda:" +
+                         std::to_string(ix));
+}
+
+py::object attn_window(py::handle q, py::handle k_cache, py::handle v_cache, py::handle ctx_len, py::handle batch,
+                       py::handle queries, py::handle last, py::handle first, py::handle scale, py::handle workspace,
+                       py::handle out, py::handle max_ctx) {
+  const int64_t B = count(batch, "B"), S = count(queries, "S");
+  const int64_t window = within(last, "window", 1, INT64_MAX), sink = within(first, "sink", 0, INT64_MAX);
+  const Queries x(q, B * S, "[B*S, Hq, D]");
+  int64_t Hkv, S_max;
+  cache_sizes(tensor(k_cache, "k_cache"), B, x.D, Hkv, S_max);
+  heads(x.Hq, Hkv);
+  const int64_t ctx = within(max_ctx, "max_ctx", 0, S_max, S_max);
+  const float sc = scale_of(scale, x.D);
+  const Bf* pk = arg<Bf>(k_cache, "k_cache", BF16, {B, Hkv, S_max, x.D}, x.ix);
+  const Bf* pv = arg<Bf>(v_cache, "v_cache", BF16, {B, Hkv, S_max, x.D}, x.ix);
+  const int32_t* pc = arg<int32_t>(ctx_len, "ctx_len", I32, {B}, x.ix);
+  const On on(x.ix);
+  const Output o(out, "out", BF16, {x.T, x.Hq * x.D}, x.ix, 16);
+  const Scratch ws(workspace,
+                   size(qmoe_attn_window_workspace(B, S, x.Hq, Hkv, x.D, window, sink, ctx), "qmoe_attn_window"), x.ix,
+                   16);
+  check(qmoe_attn_window(x.p, pk, pv, pc, B, S, x.Hq, Hkv, x.D, S_max, ctx, window, sink, sc, ws.p, ws.bytes,
+                         static_cast<Bf*>(o.p), stream(x.ix)),
+        "qmoe_attn_window");
+  return o.obj;
+}
+
+py::object attn_kv4(py::handle q, py::handle cache, py::handle ctx_len, py::handle batch, py::handle queries,
+                    py::handle last, py::handle first, py::handle scale, py::handle workspace, py::handle out,
+                    py::handle max_ctx) {
+  const int64_t B = count(batch, "B"), S = count(queries, "S");
+  const int64_t window = within(last, "window", 0, INT64_MAX), sink = within(first, "sink", 0, INT64_MAX);
+  const Queries x(q, B * S, "[B*S, Hq, D]");
+  const Cache4 c(cache, 16, 16);
+  c.holds(B, x.D);
+  same(x, c.ix);
+  heads(x.Hq, c.Hkv);
+  const int64_t ctx = within(max_ctx, "max_ctx", 0, c.S_max, c.S_max);
+  const float sc = scale_of(scale, x.D);
+  const int32_t* pc = arg<int32_t>(ctx_len, "ctx_len", I32, {B}, x.ix);
+  const On on(x.ix);
+  const Output o(out, "out", BF16, {x.T, x.Hq * x.D}, x.ix, 16);
+  const Scratch ws(workspace,
+                   size(qmoe_attn_kv4_workspace(B, S, x.Hq, c.Hkv, x.D, window, sink, ctx), "qmoe_attn_kv4"), x.ix, 16);
+  check(qmoe_attn_kv4(x.p, c.p[0], c.p[1], c.p[2], c.p[3], pc, B, S, x.Hq, c.Hkv, x.D, c.S_max, ctx, window, sink, sc,
+                      ws.p, ws.bytes, static_cast<Bf*>(o.p), stream(x.ix)),
+        "qmoe_attn_kv4");
+  return o.obj;
+}
+
+void kv4_store(py::handle k, py::handle v, py::handle cache, py::handle starts, py::handle lengths, py::handle tokens) {
+  const Cache4 c(cache, 16, any_alignment);
+  int64_t Hkv, S;
+  const at::Tensor& src = tensor(k, "k");
+  if (src.dim() != 4 || src.size(0) != c.B || src.size(1) != c.Hkv || src.size(3) != c.D)
+    refuse("k must be [B=" + std::to_string(c.B) + ", Hkv=" + std::to_string(c.Hkv) + ", S, D=" + std::to_string(c.D) +
+           "] (got " + text(src.sizes()) + ")");
+  Hkv = src.size(1);
+  S = src.size(2);
+  const int64_t n = within(tokens, "n", 0, S, S);
+  const Bf* pk = arg<Bf>(k, "k", BF16, {c.B, Hkv, S, c.D}, c.ix);
+  const Bf* pv = arg<Bf>(v, "v", BF16, {c.B, Hkv, S, c.D}, c.ix);
+  const int32_t* ps = optional_arg<int32_t>(starts, "starts", I32, {c.B}, c.ix);
+  const int32_t* pl = optional_arg<int32_t>(lengths, "lengths", I32, {c.B}, c.ix);
+  const On on(c.ix);
+  check(qmoe_kv4_store(pk, pv, S, n, ps, pl, c.B, Hkv, c.D, c.S_max, c.p[0], c.p[1], c.p[2], c.p[3], stream(c.ix)),
+        "qmoe_kv4_store");
+}
+
+py::object kv4_load(py::handle cache, py::handle entries, py::handle out) {
+  const Cache4 c(cache, 16, any_alignment);
+  const int64_t n = within(entries, "n", 0, c.S_max, c.S_max);
+  py::object to[2] = {py::none(), py::none()};
+  if (!out.is_none()) {
+    if (!PySequence_Check(out.ptr()) || THPVariable_Check(out.ptr()) || PySequence_Size(out.ptr()) != 2)
+      refuse("out must be (k, v)");
+    const py::sequence s = py::reinterpret_borrow<py::sequence>(out);
+    to[0] = s[0];
+    to[1] = s[1];
+  }
+  const On on(c.ix);
+  const Output k(to[0], "out k", BF16, {c.B, c.Hkv, n, c.D}, c.ix, 16), v(to[1], "out v", BF16, {c.B, c.Hkv, n, c.D}, c.ix, 16);
+  check(qmoe_kv4_load(c.p[0], c.p[1], c.p[2], c.p[3], c.B, c.Hkv, c.D, c.S_max, n, static_cast<Bf*>(k.p),
+                      static_cast<Bf*>(v.p), stream(c.ix)),
+        "qmoe_kv4_load");
+  return py::make_tuple(k.obj, v.obj);
+}
+
+py::object kv4_append(py::handle qkv, py::handle q_norm_w, py::handle k_norm_w, py::handle rope_cos,
+                      py::handle rope_sin, py::handle positions, py::handle slots, py::handle q_heads,
+                      py::handle kv_heads, py::handle cache, py::handle epsilon, py::handle tokens, py::handle q_out) {
+  const int64_t Hq = count(q_heads, "Hq"), Hkv = count(kv_heads, "Hkv"), S = count(tokens, "S");
+  const float eps = float(number(epsilon, "eps"));
+  const Cache4 c(cache, 4, any_alignment);
+  const int ix = c.ix;
+  const at::Tensor& cos = tensor(rope_cos, "rope_cos");
+  if (c.Hkv != Hkv)
+    refuse("cache must have Hkv=" + std::to_string(Hkv) + " heads (got " + std::to_string(c.Hkv) + ")");
+  if (cos.dim() != 2) refuse("rope_cos must be [max_pos, D / 2]");
+  const int64_t max_pos = cos.size(0), T = c.B * S, D = c.D;
+  const float* praw = arg<float>(qkv, "qkv", F32, {T, (Hq + 2 * Hkv) * D}, ix);
+  const Bf* pqn = arg<Bf>(q_norm_w, "q_norm_w", BF16, {D}, ix, any_alignment);
+  const Bf* pkn = arg<Bf>(k_norm_w, "k_norm_w", BF16, {D}, ix, any_alignment);
+  const float* pcos = arg<float>(rope_cos, "rope_cos", F32, {max_pos, D / 2}, ix);
+  const float* psin = arg<float>(rope_sin, "rope_sin", F32, {max_pos, D / 2}, ix);
+  const int32_t* pp = arg<int32_t>(positions, "positions", I32, {T}, ix);
+  const int32_t* psl = arg<int32_t>(slots, "slots", I32, {T}, ix);
+  const On on(ix);
+  const Output o(q_out, "q_out", BF16, {T, Hq, D}, ix, any_alignment);
+  check(qmoe_kv4_append(praw, pqn, pkn, pcos, psin, max_pos, pp, psl, c.B, S, Hq, Hkv, D, c.S_max, eps,
+                        static_cast<Bf*>(o.p), c.p[0], c.p[1], c.p[2], c.p[3], stream(ix)),
+        "qmoe_kv4_append");
+  return o.obj;
+}
+
 // Bytes -> a workspace tensor on GPU ix (None for 0).
 py::object workspace(int64_t bytes, const char* fn, int ix) {
   size(bytes, fn);
@@ -427,5 +576,10 @@ PYBIND11_MODULE(_native, m) {
   m.def("attn_decode_scored", &attn_decode_scored);
   m.def("kv_append", &kv_append);
   m.def("kv_evict", &kv_evict);
+  m.def("attn_window", &attn_window);
+  m.def("attn_kv4", &attn_kv4);
+  m.def("kv4_store", &kv4_store);
+  m.def("kv4_load", &kv4_load);
+  m.def("kv4_append", &kv4_append);
   m.def("workspace", &workspace);
 }

@@ -1,0 +1,358 @@
+// The cache in 4 bits: a prompt's rows into it, a decode step's projection rows
+// into it, and its values back (head_dim 128; the format is in kv4.hpp).
+#include "attn_tile.hpp"
+#include "kv4.hpp"
+
+#include <math.h>
+
+namespace qmoe {
+
+// One thread a block of 32 elements: 64 bytes in, 16 bytes and a power out.
+__global__ __launch_bounds__(256) void kv4_store_kernel(
+    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t blocks, int n, int S_src,
+    const int32_t* __restrict__ starts, const int32_t* __restrict__ lengths, int Hkv, int S_max,
+    uint8_t* __restrict__ k4, uint8_t* __restrict__ ks, uint8_t* __restrict__ v4, uint8_t* __restrict__ vs) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= blocks) return;
+  const int blk = int(i & 3);
+  const int64_t r = i >> 2;  // (b, kv head, token)
+  const int s = int(r % n);
+  const int64_t bh = r / n;
+  const int b = int(bh / Hkv);
+  const int64_t to = int64_t(starts ? starts[b] : 0) + s;
+  if (s >= (lengths ? lengths[b] : n) || to < 0 || to >= S_max) return;
+  const uint16_t* src = (blockIdx.y ? v : k) + (bh * S_src + s) * HD + blk * KV4_BLOCK;
+  float x[KV4_BLOCK];
+  int wants = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const u32x4 w = ld16(src + c * 8);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[c * 8 + 2 * e] = bf16_lo(w[e]);
+      x[c * 8 + 2 * e + 1] = bf16_hi(w[e]);
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < KV4_BLOCK; ++e) wants = max(wants, kv4_wants(x[e]));
+  const int power = kv4_power(wants);
+  u32x4 out;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    uint32_t w = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w |= kv4_code(x[c * 8 + e], power) << (4 * e);
+    out[c] = w;
+  }
+  const int64_t at = bh * S_max + to;
+  *reinterpret_cast<u32x4*>((blockIdx.y ? v4 : k4) + at * KV4_ROWB + blk * 16) = out;
+  (blockIdx.y ? vs : ks)[at * 4 + blk] = uint8_t(power);
+}
+
+// One thread a block of 32 elements: 16 bytes and a power in, 64 bytes out.
+__global__ __launch_bounds__(256) void kv4_load_kernel(
+    const uint8_t* __restrict__ k4, const uint8_t* __restrict__ ks, const uint8_t* __restrict__ v4,
+    const uint8_t* __restrict__ vs, int64_t blocks, int n, int S_max, uint16_t* __restrict__ k,
+    uint16_t* __restrict__ v) {
+  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= blocks) return;
+  const int blk = int(i & 3);
+  const int64_t r = i >> 2, at = r / n * S_max + r % n;
+  const u32x4 w = ld16((blockIdx.y ? v4 : k4) + at * KV4_ROWB + blk * 16);
+  const float scale = kv4_scale((blockIdx.y ? vs : ks)[at * 4 + blk]);
+  uint16_t* dst = (blockIdx.y ? v : k) + r * HD + blk * KV4_BLOCK;
+#pragma unroll
+  for (int c = 0; c < 4; ++c)
+    *reinterpret_cast<u32x4*>(dst + c * 8) = u32x4{kv4_pair<0>(w[c], scale), kv4_pair<1>(w[c], scale),
+                                                   kv4_pair<2>(w[c], scale), kv4_pair<3>(w[c], scale)};
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m, 64);
+  return v;
+}
+__device__ __forceinline__ int half_max(int v) {
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) v = max(v, __shfl_xor(v, m, 64));
+  return v;
+}
+
+// Half an entry into the cache: lane l holds element l of the 64 from `half` on.
+template <class T>
+__device__ __forceinline__ void kv4_put(uint8_t* codes, uint8_t* powers, int half, int l, T x) {
+  const int power = kv4_power(half_max(kv4_wants(x)));
+  uint32_t c = kv4_code(x, power);
+  c |= uint32_t(__shfl_down(int(c), 1, 64)) << 4;  // of even lanes: a byte
+  c |= uint32_t(__shfl_down(int(c), 2, 64)) << 8;
+  c |= uint32_t(__shfl_down(int(c), 4, 64)) << 16;
+  if (l % 8 == 0) *reinterpret_cast<uint32_t*>(codes + half * 32 + l / 2) = c;
+  if (l % 32 == 0) powers[half * 2 + l / 32] = uint8_t(power);
+}
+
+// One wave a (head, token): lane l holds elements l and l + 64, which RoPE pairs.
+// Queries are computed in 32 bits, as in kv_append; keys in 64, because a key next
+// to the border of two numbers is half a number off if it lands on the wrong side
+// (32 bits put about one of 3 million elements there), and they are few.
+__global__ __launch_bounds__(64) void kv4_append_kernel(
+    const float* __restrict__ raw, const uint16_t* __restrict__ qn_w, const uint16_t* __restrict__ kn_w,
+    const float* __restrict__ rope_cos, const float* __restrict__ rope_sin, const int32_t* __restrict__ positions,
+    const int32_t* __restrict__ slots, int S, int Hq, int Hkv, int S_max, int max_pos, float eps,
+    uint16_t* __restrict__ q_out, uint8_t* __restrict__ k4, uint8_t* __restrict__ ks, uint8_t* __restrict__ v4,
+    uint8_t* __restrict__ vs) {
+  const int l = threadIdx.x, head = blockIdx.x, t = blockIdx.y;
+  const float* p = raw + (int64_t(t) * (Hq + 2 * Hkv) + head) * HD;
+  float lo = p[l], hi = p[l + 64];
+  const int pos = positions[t], slot = slots[t];
+  const bool ok = pos >= 0 && pos < max_pos && slot >= 0 && slot < S_max;
+  if (!ok && head >= Hq) return;  // a rejected row: no entry, q zero
+  const int kvh = (head - Hq) % Hkv;
+  const int64_t at = (int64_t(t / S) * Hkv + kvh) * S_max + slot;
+  if (head >= Hq + Hkv) {
+    kv4_put(v4 + at * KV4_ROWB, vs + at * 4, 0, l, lo);
+    kv4_put(v4 + at * KV4_ROWB, vs + at * 4, 1, l, hi);
+    return;
+  }
+  const uint16_t* nw = head < Hq ? qn_w : kn_w;
+  const float wl = bf16_to_f32(nw[l]), wh = bf16_to_f32(nw[l + 64]);
+  const int64_t rope = int64_t(ok ? pos : 0) * (HD / 2) + l;
+  const float c = rope_cos[rope], sn = rope_sin[rope];
+  if (head < Hq) {
+    const float r = rsqrtf(wave_sum(lo * lo + hi * hi) / float(HD) + eps);
+    const float x = wl * (lo * r), y = wh * (hi * r);
+    uint16_t* dst = q_out + (int64_t(t) * Hq + head) * HD;
+    dst[l] = f32_to_bf16(ok ? x * c - y * sn : 0.0f);
+    dst[l + 64] = f32_to_bf16(ok ? y * c + x * sn : 0.0f);
+    return;
+  }
+  const double dl = lo, dh = hi;
+  const double r = 1.0 / sqrt(wave_sum64(dl * dl + dh * dh) / double(HD) + double(eps));
+  const double x = dl * r * double(wl), y = dh * r * double(wh);
+  kv4_put(k4 + at * KV4_ROWB, ks + at * 4, 0, l, x * double(c) - y * double(sn));
+  kv4_put(k4 + at * KV4_ROWB, ks + at * 4, 1, l, y * double(c) + x * double(sn));
+}
+
+// ====================================================================== attention
+struct Kv16 {
+  const uint16_t *k, *v;
+  __device__ float dot(int64_t row, const float* q) const {
+    float s = 0.0f;
+    for (int c = 0; c < HD / 8; ++c) {
+      const u32x4 w = ld16(k + row * HD + c * 8);
+      s += dot8(w, q + c * 8);
+    }
+    return s;
+  }
+  __device__ float2 value(int64_t row, int l) const {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(v)[row * (HD / 2) + l];
+    return make_float2(bf16_lo(w), bf16_hi(w));
+  }
+};
+struct Kv4 {
+  const uint8_t *k, *ks, *v, *vs;
+  __device__ float dot(int64_t row, const float* q) const {
+    float s = 0.0f;
+    for (int b = 0; b < 4; ++b) {
+      const u32x4 w = ld16(k + row * KV4_ROWB + b * 16);
+      const float scale = kv4_scale(ks[row * 4 + b]);
+      for (int c = 0; c < 4; ++c)
+        s += dot8(u32x4{kv4_pair<0>(w[c], scale), kv4_pair<1>(w[c], scale), kv4_pair<2>(w[c], scale),
+                        kv4_pair<3>(w[c], scale)},
+                  q + b * 32 + c * 8);
+    }
+    return s;
+  }
+  __device__ float2 value(int64_t row, int l) const {
+    const uint32_t w = kv4_pair<0>(v[row * KV4_ROWB + l], kv4_scale(vs[row * 4 + l / 16]));
+    return make_float2(bf16_lo(w), bf16_hi(w));
+  }
+};
+
+// One wave a (query, q head): 64 entries at a time, a lane for each one's logit,
+// then for two dims of the output.
+template <class Cache>
+__global__ __launch_bounds__(64) void attn_entries_kernel(const uint16_t* __restrict__ q, const Cache cache,
+                                                          const WinArgs w, int Hq, int Hkv, float scale_log2,
+                                                          uint16_t* __restrict__ out) {
+  __shared__ float qs[HD], ps[64];
+  const int l = threadIdx.x, h = int(blockIdx.x) % Hq;
+  const int64_t t = int(blockIdx.x) / Hq;
+  const int b = int(t / w.S);
+  const uint32_t qw = reinterpret_cast<const uint32_t*>(q)[(t * Hq + h) * (HD / 2) + l];
+  qs[2 * l] = bf16_lo(qw);
+  qs[2 * l + 1] = bf16_hi(qw);
+  __syncthreads();
+  const WinRow see = win_row(w, b, int(t % w.S));
+  const int64_t base = (int64_t(b) * Hkv + h / (Hq / Hkv)) * w.S_max;
+  float m = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  for (int part = 0; part < 2; ++part) {
+    const int from = part ? see.low : 0, to = part ? see.end : min(min(w.sink, see.low), see.end);
+    for (int k0 = from; k0 < to; k0 += 64) {
+      const int n = min(64, to - k0);
+      const float x = l < n ? cache.dot(base + k0 + l, qs) * scale_log2 : -INFINITY;
+      const float top = fmaxf(m, wave_max(x)), a = exp2f(m - top), p = l < n ? exp2f(x - top) : 0.0f;
+      m = top;
+      sum = sum * a + wave_sum(p);
+      o0 *= a;
+      o1 *= a;
+      ps[l] = p;
+      __syncthreads();
+      for (int i = 0; i < n; ++i) {
+        const float2 v = cache.value(base + k0 + i, l);
+        o0 = fmaf(ps[i], v.x, o0);
+        o1 = fmaf(ps[i], v.y, o1);
+      }
+      __syncthreads();
+    }
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+  reinterpret_cast<uint32_t*>(out)[(t * Hq + h) * (HD / 2) + l] = pack_bf16x2(o0 * inv, o1 * inv);
+}
+
+static int win_check(const char* fn, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max,
+                     int64_t max_ctx, int64_t window, int64_t sink) {
+  QMOE_REQUIRE(D == HD, "%s: head_dim must be 128 (D=%lld)", fn, (long long)D);
+  QMOE_REQUIRE(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16 && Hkv < 4096,
+               "%s: need Hq %% Hkv == 0, Hq / Hkv <= 16 and Hkv < 4096", fn);
+  QMOE_REQUIRE(B >= 0 && B < 65536 && S >= 0 && S < (1ll << 22) && B * S * Hq < (1ll << 27),
+               "%s: bad B/S (B * S * Hq must be below 2^27)", fn);
+  QMOE_REQUIRE(S_max > 0 && S_max <= (1ll << 22), "%s: S_max must be in [1, 2^22]", fn);
+  QMOE_REQUIRE(max_ctx >= 0 && max_ctx <= S_max, "%s: need 0 <= max_ctx <= S_max", fn);
+  QMOE_REQUIRE(window >= 0 && sink >= 0, "%s: window and sink must be >= 0", fn);
+  return QMOE_OK;
+}
+
+static WinArgs win_args(const int32_t* ctx_len, int64_t S, int64_t S_max, int64_t max_ctx, int64_t window,
+                        int64_t sink) {
+  WinArgs w;
+  w.ctx_len = ctx_len;
+  w.S = int(S);
+  w.S_max = int(S_max);
+  w.max_ctx = int(max_ctx);
+  w.window = int(window == 0 ? WIN_NONE : std::min<int64_t>(window, WIN_NONE));
+  w.sink = int(std::min<int64_t>(sink, WIN_NONE));
+  return w;
+}
+
+static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return x < y + uintptr_t(nb) && y < x + uintptr_t(na);
+}
+
+}  // namespace qmoe
+
+using namespace qmoe;
+
+extern "C" int64_t qmoe_attn_window_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                                              int64_t sink, int64_t max_ctx) {
+  if (window <= 0 || win_check("qmoe_attn_window_workspace", B, S, Hq, Hkv, D, 1 << 22, max_ctx, window, sink)) return -1;
+  return 0;
+}
+
+extern "C" int qmoe_attn_window(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
+                                const int32_t* ctx_len, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
+                                void* workspace, int64_t workspace_bytes, qmoe_bf16* out, qmoe_stream_t stream) {
+  const char* fn = "qmoe_attn_window";
+  QMOE_REQUIRE(B == 0 || S == 0 || (q && k_cache && v_cache && ctx_len && out), "%s: null pointer", fn);
+  if (int rc = win_check(fn, B, S, Hq, Hkv, D, S_max, max_ctx, window, sink)) return rc;
+  QMOE_REQUIRE(window > 0, "%s: window must be positive", fn);
+  QMOE_REQUIRE(scale > 0.0f && std::isfinite(scale), "%s: scale must be positive and finite", fn);
+  if (B == 0 || S == 0) return QMOE_OK;
+  QMOE_REQUIRE(aligned16(q, k_cache, v_cache, static_cast<uint8_t*>(workspace), out),
+               "%s: operands must be 16-byte aligned", fn);
+  QMOE_REQUIRE(!overlap(q, B * S * Hq * HD * 2, out, B * S * Hq * HD * 2), "%s: out overlaps q", fn);
+  hipLaunchKernelGGL(attn_entries_kernel<Kv16>, dim3(unsigned(B * S * Hq)), dim3(64), 0, as_stream(stream), q,
+                     Kv16{k_cache, v_cache}, win_args(ctx_len, S, S_max, max_ctx, window, sink), int(Hq), int(Hkv),
+                     scale * 1.4426950408889634f, out);
+  return hip_status(fn);
+}
+
+extern "C" int64_t qmoe_attn_kv4_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                                           int64_t sink, int64_t max_ctx) {
+  if (win_check("qmoe_attn_kv4_workspace", B, S, Hq, Hkv, D, 1 << 22, max_ctx, window, sink)) return -1;
+  return 0;
+}
+
+extern "C" int qmoe_attn_kv4(const qmoe_bf16* q, const uint8_t* k_cache, const uint8_t* k_scales,
+                             const uint8_t* v_cache, const uint8_t* v_scales, const int32_t* ctx_len, int64_t B,
+                             int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max, int64_t max_ctx,
+                             int64_t window, int64_t sink, float scale, void* workspace, int64_t workspace_bytes,
+                             qmoe_bf16* out, qmoe_stream_t stream) {
+  const char* fn = "qmoe_attn_kv4";
+  QMOE_REQUIRE(B == 0 || S == 0 || (q && k_cache && k_scales && v_cache && v_scales && ctx_len && out),
+               "%s: null pointer", fn);
+  if (int rc = win_check(fn, B, S, Hq, Hkv, D, S_max, max_ctx, window, sink)) return rc;
+  QMOE_REQUIRE(scale > 0.0f && std::isfinite(scale), "%s: scale must be positive and finite", fn);
+  if (B == 0 || S == 0) return QMOE_OK;
+  QMOE_REQUIRE(aligned16(q, k_cache, k_scales, v_cache, v_scales, static_cast<uint8_t*>(workspace), out),
+               "%s: operands must be 16-byte aligned", fn);
+  QMOE_REQUIRE(!overlap(q, B * S * Hq * HD * 2, out, B * S * Hq * HD * 2), "%s: out overlaps q", fn);
+  hipLaunchKernelGGL(attn_entries_kernel<Kv4>, dim3(unsigned(B * S * Hq)), dim3(64), 0, as_stream(stream), q,
+                     Kv4{k_cache, k_scales, v_cache, v_scales}, win_args(ctx_len, S, S_max, max_ctx, window, sink),
+                     int(Hq), int(Hkv), scale * 1.4426950408889634f, out);
+  return hip_status(fn);
+}
+
+static int kv4_check(const char* fn, int64_t B, int64_t Hkv, int64_t D, int64_t S_max, int64_t n) {
+  QMOE_REQUIRE(D == HD, "%s: head_dim must be 128 (D=%lld)", fn, (long long)D);
+  QMOE_REQUIRE(B >= 0 && B < 65536 && Hkv > 0 && Hkv < 65536 && S_max > 0 && S_max < (1ll << 30),
+               "%s: bad B/Hkv/S_max", fn);
+  QMOE_REQUIRE(n >= 0 && n < (1ll << 30) && B * Hkv * n < (1ll << 36), "%s: bad number of entries", fn);
+  return QMOE_OK;
+}
+
+extern "C" int qmoe_kv4_store(const qmoe_bf16* k, const qmoe_bf16* v, int64_t S_src, int64_t n, const int32_t* starts,
+                              const int32_t* lengths, int64_t B, int64_t Hkv, int64_t D, int64_t S_max,
+                              uint8_t* k_cache, uint8_t* k_scales, uint8_t* v_cache, uint8_t* v_scales,
+                              qmoe_stream_t stream) {
+  const char* fn = "qmoe_kv4_store";
+  QMOE_REQUIRE(B == 0 || n == 0 || (k && v && k_cache && k_scales && v_cache && v_scales), "%s: null pointer", fn);
+  if (int rc = kv4_check(fn, B, Hkv, D, S_max, n)) return rc;
+  QMOE_REQUIRE(S_src >= n && S_src < (1ll << 30), "%s: need n <= S_src", fn);
+  if (B == 0 || n == 0) return QMOE_OK;
+  QMOE_REQUIRE(aligned16(k, v, k_cache, v_cache), "%s: operands must be 16-byte aligned", fn);
+  const int64_t blocks = B * Hkv * n * 4;
+  hipLaunchKernelGGL(kv4_store_kernel, dim3(unsigned((blocks + 255) / 256), 2), dim3(256), 0, as_stream(stream), k, v,
+                     blocks, int(n), int(S_src), starts, lengths, int(Hkv), int(S_max), k_cache, k_scales, v_cache,
+                     v_scales);
+  return hip_status(fn);
+}
+
+extern "C" int qmoe_kv4_load(const uint8_t* k_cache, const uint8_t* k_scales, const uint8_t* v_cache,
+                             const uint8_t* v_scales, int64_t B, int64_t Hkv, int64_t D, int64_t S_max, int64_t n,
+                             qmoe_bf16* k, qmoe_bf16* v, qmoe_stream_t stream) {
+  const char* fn = "qmoe_kv4_load";
+  QMOE_REQUIRE(B == 0 || n == 0 || (k && v && k_cache && k_scales && v_cache && v_scales), "%s: null pointer", fn);
+  if (int rc = kv4_check(fn, B, Hkv, D, S_max, n)) return rc;
+  QMOE_REQUIRE(n <= S_max, "%s: need n <= S_max", fn);
+  if (B == 0 || n == 0) return QMOE_OK;
+  QMOE_REQUIRE(aligned16(k, v, k_cache, v_cache), "%s: operands must be 16-byte aligned", fn);
+  const int64_t blocks = B * Hkv * n * 4;
+  hipLaunchKernelGGL(kv4_load_kernel, dim3(unsigned((blocks + 255) / 256), 2), dim3(256), 0, as_stream(stream),
+                     k_cache, k_scales, v_cache, v_scales, blocks, int(n), int(S_max), k, v);
+  return hip_status(fn);
+}
+
+extern "C" int qmoe_kv4_append(const float* qkv, const qmoe_bf16* q_norm_w, const qmoe_bf16* k_norm_w,
+                               const float* rope_cos, const float* rope_sin, int64_t max_pos,
+                               const int32_t* positions, const int32_t* slots, int64_t B, int64_t S, int64_t Hq,
+                               int64_t Hkv, int64_t D, int64_t S_max, float eps, qmoe_bf16* q_out, uint8_t* k_cache,
+                               uint8_t* k_scales, uint8_t* v_cache, uint8_t* v_scales, qmoe_stream_t stream) {
+  const char* fn = "qmoe_kv4_append";
+  QMOE_REQUIRE(q_norm_w && k_norm_w && rope_cos && rope_sin &&
+                   (B == 0 || S == 0 || (qkv && positions && slots && q_out && k_cache && k_scales && v_cache && v_scales)),
+               "%s: null pointer", fn);
+  if (int rc = kv4_check(fn, B, Hkv, D, S_max, 0)) return rc;
+  QMOE_REQUIRE(Hq > 0 && Hq % Hkv == 0 && Hq < 65536 && Hq + 2 * Hkv < 65536, "%s: bad head counts", fn);
+  QMOE_REQUIRE(S >= 0 && S < 65536 && B * S < 65536, "%s: B * S must be below 65536", fn);
+  QMOE_REQUIRE(max_pos > 0, "%s: bad max_pos", fn);
+  if (B == 0 || S == 0) return QMOE_OK;
+  QMOE_REQUIRE(reinterpret_cast<uintptr_t>(k_cache) % 4 == 0 && reinterpret_cast<uintptr_t>(v_cache) % 4 == 0,
+               "%s: caches must be 4-byte aligned", fn);
+  hipLaunchKernelGGL(kv4_append_kernel, dim3(unsigned(Hq + 2 * Hkv), unsigned(B * S)), dim3(64), 0, as_stream(stream),
+                     qkv, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slots, int(S), int(Hq), int(Hkv),
+                     int(S_max), int(std::min<int64_t>(max_pos, 1ll << 30)), eps, q_out, k_cache, k_scales, v_cache,
+                     v_scales);
+  return hip_status(fn);
+}

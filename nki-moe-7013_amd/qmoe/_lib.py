@@ -88,6 +88,13 @@ PROTOTYPES = {
     "qmoe_kv_append": (c_int, [P, P, P, P, P, I64, P, P, I64, I64, I64, I64, I64, c_float, P, P, P, P, P, P]),
     "qmoe_kv_evict": (c_int, [P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, P, I64, I64, P, P, P, P, P]),
     "qmoe_kv_evict_workspace": (c_int64, [I64, I64, I64, I64]),
+    "qmoe_attn_window": (c_int, [P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, c_float, P, I64, P, P]),
+    "qmoe_attn_window_workspace": (c_int64, [I64, I64, I64, I64, I64, I64, I64, I64]),
+    "qmoe_attn_kv4": (c_int, [P, P, P, P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, c_float, P, I64, P, P]),
+    "qmoe_attn_kv4_workspace": (c_int64, [I64, I64, I64, I64, I64, I64, I64, I64]),
+    "qmoe_kv4_store": (c_int, [P, P, I64, I64, P, P, I64, I64, I64, I64, P, P, P, P, P]),
+    "qmoe_kv4_load": (c_int, [P, P, P, P, I64, I64, I64, I64, I64, P, P, P]),
+    "qmoe_kv4_append": (c_int, [P, P, P, P, P, I64, P, P, I64, I64, I64, I64, I64, I64, c_float, P, P, P, P, P, P]),
 }
 
 

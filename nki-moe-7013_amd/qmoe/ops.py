@@ -888,6 +888,81 @@ def kv_evict(k_cache: torch.Tensor, v_cache: torch.Tensor, scores: torch.Tensor,
     _native().kv_evict(k_cache, v_cache, scores, slot_pos, ctx_len, budget, recent, sink, out, workspace)
 
 
+# ----------------------------------------------------------------- windows and caches in 4 bits
+def attn_window_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, window: int, sink: int, max_ctx: int,
+                          device) -> Optional[torch.Tensor]:
+    """Workspace of :func:`attn_window` (``None`` when it needs none)."""
+    return _new_workspace("qmoe_attn_window_workspace", device, B, S, Hq, Hkv, D, window, sink, max_ctx)
+
+
+def attn_window(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ctx_len: torch.Tensor, B: int, S: int,
+                window: int, sink: int = 0, scale: Optional[float] = None,
+                workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                max_ctx: Optional[int] = None) -> torch.Tensor:
+    """Attention of ``q[B*S, Hq, D]`` in which a query sees the last ``window``
+    entries up to its own and the first ``sink`` ones of ``k_cache/v_cache[B,
+    Hkv, S_max, D]``.  Query s of row b stands at index ``ctx_len[b] - 1 + s``
+    (decode: S = 1 and ``ctx_len``, i32 ``[B]`` on the device, counts the new
+    entry; a prompt: ``ctx_len = 1``; a chunk whose first token is entry e: ``e +
+    1``); none sees entries from ``max_ctx`` on (default ``S_max``; a context
+    bucket sizes the launch, and the last bits go with it).  A query that sees
+    nothing gets zeros.  ``out`` is not ``q``.  Returns ``[B*S, Hq*D]``."""
+    return _native().attn_window(q, k_cache, v_cache, ctx_len, B, S, window, sink, scale, workspace, out, max_ctx)
+
+
+KV4 = Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]
+
+
+def kv4_cache(B: int, Hkv: int, S_max: int, D: int, device) -> KV4:
+    """An empty cache in 4 bits, ``(k, k_scales, v, v_scales)``: e2m1 numbers, two
+    a byte, u8 ``[B, Hkv, S_max, D / 2]``, and the power of two of every 32 of
+    them, u8 ``[B, Hkv, S_max, D / 32]``."""
+    k = torch.zeros(B, Hkv, S_max, D // 2, dtype=torch.uint8, device=device)
+    s = torch.zeros(B, Hkv, S_max, D // 32, dtype=torch.uint8, device=device)
+    return k, s, torch.zeros_like(k), torch.zeros_like(s)
+
+
+def attn_kv4_workspace(B: int, S: int, Hq: int, Hkv: int, D: int, window: int, sink: int, max_ctx: int,
+                       device) -> Optional[torch.Tensor]:
+    """Workspace of :func:`attn_kv4` (``None`` when it needs none)."""
+    return _new_workspace("qmoe_attn_kv4_workspace", device, B, S, Hq, Hkv, D, window, sink, max_ctx)
+
+
+def attn_kv4(q: torch.Tensor, cache: KV4, ctx_len: torch.Tensor, B: int, S: int, window: int = 0, sink: int = 0,
+             scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None,
+             out: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None) -> torch.Tensor:
+    """:func:`attn_window` over a cache in 4 bits (:func:`kv4_cache`); ``window`` 0:
+    a query sees every entry up to its own."""
+    return _native().attn_kv4(q, cache, ctx_len, B, S, window, sink, scale, workspace, out, max_ctx)
+
+
+def kv4_store(k: torch.Tensor, v: torch.Tensor, cache: KV4, starts: Optional[torch.Tensor] = None,
+              lengths: Optional[torch.Tensor] = None, n: Optional[int] = None) -> None:
+    """Tokens ``[0, n)`` (default: all) of the bf16 rows ``k, v[B, Hkv, S, D]`` into
+    a cache in 4 bits: token s of row b becomes entry ``starts[b] + s`` (i32
+    ``[B]``, default 0).  Only the first ``lengths[b]`` tokens are stored, and only
+    into entries that the cache has; the others stay as they were."""
+    _native().kv4_store(k, v, cache, starts, lengths, n)
+
+
+def kv4_load(cache: KV4, n: Optional[int] = None,
+             out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Entries ``[0, n)`` (default: all) of a cache in 4 bits as the bf16 rows
+    ``(k, v)[B, Hkv, n, D]`` that they stand for."""
+    return _native().kv4_load(cache, n, out)
+
+
+def kv4_append(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor, rope_cos: torch.Tensor,
+               rope_sin: torch.Tensor, positions: torch.Tensor, slots: torch.Tensor, Hq: int, Hkv: int, cache: KV4,
+               eps: float, S: int = 1, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`kv_append` into a cache in 4 bits, ``S`` tokens a row: the raw
+    projection ``qkv[B*S, (Hq+2Hkv)*D]`` (f32), token t = b * S + s at
+    ``positions[t]`` into entry ``slots[t]`` of row b (the slots of a row differ).
+    Returns ``q[B*S, Hq, D]``, whose bits are ``kv_append``'s."""
+    return _native().kv4_append(qkv, q_norm_w, k_norm_w, rope_cos, rope_sin, positions, slots, Hq, Hkv, cache, eps, S,
+                                q_out)
+
+
 # ----------------------------------------------------------------- embedding / greedy argmax
 def embed(ids: torch.Tensor, table: torch.Tensor, out: Optional[torch.Tensor] = None,
           err: Optional[torch.Tensor] = None) -> torch.Tensor:
