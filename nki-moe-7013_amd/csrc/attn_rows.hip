@@ -22,6 +22,7 @@
 //                          the attention left each row's lse = m + log2 l.
 #include "attn_tile.hpp"
 #include "common.hpp"
+#include "window.hpp"
 
 #include <math.h>
 
@@ -64,6 +65,7 @@ struct ArArgs {
   // start with the prefix when joint.  NS = pre.records() + own.records() a row.
   int NS, n_pre, joint, nb_pre, nb_own;  // nb: blocks of 32 rows
   ArKind pre, own;
+  WinArgs win;  // of a windowed attention
 };
 
 // r / G for 0 <= r < 2^32 / G, by a multiplication
@@ -79,6 +81,55 @@ __device__ __forceinline__ int ar_sees(const ArArgs& a, int b, int s) {
 }
 
 __device__ __forceinline__ float ar_lse(float m, float l) { return l > 0.0f ? m + __log2f(l) : INFINITY; }
+
+// A lane's row of an item: its packed row (of `rows`), query and query row.
+struct ArRow {
+  int run, kvh, b, rw, row, rows, sq;
+  int64_t qrow;
+  bool live;
+};
+
+// The item's rows as a record of the run, or, where it is the only one, as output.
+template <bool stream>
+__device__ __forceinline__ void ar_finish(const ArArgs& a, const ArKind kd, const bool pre, uint8_t* smem,
+                                          FlashRows& st, const ArRow r) {
+  const int lane = threadIdx.x & 63, hl = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  if (stream && !kd.split) {
+    flash_join(smem, st);
+    if (wave) return;
+  }
+  const int rec_run = stream && kd.split ? r.run * 4 + wave : r.run;
+  const float l = st.row_sum();
+  if (!r.live) return;
+  if (a.NS > 1) {
+    const int64_t blk = pre ? (int64_t(rec_run) * a.Hkv + r.kvh) * a.nb_pre + r.rw / 32
+                            : int64_t(a.pre.records()) * a.Hkv * a.nb_pre +
+                                  ((int64_t(rec_run) * a.B + r.b) * a.Hkv + r.kvh) * a.nb_own + r.rw / 32;
+    float* rec = a.part + blk * AR_REC;
+    if (hl == 0) *reinterpret_cast<float2*>(rec + (lane & 31) * 2) = make_float2(st.m, l);
+#pragma unroll
+    for (int c = 0; c < 16; ++c)
+      *reinterpret_cast<float4*>(rec + 64 + (c * 64 + lane) * 4) =
+          make_float4(st.o[c >> 2][(c & 3) * 4], st.o[c >> 2][(c & 3) * 4 + 1], st.o[c >> 2][(c & 3) * 4 + 2],
+                      st.o[c >> 2][(c & 3) * 4 + 3]);
+    return;
+  }
+  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+  uint16_t* op = a.out + r.qrow * HD;
+#pragma unroll
+  for (int db = 0; db < 4; ++db)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      u32x2 w;
+      w.x = pack_bf16x2(st.o[db][g * 4 + 0] * inv, st.o[db][g * 4 + 1] * inv);
+      w.y = pack_bf16x2(st.o[db][g * 4 + 2] * inv, st.o[db][g * 4 + 3] * inv);
+      *reinterpret_cast<u32x2*>(op + db * 32 + g * 8 + hl * 4) = w;
+    }
+  if (a.lse && hl == 0 && !pre)
+    a.lse[(int64_t(r.b) * a.Hkv + r.kvh) * r.rows + r.row] =
+        a.lengths && r.sq >= a.lengths[r.b] ? INFINITY : ar_lse(st.m, l);
+}
 
 template <bool stream>
 __device__ __forceinline__ void ar_item(const ArArgs& a, const ArKind kd, const bool pre, uint8_t* smem) {
@@ -145,46 +196,13 @@ __device__ __forceinline__ void ar_item(const ArArgs& a, const ArKind kd, const 
         last = min(ar_sees(a, b, ar_div(min(rw + 31, rows - 1), a.g_magic)), end) - 1 - k0;
       }
     }
+    const Causal see{lim, __builtin_amdgcn_readfirstlane(first), __builtin_amdgcn_readfirstlane(last)};
     if constexpr (stream)
-      stream_segment(smem, kk + base, vv + base, n, lim, a.scale_log2, st);
+      stream_segment(smem, kk + base, vv + base, n, see, a.scale_log2, st);
     else
-      flash_segment(smem, kk + base, vv + base, n, lim, __builtin_amdgcn_readfirstlane(first),
-                    __builtin_amdgcn_readfirstlane(last), a.scale_log2, st);
+      flash_segment(smem, kk + base, vv + base, n, see, a.scale_log2, st);
   }
-  if (stream && !kd.split) {
-    flash_join(smem, st);
-    if (wave) return;
-  }
-  const int rec_run = stream && kd.split ? run * 4 + wave : run;
-  const float l = st.row_sum();
-  if (!live) return;
-  if (a.NS > 1) {
-    const int64_t blk = pre ? (int64_t(rec_run) * a.Hkv + kvh) * a.nb_pre + rw / 32
-                            : int64_t(a.pre.records()) * a.Hkv * a.nb_pre +
-                                  ((int64_t(rec_run) * a.B + b) * a.Hkv + kvh) * a.nb_own + rw / 32;
-    float* rec = a.part + blk * AR_REC;
-    if (hl == 0) *reinterpret_cast<float2*>(rec + (lane & 31) * 2) = make_float2(st.m, l);
-#pragma unroll
-    for (int c = 0; c < 16; ++c)
-      *reinterpret_cast<float4*>(rec + 64 + (c * 64 + lane) * 4) =
-          make_float4(st.o[c >> 2][(c & 3) * 4], st.o[c >> 2][(c & 3) * 4 + 1], st.o[c >> 2][(c & 3) * 4 + 2],
-                      st.o[c >> 2][(c & 3) * 4 + 3]);
-    return;
-  }
-  const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-  uint16_t* op = a.out + qrow * HD;
-#pragma unroll
-  for (int db = 0; db < 4; ++db)
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      u32x2 w;
-      w.x = pack_bf16x2(st.o[db][g * 4 + 0] * inv, st.o[db][g * 4 + 1] * inv);
-      w.y = pack_bf16x2(st.o[db][g * 4 + 2] * inv, st.o[db][g * 4 + 3] * inv);
-      *reinterpret_cast<u32x2*>(op + db * 32 + g * 8 + hl * 4) = w;
-    }
-  if (a.lse && hl == 0 && !pre)
-    a.lse[(int64_t(b) * a.Hkv + kvh) * rows + row] =
-        a.lengths && sq >= a.lengths[b] ? INFINITY : ar_lse(st.m, l);
+  ar_finish<stream>(a, kd, pre, smem, st, ArRow{run, kvh, b, rw, row, rows, sq, qrow, live});
 }
 
 // Both kinds of item in one launch: the prefix's tiles are bound by the matrix
@@ -207,6 +225,56 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
   } else {
     ar_item<STREAMS>(a, kd, pre, smem);
   }
+}
+
+// An item of a windowed attention: row tile, kv head, sequence and a run of the keys
+// that the tile's queries see, the window's behind the first ones that stay (the
+// windows of consecutive queries are one run of rows).
+template <bool stream>
+__device__ __forceinline__ void aw_item(const ArArgs& a, uint8_t* smem) {
+  const int lane = threadIdx.x & 63, hl = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+  const ArKind kd = a.own;
+  constexpr int KS = stream ? 4 * AP_KT : AP_KT, ROWS = stream ? 32 : 128;
+  const int G = a.Hq / a.Hkv, rows = a.S * G, grp = a.B * a.Hkv;
+  const int x = int(blockIdx.x), y = x % (grp * kd.runs), z = y % grp;
+  const int run = y / grp, b = z / a.Hkv, kvh = z % a.Hkv, r0 = (kd.rts - 1 - x / (grp * kd.runs)) * ROWS;
+  const int rw = r0 + (stream ? 0 : wave * 32);
+  const int row = rw + (lane & 31);
+  const bool live = row < rows, wlive = rw < rows;
+  const int rq = live ? row : rows - 1, sq = ar_div(rq, a.g_magic);
+  const int64_t qrow = (int64_t(b) * a.S + sq) * a.Hq + kvh * G + (rq - sq * G);
+  FlashRows st;
+  st.start(live ? a.q + qrow * HD : nullptr, hl);
+  int n;
+  Windowed see;
+  see.sink = a.win.sink;
+  see.g = win_run(a.win, win_row(a.win, b, ar_div(r0, a.g_magic)).low,
+                  win_row(a.win, b, ar_div(min(r0 + ROWS, rows) - 1, a.g_magic)).end, &n);
+  const WinRow own = win_row(a.win, b, sq);
+  see.low = own.low;
+  see.end = own.end;
+  const WinRow w0 = win_row(a.win, b, ar_div(wlive ? rw : r0, a.g_magic));
+  const WinRow w1 = win_row(a.win, b, ar_div(wlive ? min(rw + 31, rows - 1) : r0, a.g_magic));
+  see.first = __builtin_amdgcn_readfirstlane(wlive ? see.g.key(w0.end - 1) : -1);
+  see.last = __builtin_amdgcn_readfirstlane(wlive ? see.g.key(w1.end - 1) : -1);
+  see.from = __builtin_amdgcn_readfirstlane(w1.low <= see.sink ? 0 : see.g.key(w1.low));
+  see.to = __builtin_amdgcn_readfirstlane(w0.low <= see.sink ? 0 : see.g.key(w0.low));
+  const int k0 = run * kd.run * KS, k1 = min(n, k0 + kd.run * KS);
+  if (k0 < k1) {
+    const int64_t base = (int64_t(b) * a.Hkv + kvh) * a.S_max * HD;
+    if constexpr (stream)
+      stream_segment(smem, a.k + base, a.v + base, k0, k1, see, a.scale_log2, st);
+    else
+      flash_segment(smem, a.k + base, a.v + base, k0, k1, see, a.scale_log2, st);
+  }
+  ar_finish<stream>(a, kd, false, smem, st, ArRow{run, kvh, b, rw, row, rows, sq, qrow, live});
+}
+
+template <bool STREAM>
+__global__ __launch_bounds__(256, 2) void attn_window_kernel(const ArArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];
+  aw_item<STREAM>(a, smem);
 }
 
 // Joins the runs of 32 packed rows of a kv head (8 x 101 queries, 2 runs, 8 us; 64
@@ -580,6 +648,16 @@ static int64_t ar_part_bytes(const ArArgs& a) {
   return blocks * AR_REC * int64_t(sizeof(float));
 }
 
+static int ar_merge(const char* fn, const ArArgs& a, hipStream_t s) {
+  if (a.NS == 1) return QMOE_OK;
+  const int64_t blocks = ar_ceil(int64_t(a.B) * a.S * (a.Hq / a.Hkv), 32) * a.Hkv;
+  if (a.NS >= AR_MANY_RUNS)
+    hipLaunchKernelGGL(attn_rows_merge_kernel<4>, dim3(unsigned(blocks), 16), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL(attn_rows_merge_kernel<1>, dim3(unsigned(blocks), 4), dim3(256), 0, s, a);
+  return hip_status(fn);
+}
+
 static int ar_launch(const char* fn, ArArgs& a, int64_t grid, hipStream_t s) {
   const bool own = grid > a.n_pre, tiles = (a.n_pre && !a.pre.stream) || (own && !a.own.stream);
   const bool streams = (a.n_pre && a.pre.stream) || (own && a.own.stream);
@@ -590,14 +668,8 @@ static int ar_launch(const char* fn, ArArgs& a, int64_t grid, hipStream_t s) {
     hipLaunchKernelGGL((attn_rows_kernel<true, false>), g, t, 0, s, a);
   else
     hipLaunchKernelGGL((attn_rows_kernel<false, true>), g, t, 0, s, a);
-  int rc = hip_status(fn);
-  if (rc || a.NS == 1) return rc;
-  const int64_t blocks = ar_ceil(int64_t(a.B) * a.S * (a.Hq / a.Hkv), 32) * a.Hkv;
-  if (a.NS >= AR_MANY_RUNS)
-    hipLaunchKernelGGL(attn_rows_merge_kernel<4>, dim3(unsigned(blocks), 16), t, 0, s, a);
-  else
-    hipLaunchKernelGGL(attn_rows_merge_kernel<1>, dim3(unsigned(blocks), 4), t, 0, s, a);
-  return hip_status(fn);
+  const int rc = hip_status(fn);
+  return rc ? rc : ar_merge(fn, a, s);
 }
 
 // Limits shared by both entry points; B * S may be 0.
@@ -776,4 +848,55 @@ extern "C" int qmoe_attn_prefill_scored(const qmoe_bf16* q, const qmoe_bf16* k_c
   hipLaunchKernelGGL(attn_colsum_add_kernel, dim3(unsigned(int64_t(B) * Hkv * c.nkt * (CS_KEYS / 64))),
                      dim3(256), 0, as_stream(stream), c);
   return hip_status(fn);
+}
+
+namespace qmoe {
+static ArArgs aw_args(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_max, int64_t max_ctx, int64_t window,
+                      int64_t sink, int64_t* grid) {
+  ArArgs a = ar_args(B, S, Hq, Hkv, S_max);
+  a.max_ctx = int(max_ctx);
+  a.win = win_args(S, S_max, max_ctx, window, sink);
+  // keys of a row tile at most: streams and tiles of several sequences' rows do not occur
+  const int64_t G = Hq / Hkv, tile = std::min<int64_t>(S, (S * G <= 64 ? 32 : 128) / G + 2);
+  ar_plan(a, std::min<int64_t>(max_ctx, int64_t(a.win.window) + a.win.sink + tile - 1), grid);
+  return a;
+}
+}  // namespace qmoe
+
+extern "C" int64_t qmoe_attn_window_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
+                                              int64_t sink, int64_t max_ctx) {
+  if (window <= 0 || win_check("qmoe_attn_window_workspace", B, S, Hq, Hkv, D, AR_MAX_KEYS, max_ctx, window, sink, 1.0f))
+    return -1;
+  if (B == 0 || S == 0) return 0;
+  int64_t grid;
+  return ar_part_bytes(aw_args(B, S, Hq, Hkv, AR_MAX_KEYS, max_ctx, window, sink, &grid));
+}
+
+extern "C" int qmoe_attn_window(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
+                                const int32_t* ctx_len, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
+                                int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
+                                void* workspace, int64_t workspace_bytes, qmoe_bf16* out, qmoe_stream_t stream) {
+  const char* fn = "qmoe_attn_window";
+  QMOE_REQUIRE(B == 0 || S == 0 || (q && k_cache && v_cache && ctx_len && out), "%s: null pointer", fn);
+  if (int rc = win_check(fn, B, S, Hq, Hkv, D, S_max, max_ctx, window, sink, scale)) return rc;
+  QMOE_REQUIRE(window > 0, "%s: window must be positive", fn);
+  if (B == 0 || S == 0) return QMOE_OK;
+  int64_t grid;
+  ArArgs a = aw_args(B, S, Hq, Hkv, S_max, max_ctx, window, sink, &grid);
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.win.ctx_len = ctx_len;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.part = static_cast<float*>(workspace);
+  if (int rc = win_operands(fn, grid, ar_part_bytes(a), workspace, workspace_bytes, q, out, B * S * Hq,
+                            aligned16(k_cache, v_cache)))
+    return rc;
+  if (a.own.stream)
+    hipLaunchKernelGGL(attn_window_kernel<true>, dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(attn_window_kernel<false>, dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
+  if (int rc = hip_status(fn)) return rc;
+  return ar_merge(fn, a, as_stream(stream));
 }

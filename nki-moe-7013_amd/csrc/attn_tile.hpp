@@ -74,18 +74,94 @@ struct FlashRows {
 
 constexpr int FL_SMEM = 4 * AP_TILE;  // K0, K1, V0, V1
 
-// Attends a workgroup's 4 x 32 query rows to keys [0, n_keys) of k / v (rows
-// of HD bf16; n_keys >= 1), adding to each wave's state.  Lane's row sees keys
-// [0, lim]; every row of the wave sees [0, first] and none a key past last
-// (wave-uniform; last < 0: the wave has no row, it only helps to load).
+// What the queries of a wave see of a run of keys.  Lane's row sees keys [0, lim];
+// every row of the wave sees [0, first] and none a key past last (wave-uniform;
+// last < 0: the wave has no row, it only helps to load).
+struct Causal {
+  int lim, first, last;
+  __device__ __forceinline__ bool sees(int key) const { return key <= lim; }
+  __device__ __forceinline__ bool all_see(int k0, int k1) const { return k1 <= first; }
+  __device__ __forceinline__ bool none_sees(int k0, int k1) const { return k0 > last; }
+};
+
+// A window's run leaves a gap: key `at` + i is the cache's row at + gap + i, and the
+// keys before it, the first entries that stay visible, are rows of their own number.
+struct Gap {
+  int at, gap;
+  __device__ __forceinline__ int row(int key) const { return key < at ? key : key + gap; }
+  __device__ __forceinline__ int key(int row) const { return row < at ? row : max(row - gap, at - 1); }
+};
+
+// Lane's query sees the rows [low, end) and [0, sink) below end; keys [from, ...) lie
+// in the window of every row of the wave, keys [at, to) of none.
+struct Windowed {
+  Gap g;
+  int low, end, sink, first, last, from, to;
+  __device__ __forceinline__ bool sees(int key) const {
+    const int r = g.row(key);
+    return r < end && (r >= low || r < sink);
+  }
+  __device__ __forceinline__ bool all_see(int k0, int k1) const { return k1 <= first && k0 >= from; }
+  __device__ __forceinline__ bool none_sees(int k0, int k1) const { return k0 > last || (k0 >= g.at && k1 < to); }
+};
+
+// Tiles of keys [k0, k0 + n_keys) of a cache in bf16, global -> LDS by DMA (every wave
+// of the workgroup loads a quarter); rows past the last are zeros.
+// wave w loads rows [16 w, 16 w + 16) of a tile with four instructions of 4
+// rows; lane j fills slot j % 16 of row 16 w + 4 i + j / 16 (the swizzles are
+// their own inverses; from one i to the next the V chunk stays, the K chunk
+// flips bits 2-3)
+template <bool GAP>
+struct TilesBf16 {
+  pipe::i32x4 rk, rv;
+  uint32_t koff, voff, lds0;
+  int wave;
+  Gap g;
+  int key0;  // of this lane's row in the first tile (GAP)
+  // rows: rows of k / v that the run may touch (GAP: k0 is a key, else the run starts at row 0)
+  __device__ __forceinline__ void start(uint8_t* smem, const uint16_t* k, const uint16_t* v, int rows, int k0, Gap gap) {
+    const int lane = threadIdx.x & 63, lr = lane >> 4, ls16 = lane & 15;
+    wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
+    rk = pipe::make_rsrc(k, uint32_t(rows) * AP_ROWB);
+    rv = pipe::make_rsrc(v, uint32_t(rows) * AP_ROWB);
+    koff = uint32_t((16 * wave + lr) * AP_ROWB + ap_kslot(lr, ls16) * 16);
+    voff = uint32_t((16 * wave + lr) * AP_ROWB + ap_vslot(lr, ls16) * 16);
+    lds0 = uint32_t(reinterpret_cast<uintptr_t>(smem));
+    if constexpr (GAP) {
+      g = gap;
+      key0 = k0 + 16 * wave + lr;
+      koff += uint32_t(k0) * AP_ROWB;
+      voff += uint32_t(k0) * AP_ROWB;
+    }
+  }
+  __device__ __forceinline__ uint32_t skip(int kt, int i) const {
+    if constexpr (GAP) return key0 + kt * AP_KT + 4 * i >= g.at ? uint32_t(g.gap) * AP_ROWB : 0u;
+    return 0u;
+  }
+  __device__ __forceinline__ void load_k(int kt, int buf) {
+    const uint32_t dst = lds0 + uint32_t(buf * AP_TILE + wave * 4096), adv = uint32_t(kt) * AP_TILE;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pipe::dma16(dst + i * 1024, (koff ^ (i * 64)) + (adv + i * 1024) + skip(kt, i), rk, 0);
+  }
+  __device__ __forceinline__ void load_v(int kt, int buf) {
+    const uint32_t dst = lds0 + uint32_t((2 + buf) * AP_TILE + wave * 4096), adv = uint32_t(kt) * AP_TILE;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) pipe::dma16(dst + i * 1024, voff + (adv + i * 1024) + skip(kt, i), rv, 0);
+  }
+  // the first tiles but V(1), and everything requested, in LDS (before a barrier)
+  __device__ __forceinline__ void landed_but_one() const { pipe::wait_vm<4>(); }
+  __device__ __forceinline__ void landed() const { pipe::wait_vm<0>(); }
+};
+
+// Attends a workgroup's 4 x 32 query rows to n_kt tiles of 64 keys (the first is key
+// k0 to `see`), adding to each wave's state.
 //
-// K and V tiles of 64 keys go global -> LDS by DMA, two buffers each, rows past
-// n_keys as zeros; the S^T MFMAs of step kt + 1 are issued before the softmax
-// and the O^T MFMAs of step kt, so that its VALU work runs while the matrix
-// pipe is busy; one barrier a step, after which K(kt + 3) and V(kt + 2) are
-// requested.  The maximum is lazy: O and l are rescaled only when a row's
-// tile maximum exceeds it by more than AP_TAU, so p stays below 2^AP_TAU and
-// O / l is the same.  Every wave of the workgroup calls this alike.
+// Tiles come from `tiles`, two LDS buffers for K and V each; the S^T MFMAs of step
+// kt + 1 are issued before the softmax and the O^T MFMAs of step kt, so that its
+// VALU work runs while the matrix pipe is busy; one barrier a step, after which
+// K(kt + 3) and V(kt + 2) are requested.  The maximum is lazy: O and l are rescaled
+// only when a row's tile maximum exceeds it by more than AP_TAU, so p stays below
+// 2^AP_TAU and O / l is the same.  Every wave of the workgroup calls this alike.
 //
 // The weights are rounded to bf16 for the product with V, whose MFMA takes both
 // operands in the cache's type (half a step, 2^-9 to 2^-8 of each weight), and l
@@ -93,31 +169,10 @@ constexpr int FL_SMEM = 4 * AP_TILE;  // K0, K1, V0, V1
 // any value up to 2^8 rather than 1, so it is rounded too: relative error of a
 // chunk's outputs against 64 bits 0.0021-0.0023, of which the rounding of the
 // output itself is 0.0016-0.0017 (stream_segment, whose maximum is exact: 0.0018).
-__device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
-                                              int lim, int first, int last, float scale_log2, FlashRows& st) {
+template <class Tiles, class See>
+__device__ __forceinline__ void flash_tiles(uint8_t* smem, Tiles& tiles, int n_kt, int k0, const See& see,
+                                            float scale_log2, FlashRows& st) {
   const int t = threadIdx.x, lane = t & 63, hl = lane >> 5;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int n_kt = (n_keys + AP_KT - 1) / AP_KT;
-  const pipe::i32x4 rk = pipe::make_rsrc(k, uint32_t(n_keys) * AP_ROWB);
-  const pipe::i32x4 rv = pipe::make_rsrc(v, uint32_t(n_keys) * AP_ROWB);
-  // wave w loads rows [16 w, 16 w + 16) of a tile with four instructions of 4
-  // rows; lane j fills slot j % 16 of row 16 w + 4 i + j / 16 (the swizzles are
-  // their own inverses; from one i to the next the V chunk stays, the K chunk
-  // flips bits 2-3)
-  const int lr = lane >> 4, ls16 = lane & 15;
-  const uint32_t koff = uint32_t((16 * wave + lr) * AP_ROWB + ap_kslot(lr, ls16) * 16);
-  const uint32_t voff = uint32_t((16 * wave + lr) * AP_ROWB + ap_vslot(lr, ls16) * 16);
-  const uint32_t lds0 = uint32_t(reinterpret_cast<uintptr_t>(smem));
-  auto dma_k = [&](int kt, int buf) {
-    const uint32_t dst = lds0 + uint32_t(buf * AP_TILE + wave * 4096), adv = uint32_t(kt) * AP_TILE;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) pipe::dma16(dst + i * 1024, (koff ^ (i * 64)) + (adv + i * 1024), rk, 0);
-  };
-  auto dma_v = [&](int kt, int buf) {
-    const uint32_t dst = lds0 + uint32_t((2 + buf) * AP_TILE + wave * 4096), adv = uint32_t(kt) * AP_TILE;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) pipe::dma16(dst + i * 1024, voff + (adv + i * 1024), rv, 0);
-  };
   auto qk = [&](int buf, f32x16 (&sc)[2]) {
     const uint8_t* kp = smem + buf * AP_TILE + (lane & 31) * AP_ROWB;
 #pragma unroll
@@ -139,15 +194,15 @@ __device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, 
   for (int db = 0; db < 4; ++db) vdb[db] = vlane + uint32_t(64 * (db ^ ve));
 
   auto softmax_pv = [&](int buf, int kv0, f32x16 (&sc)[2]) {
-    const bool live1 = kv0 + 32 <= last;
-    if (kv0 + AP_KT - 1 > first) {
+    const bool live1 = !see.none_sees(kv0 + 32, kv0 + AP_KT - 1);
+    if (!see.all_see(kv0, kv0 + AP_KT - 1)) {
       asm volatile("");  // keeps this a branch: the mask is not worth computing on every step
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           const int key = kv0 + kb * 32 + (i >> 2) * 8 + hl * 4 + (i & 3);
-          if (key > lim) sc[kb][i] = -INFINITY;
+          if (!see.sees(key)) sc[kb][i] = -INFINITY;
         }
     }
     float mx[11];  // maximum as a tree of 3-input maxima
@@ -208,36 +263,36 @@ __device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, 
   };
 
   __syncthreads();  // an earlier segment's LDS reads are done
-  dma_k(0, 0);
-  dma_v(0, 0);
+  tiles.load_k(0, 0);
+  tiles.load_v(0, 0);
   if (n_kt > 1) {
-    dma_k(1, 1);
-    dma_v(1, 1);
-    pipe::wait_vm<4>();
+    tiles.load_k(1, 1);
+    tiles.load_v(1, 1);
+    tiles.landed_but_one();
   } else {
-    pipe::wait_vm<0>();
+    tiles.landed();
   }
   __syncthreads();  // K(0), V(0), K(1) visible
   // end of step kt: K(kt + 2) and V(kt + 1) have landed; K(kt + 1)'s and V(kt)'s
   // buffers are free
   auto turn = [&](int kt) {
     const int buf = kt & 1;
-    pipe::wait_vm<0>();
+    tiles.landed();
     __syncthreads();
-    if (kt + 3 < n_kt) dma_k(kt + 3, buf ^ 1);
-    if (kt + 2 < n_kt) dma_v(kt + 2, buf);
+    if (kt + 3 < n_kt) tiles.load_k(kt + 3, buf ^ 1);
+    if (kt + 2 < n_kt) tiles.load_v(kt + 2, buf);
   };
   f32x16 sc[2], sn[2];
   qk(0, sc);
   if (n_kt > 2) {
     __syncthreads();  // every wave is done with K(0)'s buffer
-    dma_k(2, 0);
+    tiles.load_k(2, 0);
   }
   // steps in pairs, the score registers swapping roles
   auto one = [&](int kt, f32x16 (&cur)[2], f32x16 (&nxt)[2], auto has_next) {
-    const int kv0 = kt * AP_KT, buf = kt & 1;
+    const int kv0 = k0 + kt * AP_KT, buf = kt & 1;
     if constexpr (decltype(has_next)::value) qk(buf ^ 1, nxt);
-    if (kv0 <= last) softmax_pv(buf, kv0, cur);
+    if (!see.none_sees(kv0, kv0 + AP_KT - 1)) softmax_pv(buf, kv0, cur);
     turn(kt);
   };
   int kt = 0;
@@ -253,34 +308,56 @@ __device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, 
   }
 }
 
+// Keys [0, n_keys) of k / v (rows of HD bf16; n_keys >= 1).
+__device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
+                                              const Causal& see, float scale_log2, FlashRows& st) {
+  TilesBf16<false> tiles;
+  tiles.start(smem, k, v, n_keys, 0, Gap{0, 0});
+  flash_tiles(smem, tiles, (n_keys + AP_KT - 1) / AP_KT, 0, see, scale_log2, st);
+}
+
+// Keys [k0, k1) (k0 < k1) of a window's run over a cache's rows.
+__device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int k0, int k1,
+                                              const Windowed& see, float scale_log2, FlashRows& st) {
+  TilesBf16<true> tiles;
+  tiles.start(smem, k, v, see.g.row(k1 - 1) + 1, k0, see.g);
+  flash_tiles(smem, tiles, (k1 - k0 + AP_KT - 1) / AP_KT, k0, see, scale_log2, st);
+}
+
 // Few query rows (up to 32) over many keys, where the keys' stream is what costs:
 // every wave of the workgroup holds the same rows and takes its own 64-key tiles
 // w, w + 4, ... of keys [0, n_keys) of k / v.  K rows go from memory straight
 // into A-operand registers and V by DMA into the wave's own LDS tile, every load
 // of a tile in flight at once and no barrier between the waves; flash_join adds
-// up their states.  Lane's row sees keys [0, lim].  Weights in bf16 for the MFMA with V
-// and l in 32 bits, as in flash_segment.
-__device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
-                                               int lim, float scale_log2, FlashRows& st) {
+// up their states.  Weights in bf16 for the MFMA with V and l in 32 bits, as in
+// flash_tiles.  k0, k1: the run's keys [k0, k1), which start at 0 without a gap.
+template <bool GAP, class See>
+__device__ __forceinline__ void stream_keys(uint8_t* smem, const uint16_t* k, const uint16_t* v, int k_first, int n_keys,
+                                            const See& see, Gap g, float scale_log2, FlashRows& st) {
   const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   uint8_t* vb = smem + wave * AP_TILE;
   const int vg = lane >> 4, ve = (lane >> 2) & 3, vq = lane & 3;
   const uint32_t vlane = uint32_t((4 * (vg >> 1) + ve) * AP_ROWB +
                                   (((2 * (vg & 1) + (vq >> 1)) ^ (2 * (ve >> 1))) * 16) + 8 * (vq & 1));
-  const pipe::i32x4 rv = pipe::make_rsrc(v, uint32_t(n_keys) * AP_ROWB);  // rows past the end read as zeros
+  const int rows = GAP ? g.row(n_keys - 1) + 1 : n_keys;
+  const pipe::i32x4 rv = pipe::make_rsrc(v, uint32_t(rows) * AP_ROWB);  // rows past the end read as zeros
   const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>(smem)) + uint32_t(wave * AP_TILE);
   const uint32_t voff = uint32_t((lane >> 4) * AP_ROWB + ap_vslot(lane >> 4, lane & 15) * 16);
 #pragma unroll 1
-  for (int k0 = wave * AP_KT; k0 < n_keys; k0 += 4 * AP_KT) {
+  for (int k0 = (GAP ? k_first : 0) + wave * AP_KT; k0 < n_keys; k0 += 4 * AP_KT) {
     const int last = min(AP_KT, n_keys - k0) - 1;  // rows past it repeat it (their p is 0)
     u32x4 ka[2][HD / 16];
     wave_lds_sync();  // the last tile's V reads are done
 #pragma unroll
-    for (int i = 0; i < 16; ++i) pipe::dma16(lds + i * 1024, voff + uint32_t(k0 + 4 * i) * AP_ROWB, rv, 0);
+    for (int i = 0; i < 16; ++i) {
+      const uint32_t skip = GAP && k0 + 4 * i + (lane >> 4) >= g.at ? uint32_t(g.gap) * AP_ROWB : 0u;
+      pipe::dma16(lds + i * 1024, voff + uint32_t(k0 + 4 * i) * AP_ROWB + skip, rv, 0);
+    }
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb) {
-      const uint16_t* kp = k + int64_t(k0 + min(mb * 32 + col, last)) * HD + hl * 8;
+      const int key = k0 + min(mb * 32 + col, last);
+      const uint16_t* kp = k + int64_t(GAP ? g.row(key) : key) * HD + hl * 8;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) ka[mb][ks] = ld16(kp + ks * 16);
     }
@@ -293,14 +370,13 @@ __device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k,
         sc[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka[mb][ks]), st.qf[ks], sc[mb], 0,
                                                          0, 0);
     }
-    const int see = min(lim - k0, last);
     float m = -INFINITY;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int key = mb * 32 + (e >> 2) * 8 + hl * 4 + (e & 3);
-        sc[mb][e] = key <= see ? sc[mb][e] * scale_log2 : -INFINITY;
+        sc[mb][e] = key <= last && see.sees(k0 + key) ? sc[mb][e] * scale_log2 : -INFINITY;
         m = fmaxf(m, sc[mb][e]);
       }
     {
@@ -345,6 +421,15 @@ __device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k,
       }
     }
   }
+}
+
+__device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
+                                               const Causal& see, float scale_log2, FlashRows& st) {
+  stream_keys<false>(smem, k, v, 0, n_keys, see, Gap{0, 0}, scale_log2, st);
+}
+__device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int k0, int k1,
+                                               const Windowed& see, float scale_log2, FlashRows& st) {
+  stream_keys<true>(smem, k, v, k0, k1, see, see.g, scale_log2, st);
 }
 
 // The four waves' states of the same rows into wave 0's, through LDS in register

@@ -2,6 +2,7 @@
 // into it, and its values back (head_dim 128; the format is in kv4.hpp).
 #include "attn_tile.hpp"
 #include "kv4.hpp"
+#include "window.hpp"
 
 #include <math.h>
 
@@ -133,21 +134,6 @@ __global__ __launch_bounds__(64) void kv4_append_kernel(
 }
 
 // ====================================================================== attention
-struct Kv16 {
-  const uint16_t *k, *v;
-  __device__ float dot(int64_t row, const float* q) const {
-    float s = 0.0f;
-    for (int c = 0; c < HD / 8; ++c) {
-      const u32x4 w = ld16(k + row * HD + c * 8);
-      s += dot8(w, q + c * 8);
-    }
-    return s;
-  }
-  __device__ float2 value(int64_t row, int l) const {
-    const uint32_t w = reinterpret_cast<const uint32_t*>(v)[row * (HD / 2) + l];
-    return make_float2(bf16_lo(w), bf16_hi(w));
-  }
-};
 struct Kv4 {
   const uint8_t *k, *ks, *v, *vs;
   __device__ float dot(int64_t row, const float* q) const {
@@ -209,68 +195,13 @@ __global__ __launch_bounds__(64) void attn_entries_kernel(const uint16_t* __rest
   reinterpret_cast<uint32_t*>(out)[(t * Hq + h) * (HD / 2) + l] = pack_bf16x2(o0 * inv, o1 * inv);
 }
 
-static int win_check(const char* fn, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max,
-                     int64_t max_ctx, int64_t window, int64_t sink) {
-  QMOE_REQUIRE(D == HD, "%s: head_dim must be 128 (D=%lld)", fn, (long long)D);
-  QMOE_REQUIRE(Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && Hq / Hkv <= 16 && Hkv < 4096,
-               "%s: need Hq %% Hkv == 0, Hq / Hkv <= 16 and Hkv < 4096", fn);
-  QMOE_REQUIRE(B >= 0 && B < 65536 && S >= 0 && S < (1ll << 22) && B * S * Hq < (1ll << 27),
-               "%s: bad B/S (B * S * Hq must be below 2^27)", fn);
-  QMOE_REQUIRE(S_max > 0 && S_max <= (1ll << 22), "%s: S_max must be in [1, 2^22]", fn);
-  QMOE_REQUIRE(max_ctx >= 0 && max_ctx <= S_max, "%s: need 0 <= max_ctx <= S_max", fn);
-  QMOE_REQUIRE(window >= 0 && sink >= 0, "%s: window and sink must be >= 0", fn);
-  return QMOE_OK;
-}
-
-static WinArgs win_args(const int32_t* ctx_len, int64_t S, int64_t S_max, int64_t max_ctx, int64_t window,
-                        int64_t sink) {
-  WinArgs w;
-  w.ctx_len = ctx_len;
-  w.S = int(S);
-  w.S_max = int(S_max);
-  w.max_ctx = int(max_ctx);
-  w.window = int(window == 0 ? WIN_NONE : std::min<int64_t>(window, WIN_NONE));
-  w.sink = int(std::min<int64_t>(sink, WIN_NONE));
-  return w;
-}
-
-static bool overlap(const void* a, int64_t na, const void* b, int64_t nb) {
-  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-  return x < y + uintptr_t(nb) && y < x + uintptr_t(na);
-}
-
 }  // namespace qmoe
 
 using namespace qmoe;
 
-extern "C" int64_t qmoe_attn_window_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
-                                              int64_t sink, int64_t max_ctx) {
-  if (window <= 0 || win_check("qmoe_attn_window_workspace", B, S, Hq, Hkv, D, 1 << 22, max_ctx, window, sink)) return -1;
-  return 0;
-}
-
-extern "C" int qmoe_attn_window(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
-                                const int32_t* ctx_len, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
-                                int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
-                                void* workspace, int64_t workspace_bytes, qmoe_bf16* out, qmoe_stream_t stream) {
-  const char* fn = "qmoe_attn_window";
-  QMOE_REQUIRE(B == 0 || S == 0 || (q && k_cache && v_cache && ctx_len && out), "%s: null pointer", fn);
-  if (int rc = win_check(fn, B, S, Hq, Hkv, D, S_max, max_ctx, window, sink)) return rc;
-  QMOE_REQUIRE(window > 0, "%s: window must be positive", fn);
-  QMOE_REQUIRE(scale > 0.0f && std::isfinite(scale), "%s: scale must be positive and finite", fn);
-  if (B == 0 || S == 0) return QMOE_OK;
-  QMOE_REQUIRE(aligned16(q, k_cache, v_cache, static_cast<uint8_t*>(workspace), out),
-               "%s: operands must be 16-byte aligned", fn);
-  QMOE_REQUIRE(!overlap(q, B * S * Hq * HD * 2, out, B * S * Hq * HD * 2), "%s: out overlaps q", fn);
-  hipLaunchKernelGGL(attn_entries_kernel<Kv16>, dim3(unsigned(B * S * Hq)), dim3(64), 0, as_stream(stream), q,
-                     Kv16{k_cache, v_cache}, win_args(ctx_len, S, S_max, max_ctx, window, sink), int(Hq), int(Hkv),
-                     scale * 1.4426950408889634f, out);
-  return hip_status(fn);
-}
-
 extern "C" int64_t qmoe_attn_kv4_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
                                            int64_t sink, int64_t max_ctx) {
-  if (win_check("qmoe_attn_kv4_workspace", B, S, Hq, Hkv, D, 1 << 22, max_ctx, window, sink)) return -1;
+  if (win_check("qmoe_attn_kv4_workspace", B, S, Hq, Hkv, D, 1 << 22, max_ctx, window, sink, 1.0f)) return -1;
   return 0;
 }
 
@@ -282,15 +213,15 @@ extern "C" int qmoe_attn_kv4(const qmoe_bf16* q, const uint8_t* k_cache, const u
   const char* fn = "qmoe_attn_kv4";
   QMOE_REQUIRE(B == 0 || S == 0 || (q && k_cache && k_scales && v_cache && v_scales && ctx_len && out),
                "%s: null pointer", fn);
-  if (int rc = win_check(fn, B, S, Hq, Hkv, D, S_max, max_ctx, window, sink)) return rc;
-  QMOE_REQUIRE(scale > 0.0f && std::isfinite(scale), "%s: scale must be positive and finite", fn);
+  if (int rc = win_check(fn, B, S, Hq, Hkv, D, S_max, max_ctx, window, sink, scale)) return rc;
   if (B == 0 || S == 0) return QMOE_OK;
-  QMOE_REQUIRE(aligned16(q, k_cache, k_scales, v_cache, v_scales, static_cast<uint8_t*>(workspace), out),
-               "%s: operands must be 16-byte aligned", fn);
-  QMOE_REQUIRE(!overlap(q, B * S * Hq * HD * 2, out, B * S * Hq * HD * 2), "%s: out overlaps q", fn);
+  if (int rc = win_operands(fn, 1, 0, workspace, workspace_bytes, q, out, B * S * Hq,
+                            aligned16(k_cache, k_scales, v_cache, v_scales)))
+    return rc;
+  WinArgs w = win_args(S, S_max, max_ctx, window, sink);
+  w.ctx_len = ctx_len;
   hipLaunchKernelGGL(attn_entries_kernel<Kv4>, dim3(unsigned(B * S * Hq)), dim3(64), 0, as_stream(stream), q,
-                     Kv4{k_cache, k_scales, v_cache, v_scales}, win_args(ctx_len, S, S_max, max_ctx, window, sink),
-                     int(Hq), int(Hkv), scale * 1.4426950408889634f, out);
+                     Kv4{k_cache, k_scales, v_cache, v_scales}, w, int(Hq), int(Hkv), scale * 1.4426950408889634f, out);
   return hip_status(fn);
 }
 

@@ -1,5 +1,4 @@
-// Entries of the 4-bit cache (head_dim 128) and what a query of a windowed
-// attention sees.
+// Entries of the 4-bit cache (head_dim 128).
 //
 // An entry is 128 e2m1 numbers, two a byte with the even element in the low half,
 // and a power of two (a byte p for 2^(p - 127)) for every 32 of them: the block
@@ -63,23 +62,6 @@ __device__ __forceinline__ float kv4_scale(uint32_t power) {
 template <int B>
 __device__ __forceinline__ uint32_t kv4_pair(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, B));
-}
-
-// ---------------------------------------------------------------------- windows
-constexpr int WIN_NONE = 1 << 30;  // no window: past every length
-
-// Query s of row b stands at index p = ctx_len[b] - 1 + s and sees the entries
-// e <= p with e > p - window or e < sink, and none from max_ctx on.
-struct WinArgs {
-  const int32_t* ctx_len;
-  int S, S_max, max_ctx, window, sink;
-};
-struct WinRow {
-  int low, end;  // sees [low, end) and [0, min(sink, end))
-};
-__device__ __forceinline__ WinRow win_row(const WinArgs& w, int b, int s) {
-  const int n = min(max(w.ctx_len[b], -w.S), w.S_max) + s;  // p + 1
-  return {max(n - w.window, 0), min(max(n, 0), w.max_ctx)};
 }
 
 }  // namespace qmoe
