@@ -22,6 +22,7 @@
 //                          the attention left each row's lse = m + log2 l.
 #include "attn_tile.hpp"
 #include "common.hpp"
+#include "kv4.hpp"
 #include "window.hpp"
 
 #include <math.h>
@@ -66,13 +67,8 @@ struct ArArgs {
   int NS, n_pre, joint, nb_pre, nb_own;  // nb: blocks of 32 rows
   ArKind pre, own;
   WinArgs win;  // of a windowed attention
+  Cache4 kv4;   // its cache, when that is in 4 bits
 };
-
-// r / G for 0 <= r < 2^32 / G, by a multiplication
-__host__ __device__ __forceinline__ uint32_t ar_magic(uint32_t G) {
-  return G == 1 ? 0u : uint32_t(((1ull << 32) + G - 1) / G);
-}
-__device__ __forceinline__ int ar_div(uint32_t r, uint32_t magic) { return int(magic ? __umulhi(r, magic) : r); }
 
 // Own entries that query s of batch row b sees.
 __device__ __forceinline__ int ar_sees(const ArArgs& a, int b, int s) {
@@ -230,7 +226,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
 // An item of a windowed attention: row tile, kv head, sequence and a run of the keys
 // that the tile's queries see, the window's behind the first ones that stay (the
 // windows of consecutive queries are one run of rows).
-template <bool stream>
+template <bool stream, bool KV4>
 __device__ __forceinline__ void aw_item(const ArArgs& a, uint8_t* smem) {
   const int lane = threadIdx.x & 63, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
@@ -262,8 +258,11 @@ __device__ __forceinline__ void aw_item(const ArArgs& a, uint8_t* smem) {
   see.to = __builtin_amdgcn_readfirstlane(w0.low <= see.sink ? 0 : see.g.key(w0.low));
   const int k0 = run * kd.run * KS, k1 = min(n, k0 + kd.run * KS);
   if (k0 < k1) {
-    const int64_t base = (int64_t(b) * a.Hkv + kvh) * a.S_max * HD;
-    if constexpr (stream)
+    const int64_t at = (int64_t(b) * a.Hkv + kvh) * a.S_max, base = at * HD;
+    if constexpr (KV4)
+      flash_segment(smem, a.kv4.k + at * KV4_ROWB, a.kv4.ks + at * 4, a.kv4.v + at * KV4_ROWB, a.kv4.vs + at * 4, k0, k1,
+                    see, a.scale_log2, st);
+    else if constexpr (stream)
       stream_segment(smem, a.k + base, a.v + base, k0, k1, see, a.scale_log2, st);
     else
       flash_segment(smem, a.k + base, a.v + base, k0, k1, see, a.scale_log2, st);
@@ -271,10 +270,10 @@ __device__ __forceinline__ void aw_item(const ArArgs& a, uint8_t* smem) {
   ar_finish<stream>(a, kd, false, smem, st, ArRow{run, kvh, b, rw, row, rows, sq, qrow, live});
 }
 
-template <bool STREAM>
+template <bool STREAM, bool KV4>
 __global__ __launch_bounds__(256, 2) void attn_window_kernel(const ArArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];
-  aw_item<STREAM>(a, smem);
+  aw_item<STREAM, KV4>(a, smem);
 }
 
 // Joins the runs of 32 packed rows of a kv head (8 x 101 queries, 2 runs, 8 us; 64
@@ -861,6 +860,29 @@ static ArArgs aw_args(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_m
   ar_plan(a, std::min<int64_t>(max_ctx, int64_t(a.win.window) + a.win.sink + tile - 1), grid);
   return a;
 }
+
+int64_t attn_kv4_tiles_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
+                                 int64_t sink) {
+  int64_t grid;
+  return ar_part_bytes(aw_args(B, S, Hq, Hkv, AR_MAX_KEYS, max_ctx, window, sink, &grid));
+}
+
+int attn_kv4_tiles(const char* fn, const uint16_t* q, const Cache4& cache, const int32_t* ctx_len, int64_t B, int64_t S,
+                   int64_t Hq, int64_t Hkv, int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
+                   void* workspace, int64_t workspace_bytes, uint16_t* out, hipStream_t stream) {
+  int64_t grid;
+  ArArgs a = aw_args(B, S, Hq, Hkv, S_max, max_ctx, window, sink, &grid);
+  a.q = q;
+  a.kv4 = cache;
+  a.win.ctx_len = ctx_len;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.out = out;
+  a.part = static_cast<float*>(workspace);
+  if (int rc = win_operands(fn, grid, ar_part_bytes(a), workspace, workspace_bytes, q, out, B * S * Hq, true)) return rc;
+  hipLaunchKernelGGL((attn_window_kernel<false, true>), dim3(unsigned(grid)), dim3(256), 0, stream, a);
+  if (int rc = hip_status(fn)) return rc;
+  return ar_merge(fn, a, stream);
+}
 }  // namespace qmoe
 
 extern "C" int64_t qmoe_attn_window_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
@@ -894,9 +916,9 @@ extern "C" int qmoe_attn_window(const qmoe_bf16* q, const qmoe_bf16* k_cache, co
                             aligned16(k_cache, v_cache)))
     return rc;
   if (a.own.stream)
-    hipLaunchKernelGGL(attn_window_kernel<true>, dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
+    hipLaunchKernelGGL((attn_window_kernel<true, false>), dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
   else
-    hipLaunchKernelGGL(attn_window_kernel<false>, dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
+    hipLaunchKernelGGL((attn_window_kernel<false, false>), dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
   if (int rc = hip_status(fn)) return rc;
   return ar_merge(fn, a, as_stream(stream));
 }

@@ -2,7 +2,6 @@
 // into it, and its values back (head_dim 128; the format is in kv4.hpp).
 #include "attn_tile.hpp"
 #include "kv4.hpp"
-#include "window.hpp"
 
 #include <math.h>
 
@@ -133,97 +132,9 @@ __global__ __launch_bounds__(64) void kv4_append_kernel(
   kv4_put(k4 + at * KV4_ROWB, ks + at * 4, 1, l, y * double(c) + x * double(sn));
 }
 
-// ====================================================================== attention
-struct Kv4 {
-  const uint8_t *k, *ks, *v, *vs;
-  __device__ float dot(int64_t row, const float* q) const {
-    float s = 0.0f;
-    for (int b = 0; b < 4; ++b) {
-      const u32x4 w = ld16(k + row * KV4_ROWB + b * 16);
-      const float scale = kv4_scale(ks[row * 4 + b]);
-      for (int c = 0; c < 4; ++c)
-        s += dot8(u32x4{kv4_pair<0>(w[c], scale), kv4_pair<1>(w[c], scale), kv4_pair<2>(w[c], scale),
-                        kv4_pair<3>(w[c], scale)},
-                  q + b * 32 + c * 8);
-    }
-    return s;
-  }
-  __device__ float2 value(int64_t row, int l) const {
-    const uint32_t w = kv4_pair<0>(v[row * KV4_ROWB + l], kv4_scale(vs[row * 4 + l / 16]));
-    return make_float2(bf16_lo(w), bf16_hi(w));
-  }
-};
-
-// One wave a (query, q head): 64 entries at a time, a lane for each one's logit,
-// then for two dims of the output.
-template <class Cache>
-__global__ __launch_bounds__(64) void attn_entries_kernel(const uint16_t* __restrict__ q, const Cache cache,
-                                                          const WinArgs w, int Hq, int Hkv, float scale_log2,
-                                                          uint16_t* __restrict__ out) {
-  __shared__ float qs[HD], ps[64];
-  const int l = threadIdx.x, h = int(blockIdx.x) % Hq;
-  const int64_t t = int(blockIdx.x) / Hq;
-  const int b = int(t / w.S);
-  const uint32_t qw = reinterpret_cast<const uint32_t*>(q)[(t * Hq + h) * (HD / 2) + l];
-  qs[2 * l] = bf16_lo(qw);
-  qs[2 * l + 1] = bf16_hi(qw);
-  __syncthreads();
-  const WinRow see = win_row(w, b, int(t % w.S));
-  const int64_t base = (int64_t(b) * Hkv + h / (Hq / Hkv)) * w.S_max;
-  float m = -INFINITY, sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int part = 0; part < 2; ++part) {
-    const int from = part ? see.low : 0, to = part ? see.end : min(min(w.sink, see.low), see.end);
-    for (int k0 = from; k0 < to; k0 += 64) {
-      const int n = min(64, to - k0);
-      const float x = l < n ? cache.dot(base + k0 + l, qs) * scale_log2 : -INFINITY;
-      const float top = fmaxf(m, wave_max(x)), a = exp2f(m - top), p = l < n ? exp2f(x - top) : 0.0f;
-      m = top;
-      sum = sum * a + wave_sum(p);
-      o0 *= a;
-      o1 *= a;
-      ps[l] = p;
-      __syncthreads();
-      for (int i = 0; i < n; ++i) {
-        const float2 v = cache.value(base + k0 + i, l);
-        o0 = fmaf(ps[i], v.x, o0);
-        o1 = fmaf(ps[i], v.y, o1);
-      }
-      __syncthreads();
-    }
-  }
-  const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-  reinterpret_cast<uint32_t*>(out)[(t * Hq + h) * (HD / 2) + l] = pack_bf16x2(o0 * inv, o1 * inv);
-}
-
 }  // namespace qmoe
 
 using namespace qmoe;
-
-extern "C" int64_t qmoe_attn_kv4_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
-                                           int64_t sink, int64_t max_ctx) {
-  if (win_check("qmoe_attn_kv4_workspace", B, S, Hq, Hkv, D, 1 << 22, max_ctx, window, sink, 1.0f)) return -1;
-  return 0;
-}
-
-extern "C" int qmoe_attn_kv4(const qmoe_bf16* q, const uint8_t* k_cache, const uint8_t* k_scales,
-                             const uint8_t* v_cache, const uint8_t* v_scales, const int32_t* ctx_len, int64_t B,
-                             int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t S_max, int64_t max_ctx,
-                             int64_t window, int64_t sink, float scale, void* workspace, int64_t workspace_bytes,
-                             qmoe_bf16* out, qmoe_stream_t stream) {
-  const char* fn = "qmoe_attn_kv4";
-  QMOE_REQUIRE(B == 0 || S == 0 || (q && k_cache && k_scales && v_cache && v_scales && ctx_len && out),
-               "%s: null pointer", fn);
-  if (int rc = win_check(fn, B, S, Hq, Hkv, D, S_max, max_ctx, window, sink, scale)) return rc;
-  if (B == 0 || S == 0) return QMOE_OK;
-  if (int rc = win_operands(fn, 1, 0, workspace, workspace_bytes, q, out, B * S * Hq,
-                            aligned16(k_cache, k_scales, v_cache, v_scales)))
-    return rc;
-  WinArgs w = win_args(S, S_max, max_ctx, window, sink);
-  w.ctx_len = ctx_len;
-  hipLaunchKernelGGL(attn_entries_kernel<Kv4>, dim3(unsigned(B * S * Hq)), dim3(64), 0, as_stream(stream), q,
-                     Kv4{k_cache, k_scales, v_cache, v_scales}, w, int(Hq), int(Hkv), scale * 1.4426950408889634f, out);
-  return hip_status(fn);
-}
 
 static int kv4_check(const char* fn, int64_t B, int64_t Hkv, int64_t D, int64_t S_max, int64_t n) {
   QMOE_REQUIRE(D == HD, "%s: head_dim must be 128 (D=%lld)", fn, (long long)D);

@@ -9,6 +9,12 @@
 
 namespace qmoe {
 
+// r / G for 0 <= r < 2^32 / G, by a multiplication
+__host__ __device__ __forceinline__ uint32_t ar_magic(uint32_t G) {
+  return G == 1 ? 0u : uint32_t(((1ull << 32) + G - 1) / G);
+}
+__device__ __forceinline__ int ar_div(uint32_t r, uint32_t magic) { return int(magic ? __umulhi(r, magic) : r); }
+
 constexpr int WIN_NONE = 1 << 30;  // no window: past every length
 
 // Query s of row b stands at index p = ctx_len[b] - 1 + s and sees the entries
@@ -34,7 +40,19 @@ __device__ __forceinline__ Gap win_run(const WinArgs& w, int low, int end, int* 
   return {stay, max(low - stay, 0)};
 }
 
+// A cache in 4 bits: numbers [B][Hkv][S_max][64] and powers [B][Hkv][S_max][4].
+struct Cache4 {
+  const uint8_t *k, *ks, *v, *vs;
+};
+
 // ---------------------------------------------------------------------- host
+// qmoe_attn_kv4's many rows (S * Hq / Hkv > 64), on the tiles of attn_rows.hip.
+int64_t attn_kv4_tiles_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
+                                 int64_t sink);
+int attn_kv4_tiles(const char* fn, const uint16_t* q, const Cache4& cache, const int32_t* ctx_len, int64_t B, int64_t S,
+                   int64_t Hq, int64_t Hkv, int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
+                   void* workspace, int64_t workspace_bytes, uint16_t* out, hipStream_t stream);
+
 inline WinArgs win_args(int64_t S, int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink) {
   WinArgs w{};
   w.S = int(S);
