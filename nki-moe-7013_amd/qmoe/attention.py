@@ -173,14 +173,49 @@ class BoundedKVCache(KVCache):
         self.slot_pos = torch.full((B, n_kv, state.capacity), -1, dtype=torch.int32, device=dev)
 
 
+class PromptRows:
+    """A prompt's keys and values in bf16, before they go to a cache in 4 bits: one
+    scratch cache for all layers, which run one after another."""
+
+    def __init__(self):
+        self.cache: Optional[KVCache] = None
+
+    def of(self, B: int, n_kv: int, S: int, head_dim: int, device) -> KVCache:
+        c = self.cache
+        if c is None or c.k.shape[:2] != (B, n_kv) or c.capacity < S or c.k.device != device:
+            c = self.cache = KVCache(B, n_kv, S, head_dim, device)
+        return c
+
+
+class KV4Cache(KVCache):
+    """One layer's cache in 4 bits (:func:`qmoe.ops.kv4_cache`); a token's cache
+    index is its position, as in a :class:`KVCache`.  Unpacks as the bf16 ``(K,
+    V)`` that its entries stand for (new tensors: writing to them changes no
+    entry)."""
+
+    def __init__(self, B: int, n_kv: int, S_max: int, head_dim: int, device, rows: Optional[PromptRows] = None):
+        self.tensors = ops.kv4_cache(B, n_kv, S_max, head_dim, device)
+        self.k, self.v = self.tensors[0], self.tensors[2]  # the codes
+        self.rows = PromptRows() if rows is None else rows
+
+    def __iter__(self):
+        return iter(ops.kv4_load(self.tensors))
+
+    def __getitem__(self, i):
+        return ops.kv4_load(self.tensors)[i]
+
+
 class Attention:
     """One layer's attention.  ``forward`` adds ``o_proj(attn(x))`` to the fp32
     residual stream in place (the residual add of qwen_with_nki.py:10200 fused
-    into the o_proj epilogue)."""
+    into the o_proj epilogue).  With a ``window`` a query sees the last ``window``
+    positions up to its own and the first ``sink`` ones."""
 
-    def __init__(self, wqkv, q_norm, k_norm, wo, n_q: int, n_kv: int, head_dim: int, eps: float):
+    def __init__(self, wqkv, q_norm, k_norm, wo, n_q: int, n_kv: int, head_dim: int, eps: float, window: int = 0,
+                 sink: int = 0):
         self.wqkv, self.q_norm, self.k_norm, self.wo = wqkv, q_norm, k_norm, wo
         self.n_q, self.n_kv, self.head_dim, self.eps = n_q, n_kv, head_dim, eps
+        self.window, self.sink = window, sink
         self.scale = 1.0 / math.sqrt(head_dim)
         self._ws = {}
 
@@ -225,10 +260,18 @@ class Attention:
         :class:`BoundedKVCache`: a decode row's entry goes to slot
         ``state.slots[b]`` and the weights of its attention to the scores; a
         prompt (``start`` 0, ``state.lengths`` real tokens a row) is attended
-        in full and then cut down to the budget.
+        in full and then cut down to the budget.  Neither goes with a window.
+
+        A :class:`KV4Cache`: a prompt (``start`` 0) attends its own keys and values
+        in bf16 and leaves them in 4 bits; steps and later chunks attend the
+        entries.
         """
         if cache.prefix is not None or isinstance(cache, BoundedKVCache):
+            if self.window:
+                raise ValueError("a shared prefix or a bounded cache has no window")
             o = self._special(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
+        elif self.window or isinstance(cache, KV4Cache):
+            o = self._windowed(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
         else:
             o = self._plain(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
         key = ("oproj", o.shape[0])
@@ -314,13 +357,9 @@ class Attention:
             ops.kv_evict(own.k, own.v, scores, pos, st.lengths, st.budget, st.recent, st.sink,
                          out=(cache.k, cache.v, cache.scores, cache.slot_pos))
             return o
-        gemv = ops.qkv_norm_rope_workspace(B, x.shape[1], self.n_q, self.n_kv, self.head_dim) > 0
-        if norm is not None:
-            raw = ops.gemv_rmsnorm(x, norm[0], norm[1], self.wqkv, _lib.GEMM_STORE_F32)
-        elif gemv or self._skinny_decode(x, B):
-            raw = ops.gemm(x, self.wqkv, _lib.GEMM_STORE_F32)
-        else:
-            raw = self._raw_of_any(x) if bounded else None
+        raw = self._raw(x, B, norm)
+        if raw is None and bounded:
+            raw = self._raw_of_any(x)
         if not bounded:
             if raw is None:
                 q = ops.qkv_norm_rope(x, self.wqkv, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, B, 1,
@@ -334,6 +373,47 @@ class Attention:
         q = ops.kv_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, st.slots, self.n_q, self.n_kv,
                           cache.k, cache.v, self.eps, scores=cache.scores, slot_pos=cache.slot_pos)
         return ops.attn_decode_scored(q, cache.k, cache.v, st.ctx, cache.scores, self.scale, max_ctx=max_ctx)
+
+    def _raw(self, x: torch.Tensor, rows: int, norm: Optional[tuple]) -> Optional[torch.Tensor]:
+        """The raw f32 projection of a step's rows (``None``: ``qkv_norm_rope``'s)."""
+        if norm is not None:
+            return ops.gemv_rmsnorm(x, norm[0], norm[1], self.wqkv, _lib.GEMM_STORE_F32)
+        gemv = ops.qkv_norm_rope_workspace(rows, x.shape[1], self.n_q, self.n_kv, self.head_dim) > 0
+        return ops.gemm(x, self.wqkv, _lib.GEMM_STORE_F32) if gemv or self._skinny_decode(x, rows) else None
+
+    def _windowed(self, x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm) -> torch.Tensor:
+        """Attention outputs ``[B*S, Hq*D]`` with a window, over a cache in 4 bits, or both."""
+        four = isinstance(cache, KV4Cache)
+        if norm is not None and B * S != 1:
+            raise ValueError("the fused input norm takes one fp32 row on the GEMV path")
+        prompt = four and S > 1 and not isinstance(start, torch.Tensor) and start == 0
+        raw = self._raw(x, B * S, norm) if S == 1 or (four and not prompt) else None
+        if raw is None and four and not prompt:
+            raw = self._raw_of_any(x)
+        first = positions if S == 1 else positions.view(B, S)[:, 0]
+        top = max_ctx
+        if S > 1 and not isinstance(start, torch.Tensor):
+            top = min(cache.capacity, start + S)
+        if four and not prompt:
+            q = ops.kv4_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, positions, self.n_q,
+                               self.n_kv, cache.tensors, self.eps, S=S)
+            return ops.attn_kv4(q, cache.tensors, first + 1, B, S, self.window, self.sink, self.scale, max_ctx=top)
+        own = cache.rows.of(B, self.n_kv, S, self.head_dim, x.device) if four else cache
+        if raw is not None:
+            q = ops.kv_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, positions, self.n_q,
+                              self.n_kv, own.k, own.v, self.eps)
+        else:
+            n = ops.qkv_norm_rope_workspace(B * S, x.shape[1], self.n_q, self.n_kv, self.head_dim)
+            ws = torch.empty(n // 4, dtype=torch.float32, device=x.device) if n > 0 else None
+            q = ops.qkv_norm_rope(x, self.wqkv, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, B, S,
+                                  self.n_q, self.n_kv, own.k, own.v, self.eps, workspace=ws)
+        if four:
+            ops.kv4_store(own.k, own.v, cache.tensors, n=S)
+            top = S
+        if not self.window:
+            return ops.attn_prefill(q, own.k, own.v, B, S, 0, self.scale,
+                                    workspace=ops.attn_prefill_workspace(B, S, self.n_q, self.head_dim, x.device))
+        return ops.attn_window(q, own.k, own.v, first + 1, B, S, self.window, self.sink, self.scale, max_ctx=top)
 
     def _raw_of_any(self, x: torch.Tensor) -> torch.Tensor:
         """The raw projection of rows that ``_skinny_decode`` leaves to

@@ -45,6 +45,11 @@ def parse_args(argv=None):
     p.add_argument("--do-sample", action="store_true")
     p.add_argument("--speculation-length", type=int, default=0,
                    help="prompt-lookup speculation: tokens verified per step (the reference ships 5); 0 = off")
+    p.add_argument("--kv-cache-bits", type=int, default=16, choices=[16, 4],
+                   help="bits of a cached key's or value's element")
+    p.add_argument("--attention-window", type=int, default=None,
+                   help="positions a token sees up to its own (0: all; default: what config.json says)")
+    p.add_argument("--attention-sink", type=int, default=0, help="first positions it sees besides the window's")
     return p.parse_args(argv)
 
 
@@ -55,7 +60,8 @@ def prepare_inference(model_cls, args):
         batch_size=kw.get("batch_size", 1), seq_len=kw.get("seq_len", 640),
         max_length=kw.get("seq_len", 640), torch_dtype=kw.get("torch_dtype", "bfloat16"),
         tp_degree=kw.get("tp_degree", 1), seed=kw.get("seed", 0),
-        speculation_length=kw.get("speculation_length", 0))
+        speculation_length=kw.get("speculation_length", 0), kv_cache_bits=kw.get("kv_cache_bits", 16),
+        attention_window=kw.get("attention_window"), attention_sink=kw.get("attention_sink", 0))
     path = args.model_path
     load_config = None
     if path and os.path.isfile(os.path.join(path, "config.json")):

@@ -33,8 +33,8 @@ from typing import Any, Callable, Dict, List, Optional
 import torch
 
 from . import _lib, ops, weights
-from .attention import (Attention, BoundedKVCache, CacheBudget, KVCache, SharedPrefix, check_budget, default_recent,
-                        rope_tables)
+from .attention import (Attention, BoundedKVCache, CacheBudget, KV4Cache, KVCache, PromptRows, SharedPrefix,
+                        check_budget, default_recent, rope_tables)
 from .config import Qwen3MoeShape
 from .moe import MoEBlock
 
@@ -78,6 +78,20 @@ class MoENeuronConfig:
         self.kv_cache_slack = int(kwargs.pop("kv_cache_slack", 64))
         if self.kv_cache_budget < 0:
             raise ValueError("kv_cache_budget must be >= 0")
+        # bits of a cache's element: 16 (bf16), or 4 (e2m1 numbers with a power of two
+        # for every 32 of them)
+        self.kv_cache_bits = int(kwargs.pop("kv_cache_bits", 16))
+        if self.kv_cache_bits not in (4, 16):
+            raise ValueError("kv_cache_bits must be 16 or 4")
+        # positions that a query sees up to its own (0: all; None: what the model's
+        # config says), and the first ones that it sees besides
+        window = kwargs.pop("attention_window", None)
+        self.attention_window = None if window is None else int(window)
+        self.attention_sink = int(kwargs.pop("attention_sink", 0))
+        if (self.attention_window or 0) < 0 or self.attention_sink < 0:
+            raise ValueError("attention_window and attention_sink must be >= 0")
+        if self.kv_cache_budget and self.kv_cache_bits != 16:
+            raise ValueError("kv_cache_budget keeps entries in bf16 (kv_cache_bits=16)")
         self.seed = int(kwargs.pop("seed", 0))
         self.extra = kwargs  # every other generate-mode flag, accepted and ignored
 
@@ -115,6 +129,20 @@ class Qwen3MoeInferenceConfig:
         self.router_dtype = torch.float32
         self.router_act_fn = "softmax"
         self.normalize_top_k_affinities = True
+
+    def window(self) -> int:
+        """Positions that a query sees up to its own (0: all of them):
+        ``neuron_config.attention_window``, or the checkpoint's ``sliding_window``
+        where its ``use_sliding_window`` is set."""
+        w = self.neuron_config.attention_window
+        if w is None:
+            w = getattr(self, "sliding_window", None) if getattr(self, "use_sliding_window", False) else 0
+        w = int(w or 0)
+        if w < 0:
+            raise ValueError(f"sliding_window must not be negative (got {w})")
+        if w and self.neuron_config.kv_cache_budget:
+            raise ValueError("kv_cache_budget keeps entries by their weight: it goes with no attention window")
+        return w
 
     def shape(self) -> Qwen3MoeShape:
         return Qwen3MoeShape(**{k: getattr(self, k) for k in Qwen3MoeShape().to_dict()})
@@ -170,7 +198,8 @@ class NeuronQwen3MoeDecoderLayer:
         self.input_layernorm = RMSNormWeight(w["input_layernorm"], c.rms_norm_eps)
         self.post_attention_layernorm = RMSNormWeight(w["post_attention_layernorm"], c.rms_norm_eps)
         self.self_attn = Attention(w["wqkv"], w["q_norm"], w["k_norm"], w["wo"], c.num_attention_heads,
-                                   c.num_key_value_heads, c.head_dim, c.rms_norm_eps)
+                                   c.num_key_value_heads, c.head_dim, c.rms_norm_eps, c.window(),
+                                   c.neuron_config.attention_sink)
         self.mlp = MoEBlock(w["router"], w["w13"], w["w2"], c.num_experts_per_tok)
         self.cache: Optional[KVCache] = None
         self._rope = None  # (cos, sin) built from head_dim / rope_theta on first use
@@ -229,8 +258,8 @@ class NeuronQwen3MoeDecoderLayer:
         * ``position_ids[B, S]`` (default ``0..S-1``): row b holds consecutive
           positions; a chunk with S > 1 starts at the same position in every
           row; position == cache index.
-        * ``past_key_value``: a :class:`KVCache` or a ``(K, V)`` pair of bf16
-          ``[B, Hkv, S_max, D]`` tensors, updated in place.  Without it the
+        * ``past_key_value``: a :class:`KVCache` (a :class:`KV4Cache` too) or a ``(K,
+          V)`` pair of bf16 ``[B, Hkv, S_max, D]`` tensors, updated in place.  Without it the
           layer keeps its own cache, allocated on first use with room for
           ``neuron_config.max_length + 1`` positions (reallocated by a chunk
           that starts at position 0 and does not fit).
@@ -269,7 +298,8 @@ class NeuronQwen3MoeDecoderLayer:
         if past_key_value is None and int(starts.min()) == 0 \
                 and (cache is None or cache.k.shape[0] != B or cache.capacity < end):
             cap = max(end, int(self.config.neuron_config.max_length) + 1)
-            cache = KVCache(B, self.config.num_key_value_heads, cap, self.config.head_dim, dev)
+            make = KV4Cache if self.config.neuron_config.kv_cache_bits == 4 else KVCache
+            cache = make(B, self.config.num_key_value_heads, cap, self.config.head_dim, dev)
         if cache is None or cache.k.shape[0] != B:
             raise ValueError("no KV cache for this batch: start at position 0 or pass past_key_value")
         if cache.capacity < end:
@@ -334,7 +364,8 @@ class NeuronQwen3MoeModel:
         self.embed_err = torch.zeros(1, dtype=torch.int32, device=dev)
 
     def allocate_cache(self, B: int, S_max: int):
-        """A contiguous cache of ``S_max`` entries a row in every layer, or, with
+        """A contiguous cache of ``S_max`` entries a row in every layer, in bf16 or with
+        ``neuron_config.kv_cache_bits`` 4 in 4 bits, or, with
         ``neuron_config.kv_cache_budget``, a bounded one.  A shared prefix goes
         with the caches that had it."""
         c, n = self.config, self.config.neuron_config
@@ -346,8 +377,10 @@ class NeuronQwen3MoeModel:
             for l in self.layers:
                 l.cache = BoundedKVCache(self.budget, c.num_key_value_heads, c.head_dim)
             return
+        dev, rows = self.embed_tokens.device, PromptRows()
         for l in self.layers:
-            l.cache = KVCache(B, c.num_key_value_heads, S_max, c.head_dim, self.embed_tokens.device)
+            l.cache = (KV4Cache(B, c.num_key_value_heads, S_max, c.head_dim, dev, rows) if n.kv_cache_bits == 4
+                       else KVCache(B, c.num_key_value_heads, S_max, c.head_dim, dev))
 
     def hidden(self, input_ids: torch.Tensor, positions: torch.Tensor, B: int, S: int, start,
                h_buf: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None) -> torch.Tensor:
@@ -363,6 +396,10 @@ class NeuronQwen3MoeModel:
     def caches(self):
         return [l.cache for l in self.layers]
 
+    def plain_attention(self) -> bool:
+        """Whether caches are in bf16 and a query sees every position up to its own."""
+        return self.config.neuron_config.kv_cache_bits == 16 and self.config.window() == 0
+
     def set_prefix(self, input_ids: torch.Tensor, budget: int = 0, recent: int = 0, sink: int = 0) -> None:
         """Runs ``input_ids[1, P]`` and makes its keys and values (cut down to
         ``budget`` entries a kv head, if that is fewer) the prefix of every
@@ -371,6 +408,8 @@ class NeuronQwen3MoeModel:
         if self.budget is not None:
             raise ValueError("a prefix is shared by contiguous caches (kv_cache_budget is set); "
                              "pass budget here to keep part of the prefix")
+        if P and not self.plain_attention():
+            raise ValueError("a prefix is shared by caches in bf16 without an attention window")
         if P >= self.rope_full[0].shape[0]:
             raise ValueError(f"a prefix of {P} tokens leaves no position of {self.rope_full[0].shape[0]} to continue at")
         if budget:
@@ -693,16 +732,16 @@ class NeuronQwen3MoeForCausalLM:
 
     def _check_steps(self, first: int, end: int) -> None:
         """Refuses steps at positions outside ``[0, _positions())`` on caches with a
-        prefix or a budget: there the step's entry is rejected, its zero query
-        gives every entry the same weight, and a bounded row moves on to a slot
-        that holds nothing.  (A plain cache's step is a zero row.)"""
-        if not self._contiguous() and (first < 0 or end > self._positions()):
+        prefix, a budget, a window or 4 bits: there the step's entry is rejected, its
+        zero query gives every entry the same weight, and a bounded row moves on to
+        a slot that holds nothing.  (A plain cache's step is a zero row.)"""
+        if not self._plain() and (first < 0 or end > self._positions()):
             raise ValueError(f"steps at positions {first} to {end - 1}: there are {self._positions()}"
                              + (f" after a prefix of {self.model.base}" if self.model.base else ""))
 
     def _top(self, pos: torch.Tensor, n_steps: int) -> int:
         """The largest of a batch's positions, from which ``n_steps`` steps may go on."""
-        if self._contiguous():
+        if self._plain():
             return int(pos.max())
         low, top = torch.stack(torch.aminmax(pos)).tolist()
         self._check_steps(low, top + n_steps)
@@ -710,6 +749,9 @@ class NeuronQwen3MoeForCausalLM:
 
     def _contiguous(self) -> bool:
         return self.model.budget is None and not self.model.base
+
+    def _plain(self) -> bool:
+        return self._contiguous() and self.model.plain_attention()
 
     # -- forward ---------------------------------------------------------------
     def prefill(self, input_ids: torch.Tensor, lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -763,9 +805,10 @@ class NeuronQwen3MoeForCausalLM:
         if budget is not None:
             budget.make_room(self.model.caches())
             ctx = max(budget.used) + 1
-        # the bucket of the captured step: the operators on a prefix or a bounded
-        # cache cut their work by it, so eager and captured steps give the same bits
-        bucket = None if self._contiguous() else self._bucket(ctx)
+        # the bucket of the captured step: the operators on a prefix, a bounded cache, a
+        # window or 4 bits cut their work by it, so eager and captured steps give the
+        # same bits
+        bucket = None if self._plain() else self._bucket(ctx)
         h = self.model.hidden(token_ids.to(dev).view(B, 1), pos, B, 1, 0, max_ctx=bucket)
         if budget is not None:
             budget.slots.add_(1)
