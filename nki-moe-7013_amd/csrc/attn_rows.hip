@@ -226,17 +226,16 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
 // An item of a windowed attention: row tile, kv head, sequence and a run of the keys
 // that the tile's queries see, the window's behind the first ones that stay (the
 // windows of consecutive queries are one run of rows).
-template <bool stream, bool KV4>
-__device__ __forceinline__ void aw_item(const ArArgs& a, uint8_t* smem) {
+template <bool KV4>
+__global__ __launch_bounds__(256, 2) void attn_window_kernel(const ArArgs a) {
+  __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];
   const int lane = threadIdx.x & 63, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   const ArKind kd = a.own;
-  constexpr int KS = stream ? 4 * AP_KT : AP_KT, ROWS = stream ? 32 : 128;
   const int G = a.Hq / a.Hkv, rows = a.S * G, grp = a.B * a.Hkv;
   const int x = int(blockIdx.x), y = x % (grp * kd.runs), z = y % grp;
-  const int run = y / grp, b = z / a.Hkv, kvh = z % a.Hkv, r0 = (kd.rts - 1 - x / (grp * kd.runs)) * ROWS;
-  const int rw = r0 + (stream ? 0 : wave * 32);
-  const int row = rw + (lane & 31);
+  const int run = y / grp, b = z / a.Hkv, kvh = z % a.Hkv, r0 = (kd.rts - 1 - x / (grp * kd.runs)) * 128;
+  const int rw = r0 + wave * 32, row = rw + (lane & 31);
   const bool live = row < rows, wlive = rw < rows;
   const int rq = live ? row : rows - 1, sq = ar_div(rq, a.g_magic);
   const int64_t qrow = (int64_t(b) * a.S + sq) * a.Hq + kvh * G + (rq - sq * G);
@@ -246,7 +245,7 @@ __device__ __forceinline__ void aw_item(const ArArgs& a, uint8_t* smem) {
   Windowed see;
   see.sink = a.win.sink;
   see.g = win_run(a.win, win_row(a.win, b, ar_div(r0, a.g_magic)).low,
-                  win_row(a.win, b, ar_div(min(r0 + ROWS, rows) - 1, a.g_magic)).end, &n);
+                  win_row(a.win, b, ar_div(min(r0 + 128, rows) - 1, a.g_magic)).end, &n);
   const WinRow own = win_row(a.win, b, sq);
   see.low = own.low;
   see.end = own.end;
@@ -256,24 +255,16 @@ __device__ __forceinline__ void aw_item(const ArArgs& a, uint8_t* smem) {
   see.last = __builtin_amdgcn_readfirstlane(wlive ? see.g.key(w1.end - 1) : -1);
   see.from = __builtin_amdgcn_readfirstlane(w1.low <= see.sink ? 0 : see.g.key(w1.low));
   see.to = __builtin_amdgcn_readfirstlane(w0.low <= see.sink ? 0 : see.g.key(w0.low));
-  const int k0 = run * kd.run * KS, k1 = min(n, k0 + kd.run * KS);
+  const int k0 = run * kd.run * AP_KT, k1 = min(n, k0 + kd.run * AP_KT);
   if (k0 < k1) {
-    const int64_t at = (int64_t(b) * a.Hkv + kvh) * a.S_max, base = at * HD;
+    const int64_t at = (int64_t(b) * a.Hkv + kvh) * a.S_max;
     if constexpr (KV4)
       flash_segment(smem, a.kv4.k + at * KV4_ROWB, a.kv4.ks + at * 4, a.kv4.v + at * KV4_ROWB, a.kv4.vs + at * 4, k0, k1,
                     see, a.scale_log2, st);
-    else if constexpr (stream)
-      stream_segment(smem, a.k + base, a.v + base, k0, k1, see, a.scale_log2, st);
     else
-      flash_segment(smem, a.k + base, a.v + base, k0, k1, see, a.scale_log2, st);
+      flash_segment(smem, a.k + at * HD, a.v + at * HD, k0, k1, see, a.scale_log2, st);
   }
-  ar_finish<stream>(a, kd, false, smem, st, ArRow{run, kvh, b, rw, row, rows, sq, qrow, live});
-}
-
-template <bool STREAM, bool KV4>
-__global__ __launch_bounds__(256, 2) void attn_window_kernel(const ArArgs a) {
-  __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];
-  aw_item<STREAM, KV4>(a, smem);
+  ar_finish<false>(a, kd, false, smem, st, ArRow{run, kvh, b, rw, row, rows, sq, qrow, live});
 }
 
 // Joins the runs of 32 packed rows of a kv head (8 x 101 queries, 2 runs, 8 us; 64
@@ -855,70 +846,38 @@ static ArArgs aw_args(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_m
   ArArgs a = ar_args(B, S, Hq, Hkv, S_max);
   a.max_ctx = int(max_ctx);
   a.win = win_args(S, S_max, max_ctx, window, sink);
-  // keys of a row tile at most: streams and tiles of several sequences' rows do not occur
-  const int64_t G = Hq / Hkv, tile = std::min<int64_t>(S, (S * G <= 64 ? 32 : 128) / G + 2);
+  // keys of a row tile at most (its rows are one sequence's)
+  const int64_t tile = std::min<int64_t>(S, 128 / (Hq / Hkv) + 2);
   ar_plan(a, std::min<int64_t>(max_ctx, int64_t(a.win.window) + a.win.sink + tile - 1), grid);
   return a;
 }
 
-int64_t attn_kv4_tiles_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
-                                 int64_t sink) {
+int64_t attn_window_tiles_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
+                                    int64_t sink) {
   int64_t grid;
   return ar_part_bytes(aw_args(B, S, Hq, Hkv, AR_MAX_KEYS, max_ctx, window, sink, &grid));
 }
 
-int attn_kv4_tiles(const char* fn, const uint16_t* q, const Cache4& cache, const int32_t* ctx_len, int64_t B, int64_t S,
-                   int64_t Hq, int64_t Hkv, int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
-                   void* workspace, int64_t workspace_bytes, uint16_t* out, hipStream_t stream) {
+int attn_window_tiles(const char* fn, const uint16_t* q, const uint16_t* k, const uint16_t* v, const Cache4* cache,
+                      const int32_t* ctx_len, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_max,
+                      int64_t max_ctx, int64_t window, int64_t sink, float scale, void* workspace,
+                      int64_t workspace_bytes, uint16_t* out, hipStream_t stream) {
   int64_t grid;
   ArArgs a = aw_args(B, S, Hq, Hkv, S_max, max_ctx, window, sink, &grid);
   a.q = q;
-  a.kv4 = cache;
+  a.k = k;
+  a.v = v;
+  if (cache) a.kv4 = *cache;
   a.win.ctx_len = ctx_len;
   a.scale_log2 = scale * 1.4426950408889634f;
   a.out = out;
   a.part = static_cast<float*>(workspace);
-  if (int rc = win_operands(fn, grid, ar_part_bytes(a), workspace, workspace_bytes, q, out, B * S * Hq, true)) return rc;
-  hipLaunchKernelGGL((attn_window_kernel<false, true>), dim3(unsigned(grid)), dim3(256), 0, stream, a);
+  if (int rc = win_operands(fn, grid, ar_part_bytes(a), workspace, workspace_bytes, q, out, B * S * Hq)) return rc;
+  if (cache)
+    hipLaunchKernelGGL(attn_window_kernel<true>, dim3(unsigned(grid)), dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL(attn_window_kernel<false>, dim3(unsigned(grid)), dim3(256), 0, stream, a);
   if (int rc = hip_status(fn)) return rc;
   return ar_merge(fn, a, stream);
 }
 }  // namespace qmoe
-
-extern "C" int64_t qmoe_attn_window_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D, int64_t window,
-                                              int64_t sink, int64_t max_ctx) {
-  if (window <= 0 || win_check("qmoe_attn_window_workspace", B, S, Hq, Hkv, D, AR_MAX_KEYS, max_ctx, window, sink, 1.0f))
-    return -1;
-  if (B == 0 || S == 0) return 0;
-  int64_t grid;
-  return ar_part_bytes(aw_args(B, S, Hq, Hkv, AR_MAX_KEYS, max_ctx, window, sink, &grid));
-}
-
-extern "C" int qmoe_attn_window(const qmoe_bf16* q, const qmoe_bf16* k_cache, const qmoe_bf16* v_cache,
-                                const int32_t* ctx_len, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
-                                int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
-                                void* workspace, int64_t workspace_bytes, qmoe_bf16* out, qmoe_stream_t stream) {
-  const char* fn = "qmoe_attn_window";
-  QMOE_REQUIRE(B == 0 || S == 0 || (q && k_cache && v_cache && ctx_len && out), "%s: null pointer", fn);
-  if (int rc = win_check(fn, B, S, Hq, Hkv, D, S_max, max_ctx, window, sink, scale)) return rc;
-  QMOE_REQUIRE(window > 0, "%s: window must be positive", fn);
-  if (B == 0 || S == 0) return QMOE_OK;
-  int64_t grid;
-  ArArgs a = aw_args(B, S, Hq, Hkv, S_max, max_ctx, window, sink, &grid);
-  a.q = q;
-  a.k = k_cache;
-  a.v = v_cache;
-  a.win.ctx_len = ctx_len;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  a.out = out;
-  a.part = static_cast<float*>(workspace);
-  if (int rc = win_operands(fn, grid, ar_part_bytes(a), workspace, workspace_bytes, q, out, B * S * Hq,
-                            aligned16(k_cache, v_cache)))
-    return rc;
-  if (a.own.stream)
-    hipLaunchKernelGGL((attn_window_kernel<true, false>), dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
-  else
-    hipLaunchKernelGGL((attn_window_kernel<false, false>), dim3(unsigned(grid)), dim3(256), 0, as_stream(stream), a);
-  if (int rc = hip_status(fn)) return rc;
-  return ar_merge(fn, a, as_stream(stream));
-}

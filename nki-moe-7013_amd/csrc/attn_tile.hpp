@@ -330,34 +330,28 @@ __device__ __forceinline__ void flash_segment(uint8_t* smem, const uint16_t* k, 
 // into A-operand registers and V by DMA into the wave's own LDS tile, every load
 // of a tile in flight at once and no barrier between the waves; flash_join adds
 // up their states.  Weights in bf16 for the MFMA with V and l in 32 bits, as in
-// flash_tiles.  k0, k1: the run's keys [k0, k1), which start at 0 without a gap.
-template <bool GAP, class See>
-__device__ __forceinline__ void stream_keys(uint8_t* smem, const uint16_t* k, const uint16_t* v, int k_first, int n_keys,
-                                            const See& see, Gap g, float scale_log2, FlashRows& st) {
+// flash_tiles.
+__device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
+                                               const Causal& seen, float scale_log2, FlashRows& st) {
   const int lane = threadIdx.x & 63, col = lane & 31, hl = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
   uint8_t* vb = smem + wave * AP_TILE;
   const int vg = lane >> 4, ve = (lane >> 2) & 3, vq = lane & 3;
   const uint32_t vlane = uint32_t((4 * (vg >> 1) + ve) * AP_ROWB +
                                   (((2 * (vg & 1) + (vq >> 1)) ^ (2 * (ve >> 1))) * 16) + 8 * (vq & 1));
-  const int rows = GAP ? g.row(n_keys - 1) + 1 : n_keys;
-  const pipe::i32x4 rv = pipe::make_rsrc(v, uint32_t(rows) * AP_ROWB);  // rows past the end read as zeros
+  const pipe::i32x4 rv = pipe::make_rsrc(v, uint32_t(n_keys) * AP_ROWB);  // rows past the end read as zeros
   const uint32_t lds = uint32_t(reinterpret_cast<uintptr_t>(smem)) + uint32_t(wave * AP_TILE);
   const uint32_t voff = uint32_t((lane >> 4) * AP_ROWB + ap_vslot(lane >> 4, lane & 15) * 16);
 #pragma unroll 1
-  for (int k0 = (GAP ? k_first : 0) + wave * AP_KT; k0 < n_keys; k0 += 4 * AP_KT) {
+  for (int k0 = wave * AP_KT; k0 < n_keys; k0 += 4 * AP_KT) {
     const int last = min(AP_KT, n_keys - k0) - 1;  // rows past it repeat it (their p is 0)
     u32x4 ka[2][HD / 16];
     wave_lds_sync();  // the last tile's V reads are done
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const uint32_t skip = GAP && k0 + 4 * i + (lane >> 4) >= g.at ? uint32_t(g.gap) * AP_ROWB : 0u;
-      pipe::dma16(lds + i * 1024, voff + uint32_t(k0 + 4 * i) * AP_ROWB + skip, rv, 0);
-    }
+    for (int i = 0; i < 16; ++i) pipe::dma16(lds + i * 1024, voff + uint32_t(k0 + 4 * i) * AP_ROWB, rv, 0);
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb) {
-      const int key = k0 + min(mb * 32 + col, last);
-      const uint16_t* kp = k + int64_t(GAP ? g.row(key) : key) * HD + hl * 8;
+      const uint16_t* kp = k + int64_t(k0 + min(mb * 32 + col, last)) * HD + hl * 8;
 #pragma unroll
       for (int ks = 0; ks < HD / 16; ++ks) ka[mb][ks] = ld16(kp + ks * 16);
     }
@@ -370,13 +364,14 @@ __device__ __forceinline__ void stream_keys(uint8_t* smem, const uint16_t* k, co
         sc[mb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, ka[mb][ks]), st.qf[ks], sc[mb], 0,
                                                          0, 0);
     }
+    const int see = min(seen.lim - k0, last);
     float m = -INFINITY;
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
         const int key = mb * 32 + (e >> 2) * 8 + hl * 4 + (e & 3);
-        sc[mb][e] = key <= last && see.sees(k0 + key) ? sc[mb][e] * scale_log2 : -INFINITY;
+        sc[mb][e] = key <= see ? sc[mb][e] * scale_log2 : -INFINITY;
         m = fmaxf(m, sc[mb][e]);
       }
     {
@@ -421,15 +416,6 @@ __device__ __forceinline__ void stream_keys(uint8_t* smem, const uint16_t* k, co
       }
     }
   }
-}
-
-__device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int n_keys,
-                                               const Causal& see, float scale_log2, FlashRows& st) {
-  stream_keys<false>(smem, k, v, 0, n_keys, see, Gap{0, 0}, scale_log2, st);
-}
-__device__ __forceinline__ void stream_segment(uint8_t* smem, const uint16_t* k, const uint16_t* v, int k0, int k1,
-                                               const Windowed& see, float scale_log2, FlashRows& st) {
-  stream_keys<true>(smem, k, v, k0, k1, see, see.g, scale_log2, st);
 }
 
 // The four waves' states of the same rows into wave 0's, through LDS in register

@@ -46,12 +46,14 @@ struct Cache4 {
 };
 
 // ---------------------------------------------------------------------- host
-// qmoe_attn_kv4's many rows (S * Hq / Hkv > 64), on the tiles of attn_rows.hip.
-int64_t attn_kv4_tiles_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
-                                 int64_t sink);
-int attn_kv4_tiles(const char* fn, const uint16_t* q, const Cache4& cache, const int32_t* ctx_len, int64_t B, int64_t S,
-                   int64_t Hq, int64_t Hkv, int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink, float scale,
-                   void* workspace, int64_t workspace_bytes, uint16_t* out, hipStream_t stream);
+// The calls of many rows (S * Hq / Hkv > 64), on the tiles of attn_rows.hip; cache: in
+// 4 bits, instead of k and v.
+int64_t attn_window_tiles_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
+                                    int64_t sink);
+int attn_window_tiles(const char* fn, const uint16_t* q, const uint16_t* k, const uint16_t* v, const Cache4* cache,
+                      const int32_t* ctx_len, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_max,
+                      int64_t max_ctx, int64_t window, int64_t sink, float scale, void* workspace,
+                      int64_t workspace_bytes, uint16_t* out, hipStream_t stream);
 
 inline WinArgs win_args(int64_t S, int64_t S_max, int64_t max_ctx, int64_t window, int64_t sink) {
   WinArgs w{};
@@ -79,11 +81,11 @@ inline int win_check(const char* fn, int64_t B, int64_t S, int64_t Hq, int64_t H
 }
 
 // The rest of the checks, of B * S > 0 queries: the grid, `need` bytes of workspace,
-// alignments (`caches`: whether those are 16-byte aligned) and an output that is not q.
+// alignments and an output that is not q.
 inline int win_operands(const char* fn, int64_t grid, int64_t need, const void* workspace, int64_t workspace_bytes,
-                        const qmoe_bf16* q, const qmoe_bf16* out, int64_t heads, bool caches) {
+                        const qmoe_bf16* q, const qmoe_bf16* out, int64_t heads) {
   QMOE_REQUIRE(grid < (1ll << 31), "%s: grid too large", fn);
-  QMOE_REQUIRE(caches && aligned16(q, static_cast<const uint8_t*>(workspace), out),
+  QMOE_REQUIRE(aligned16(q, static_cast<const uint8_t*>(workspace), out),
                "%s: operands must be 16-byte aligned", fn);
   const uintptr_t x = reinterpret_cast<uintptr_t>(q), y = reinterpret_cast<uintptr_t>(out);
   QMOE_REQUIRE((x < y ? y - x : x - y) >= uintptr_t(heads * AP_ROWB), "%s: out overlaps q", fn);

@@ -293,6 +293,33 @@ def test_attn_kv4(dev, case, windowed):
     assert not bool(got[blind].any())
 
 
+@pytest.mark.parametrize("B,S,S_max,Hq,Hkv,window,ctx", [
+    # every workgroup takes an even share of all keys (long batches)
+    (33, 1, 18000, 8, 8, 0, [18000 - 541 * i for i in range(33)]),
+    (64, 1, 9000, 32, 8, 0, [9000 - 300 * (i % 31) for i in range(64)]),
+    (16, 1, 32768, 64, 4, 0, [0, 32768, 1, 5, 0, 20000, 32767, 31000] * 2),
+    (17, 5, 17000, 32, 4, 0, [17000 - 1000 * i for i in range(17)]),        # three row tiles an item
+    (300, 1, 9000, 2, 1, 8500, [30 * i for i in range(300)]),               # more sequences than threads
+    (12, 3, 34000, 16, 4, 33000, [34000, 1, -1, 33990] * 3),
+], ids=lambda x: str(x) if isinstance(x, int) else "")
+def test_attn_kv4_of_long_batches(dev, B, S, S_max, Hq, Hkv, window, ctx):
+    announce(f"attn_kv4 long {B} {S} {S_max} {Hq} {Hkv} {window}")
+    g = _gen(dev, B)
+    q = bf16_randn((B * S, Hq, D), g, dev, 2.0)
+    cache = ops.kv4_cache(B, Hkv, S_max, D, dev)
+    for b in range(B):
+        rows = [bf16_randn((1, Hkv, S_max, D), g, dev) for _ in range(2)]
+        ops.kv4_store(*rows, tuple(t[b:b + 1] for t in cache))
+    got = ops.attn_kv4(q, cache, _i32(ctx, dev), B, S, window, 4 if window else 0)
+    again = ops.attn_kv4(q, cache, _i32(ctx, dev), B, S, window, 4 if window else 0)
+    torch.cuda.synchronize()
+    assert torch.equal(got, again) and not bool(torch.isnan(got).any())
+    for b in sorted({0, 1, 2, B // 2, B - 2, B - 1}):
+        one = slice(b * S, (b + 1) * S)
+        k, v = (ref.values(c[b:b + 1], p[b:b + 1]) for c, p in (cache[:2], cache[2:]))
+        _within(got[one], *ref.window(q[one], k, v, [ctx[b]], 1, S, window, 4 if window else 0, S_max, SCALE), f"row {b}")
+
+
 @pytest.mark.parametrize("scale", [1.0, 1e-3, 0.5])
 def test_scales(dev, scale):
     g = _gen(dev, 3)
