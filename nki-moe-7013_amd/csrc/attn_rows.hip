@@ -243,18 +243,18 @@ __global__ __launch_bounds__(256, 2) void attn_window_kernel(const ArArgs a) {
   st.start(live ? a.q + qrow * HD : nullptr, hl);
   int n;
   Windowed see;
-  see.sink = a.win.sink;
   see.g = win_run(a.win, win_row(a.win, b, ar_div(r0, a.g_magic)).low,
                   win_row(a.win, b, ar_div(min(r0 + 128, rows) - 1, a.g_magic)).end, &n);
   const WinRow own = win_row(a.win, b, sq);
-  see.low = own.low;
-  see.end = own.end;
+  see.stay = see.g.at;
+  see.low = own.low <= a.win.sink ? 0 : see.g.key(own.low);
+  see.lim = see.g.key(own.end - 1);
   const WinRow w0 = win_row(a.win, b, ar_div(wlive ? rw : r0, a.g_magic));
   const WinRow w1 = win_row(a.win, b, ar_div(wlive ? min(rw + 31, rows - 1) : r0, a.g_magic));
   see.first = __builtin_amdgcn_readfirstlane(wlive ? see.g.key(w0.end - 1) : -1);
   see.last = __builtin_amdgcn_readfirstlane(wlive ? see.g.key(w1.end - 1) : -1);
-  see.from = __builtin_amdgcn_readfirstlane(w1.low <= see.sink ? 0 : see.g.key(w1.low));
-  see.to = __builtin_amdgcn_readfirstlane(w0.low <= see.sink ? 0 : see.g.key(w0.low));
+  see.from = __builtin_amdgcn_readfirstlane(w1.low <= a.win.sink ? 0 : see.g.key(w1.low));
+  see.to = __builtin_amdgcn_readfirstlane(w0.low <= a.win.sink ? 0 : see.g.key(w0.low));
   const int k0 = run * kd.run * AP_KT, k1 = min(n, k0 + kd.run * AP_KT);
   if (k0 < k1) {
     const int64_t at = (int64_t(b) * a.Hkv + kvh) * a.S_max;

@@ -79,7 +79,8 @@ constexpr int FL_SMEM = 4 * AP_TILE;  // K0, K1, V0, V1
 // last < 0: the wave has no row, it only helps to load).
 struct Causal {
   int lim, first, last;
-  __device__ __forceinline__ bool sees(int key) const { return key <= lim; }
+  // Logits of the keys k0 + i, or -inf
+  __device__ __forceinline__ float mask(float x, int k0, int i) const { return k0 + i > lim ? -INFINITY : x; }
   __device__ __forceinline__ bool all_see(int k0, int k1) const { return k1 <= first; }
   __device__ __forceinline__ bool none_sees(int k0, int k1) const { return k0 > last; }
 };
@@ -92,17 +93,17 @@ struct Gap {
   __device__ __forceinline__ int key(int row) const { return row < at ? row : max(row - gap, at - 1); }
 };
 
-// Lane's query sees the rows [low, end) and [0, sink) below end; keys [from, ...) lie
-// in the window of every row of the wave, keys [at, to) of none.
+// Lane's query sees the keys [low, lim] and [0, stay) up to lim; keys [from, ...) lie in
+// the window of every row of the wave, keys [stay, to) in that of none.
 struct Windowed {
   Gap g;
-  int low, end, sink, first, last, from, to;
-  __device__ __forceinline__ bool sees(int key) const {
-    const int r = g.row(key);
-    return r < end && (r >= low || r < sink);
+  int low, lim, stay, first, last, from, to;
+  __device__ __forceinline__ float mask(float x, int k0, int i) const {
+    const bool hidden = (k0 + i > lim) | ((k0 + i < low) & (k0 + i >= stay));  // no branches
+    return hidden ? -INFINITY : x;
   }
   __device__ __forceinline__ bool all_see(int k0, int k1) const { return k1 <= first && k0 >= from; }
-  __device__ __forceinline__ bool none_sees(int k0, int k1) const { return k0 > last || (k0 >= g.at && k1 < to); }
+  __device__ __forceinline__ bool none_sees(int k0, int k1) const { return k0 > last || (k0 >= stay && k1 < to); }
 };
 
 // Tiles of keys [k0, k0 + n_keys) of a cache in bf16, global -> LDS by DMA (every wave
@@ -200,10 +201,8 @@ __device__ __forceinline__ void flash_tiles(uint8_t* smem, Tiles& tiles, int n_k
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = kv0 + kb * 32 + (i >> 2) * 8 + hl * 4 + (i & 3);
-          if (!see.sees(key)) sc[kb][i] = -INFINITY;
-        }
+        for (int i = 0; i < 16; ++i)
+          sc[kb][i] = see.mask(sc[kb][i], kv0 + hl * 4, kb * 32 + (i >> 2) * 8 + (i & 3));
     }
     float mx[11];  // maximum as a tree of 3-input maxima
 #pragma unroll
