@@ -495,7 +495,7 @@ py::object attn_kv4(py::handle q, py::handle cache, py::handle ctx_len, py::hand
 }
 
 void kv4_store(py::handle k, py::handle v, py::handle cache, py::handle starts, py::handle lengths, py::handle tokens) {
-  const Cache4 c(cache, 16, any_alignment);
+  const Cache4 c(cache, 16, 4);
   int64_t Hkv, S;
   const at::Tensor& src = tensor(k, "k");
   if (src.dim() != 4 || src.size(0) != c.B || src.size(1) != c.Hkv || src.size(3) != c.D)

@@ -7,64 +7,94 @@
 
 namespace qmoe {
 
-// One thread a block of 32 elements: 64 bytes in, 16 bytes and a power out.
-__global__ __launch_bounds__(256) void kv4_store_kernel(
-    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int64_t blocks, int n, int S_src,
-    const int32_t* __restrict__ starts, const int32_t* __restrict__ lengths, int Hkv, int S_max,
-    uint8_t* __restrict__ k4, uint8_t* __restrict__ ks, uint8_t* __restrict__ v4, uint8_t* __restrict__ vs) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= blocks) return;
-  const int blk = int(i & 3);
-  const int64_t r = i >> 2;  // (b, kv head, token)
-  const int s = int(r % n);
-  const int64_t bh = r / n;
-  const int b = int(bh / Hkv);
-  const int64_t to = int64_t(starts ? starts[b] : 0) + s;
-  if (s >= (lengths ? lengths[b] : n) || to < 0 || to >= S_max) return;
-  const uint16_t* src = (blockIdx.y ? v : k) + (bh * S_src + s) * HD + blk * KV4_BLOCK;
-  float x[KV4_BLOCK];
-  int wants = 0;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const u32x4 w = ld16(src + c * 8);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[c * 8 + 2 * e] = bf16_lo(w[e]);
-      x[c * 8 + 2 * e + 1] = bf16_hi(w[e]);
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < KV4_BLOCK; ++e) wants = max(wants, kv4_wants(x[e]));
-  const int power = kv4_power(wants);
-  u32x4 out;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    uint32_t w = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w |= kv4_code(x[c * 8 + e], power) << (4 * e);
-    out[c] = w;
-  }
-  const int64_t at = bh * S_max + to;
-  *reinterpret_cast<u32x4*>((blockIdx.y ? v4 : k4) + at * KV4_ROWB + blk * 16) = out;
-  (blockIdx.y ? vs : ks)[at * 4 + blk] = uint8_t(power);
+// Rows go through in chunks of KS_ROWS of a (sequence, kv head), 16 lanes a row: lane
+// p % 16 has 8 elements, 16 bytes in bf16 and 4 in codes, so that a wave's loads and
+// stores are whole lines; all of a thread's loads are in flight at once.
+constexpr int KS_UNROLL = 4, KS_ROWS = 16 * KS_UNROLL;
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+  return uint32_t(__builtin_amdgcn_update_dpp(0, int(v), CTRL, 0xf, 0xf, true));
+}
+constexpr int DPP_XOR1 = 0xb1, DPP_XOR2 = 0x4e;         // quad_perm [1,0,3,2], [2,3,0,1]
+constexpr int DPP_ROR4 = 0x124, DPP_ROR8 = 0x128;       // row_ror
+
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+// Two bf16 values as numbers of the power's multiples (nearest, ties to even, what is
+// past 6 to 6), to byte B of w.
+template <int B>
+__device__ __forceinline__ uint32_t kv4_pack(uint32_t w, uint32_t x, float scale) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(w, __builtin_bit_cast(bf16x2_t, x), scale, B);
 }
 
-// One thread a block of 32 elements: 16 bytes and a power in, 64 bytes out.
+__global__ __launch_bounds__(256) void kv4_store_kernel(
+    const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int chunks, int n, int S_src,
+    const int32_t* __restrict__ starts, const int32_t* __restrict__ lengths, int Hkv, int S_max,
+    uint8_t* __restrict__ k4, uint8_t* __restrict__ ks, uint8_t* __restrict__ v4, uint8_t* __restrict__ vs) {
+  const int bh = int(blockIdx.x) / chunks, b = bh / Hkv, p = threadIdx.x & 15;
+  const int s0 = int(blockIdx.x) % chunks * KS_ROWS + int(threadIdx.x) / 16;
+  const int len = lengths ? min(lengths[b], n) : n;
+  const int64_t start = starts ? starts[b] : 0;
+  const uint16_t* src = (blockIdx.y ? v : k) + int64_t(bh) * S_src * HD + p * 8;
+  u32x4 x[KS_UNROLL];
+#pragma unroll
+  for (int u = 0; u < KS_UNROLL; ++u) {
+    const int s = s0 + 16 * u;
+    x[u] = s < len ? ld16(src + int64_t(s) * HD) : u32x4{0u, 0u, 0u, 0u};
+  }
+  uint8_t* codes = (blockIdx.y ? v4 : k4) + int64_t(bh) * S_max * KV4_ROWB + p * 4;
+  uint32_t* powers = reinterpret_cast<uint32_t*>((blockIdx.y ? vs : ks) + int64_t(bh) * S_max * 4);
+#pragma unroll
+  for (int u = 0; u < KS_UNROLL; ++u) {
+    // the block's largest magnitude, over its four lanes: bf16's bits without the sign
+    // are in the order of the magnitudes
+    uint32_t top = pk_max(pk_max(x[u].x & 0x7fff7fffu, x[u].y & 0x7fff7fffu),
+                          pk_max(x[u].z & 0x7fff7fffu, x[u].w & 0x7fff7fffu));
+    top = pk_max(top, dpp_u32<DPP_XOR1>(top));
+    top = pk_max(top, dpp_u32<DPP_XOR2>(top));
+    const int power = kv4_power(kv4_wants(__uint_as_float(max(top << 16, top & 0xffff0000u))));
+    const float scale = kv4_scale(uint32_t(power));
+    uint32_t c = kv4_pack<0>(0u, x[u].x, scale);
+    c = kv4_pack<1>(c, x[u].y, scale);
+    c = kv4_pack<2>(c, x[u].z, scale);
+    c = kv4_pack<3>(c, x[u].w, scale);
+    uint32_t all = uint32_t(power) << (8 * (p >> 2));  // the row's four powers
+    all |= dpp_u32<DPP_ROR4>(all);
+    all |= dpp_u32<DPP_ROR8>(all);
+    const int s = s0 + 16 * u;
+    const int64_t to = start + s;
+    if (s < len && to >= 0 && to < S_max) {
+      *reinterpret_cast<uint32_t*>(codes + to * KV4_ROWB) = power == KV4_NAN ? 0u : c;
+      if (p == 0) powers[to] = all;
+    }
+  }
+}
+
 __global__ __launch_bounds__(256) void kv4_load_kernel(
     const uint8_t* __restrict__ k4, const uint8_t* __restrict__ ks, const uint8_t* __restrict__ v4,
-    const uint8_t* __restrict__ vs, int64_t blocks, int n, int S_max, uint16_t* __restrict__ k,
-    uint16_t* __restrict__ v) {
-  const int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= blocks) return;
-  const int blk = int(i & 3);
-  const int64_t r = i >> 2, at = r / n * S_max + r % n;
-  const u32x4 w = ld16((blockIdx.y ? v4 : k4) + at * KV4_ROWB + blk * 16);
-  const float scale = kv4_scale((blockIdx.y ? vs : ks)[at * 4 + blk]);
-  uint16_t* dst = (blockIdx.y ? v : k) + r * HD + blk * KV4_BLOCK;
+    const uint8_t* __restrict__ vs, int chunks, int n, int S_max, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
+  const int bh = int(blockIdx.x) / chunks, p = threadIdx.x & 15;
+  const int s0 = int(blockIdx.x) % chunks * KS_ROWS + int(threadIdx.x) / 16;
+  const uint8_t* codes = (blockIdx.y ? v4 : k4) + int64_t(bh) * S_max * KV4_ROWB + p * 4;
+  const uint8_t* powers = (blockIdx.y ? vs : ks) + int64_t(bh) * S_max * 4 + (p >> 2);
+  uint16_t* dst = (blockIdx.y ? v : k) + int64_t(bh) * n * HD + p * 8;
+  uint32_t w[KS_UNROLL], power[KS_UNROLL];
 #pragma unroll
-  for (int c = 0; c < 4; ++c)
-    *reinterpret_cast<u32x4*>(dst + c * 8) = u32x4{kv4_pair<0>(w[c], scale), kv4_pair<1>(w[c], scale),
-                                                   kv4_pair<2>(w[c], scale), kv4_pair<3>(w[c], scale)};
+  for (int u = 0; u < KS_UNROLL; ++u) {
+    const int s = min(s0 + 16 * u, n - 1);
+    w[u] = *reinterpret_cast<const uint32_t*>(codes + int64_t(s) * KV4_ROWB);
+    power[u] = powers[int64_t(s) * 4];
+  }
+#pragma unroll
+  for (int u = 0; u < KS_UNROLL; ++u) {
+    const float scale = kv4_scale(power[u]);
+    if (s0 + 16 * u < n)
+      *reinterpret_cast<u32x4*>(dst + int64_t(s0 + 16 * u) * HD) = u32x4{
+          kv4_pair<0>(w[u], scale), kv4_pair<1>(w[u], scale), kv4_pair<2>(w[u], scale), kv4_pair<3>(w[u], scale)};
+  }
 }
 
 __device__ __forceinline__ double wave_sum64(double v) {
@@ -154,9 +184,12 @@ extern "C" int qmoe_kv4_store(const qmoe_bf16* k, const qmoe_bf16* v, int64_t S_
   QMOE_REQUIRE(S_src >= n && S_src < (1ll << 30), "%s: need n <= S_src", fn);
   if (B == 0 || n == 0) return QMOE_OK;
   QMOE_REQUIRE(aligned16(k, v, k_cache, v_cache), "%s: operands must be 16-byte aligned", fn);
-  const int64_t blocks = B * Hkv * n * 4;
-  hipLaunchKernelGGL(kv4_store_kernel, dim3(unsigned((blocks + 255) / 256), 2), dim3(256), 0, as_stream(stream), k, v,
-                     blocks, int(n), int(S_src), starts, lengths, int(Hkv), int(S_max), k_cache, k_scales, v_cache,
+  QMOE_REQUIRE((reinterpret_cast<uintptr_t>(k_scales) | reinterpret_cast<uintptr_t>(v_scales)) % 4 == 0,
+               "%s: scales must be 4-byte aligned", fn);
+  const int64_t chunks = (n + KS_ROWS - 1) / KS_ROWS;
+  QMOE_REQUIRE(B * Hkv * chunks < (1ll << 31), "%s: grid too large", fn);
+  hipLaunchKernelGGL(kv4_store_kernel, dim3(unsigned(B * Hkv * chunks), 2), dim3(256), 0, as_stream(stream), k, v,
+                     int(chunks), int(n), int(S_src), starts, lengths, int(Hkv), int(S_max), k_cache, k_scales, v_cache,
                      v_scales);
   return hip_status(fn);
 }
@@ -170,9 +203,10 @@ extern "C" int qmoe_kv4_load(const uint8_t* k_cache, const uint8_t* k_scales, co
   QMOE_REQUIRE(n <= S_max, "%s: need n <= S_max", fn);
   if (B == 0 || n == 0) return QMOE_OK;
   QMOE_REQUIRE(aligned16(k, v, k_cache, v_cache), "%s: operands must be 16-byte aligned", fn);
-  const int64_t blocks = B * Hkv * n * 4;
-  hipLaunchKernelGGL(kv4_load_kernel, dim3(unsigned((blocks + 255) / 256), 2), dim3(256), 0, as_stream(stream),
-                     k_cache, k_scales, v_cache, v_scales, blocks, int(n), int(S_max), k, v);
+  const int64_t chunks = (n + KS_ROWS - 1) / KS_ROWS;
+  QMOE_REQUIRE(B * Hkv * chunks < (1ll << 31), "%s: grid too large", fn);
+  hipLaunchKernelGGL(kv4_load_kernel, dim3(unsigned(B * Hkv * chunks), 2), dim3(256), 0, as_stream(stream), k_cache,
+                     k_scales, v_cache, v_scales, int(chunks), int(n), int(S_max), k, v);
   return hip_status(fn);
 }
 

@@ -23,7 +23,7 @@ def kv4(l, q=A, k=2 * A, ks=7 * A, v=3 * A, vs=8 * A, ctx=4, B=2, S=1, Hq=32, Hk
 
 
 def store(l, k=A, v=2 * A, S_src=16, n=16, starts=NONE, lengths=NONE, B=2, Hkv=4, D=128, S_max=64, k4=3 * A, ks=4,
-          v4=5 * A, vs=6):
+          v4=5 * A, vs=8):
     return l.qmoe_kv4_store(k, v, S_src, n, starts, lengths, B, Hkv, D, S_max, k4, ks, v4, vs, NONE)
 
 
@@ -58,7 +58,7 @@ REFUSED += [
     (store, dict(D=64), "head_dim"), (store, dict(B=-1), "bad B"), (store, dict(Hkv=0), "bad B"),
     (store, dict(S_max=0), "bad B"), (store, dict(n=-1), "entries"), (store, dict(n=17), "n <= S_src"),
     (store, dict(k=A + 8), "aligned"), (store, dict(v=2 * A + 2), "aligned"), (store, dict(k4=3 * A + 4), "aligned"),
-    (store, dict(v4=5 * A + 1), "aligned"), (store, dict(B=60000, Hkv=60000, n=1 << 20, S_src=1 << 20), "entries"),
+    (store, dict(v4=5 * A + 1), "aligned"), (store, dict(ks=6), "4-byte"), (store, dict(vs=9), "4-byte"), (store, dict(B=60000, Hkv=60000, n=1 << 20, S_src=1 << 20), "entries"),
     (load, dict(k=NONE), "null pointer"), (load, dict(vs=NONE), "null pointer"), (load, dict(D=256), "head_dim"),
     (load, dict(n=65), "n <= S_max"), (load, dict(n=-1), "entries"), (load, dict(k=5 * A + 2), "aligned"),
     (load, dict(k4=A + 4), "aligned"),
