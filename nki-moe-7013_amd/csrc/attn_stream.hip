@@ -26,12 +26,12 @@ struct AsArgs {
   const uint16_t *q, *k, *v;
   Cache4 c;  // instead of k and v
   WinArgs win;
-  int B, Hq, Hkv, rts;  // rts: row tiles of a (sequence, kv head)
+  int B, Hq, Hkv, G, rts;  // G: Hq / Hkv; rts: row tiles of a (sequence, kv head)
   int waves, runs, run;  // waves of a workgroup; runs of `run` keys that an item is cut into
   int wgs;               // or workgroups that share all items' keys evenly (0: runs)
   uint32_t g_magic;
   float scale_log2;
-  float* part;  // [runs][B * Hkv * rts][AS_REC], when runs > 1, or [wgs][2][AS_REC]
+  float* part;  // [runs][rts][B][Hkv][AS_REC], when runs > 1, or [wgs][2][AS_REC]
   uint16_t* out;
 };
 
@@ -64,7 +64,7 @@ __device__ __forceinline__ AsRun as_run(const AsArgs& a, int b, int r0, int r1) 
 // places in the cache beside bf16's tiles are more than the registers hold).
 constexpr int AS_STEP = AS_CUT * AS_TILE;
 __device__ __forceinline__ int as_steps(const AsArgs& a, int b, int rt) {
-  const int r0 = rt * AS_ROWS, rows = a.win.S * (a.Hq / a.Hkv);
+  const int r0 = rt * AS_ROWS, rows = a.win.S * a.G;
   const int n = as_run<true>(a, b, r0, min(r0 + AS_ROWS, rows) - 1).n;
   return max((n + AS_STEP - 1) / AS_STEP, 1);
 }
@@ -228,11 +228,21 @@ __device__ __forceinline__ void as_piece(const AsArgs& a, const AsRun& kr, int b
                                          float* part, uint8_t (*smem)[AS_TILE * AP_ROWB], float2 (*sml)[AS_ROWS]) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(int(threadIdx.x) >> 6);
-  const int G = a.Hq / a.Hkv, r0 = rt * AS_ROWS, r1 = min(r0 + AS_ROWS, a.win.S * G) - 1;
+  const int r0 = rt * AS_ROWS, r1 = min(r0 + AS_ROWS, a.win.S * a.G) - 1;
   const Gap gap = kr.gap;
   const int row = min(r0 + r, r1), sq = ar_div(row, a.g_magic);
   const bool live = r0 + r <= r1;
-  const int64_t qrow = (int64_t(b) * a.win.S + sq) * a.Hq + kvh * G + (row - sq * G);
+  const int64_t qrow = (int64_t(b) * a.win.S + sq) * a.Hq + kvh * a.G + (row - sq * a.G);
+  using Tile = std::conditional_t<FOUR, AsTile4, AsTile16>;
+  // Q^T as B operands, in the order of the K operands' dims (ahead of the cache's loads,
+  // behind which the first product would wait for it)
+  bf16x8 qf[4];
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    const u32x4 w = live ? ld16(a.q + qrow * HD + Tile::dim(g, ks)) : u32x4{0u, 0u, 0u, 0u};
+    qf[ks] = __builtin_bit_cast(bf16x8, w);
+  }
+  __builtin_amdgcn_sched_barrier(0);
   // this lane's row sees the keys [0, stay) and [all, ...) up to row own.end
   const WinRow own = win_row(a.win, b, sq);
   const int all = own.low <= a.win.sink ? 0 : gap.key(own.low);
@@ -240,7 +250,6 @@ __device__ __forceinline__ void as_piece(const AsArgs& a, const AsRun& kr, int b
   const int from = kr.last.low <= a.win.sink ? 0 : gap.key(kr.last.low);
   const int upto = min(gap.key(kr.first.end - 1) + 1, k1);
 
-  using Tile = std::conditional_t<FOUR, AsTile4, AsTile16>;
   Tile tile;
   const int w0 = k0 + wave * AS_TILE;
   if (k0 < k1)
@@ -248,13 +257,6 @@ __device__ __forceinline__ void as_piece(const AsArgs& a, const AsRun& kr, int b
   if (w0 < k1) {
     tile.load_k(w0, r, g);
     tile.load_v(w0, r, g);
-  }
-  // Q^T as B operands, in the order of the K operands' dims
-  bf16x8 qf[4];
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) {
-    const u32x4 w = live ? ld16(a.q + qrow * HD + Tile::dim(g, ks)) : u32x4{0u, 0u, 0u, 0u};
-    qf[ks] = __builtin_bit_cast(bf16x8, w);
   }
   f32x4 o[8];  // O^T: dims 16 dt + 4 g + [0, 4) of row r
 #pragma unroll
@@ -380,20 +382,21 @@ __device__ __forceinline__ void as_piece(const AsArgs& a, const AsRun& kr, int b
   if (part && wave == 0 && g == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(M, L);
 }
 
-// Workgroup = (run, item).
+// Workgroup = (kv head, sequence, run of a row tile): heads and sequences are fastest, so
+// the row tiles that share a head's keys are on one XCD when there are a multiple of 8
+// of those.
 template <bool FOUR, int WAVES>
 __global__ __launch_bounds__(WAVES * 64, 8 / WAVES) void attn_stream_kernel(const AsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES][AS_TILE * AP_ROWB];
   __shared__ float2 sml[WAVES][AS_ROWS];
-  // (sequence, kv head) fastest, so the row tiles that share its keys are on one XCD
-  // when their number is a multiple of 8
-  const int grp = a.B * a.Hkv, x = int(blockIdx.x), z = x % grp, y = x / grp, rt = y % a.rts, run = y / a.rts;
-  const int b = z / a.Hkv, r0 = rt * AS_ROWS, r1 = min(r0 + AS_ROWS, a.win.S * (a.Hq / a.Hkv)) - 1;
+  const int kvh = blockIdx.x, b = blockIdx.y, z = blockIdx.z;
+  const int run = a.rts == 1 ? z : z / a.rts, rt = z - run * a.rts;
+  const int r0 = rt * AS_ROWS, r1 = min(r0 + AS_ROWS, a.win.S * a.G) - 1;
   const AsRun kr = as_run<FOUR>(a, b, r0, r1);
   const int k0 = run * a.run;
   if (run > 0 && k0 >= kr.n) return;  // the merge knows how many runs there are
-  float* part = a.runs > 1 ? a.part + (int64_t(run) * grp * a.rts + z * a.rts + rt) * AS_REC : nullptr;
-  as_piece<FOUR, WAVES>(a, kr, b, z % a.Hkv, rt, k0, min(kr.n, k0 + a.run), part, smem, sml);
+  float* part = a.runs > 1 ? a.part + ((int64_t(z) * a.B + b) * a.Hkv + kvh) * AS_REC : nullptr;
+  as_piece<FOUR, WAVES>(a, kr, b, kvh, rt, k0, min(kr.n, k0 + a.run), part, smem, sml);
 }
 
 // Workgroup = its share of all steps: the end of an item, whole items, the beginning of
@@ -419,7 +422,7 @@ __global__ __launch_bounds__(AS_CUT * 64, 8 / AS_CUT) void attn_stream_cut_kerne
     for (int n; off >= (n = as_steps(a, b, rt)); ++rt) off -= n;
   }
   while (s < end) {
-    const int r0 = rt * AS_ROWS, r1 = min(r0 + AS_ROWS, a.win.S * (a.Hq / a.Hkv)) - 1;
+    const int r0 = rt * AS_ROWS, r1 = min(r0 + AS_ROWS, a.win.S * a.G) - 1;
     const AsRun kr = as_run<true>(a, b, r0, r1);
     const int steps = max((kr.n + AS_STEP - 1) / AS_STEP, 1), take = min(steps - off, end - s);
     float* part = take == steps ? nullptr : a.part + (int64_t(w) * 2 + (off == 0)) * AS_REC;
@@ -444,9 +447,8 @@ __global__ __launch_bounds__(256) void attn_stream_merge_kernel(const AsArgs a) 
   __shared__ f32x4 so[4][64];
   __shared__ float2 sml[4][64];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4, wave = threadIdx.x >> 6;
-  const int dt = int(blockIdx.x) & 7, item = int(blockIdx.x) >> 3;
-  const int G = a.Hq / a.Hkv, rows = a.win.S * G;
-  const int rt = item % a.rts, z = item / a.rts, b = z / a.Hkv, kvh = z % a.Hkv, r0 = rt * AS_ROWS;
+  const int dt = int(blockIdx.x) & 7, kvh = int(blockIdx.x) >> 3, b = blockIdx.y, rt = blockIdx.z;
+  const int rows = a.win.S * a.G, r0 = rt * AS_ROWS;
   int pieces;
   const float *p0, *p1;  // the first piece's record and the second one's, then every `next`
   int64_t next;
@@ -466,7 +468,7 @@ __global__ __launch_bounds__(256) void attn_stream_merge_kernel(const AsArgs a) 
   } else {
     pieces = max((as_run<FOUR>(a, b, r0, min(r0 + AS_ROWS, rows) - 1).n + a.run - 1) / a.run, 1);
     next = int64_t(a.B) * a.Hkv * a.rts * AS_REC;
-    p0 = a.part + int64_t(item) * AS_REC;
+    p0 = a.part + ((int64_t(rt) * a.B + b) * a.Hkv + kvh) * AS_REC;
     p1 = p0 + next;
   }
   const int row = r0 + r;
@@ -518,7 +520,7 @@ __global__ __launch_bounds__(256) void attn_stream_merge_kernel(const AsArgs a) 
   }
   const float inv = L > 0.0f ? 1.0f / L : 0.0f;
   const int sq = ar_div(row, a.g_magic);
-  *reinterpret_cast<u32x2*>(a.out + ((int64_t(b) * a.win.S + sq) * a.Hq + kvh * G + (row - sq * G)) * HD + dt * 16 + g * 4) =
+  *reinterpret_cast<u32x2*>(a.out + ((int64_t(b) * a.win.S + sq) * a.Hq + kvh * a.G + (row - sq * a.G)) * HD + dt * 16 + g * 4) =
       u32x2{pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
 }
 
@@ -531,6 +533,7 @@ static AsArgs as_args(bool four, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, 
   a.B = int(B);
   a.Hq = int(Hq);
   a.Hkv = int(Hkv);
+  a.G = int(G);
   a.rts = int((S * G + AS_ROWS - 1) / AS_ROWS);
   a.g_magic = ar_magic(uint32_t(G));
   // a run's keys at most: the windows of a tile's queries, and the gap's alignment
@@ -564,10 +567,11 @@ static int64_t as_bytes(const AsArgs& a) {
 }
 
 template <bool FOUR>
-static int as_launch(const char* fn, const AsArgs& a, int64_t grid, hipStream_t s) {
-  const dim3 g{unsigned(grid)}, merge{unsigned(int64_t(a.B) * a.Hkv * a.rts * 8)};
+static int as_launch(const char* fn, const AsArgs& a, hipStream_t s) {
+  const dim3 g{unsigned(a.Hkv), unsigned(a.B), unsigned(a.runs * a.rts)};
+  const dim3 merge{unsigned(a.Hkv * 8), unsigned(a.B), unsigned(a.rts)};
   if (a.wgs)
-    hipLaunchKernelGGL(attn_stream_cut_kernel, g, dim3(AS_CUT * 64), 0, s, a);
+    hipLaunchKernelGGL(attn_stream_cut_kernel, dim3(unsigned(a.wgs)), dim3(AS_CUT * 64), 0, s, a);
   else if (a.waves == 8)
     hipLaunchKernelGGL((attn_stream_kernel<FOUR, 8>), g, dim3(512), 0, s, a);
   else
@@ -606,7 +610,7 @@ static int attend(const char* fn, bool four, const qmoe_bf16* q, const qmoe_bf16
   a.scale_log2 = scale * 1.4426950408889634f;
   a.part = static_cast<float*>(workspace);
   a.out = out;
-  return four ? as_launch<true>(fn, a, grid, as_stream(stream)) : as_launch<false>(fn, a, grid, as_stream(stream));
+  return four ? as_launch<true>(fn, a, as_stream(stream)) : as_launch<false>(fn, a, as_stream(stream));
 }
 
 static int64_t workspace(const char* fn, bool four, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t D,
