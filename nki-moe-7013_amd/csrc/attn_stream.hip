@@ -78,46 +78,48 @@ struct AsTotal {
   __device__ __forceinline__ int begin(int w) const { return int(int64_t(w) * T / W); }
   __device__ __forceinline__ int owner(int step) const { return int((int64_t(step + 1) * W - 1) / T); }
 };
-// Sums the steps of all sequences (256 threads) and of those before a place: `find`
-// says of a sequence's first step and number of steps whether it is the place, whose
-// sequence and first step everyone gets.
+__device__ __forceinline__ int wave_scan(int v) {  // inclusive
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_SHR(1), 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_SHR(2), 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_SHR(4), 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_SHR(8), 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_BCAST15, 0xa, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, QMOE_DPP_ROW_BCAST31, 0xc, 0xf, false);
+  return v;
+}
+// Sums the steps of all sequences, and finds the place that `find` says yes to, given
+// the total, a sequence, its first step and its number of steps.  Every wave does it
+// for itself, 64 sequences at a time.
 struct AsPlace {
   int b, first;
 };
 template <class Find>
-__device__ __forceinline__ AsTotal as_total(const AsArgs& a, int (&lds)[8], AsPlace* place, Find find) {
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6, per = (a.B + 255) / 256;
-  const int b0 = min(t * per, a.B), b1 = min(b0 + per, a.B);
-  int sum = 0;
-  for (int b = b0; b < b1; ++b) sum += as_row_steps(a, b);
-  sum *= a.Hkv;
-  int upto = sum;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int v = __shfl_up(upto, d, 64);
-    upto += lane >= d ? v : 0;
-  }
-  if (lane == 63) lds[wave] = upto;
-  __syncthreads();
-  int before = upto - sum;
+__device__ __forceinline__ AsTotal as_total(const AsArgs& a, AsPlace* place, Find find) {
+  const int lane = threadIdx.x & 63;
   AsTotal tot{0, 0};
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    before += w < wave ? lds[w] : 0;
-    tot.T += lds[w];
+  int n = 0, upto = 0;
+  for (int c = 0; c < a.B; c += 64) {
+    n = c + lane < a.B ? as_row_steps(a, c + lane) * a.Hkv : 0;
+    upto = wave_scan(n);
+    tot.T += __builtin_amdgcn_readlane(upto, 63);
   }
-  tot.T = __builtin_amdgcn_readfirstlane(tot.T);
   tot.W = min(a.wgs, tot.T);
-  for (int b = b0; b < b1; ++b) {
-    const int n = b1 - b0 == 1 ? sum : as_row_steps(a, b) * a.Hkv;
-    if (find(tot, b, before, n)) {
-      lds[4] = b;
-      lds[5] = before;
+  int before = 0;
+  *place = AsPlace{0, 0};
+  for (int c = 0; c < a.B; c += 64) {
+    if (a.B > 64) {
+      n = c + lane < a.B ? as_row_steps(a, c + lane) * a.Hkv : 0;
+      upto = wave_scan(n);
     }
-    before += n;
+    const int first = before + upto - n;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(c + lane < a.B && find(tot, c + lane, first, n));
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      *place = AsPlace{c + l, __builtin_amdgcn_readlane(first, l)};
+      break;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
-  __syncthreads();
-  *place = AsPlace{__builtin_amdgcn_readfirstlane(lds[4]), __builtin_amdgcn_readfirstlane(lds[5])};
   return tot;
 }
 
@@ -404,10 +406,9 @@ __global__ __launch_bounds__(WAVES * 64, 8 / WAVES) void attn_stream_kernel(cons
 __global__ __launch_bounds__(AS_CUT * 64, 8 / AS_CUT) void attn_stream_cut_kernel(const AsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[AS_CUT][AS_TILE * AP_ROWB];
   __shared__ float2 sml[AS_CUT][AS_ROWS];
-  __shared__ int lds[8];
   const int w = int(blockIdx.x);
   AsPlace at;
-  const AsTotal tot = as_total(a, lds, &at, [&](const AsTotal& t, int, int first, int n) {
+  const AsTotal tot = as_total(a, &at, [&](const AsTotal& t, int, int first, int n) {
     const int s = w < t.W ? t.begin(w) : -1;
     return s >= first && s < first + n;
   });
@@ -453,9 +454,8 @@ __global__ __launch_bounds__(256) void attn_stream_merge_kernel(const AsArgs a) 
   const float *p0, *p1;  // the first piece's record and the second one's, then every `next`
   int64_t next;
   if constexpr (CUT) {
-    __shared__ int lds[8];
     AsPlace at;
-    const AsTotal tot = as_total(a, lds, &at, [&](const AsTotal&, int c, int, int) { return c == b; });
+    const AsTotal tot = as_total(a, &at, [&](const AsTotal&, int c, int, int) { return c == b; });
     int first = at.first + kvh * as_row_steps(a, b);
     for (int i = 0; i < rt; ++i) first += as_steps(a, b, i);
     // workgroup w0 began the item (its second record), the next ones went on (their first)
@@ -555,8 +555,8 @@ static AsArgs as_args(bool four, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, 
   a.run = int((steps + want - 1) / want * step);
   a.runs = int((steps * step + a.run - 1) / a.run);
   // An even share of all keys for each place once that is 16 steps and more (runs /
-  // shares: 32 rows of up to 16384 47.5 / 44.0 us, 64 of 32768 150 / 140; but 64 of 4096 27.5 /
-  // 31.7, for a share begins and ends inside items).
+  // shares: 32 rows of up to 16384 47.5 / 41.8 us, 64 of 32768 150 / 138; but 64 of 4096 25.4 /
+  // 29.6, for a share begins and ends inside items).
   a.wgs = four && B > 1 && items < 4 * places && items * steps >= 16 * places ? int(places) : 0;
   *grid = a.wgs ? a.wgs : items * a.runs;
   return a;
