@@ -18,7 +18,6 @@ namespace qmoe {
 
 constexpr int AS_ROWS = 16;             // query rows of an item
 constexpr int AS_TILE = 64;             // keys of a wave's step
-constexpr int AS_MAX_ROWS = 64;         // rows of a (sequence, kv head): past them tiles share the keys
 constexpr int AS_REC = 2 * AS_ROWS + AS_ROWS * HD;  // record of a piece: (m, l) of the rows, O in register order
 constexpr int AS_CUT = 4;               // waves of a workgroup that takes a share of the keys
 
@@ -561,6 +560,19 @@ static AsArgs as_args(bool four, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, 
   *grid = a.wgs ? a.wgs : items * a.runs;
   return a;
 }
+
+// Whether rows go as streams: up to 64 of a (sequence, kv head), and more while that is
+// at most four steps a CU in all.  A stream's 16 rows take nearly twice as long over many
+// keys as their share of a tile's 128, but end sooner over few (1 x 100 queries on 1000
+// entries in 4 bits, tiles / streams: 15.4 / 10.4 us; 8 x 12 with a window of 512 14.5 /
+// 12.3; but 8 x 24 16.2 / 17.5, a prompt of 640 with a window of 250 14.5 / 21.5).
+static bool as_few(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
+                   int64_t sink) {
+  const int64_t rows = S * (Hq / Hkv), items = B * Hkv * ((rows + AS_ROWS - 1) / AS_ROWS);
+  const int64_t seen = std::min<int64_t>(window, WIN_NONE) + std::min<int64_t>(sink, WIN_NONE);
+  const int64_t keys = window ? std::min(max_ctx, seen) : max_ctx;
+  return rows <= 64 || items * ((keys + AS_STEP - 1) / AS_STEP) <= 4 * std::max(current_device_cus(), 1);
+}
 static int64_t as_bytes(const AsArgs& a) {
   const int64_t records = a.wgs ? 2 * int64_t(a.wgs) : a.runs > 1 ? int64_t(a.runs) * a.B * a.Hkv * a.rts : 0;
   return records * AS_REC * int64_t(sizeof(float));
@@ -596,7 +608,7 @@ static int attend(const char* fn, bool four, const qmoe_bf16* q, const qmoe_bf16
                   int64_t workspace_bytes, qmoe_bf16* out, qmoe_stream_t stream) {
   if (B == 0 || S == 0) return QMOE_OK;
   QMOE_REQUIRE(aligned16(k, v, cache.k, cache.ks, cache.v, cache.vs), "%s: operands must be 16-byte aligned", fn);
-  if (S * (Hq / Hkv) > AS_MAX_ROWS)
+  if (!as_few(B, S, Hq, Hkv, max_ctx, window, sink))
     return attn_window_tiles(fn, q, k, v, four ? &cache : nullptr, ctx_len, B, S, Hq, Hkv, S_max, max_ctx, window, sink,
                              scale, workspace, workspace_bytes, out, as_stream(stream));
   int64_t grid;
@@ -618,7 +630,8 @@ static int64_t workspace(const char* fn, bool four, int64_t B, int64_t S, int64_
   const int64_t most = 1ll << 22;
   if (win_check(fn, B, S, Hq, Hkv, D, most, max_ctx, window, sink, 1.0f)) return -1;
   if (B == 0 || S == 0) return 0;
-  if (S * (Hq / Hkv) > AS_MAX_ROWS) return attn_window_tiles_workspace(B, S, Hq, Hkv, max_ctx, window, sink);
+  if (!as_few(B, S, Hq, Hkv, max_ctx, window, sink))
+    return attn_window_tiles_workspace(B, S, Hq, Hkv, max_ctx, window, sink);
   int64_t grid;
   return as_bytes(as_args(four, B, S, Hq, Hkv, most, max_ctx, window, sink, &grid));
 }

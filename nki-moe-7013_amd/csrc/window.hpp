@@ -46,8 +46,8 @@ struct Cache4 {
 };
 
 // ---------------------------------------------------------------------- host
-// The calls of many rows (S * Hq / Hkv > 64), on the tiles of attn_rows.hip; cache: in
-// 4 bits, instead of k and v.
+// The calls of many rows, on the tiles of attn_rows.hip; cache: in 4 bits, instead of k
+// and v.
 int64_t attn_window_tiles_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
                                     int64_t sink);
 int attn_window_tiles(const char* fn, const uint16_t* q, const uint16_t* k, const uint16_t* v, const Cache4* cache,

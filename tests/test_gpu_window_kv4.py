@@ -236,6 +236,15 @@ ATTEND = [
     (1, 700, 700, 4, 4, [-40], 33, 3, None),
     (1, 1100, 1100, 8, 1, [1], 1 << 30, 0, None),
     (3, 40, 3000, 16, 2, [2961, 1, 2000], 2500, 4, None),
+    (1, 1500, 1700, 8, 8, [201], 700, 7, None),           # tiles: one head a group
+    (1, 1400, 1400, 4, 4, [-40], 900, 3, None),
+    (2, 700, 900, 12, 4, [1, 201], 300, 65, None),
+    (2, 600, 700, 32, 4, [1, 90], 1, 0, None),
+    (2, 600, 700, 32, 4, [1, 90], 1, 1, None),
+    (2, 600, 700, 32, 4, [1, 101], 33, 40, 500),
+    (1, 1000, 1000, 16, 1, [5], 64, 64, None),            # and queries past the cache
+    (2, 600, 64, 32, 4, [1, 30], 100, 0, 0),              # nothing to see at all
+    (3, 1, 64, 32, 4, [1, 30, 64], 100, 2, 0),
 ]
 
 
