@@ -102,7 +102,10 @@ struct Tiles4 {
     rks = kv4_rsrc(ks, int64_t(rows) * 4);
     rvs = kv4_rsrc(vs, int64_t(rows) * 4);
     smem = lds;
-    row = int(threadIdx.x) >> 2;
+    // rows 2 apart next to each other: eight lanes' chunks, of K as of V, then lie in
+    // eight places
+    const int q = int(threadIdx.x) >> 2;
+    row = (q & ~3) | (q & 1) << 1 | ((q >> 1) & 1);
     blk = int(threadIdx.x) & 3;
     key = k0 + row;
     n_kt = tiles;
