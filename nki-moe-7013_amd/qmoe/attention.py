@@ -270,7 +270,7 @@ class Attention:
             if self.window:
                 raise ValueError("a shared prefix or a bounded cache has no window")
             o = self._special(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
-        elif self.window or isinstance(cache, KV4Cache):
+        elif isinstance(cache, KV4Cache) or self._hides(S, cache, start, max_ctx):
             o = self._windowed(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
         else:
             o = self._plain(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
@@ -380,6 +380,14 @@ class Attention:
             return ops.gemv_rmsnorm(x, norm[0], norm[1], self.wqkv, _lib.GEMM_STORE_F32)
         gemv = ops.qkv_norm_rope_workspace(rows, x.shape[1], self.n_q, self.n_kv, self.head_dim) > 0
         return ops.gemm(x, self.wqkv, _lib.GEMM_STORE_F32) if gemv or self._skinny_decode(x, rows) else None
+
+    def _hides(self, S: int, cache: KVCache, start, max_ctx: Optional[int]) -> bool:
+        """Whether the window leaves out an entry that some query could see: none in a
+        bucket or up to a prompt's end that is no longer than it."""
+        end = cache.capacity if max_ctx is None else min(max_ctx, cache.capacity)
+        if S > 1 and not isinstance(start, torch.Tensor):
+            end = min(end, start + S)
+        return 0 < self.window < end
 
     def _windowed(self, x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm) -> torch.Tensor:
         """Attention outputs ``[B*S, Hq*D]`` with a window, over a cache in 4 bits, or both."""

@@ -287,6 +287,25 @@ def test_attention_layer(dev, B, S, chunk, window, sink, four):
         first += count
 
 
+def test_a_window_that_hides_nothing_takes_the_plain_path(dev):
+    """Up to the window's length a layer's outputs are those without one, bit for bit;
+    past it they differ."""
+    plain, g = _attention(dev, 3, 0, 0)
+    at = Attention(plain.wqkv, plain.q_norm, plain.k_norm, plain.wo, HQ, HKV, D, 1e-6, 40, 0)
+    cos, sin = rope_tables(D, 100, 1e6, dev)
+    a, b = KVCache(2, HKV, 100, D, dev), KVCache(2, HKV, 100, D, dev)
+    first = 0
+    for n, bucket, same in ((38, None, True), (1, 40, True), (1, 40, True), (1, 64, False), (20, None, False)):
+        x = bf16_randn((2 * n, H), g, dev)
+        pos = (first + torch.arange(n, dtype=torch.int32, device=dev)).repeat(2)
+        out = [torch.zeros(2 * n, H, device=dev) for _ in range(2)]
+        for layer, cache, res in ((plain, a, out[0]), (at, b, out[1])):
+            layer.forward(x, res, pos, 2, n, cache, cos, sin, first, max_ctx=bucket)
+        assert torch.equal(*out) == same
+        assert torch.equal(a.k, b.k) and torch.equal(a.v, b.v)
+        first += n
+
+
 def test_a_layer_with_a_window_refuses_special_caches(dev):
     from qmoe.attention import BoundedKVCache, CacheBudget, SharedPrefix
 
@@ -322,7 +341,7 @@ def test_layer_contract_with_a_window_and_four_bits(dev):
 
 
 # ------------------------------------------------------------------ the model
-OPTIONS = [dict(attention_window=24, attention_sink=3), dict(kv_cache_bits=4),
+OPTIONS = [dict(attention_window=24, attention_sink=3), dict(attention_window=260), dict(kv_cache_bits=4),
            dict(kv_cache_bits=4, attention_window=24, attention_sink=3)]
 
 
