@@ -696,7 +696,9 @@ int64_t qmoe_attn_window_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv
  * NaN has the power 255 and reads as NaN.  Bytes of 0 read as 0. */
 
 /* qmoe_attn_window over a cache in 4 bits; window 0: every entry up to the
- * query's own.  Rules, limits and workspace as there.
+ * query's own.  Rules, limits and workspace as there, but that a long batch's keys
+ * are cut by the lengths of all its rows, so that a row's last bits may differ
+ * with the other rows' lengths.
  * Replaces: the attention over the KV cache (qwen_with_nki.py:9943-9946); the
  *   reference's cache is in bf16. */
 int qmoe_attn_kv4(const qmoe_bf16* q, const uint8_t* k_cache, const uint8_t* k_scales, const uint8_t* v_cache,

@@ -932,7 +932,8 @@ def attn_kv4(q: torch.Tensor, cache: KV4, ctx_len: torch.Tensor, B: int, S: int,
              scale: Optional[float] = None, workspace: Optional[torch.Tensor] = None,
              out: Optional[torch.Tensor] = None, max_ctx: Optional[int] = None) -> torch.Tensor:
     """:func:`attn_window` over a cache in 4 bits (:func:`kv4_cache`); ``window`` 0:
-    a query sees every entry up to its own."""
+    a query sees every entry up to its own.  A long batch's keys are cut by the
+    lengths of all its rows, and a row's last bits go with the others' lengths."""
     return _native().attn_kv4(q, cache, ctx_len, B, S, window, sink, scale, workspace, out, max_ctx)
 
 

@@ -153,6 +153,47 @@ def test_graph_replays_with_changing_lengths(dev):
         assert all(torch.equal(a, b) for a, b in zip(cache, eager))
 
 
+def test_graph_replays_of_long_batches_and_chunks(dev):
+    """A step of a long batch, whose keys go in even shares, and chunks on tiles with
+    and without a window: captured once, replayed with other lengths and eager work
+    between, every replay as the eager call."""
+    B, S_max, S = 40, 12000, 40
+    announce("graph replays, long batches and chunks")
+    g = _gen(dev, 9)
+    k, v = bf16_randn((B, HKV, S_max, D), g, dev), bf16_randn((B, HKV, S_max, D), g, dev)
+    cache = ops.kv4_cache(B, HKV, S_max, D, dev)
+    ops.kv4_store(k, v, cache)
+    q = bf16_randn((B * S, HQ, D), g, dev, 2.0)
+    ctx = _i32([1] * B, dev)
+    outs = [torch.zeros(n, HQ * D, dtype=torch.bfloat16, device=dev) for n in (B, B * S, B * S)]
+
+    def calls(outs):
+        ops.attn_kv4(q[:B], cache, ctx, B, 1, out=outs[0])
+        ops.attn_kv4(q, cache, ctx, B, S, 1500, 4, out=outs[1])
+        ops.attn_window(q, k, v, ctx, B, S, 700, 4, out=outs[2])
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        calls(outs)
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        calls(outs)
+    eager = [torch.zeros_like(o) for o in outs]
+    for rep, n in enumerate([12000, 1, 5000, 0, 11999]):
+        ctx.copy_(_i32([max(-S, n - 290 * i) for i in range(B)], dev))
+        q.normal_(0.0, 2.0, generator=g)
+        graph.replay()
+        torch.cuda.synchronize()
+        calls(eager)
+        torch.cuda.synchronize()
+        for a, b in zip(outs, eager):
+            assert torch.equal(a, b), rep
+            assert not bool(torch.isnan(a).any())
+
+
 def test_calls_on_another_stream(dev):
     """Calls take the current stream, whichever it is."""
     announce("another stream")
