@@ -7,6 +7,16 @@
 //   S^T [keys x rows] = K . Q^T     O^T [dims x rows] += V^T . P^T
 // Numbers of 4 bits become bf16 in registers (v_cvt_scalef32_pk_bf16_fp4, two a step
 // with their power; exact), so queries and products are those of a bf16 cache.
+//
+// Work: 4 * 128 flops a (query head, key), 512 bytes a (kv head, key) in bf16 and 136 in 4
+// bits.  8 query heads on a kv head are 8 flops a byte, or 30: the stream from memory
+// bounds a long batch in bf16 (32 rows that see 4100 keys each, 269 MB in 48 us and 4 for
+// the merge, 5.2 TB/s in all, a large copy's rate) and a very long one in 4 bits (64 rows
+// of up to 32768, 714 MB in 138 us, 5.2 TB/s).  Shorter ones in 4 bits wait for the steps:
+// one is 128 conversions, 32 products, 64 exponentials and V through LDS a wave, with two
+// waves a SIMD (32 rows of up to 8192, 90 MB in 24 + 4 us, 3.3 TB/s).  Few keys are a chain
+// of memory round trips: lengths, queries and keys, one step or two, the join (one row of
+// 800 in 4 bits 9 us, of 516 keys in bf16 7 + 2.3).
 #include "attn_tile.hpp"
 #include "common.hpp"
 #include "kv4.hpp"
@@ -383,6 +393,14 @@ __device__ __forceinline__ void as_piece(const AsArgs& a, const AsRun& kr, int b
   if (part && wave == 0 && g == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(M, L);
 }
 
+// 64 keys a step: 16 loads of 16 bytes a lane in flight for the next K and V in bf16 (the
+// 243 registers are what two waves a SIMD have) and 10 in 4 bits.  16 query rows, since a
+// group has 8 heads: of 32 x 32 products three quarters would be of rows that are none.
+// Tried for 4 bits and not kept: the next tile but one in flight too (32 x 8192 27 -> 29 us,
+// 1 x 800 9.2 -> 10.1); V converted behind the first products (the same time); keys in
+// 4 bits and queries as two terms in 8 for the scaled products (their sums are aligned
+// to the largest term: errors of 8e-5 of the terms' magnitudes).
+//
 // Workgroup = (kv head, sequence, run of a row tile): heads and sequences are fastest, so
 // the row tiles that share a head's keys are on one XCD when there are a multiple of 8
 // of those.
@@ -401,7 +419,7 @@ __global__ __launch_bounds__(WAVES * 64, 8 / WAVES) void attn_stream_kernel(cons
 }
 
 // Workgroup = its share of all steps: the end of an item, whole items, the beginning of
-// another.
+// another.  (64 x 32768: 126-141 us; with runs of equal numbers of steps an item 150.)
 __global__ __launch_bounds__(AS_CUT * 64, 8 / AS_CUT) void attn_stream_cut_kernel(const AsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[AS_CUT][AS_TILE * AP_ROWB];
   __shared__ float2 sml[AS_CUT][AS_ROWS];
@@ -441,7 +459,8 @@ __global__ __launch_bounds__(AS_CUT * 64, 8 / AS_CUT) void attn_stream_cut_kerne
 }
 
 // Joins the pieces of an item's rows: workgroup = (item, dim tile); wave v takes the
-// pieces v, v + 4, ..., four at a time.
+// pieces v, v + 4, ..., four at a time.  Bound by latency: one round trip for the lengths
+// and one for the records (3 items 2.3 us, 32 x 4 items of 4 pieces 3.9, of shares 6.6).
 template <bool FOUR, bool CUT>
 __global__ __launch_bounds__(256) void attn_stream_merge_kernel(const AsArgs a) {
   __shared__ f32x4 so[4][64];
