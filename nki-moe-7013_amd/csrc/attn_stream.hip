@@ -12,11 +12,12 @@
 // bits.  8 query heads on a kv head are 8 flops a byte, or 30: the stream from memory
 // bounds a long batch in bf16 (32 rows that see 4100 keys each, 269 MB in 48 us and 4 for
 // the merge, 5.2 TB/s in all, a large copy's rate) and a very long one in 4 bits (64 rows
-// of up to 32768, 714 MB in 138 us, 5.2 TB/s).  Shorter ones in 4 bits wait for the steps:
-// one is 128 conversions, 32 products, 64 exponentials and V through LDS a wave, with two
-// waves a SIMD (32 rows of up to 8192, 90 MB in 24 + 4 us, 3.3 TB/s).  Few keys are a chain
-// of memory round trips: lengths, queries and keys, one step or two, the join (one row of
-// 800 in 4 bits 9 us, of 516 keys in bf16 7 + 2.3).
+// of up to 32768, 714 MB in 138 us, 5.2 TB/s).  Shorter ones in 4 bits wait for the steps,
+// of 128 conversions, 32 products, 16 exponentials and V through LDS a wave: a conversion
+// takes its SIMD 16 cycles, so two waves' steps on one 5000 (32 rows of up to 8192, 90 MB in
+// 25 us).  Few keys are a chain: lengths, queries and keys, one step or two, the join (one
+// row of 800 in 4 bits 9 us), and in bf16 what a CU takes in, 19-24 bytes a cycle, so that
+// one row's keys go to many (516 keys: 4 heads x 9 waves each alone 7.7 us, 3 x 4 waves 9.9).
 #include "attn_tile.hpp"
 #include "common.hpp"
 #include "kv4.hpp"
@@ -354,9 +355,23 @@ __device__ __forceinline__ void as_piece(const AsArgs& a, const AsRun& kr, int b
     }
   }
 
-  // the waves' states of the same rows: each wave joins its share of the eight dim tiles
   l += __shfl_xor(l, 16, 64);
   l += __shfl_xor(l, 32, 64);
+  if constexpr (WAVES == 1) {  // nothing to join
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (!live) return;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) {
+      if (part)
+        *reinterpret_cast<f32x4*>(part + 2 * AS_ROWS + (dt * 64 + lane) * 4) = o[dt];
+      else
+        *reinterpret_cast<u32x2*>(a.out + qrow * HD + dt * 16 + g * 4) =
+            u32x2{pack_bf16x2(o[dt][0] * inv, o[dt][1] * inv), pack_bf16x2(o[dt][2] * inv, o[dt][3] * inv)};
+    }
+    if (part && g == 0) *reinterpret_cast<float2*>(part + 2 * r) = make_float2(m, l);
+    return;
+  }
+  // the waves' states of the same rows: each wave joins its share of the eight dim tiles
   __syncthreads();  // V tiles free
   float* rec = reinterpret_cast<float*>(&smem[0][0]);
 #pragma unroll
@@ -405,7 +420,7 @@ __device__ __forceinline__ void as_piece(const AsArgs& a, const AsRun& kr, int b
 // the row tiles that share a head's keys are on one XCD when there are a multiple of 8
 // of those.
 template <bool FOUR, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, 8 / WAVES) void attn_stream_kernel(const AsArgs a) {
+__global__ __launch_bounds__(WAVES * 64, WAVES == 8 ? 1 : 2) void attn_stream_kernel(const AsArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[WAVES][AS_TILE * AP_ROWB];
   __shared__ float2 sml[WAVES][AS_ROWS];
   const int kvh = blockIdx.x, b = blockIdx.y, z = blockIdx.z;
@@ -543,6 +558,32 @@ __global__ __launch_bounds__(256) void attn_stream_merge_kernel(const AsArgs a) 
 }
 
 // ---------------------------------------------------------------------- host
+// Waves of a workgroup, for items of n keys at most.  us called / replayed in a graph,
+// 32 query heads over 4 kv heads:
+//  - 4 where they take all keys in one step, and no merge (1 row of 200, 4 / 8 waves:
+//    bf16 6.9 / 7.3, 4 bits 5.7 / 6.1);
+//  - 8 and no merge for a few more keys: up to 1024 of 4 bits (1 row of 800, one launch 9.4 /
+//    9.3, two 11.1 / 7.9), up to 512 of bf16, and 512 more where the items alone take half
+//    of the CUs (32 rows of 1500 in 4 bits, one launch 11.8, two 13.4; bf16, 24 rows of 600
+//    12.0 / 14.3, 32 of 1020 16.4 / 18.1; but 16 rows of 1500 in 4 bits 11.3 / 10.8);
+//  - 1, of a tile each, for few keys of bf16, whose bytes a CU takes in at its own rate (1
+//    row of 500, 8 waves / 1: 9.8 / 7.5, of 380 8.0 / 7.7 and 1.3 us more on the host; window
+//    of 512 + 4, 4 waves 9.9 / 2 waves 8.5 / 1 wave 7.7; but 1 row of 4000 9.3 / 8.6 / 9.6);
+//  - 2, of a step each, while that is up to eight workgroups a CU in bf16 (24 rows with a
+//    window of 1020, 4 / 2 waves: 16.9 / 14.7, 12 with one of 2000 15.0 / 14.4, 1 row of 4000
+//    9.3 / 8.6; but 16 rows of 8000 slower) and two waves in 4 bits (1 row of 2000 8.4 / 7.9,
+//    4 of 2048 8.2 / 7.7; but 8 of 1500 8.8 / 9.2), and the merge has 32 or 16 records;
+//  - 4 with long runs past that.
+static int as_waves(bool four, int64_t items, int64_t n, int64_t cus) {
+  const int64_t tiles = (n + AS_TILE - 1) / AS_TILE, work = items * tiles;
+  if (tiles <= 4) return 4;
+  const bool spread = !four && tiles <= 20 && 2 * work <= 3 * cus;
+  const int64_t one = 512 * ((four ? 2 : 1) + (2 * items >= cus));
+  if (n <= one && items <= cus && !(spread && tiles > 6)) return 8;
+  if (spread) return 1;
+  return items < cus && work < (four ? 2 : 8) * cus && tiles <= (four ? 32 : 64) ? 2 : 4;
+}
+
 static AsArgs as_args(bool four, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t S_max, int64_t max_ctx,
                       int64_t window, int64_t sink, int64_t* grid) {
   AsArgs a{};
@@ -554,14 +595,11 @@ static AsArgs as_args(bool four, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, 
   a.G = int(G);
   a.rts = int((S * G + AS_ROWS - 1) / AS_ROWS);
   a.g_magic = ar_magic(uint32_t(G));
-  // a run's keys at most: the windows of a tile's queries, and the gap's alignment
-  const int64_t n = std::min<int64_t>(max_ctx, int64_t(a.win.window) + a.win.sink + std::min<int64_t>(S, AS_ROWS)) + 3;
+  // an item's keys at most: the windows of its queries, and the gap's alignment
+  const int64_t seen = int64_t(a.win.window) + a.win.sink + std::min<int64_t>(S, AS_ROWS) - 1 + (four ? 3 : 0);
+  const int64_t n = std::max<int64_t>(std::min(max_ctx, seen), 1);
   const int64_t items = B * Hkv * a.rts, cus = std::max(current_device_cus(), 1);
-  // One launch of eight waves a workgroup while the keys are few: up to 1024 of 4 bits
-  // (1 row of 1000, called / replayed in a graph, 10.7 / 9.0 -> 9.8 / 9.9 us; 32 rows 13.0 /
-  // 12.7 -> 10.2; 1 row of 500 10.8 / 8.9 -> 8.0), up to 512 of bf16 (1 row of 500 10.7 -> 9.9,
-  // of 1000 11.0 -> 14.8).
-  a.waves = n <= (four ? 1024 : 512) && items <= cus ? 8 : AS_CUT;
+  a.waves = as_waves(four, items, n, cus);
   const int64_t step = a.waves * AS_TILE, steps = (n + step - 1) / step;
   // Else runs for a workgroup a CU, or for two where the rows are likely of different
   // lengths and a step takes little from memory (8 rows of up to 32000 in 4 bits, 8 / 16
@@ -569,7 +607,8 @@ static AsArgs as_args(bool four, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, 
   // with a window of 8000, 2 / 4 runs: 69 / 74), but no runs of a few steps where the
   // items alone fill the CUs (64 rows of 2000 in 4 bits, 1 / 2 runs: 16.7 / 20.0).
   const int64_t places = cus * (four && B > 1 ? 2 : 1);
-  const int64_t want = a.waves == 8 || (items >= cus && steps <= 8) ? 1 : std::max<int64_t>(places / items, 1);
+  int64_t want = a.waves == 8 || (items >= cus && steps <= 8) ? 1 : std::max<int64_t>(places / items, 1);
+  if (a.waves < AS_CUT) want = steps;
   a.run = int((steps + want - 1) / want * step);
   a.runs = int((steps * step + a.run - 1) / a.run);
   // An even share of all keys for each place once that is 16 steps and more (runs /
@@ -605,8 +644,12 @@ static int as_launch(const char* fn, const AsArgs& a, hipStream_t s) {
     hipLaunchKernelGGL(attn_stream_cut_kernel, dim3(unsigned(a.wgs)), dim3(AS_CUT * 64), 0, s, a);
   else if (a.waves == 8)
     hipLaunchKernelGGL((attn_stream_kernel<FOUR, 8>), g, dim3(512), 0, s, a);
-  else
+  else if (a.waves == AS_CUT)
     hipLaunchKernelGGL((attn_stream_kernel<FOUR, AS_CUT>), g, dim3(AS_CUT * 64), 0, s, a);
+  else if (a.waves == 2)
+    hipLaunchKernelGGL((attn_stream_kernel<FOUR, 2>), g, dim3(128), 0, s, a);
+  else
+    hipLaunchKernelGGL((attn_stream_kernel<false, 1>), g, dim3(64), 0, s, a);
   const int rc = hip_status(fn);
   if (rc || (a.wgs == 0 && a.runs == 1)) return rc;
   if (a.wgs)

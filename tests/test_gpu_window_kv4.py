@@ -329,6 +329,30 @@ def test_attn_kv4_of_long_batches(dev, B, S, S_max, Hq, Hkv, window, ctx):
         _within(got[one], *ref.window(q[one], k, v, [ctx[b]], 1, S, window, 4 if window else 0, S_max, SCALE), f"row {b}")
 
 
+@pytest.mark.parametrize("four", [False, True], ids=["bf16", "four"])
+@pytest.mark.parametrize("B,S,n,Hq,Hkv", [
+    # on both sides of where a workgroup has 1, 2, 4 and 8 waves, and a call one launch or two
+    (1, 1, 60, 32, 4), (1, 1, 256, 32, 4), (1, 1, 257, 32, 4), (1, 1, 385, 32, 4), (1, 1, 513, 8, 8), (3, 1, 1000, 32, 4),
+    (1, 1, 1030, 32, 4), (2, 1, 1280, 32, 4), (1, 1, 1290, 32, 4), (1, 1, 2045, 64, 4), (5, 1, 2050, 32, 4),
+    (1, 1, 4100, 32, 4), (34, 1, 900, 32, 4), (33, 1, 1500, 32, 4), (70, 1, 400, 32, 4), (2, 5, 700, 32, 4),
+    (1, 3, 1200, 64, 4), (1, 7, 3000, 32, 8)])
+def test_few_rows_of_any_length(dev, B, S, n, Hq, Hkv, four):
+    announce(f"few rows {B} {S} {n} {Hq} {Hkv} {'4 bits' if four else 'bf16'}")
+    g = _gen(dev, n)
+    q = bf16_randn((B * S, Hq, D), g, dev, 2.0)
+    ctx = [max(-S, n - S + 1 - 67 * i) for i in range(B)]
+    k, v = (bf16_randn((B, Hkv, n, D), g, dev) for _ in range(2))
+    for window, sink in (((0, 0),) if four else ()) + ((n, 0), (n - 10, 4), (n // 2, 5)):
+        if four:
+            cache = ops.kv4_cache(B, Hkv, n, D, dev)
+            ops.kv4_store(k, v, cache)
+            got = ops.attn_kv4(q, cache, _i32(ctx, dev), B, S, window, sink)
+            held = [ref.values(*cache[i:i + 2]) for i in (0, 2)]
+        else:
+            got, held = ops.attn_window(q, k, v, _i32(ctx, dev), B, S, window, sink), [k, v]
+        _within(got, *ref.window(q, *held, ctx, B, S, window, sink, n, SCALE), f"window {window}")
+
+
 @pytest.mark.parametrize("scale", [1.0, 1e-3, 0.5])
 def test_scales(dev, scale):
     g = _gen(dev, 3)

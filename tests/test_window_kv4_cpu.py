@@ -100,6 +100,17 @@ def test_workspace_queries():
     assert l.qmoe_attn_window_workspace(1, 1, 32, 4, 128, 0, 0, 1) == -1
 
 
+def test_workspace_queries_of_every_size():
+    """From caches of which nothing is seen on, whatever the batch, the chunk and the window."""
+    l = _lib.lib()
+    for top in (0, 1, 63, 64, 65, 256, 257, 513, 1024, 1025, 2048, 5000, 1 << 22):
+        for B, S in ((1, 1), (3, 5), (2, 100), (1, 700), (64, 1), (300, 1)):
+            for window in (1, 512, 1 << 40):
+                assert l.qmoe_attn_window_workspace(B, S, 32, 4, 128, window, 3, top) >= 0
+                assert l.qmoe_attn_kv4_workspace(B, S, 32, 4, 128, window, 3, top) >= 0
+            assert l.qmoe_attn_kv4_workspace(B, S, 32, 4, 128, 0, 0, top) >= 0
+
+
 def _cache():
     return ops.kv4_cache(2, 4, 64, 128, "cpu")
 
