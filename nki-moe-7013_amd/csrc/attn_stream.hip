@@ -12,12 +12,13 @@
 // bits.  8 query heads on a kv head are 8 flops a byte, or 30: the stream from memory
 // bounds a long batch in bf16 (32 rows that see 4100 keys each, 269 MB in 48 us and 4 for
 // the merge, 5.2 TB/s in all, a large copy's rate) and a very long one in 4 bits (64 rows
-// of up to 32768, 714 MB in 138 us, 5.2 TB/s).  Shorter ones in 4 bits wait for the steps,
-// of 128 conversions, 32 products, 16 exponentials and V through LDS a wave: a conversion
-// takes its SIMD 16 cycles, so two waves' steps on one 5000 (32 rows of up to 8192, 90 MB in
-// 25 us).  Few keys are a chain: lengths, queries and keys, one step or two, the join (one
-// row of 800 in 4 bits 9 us), and in bf16 what a CU takes in, 19-24 bytes a cycle, so that
-// one row's keys go to many (516 keys: 4 heads x 9 waves each alone 7.7 us, 3 x 4 waves 9.9).
+// of up to 32768, 714 MB in 138 us, 5.2 TB/s).  Shorter ones in 4 bits are that rate and 11 us of
+// launches, first loads, joins and the merge (32 rows of up to 8192 25 us, of up to 16384
+// 42).  Few keys are a chain: lengths, queries and keys, one step or two (of 3300 cycles in 4
+// bits: 128 conversions, 32 products, 16 exponentials, V through LDS), the join (one row of
+// 800 in 4 bits 9 us), and in it what one CU takes in, 19-24 bytes a cycle, for which a row's
+// keys in bf16 go to many CUs (516 keys, 4 heads: 9 waves each by itself 7.7 us, 3 workgroups
+// of 4 waves 9.9, in a graph).
 #include "attn_tile.hpp"
 #include "common.hpp"
 #include "kv4.hpp"
