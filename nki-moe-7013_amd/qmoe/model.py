@@ -133,10 +133,11 @@ class Qwen3MoeInferenceConfig:
     def window(self) -> int:
         """Positions that a query sees up to its own (0: all of them):
         ``neuron_config.attention_window``, or the checkpoint's ``sliding_window``
-        where its ``use_sliding_window`` is set."""
+        where its ``use_sliding_window`` is set (null: no window; absent: 4096, the
+        default of the published config class)."""
         w = self.neuron_config.attention_window
         if w is None:
-            w = getattr(self, "sliding_window", None) if getattr(self, "use_sliding_window", False) else 0
+            w = getattr(self, "sliding_window", 4096) if getattr(self, "use_sliding_window", False) else 0
         w = int(w or 0)
         if w < 0:
             raise ValueError(f"sliding_window must not be negative (got {w})")
