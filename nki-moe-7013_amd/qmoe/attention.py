@@ -38,11 +38,17 @@ CHUNK_DECODE_MAX = 16
 @dataclass
 class SharedPrefix:
     """Keys and values of the tokens that every sequence of a batch starts with,
-    held once: ``k``, ``v`` bf16 ``[Hkv, P_max, D]``, of which ``length`` entries."""
+    held once: ``k``, ``v`` bf16 ``[Hkv, P_max, D]``, of which ``length`` entries
+    that were kept of ``tokens`` (default: all of them)."""
 
     k: torch.Tensor
     v: torch.Tensor
     length: int
+    tokens: Optional[int] = None
+
+    def __post_init__(self):
+        if self.tokens is None:
+            self.tokens = self.length
 
 
 class KVCache:
@@ -260,17 +266,20 @@ class Attention:
         :class:`BoundedKVCache`: a decode row's entry goes to slot
         ``state.slots[b]`` and the weights of its attention to the scores; a
         prompt (``start`` 0, ``state.lengths`` real tokens a row) is attended
-        in full and then cut down to the budget.  Neither goes with a window.
+        in full and then cut down to the budget.  Neither goes with a window that
+        hides one of the positions that there are (those of the prefix and of the
+        RoPE tables).
 
         A :class:`KV4Cache`: a prompt (``start`` 0) attends its own keys and values
         in bf16 and leaves them in 4 bits; steps and later chunks attend the
         entries.
         """
         if cache.prefix is not None or isinstance(cache, BoundedKVCache):
-            if self.window:
+            before = 0 if cache.prefix is None else cache.prefix.tokens
+            if 0 < self.window < before + rope_cos.shape[0]:
                 raise ValueError("a shared prefix or a bounded cache has no window")
             o = self._special(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
-        elif isinstance(cache, KV4Cache) or self._hides(S, cache, start, max_ctx):
+        elif isinstance(cache, KV4Cache) or self._hides(S, cache, rope_cos, start, max_ctx):
             o = self._windowed(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
         else:
             o = self._plain(x, positions, B, S, cache, rope_cos, rope_sin, start, max_ctx, norm)
@@ -381,10 +390,11 @@ class Attention:
         gemv = ops.qkv_norm_rope_workspace(rows, x.shape[1], self.n_q, self.n_kv, self.head_dim) > 0
         return ops.gemm(x, self.wqkv, _lib.GEMM_STORE_F32) if gemv or self._skinny_decode(x, rows) else None
 
-    def _hides(self, S: int, cache: KVCache, start, max_ctx: Optional[int]) -> bool:
+    def _hides(self, S: int, cache: KVCache, rope_cos: torch.Tensor, start, max_ctx: Optional[int]) -> bool:
         """Whether the window leaves out an entry that some query could see: none in a
-        bucket or up to a prompt's end that is no longer than it."""
-        end = cache.capacity if max_ctx is None else min(max_ctx, cache.capacity)
+        bucket, up to a prompt's end or in tables that are no longer than it."""
+        end = min(cache.capacity, rope_cos.shape[0])
+        end = end if max_ctx is None else min(max_ctx, end)
         if S > 1 and not isinstance(start, torch.Tensor):
             end = min(end, start + S)
         return 0 < self.window < end

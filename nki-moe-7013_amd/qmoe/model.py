@@ -141,9 +141,18 @@ class Qwen3MoeInferenceConfig:
         w = int(w or 0)
         if w < 0:
             raise ValueError(f"sliding_window must not be negative (got {w})")
-        if w and self.neuron_config.kv_cache_budget:
+        if 0 < w < self.positions() and self.neuron_config.kv_cache_budget:
             raise ValueError("kv_cache_budget keeps entries by their weight: it goes with no attention window")
         return w
+
+    def positions(self) -> int:
+        """Positions of a sequence: what the model's RoPE tables cover."""
+        return min(int(self.max_position_embeddings), int(self.neuron_config.max_length) + 1)
+
+    def hides(self) -> bool:
+        """Whether the window hides a position from some query (one as long as the
+        sequence hides none)."""
+        return 0 < self.window() < self.positions()
 
     def shape(self) -> Qwen3MoeShape:
         return Qwen3MoeShape(**{k: getattr(self, k) for k in Qwen3MoeShape().to_dict()})
@@ -356,8 +365,7 @@ class NeuronQwen3MoeModel:
         self.norm = RMSNormWeight(params["norm"], config.rms_norm_eps)
         self.lm_head = params["lm_head"]
         dev = self.embed_tokens.device
-        max_pos = min(int(config.max_position_embeddings), int(config.neuron_config.max_length) + 1)
-        self.rope = self.rope_full = rope_tables(config.head_dim, max_pos, float(config.rope_theta), dev)
+        self.rope = self.rope_full = rope_tables(config.head_dim, config.positions(), float(config.rope_theta), dev)
         self.base = 0  # tokens of a shared prefix: the position of cache index 0, where ``rope`` starts
         self.budget: Optional[CacheBudget] = None
         self.allocations = 0  # of caches and prefixes: a captured step is good for those it was captured with
@@ -399,7 +407,7 @@ class NeuronQwen3MoeModel:
 
     def plain_attention(self) -> bool:
         """Whether caches are in bf16 and a query sees every position up to its own."""
-        return self.config.neuron_config.kv_cache_bits == 16 and self.config.window() == 0
+        return self.config.neuron_config.kv_cache_bits == 16 and not self.config.hides()
 
     def set_prefix(self, input_ids: torch.Tensor, budget: int = 0, recent: int = 0, sink: int = 0) -> None:
         """Runs ``input_ids[1, P]`` and makes its keys and values (cut down to
@@ -439,7 +447,7 @@ class NeuronQwen3MoeModel:
             for l, cache in zip(self.layers, own):
                 l.cache = cache
         for cache, m in zip(own, made):
-            cache.prefix = SharedPrefix(m.k[0], m.v[0], n)
+            cache.prefix = SharedPrefix(m.k[0], m.v[0], n, P)
         self.base = P
         self.rope = tuple(t[P:] for t in self.rope_full)
 
@@ -733,9 +741,10 @@ class NeuronQwen3MoeForCausalLM:
 
     def _check_steps(self, first: int, end: int) -> None:
         """Refuses steps at positions outside ``[0, _positions())`` on caches with a
-        prefix, a budget, a window or 4 bits: there the step's entry is rejected, its
-        zero query gives every entry the same weight, and a bounded row moves on to
-        a slot that holds nothing.  (A plain cache's step is a zero row.)"""
+        prefix, a budget, a window that hides something or 4 bits: there the step's
+        entry is rejected, its zero query gives every entry the same weight, and a
+        bounded row moves on to a slot that holds nothing.  (A plain cache's step is
+        a zero row.)"""
         if not self._plain() and (first < 0 or end > self._positions()):
             raise ValueError(f"steps at positions {first} to {end - 1}: there are {self._positions()}"
                              + (f" after a prefix of {self.model.base}" if self.model.base else ""))
