@@ -129,6 +129,7 @@ class Qwen3MoeInferenceConfig:
         self.router_dtype = torch.float32
         self.router_act_fn = "softmax"
         self.normalize_top_k_affinities = True
+        self.window()  # options that do not go together are refused before any weight is read
 
     def window(self) -> int:
         """Positions that a query sees up to its own (0: all of them):

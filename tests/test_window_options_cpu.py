@@ -104,3 +104,17 @@ def test_the_layer_takes_special_caches_unless_its_window_hides_something(monkey
     else:
         call()
     assert len(called) == (not hides)
+
+
+# ------------------------------------------------------------------ refusals
+def test_a_budget_with_a_window_that_hides_something_is_refused_by_the_config():
+    """Before any weight is read; a checkpoint's own window too."""
+    for extra, kw in ((None, dict(attention_window=32)), ({"use_sliding_window": True}, dict(max_length=5000)),
+                      ({"use_sliding_window": True, "sliding_window": 77}, {})):
+        with pytest.raises(ValueError, match="window"):
+            _config(extra, kv_cache_budget=64, **kw)
+    for extra, kw in ((None, dict(attention_window=641)), ({"use_sliding_window": True}, {}),
+                      ({"use_sliding_window": True, "sliding_window": 77}, dict(attention_window=0))):
+        assert not _config(extra, kv_cache_budget=64, **kw).hides()
+    with pytest.raises(ValueError, match="negative"):
+        _config({"sliding_window": -5, "use_sliding_window": True})
