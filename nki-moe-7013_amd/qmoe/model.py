@@ -982,6 +982,7 @@ class NeuronQwen3MoeForCausalLM:
         cap = self.model.layers[0].cache.capacity
         if T0 + max_new_tokens > cap:
             raise ValueError(f"prompt + new tokens ({T0}+{max_new_tokens}) exceed the cache ({cap})")
+        self._check_steps(T0, T0 + max_new_tokens - 1)
         self.reset()
         seq = prompt[0].tolist()
         if max_new_tokens <= 0:

@@ -118,3 +118,32 @@ def test_a_budget_with_a_window_that_hides_something_is_refused_by_the_config():
         assert not _config(extra, kv_cache_budget=64, **kw).hides()
     with pytest.raises(ValueError, match="negative"):
         _config({"sliding_window": -5, "use_sliding_window": True})
+
+
+@pytest.mark.parametrize("kw", [dict(kv_cache_bits=4), dict(attention_window=5)], ids=str)
+def test_speculation_past_the_last_position_is_refused_before_it_begins(kw):
+    """As the plain steps are: a verified token there would come from a zero query."""
+    m = _Causal(batch=1, max_position_embeddings=14, **kw)
+    assert m._positions() == 14 and m.model.caches()[0].capacity == 21
+    greedy = lambda ids, n: (m.reset(), m.prefill(ids), m.greedy_decode(ids[:, -1], n - 1, use_graph=False))
+    for new in (6, 9):
+        with pytest.raises(ValueError, match="steps at positions"):
+            greedy(_tokens(1, 10), new)
+        n = len(m.calls)
+        with pytest.raises(ValueError, match="steps at positions"):
+            m.spec_generate(_tokens(1, 10), new)
+        assert len(m.calls) == n
+    greedy(_tokens(1, 10), 5)  # the last of five tokens is not stepped
+    m.greedy_decode = lambda tok, k: torch.ones(1, 1, dtype=torch.long)
+    m._verify_graph = lambda S: pytest.fail("no candidates here")
+    out, _ = m.spec_generate(torch.arange(10).view(1, 10) + 20, 5, ngram=9, ngram_min=9)
+    assert out.shape == (1, 15)
+
+
+def test_speculation_past_the_last_position_of_plain_caches():
+    """Not refused, as the plain steps are not."""
+    m = _Causal(batch=1, max_position_embeddings=14, attention_window=14)
+    m.greedy_decode = lambda tok, k: torch.ones(1, 1, dtype=torch.long)
+    m._verify_graph = lambda S: pytest.fail("no candidates here")
+    out, _ = m.spec_generate(torch.arange(10).view(1, 10) + 20, 9, ngram=9, ngram_min=9)
+    assert out.shape == (1, 19)
