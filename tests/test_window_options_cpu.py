@@ -133,7 +133,7 @@ def test_speculation_past_the_last_position_is_refused_before_it_begins(kw):
         with pytest.raises(ValueError, match="steps at positions"):
             m.spec_generate(_tokens(1, 10), new)
         assert len(m.calls) == n
-    greedy(_tokens(1, 10), 5)  # the last of five tokens is not stepped
+    m._top(torch.tensor([10]), 4)  # four steps give five tokens with the prompt's
     m.greedy_decode = lambda tok, k: torch.ones(1, 1, dtype=torch.long)
     m._verify_graph = lambda S: pytest.fail("no candidates here")
     out, _ = m.spec_generate(torch.arange(10).view(1, 10) + 20, 5, ngram=9, ngram_min=9)
