@@ -413,8 +413,7 @@ class Attention:
         if S > 1 and not isinstance(start, torch.Tensor):
             top = min(cache.capacity, start + S)
         if four and not prompt:
-            q = ops.kv4_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, positions, positions, self.n_q,
-                               self.n_kv, cache.tensors, self.eps, S=S)
+            q = self._append4(raw, positions, B, S, cache.tensors, rope_cos, rope_sin)
             return ops.attn_kv4(q, cache.tensors, first + 1, B, S, self.window, self.sink, self.scale, max_ctx=top)
         own = cache.rows.of(B, self.n_kv, S, self.head_dim, x.device) if four else cache
         if raw is not None:
@@ -432,6 +431,27 @@ class Attention:
             return ops.attn_prefill(q, own.k, own.v, B, S, 0, self.scale,
                                     workspace=ops.attn_prefill_workspace(B, S, self.n_q, self.head_dim, x.device))
         return ops.attn_window(q, own.k, own.v, first + 1, B, S, self.window, self.sink, self.scale, max_ctx=top)
+
+    def _append4(self, raw, positions, B: int, S: int, cache: ops.KV4, rope_cos, rope_sin) -> torch.Tensor:
+        """``kv4_append`` of any number of tokens, which a call takes fewer than 65536
+        of: rows of the batch at a time, or tokens of a row that has more."""
+        def call(raw, at, cache, S, q=None):
+            return ops.kv4_append(raw, self.q_norm, self.k_norm, rope_cos, rope_sin, at, at, self.n_q, self.n_kv, cache,
+                                  self.eps, S=S, q_out=q)
+
+        most = (1 << 16) - 1
+        if B * S <= most:
+            return call(raw, positions, cache, S)
+        q = torch.empty(B * S, self.n_q, self.head_dim, dtype=torch.bfloat16, device=raw.device)
+        rows, tokens = max(most // S, 1), min(most, S)
+        for b in range(0, B, rows):
+            part = tuple(t[b:b + rows] for t in cache)
+            for s in range(0, S, tokens):
+                n = min(tokens, S - s)
+                first = b * S + s
+                to = first + part[0].shape[0] * n
+                call(raw[first:to], positions[first:to], part, n, q[first:to])
+        return q
 
     def _raw_of_any(self, x: torch.Tensor) -> torch.Tensor:
         """The raw projection of rows that ``_skinny_decode`` leaves to

@@ -9,7 +9,7 @@ import torch
 
 from qmoe import model as qm
 from qmoe import ops
-from qmoe.attention import Attention, BoundedKVCache, CacheBudget, KVCache, SharedPrefix
+from qmoe.attention import Attention, BoundedKVCache, CacheBudget, KV4Cache, KVCache, SharedPrefix
 from test_cache_model_cpu import _Causal, _tokens
 
 
@@ -147,3 +147,49 @@ def test_speculation_past_the_last_position_of_plain_caches():
     m._verify_graph = lambda S: pytest.fail("no candidates here")
     out, _ = m.spec_generate(torch.arange(10).view(1, 10) + 20, 9, ngram=9, ngram_min=9)
     assert out.shape == (1, 19)
+
+
+# ------------------------------------------------------------------ large chunks
+@pytest.mark.parametrize("B,S,calls", [(2, 5, 1), (1, 65535, 1), (64, 1024, 2), (3, 30000, 2), (7, 40000, 7),
+                                       (2, 70000, 4), (1, 131070, 2), (60000, 2, 2)])
+def test_chunks_of_any_size_go_to_a_cache_of_four_bits(monkeypatch, B, S, calls):
+    """A call of the append takes fewer than 65536 tokens: every token of a larger chunk
+    goes once, with its own position, row of the batch and query."""
+    d, h = 128, 512
+    w = torch.ones(d, dtype=torch.bfloat16)
+    a = Attention(torch.zeros(3 * d, h, dtype=torch.bfloat16), w, w, torch.zeros(h, d, dtype=torch.bfloat16), 1, 1, d,
+                  1e-6)
+    token = torch.arange(B * S, dtype=torch.float32).view(-1, 1)
+    seen, made, count = [], [], [0]
+
+    def append(qkv, qn, kn, cos, sin, positions, slots, hq, hkv, cache, eps, S=1, q_out=None):
+        n = qkv.shape[0]
+        count[0] += 1
+        assert n < 65536 and n == cache[0].shape[0] * S and torch.equal(positions, slots)
+        first = cache[0].flatten()[0] if cache[0].numel() else 0
+        row = first + torch.arange(cache[0].shape[0]).repeat_interleave(S)
+        seen.append(torch.stack([qkv[:, 0].long(), positions.long(), row]))
+        q_out = torch.empty(n, hq) if q_out is None else q_out
+        q_out.view(n, -1)[:] = (qkv[:, :1] % 251).to(q_out.dtype)  # exact in bf16
+        return q_out
+
+    def attend(q, cache, ctx, B, S, *args, **kw):
+        made.append(q)
+        return torch.zeros(B * S, d, dtype=torch.bfloat16)
+
+    monkeypatch.setattr(ops, "kv4_append", append)
+    monkeypatch.setattr(ops, "attn_kv4", attend)
+    monkeypatch.setattr(ops, "gemm", lambda *args, **kw: None)
+    monkeypatch.setattr(ops, "gemm_workspace", lambda *args: None)
+    monkeypatch.setattr(Attention, "_raw", lambda self, *args: token)
+    cache = KV4Cache(1, 1, 1, d, "cpu")
+    cache.tensors = tuple(torch.arange(B).view(B, 1, 1, 1) for _ in range(4))
+    cache.k = torch.empty(B, 1, 1 << 20, 0)
+    positions = (9 + torch.arange(S, dtype=torch.int32)).repeat(B)
+    rope = torch.zeros(1, d // 2)
+    a.forward(torch.zeros(B * S, h, dtype=torch.bfloat16)[:0], torch.zeros(0, h), positions, B, S, cache, rope, rope, 9)
+    assert count[0] == calls
+    seen = torch.cat(seen, 1)
+    assert torch.equal(seen[0], torch.arange(B * S)) and torch.equal(seen[1], positions.long())
+    assert torch.equal(seen[2], torch.arange(B).repeat_interleave(S))
+    assert torch.equal(made[0].view(B * S, -1)[:, 0].float(), token[:, 0] % 251)
