@@ -427,7 +427,7 @@ class Attention:
         if four:
             ops.kv4_store(own.k, own.v, cache.tensors, n=S)
             top = S
-        if not self.window:
+        if prompt and not 0 < self.window < S:
             return ops.attn_prefill(q, own.k, own.v, B, S, 0, self.scale,
                                     workspace=ops.attn_prefill_workspace(B, S, self.n_q, self.head_dim, x.device))
         return ops.attn_window(q, own.k, own.v, first + 1, B, S, self.window, self.sink, self.scale, max_ctx=top)

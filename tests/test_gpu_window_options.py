@@ -11,13 +11,13 @@ from test_gpu_cache_model import _model, _tokens
 pytestmark = pytest.mark.gpu
 
 
-@pytest.mark.parametrize("kind", ["plain", "prefix", "prefix cut down", "budget"])
+@pytest.mark.parametrize("kind", ["plain", "prefix", "prefix cut down", "budget", "4 bits"])
 def test_a_window_of_all_positions_changes_no_bit(dev, kind):
     """Prompts, captured and eager steps and, on plain caches, steps past the last
     position are those of a model without a window."""
     announce(f"a window of all positions, {kind}")
     B = 2
-    kw = dict(kv_cache_budget=24, kv_cache_slack=4) if kind == "budget" else {}
+    kw = {"budget": dict(kv_cache_budget=24, kv_cache_slack=4), "4 bits": dict(kv_cache_bits=4)}.get(kind, {})
     models = [_model(B, 60, **kw), _model(B, 60, attention_window=61, attention_sink=3, **kw)]
     prompts, lengths = _tokens(2, B, 33), torch.tensor([33, 20])
     steps = [_tokens(3 + i, B) for i in range(4)]

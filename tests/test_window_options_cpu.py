@@ -106,6 +106,26 @@ def test_the_layer_takes_special_caches_unless_its_window_hides_something(monkey
     assert len(called) == (not hides)
 
 
+@pytest.mark.parametrize("window,S,plain", [(0, 8, True), (8, 8, True), (7, 8, False), (9, 8, True), (20, 21, False)])
+def test_a_prompt_no_longer_than_the_window_is_attended_without_it(monkeypatch, window, S, plain):
+    """Also on its way to a cache in 4 bits."""
+    d, h = 128, 512
+    w = torch.ones(d, dtype=torch.bfloat16)
+    a = Attention(torch.zeros(3 * d, h, dtype=torch.bfloat16), w, w, torch.zeros(h, d, dtype=torch.bfloat16), 1, 1, d,
+                  1e-6, window, 2)
+    called = []
+    for name in ("attn_window", "attn_prefill"):
+        monkeypatch.setattr(ops, name, lambda *args, name=name, **kw: called.append(name) or torch.zeros(S, d))
+    for name in ("qkv_norm_rope", "gemm", "gemm_workspace", "kv4_store", "attn_prefill_workspace"):
+        monkeypatch.setattr(ops, name, lambda *args, **kw: None)
+    monkeypatch.setattr(ops, "qkv_norm_rope_workspace", lambda *args: 0)
+    rope = torch.zeros(30, d // 2)
+    for cache in (KV4Cache(1, 1, 30, d, "cpu"), KVCache(1, 1, 30, d, "cpu")):
+        a.forward(torch.zeros(S, h, dtype=torch.bfloat16), torch.zeros(S, h), torch.arange(S, dtype=torch.int32), 1, S,
+                  cache, rope, rope)
+    assert called == ["attn_prefill" if plain else "attn_window"] * 2
+
+
 # ------------------------------------------------------------------ refusals
 def test_a_budget_with_a_window_that_hides_something_is_refused_by_the_config():
     """Before any weight is read; a checkpoint's own window too."""
