@@ -225,15 +225,17 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
 
 // An item of a windowed attention: row tile, kv head, sequence and a run of the keys
 // that the tile's queries see, the window's behind the first ones that stay (the
-// windows of consecutive queries are one run of rows).  Bound by the matrix pipe with
-// the softmax's VALU work beside it, as attn_rows_kernel (2 prompts of 8192 with a window of
-// 1024 + 4: 259 GFLOP in 300 us, 860 TFLOP/s; without a window, on qmoe_attn_prefill's
-// work, 1040).  A tile's key steps are few in a window (17 of 64 keys): what is lost is
-// the masked parts of its first and last ones (5.5%) and the start of its pipeline (9%).  In
-// 4 bits a step converts its K and V on the way to LDS: 2.47 us where bf16 has 2.14 (4 x
-// 301 queries on 2900 entries, 54 GFLOP: 86-90 us with the merge, 600-630 TFLOP/s; 912
-// items of 3 runs on 512 places, a ninth of the time idle).  A prompt of 640 with a window
-// of 250 is the chain of one tile's five steps, its start and its end: 14 us.
+// windows of consecutive queries are one run of rows).  Bound by the matrix pipe with the
+// softmax's VALU work beside it, as attn_rows_kernel (2 prompts of 8192 with a window of
+// 1024 + 4: 259 GFLOP in 309-314 us a call among others, 825-840 TFLOP/s, and 368 in the
+// first calls after a pause; without a window, on qmoe_attn_prefill's work, 1040).  A
+// tile's key steps are few in a window (17 of 64 keys): what is lost is the masked parts
+// of its first and last ones (5.5%) and the start of its pipeline (9%).  In 4 bits a step
+// converts its K and V on the way to LDS: 2.47 us where bf16 has 2.14 (4 x 301 queries on
+// 2900 entries, 54 GFLOP: 86-87 us a call with the merge, 620-630 TFLOP/s, of which under
+// a profiler, that keeps the launches apart, 82 and 12; 912 items of 3 runs on 512
+// places, a ninth of the time idle).  A prompt of 640 with a window of 250 is the chain
+// of one tile's five steps, its start and its end: 14 us.
 template <bool KV4>
 __global__ __launch_bounds__(256, 2) void attn_window_kernel(const ArArgs a) {
   __shared__ __attribute__((aligned(1024))) uint8_t smem[FL_SMEM];

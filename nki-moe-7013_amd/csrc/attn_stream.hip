@@ -10,8 +10,8 @@
 //
 // Work: 4 * 128 flops a (query head, key), 512 bytes a (kv head, key) in bf16 and 136 in 4
 // bits.  8 query heads on a kv head are 8 flops a byte, or 30: the stream from memory
-// bounds a long batch in bf16 (32 rows that see 4100 keys each, 269 MB in 48 us and 4 for
-// the merge, 5.2 TB/s in all, a large copy's rate) and a very long one in 4 bits (64 rows
+// bounds a long batch in bf16 (32 rows that see 4100 keys each, 269 MB in 49 us and 5 for
+// the merge, 5.0 TB/s in all, of a large copy's 5.2) and a very long one in 4 bits (64 rows
 // of up to 32768, 714 MB in 138 us, 5.2 TB/s).  Shorter ones in 4 bits are that rate and 11 us of
 // launches, first loads, joins and the merge (32 rows of up to 8192 25 us, of up to 16384
 // 42).  Few keys are a chain: lengths, queries and keys, one step or two (of 3300 cycles in 4
@@ -624,7 +624,11 @@ static AsArgs as_args(bool four, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, 
 // at most four steps a CU in all.  A stream's 16 rows take nearly twice as long over many
 // keys as their share of a tile's 128, but end sooner over few (1 x 100 queries on 1000
 // entries in 4 bits, tiles / streams: 15.4 / 10.4 us; 8 x 12 with a window of 512 14.5 /
-// 12.3; but 8 x 24 16.2 / 17.5, a prompt of 640 with a window of 250 14.5 / 21.5).
+// 12.3; but 8 x 24 16.2 / 17.5, a prompt of 640 with a window of 250 14.5 / 21.5).  The bound
+// is where the windowed ones cross.  In 4 bits there are shapes on both sides past it: 4 x
+// 301 queries on 2900 (28 x the bound) 87 / 124, 4 x 100 on 1422 28.0 / 33.1, 6 x 46 on 1203
+// 23.2 / 24.4, but 1 x 200 on 1000 (1.6 x) 18.0 / 14.0, 1 x 392 on 392 16.7 / 14.4, 8 x 24 on
+// 2000 (3 x) 25.0 / 23.0.
 static bool as_few(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t max_ctx, int64_t window,
                    int64_t sink) {
   const int64_t rows = S * (Hq / Hkv), items = B * Hkv * ((rows + AS_ROWS - 1) / AS_ROWS);

@@ -10,9 +10,9 @@ namespace qmoe {
 // Rows go through in chunks of KS_ROWS of a (sequence, kv head), 16 lanes a row: lane
 // p % 16 has 8 elements, 16 bytes in bf16 and 4 in codes, so that a wave's loads and
 // stores are whole lines; all of a thread's loads are in flight at once.  Bound by memory:
-// 512 + 136 bytes a (token, kv head), two prompts of 8192 (42 MB each way) 8.6 us to the
-// cache and 8.2 back, 5 TB/s, of which a launch is 2; a lane a block, 32 bytes apart, took
-// 29.6 us for both instead of 17.2.
+// 512 + 136 bytes a (token, kv head), two prompts of 8192 (42 MB each way) 9.3 us to the
+// cache and 8.7 back under a profiler, 16.6 for both among other calls, 5 TB/s; a lane a
+// block, 32 bytes apart, took 29.6 us for both instead of 17.2.
 constexpr int KS_UNROLL = 4, KS_ROWS = 16 * KS_UNROLL;
 
 template <int CTRL>
@@ -124,7 +124,7 @@ __device__ __forceinline__ void kv4_put(uint8_t* codes, uint8_t* powers, int hal
 }
 
 // Bound by latency: one launch, one round trip for the row and one for the tables at its
-// position (1 row 2.9 us, 64 rows 3.8; 20 KB of the projection a row of 40 heads).
+// position (1 row 3.2 us, 64 rows 3.9; 20 KB of the projection a row of 40 heads).
 // One wave a (head, token): lane l holds elements l and l + 64, which RoPE pairs.
 // Queries are computed in 32 bits, as in kv_append; keys in 64, because a key next
 // to the border of two numbers is half a number off if it lands on the wrong side
