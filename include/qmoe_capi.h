@@ -670,8 +670,8 @@ int64_t qmoe_kv_evict_workspace(int64_t B, int64_t Hkv, int64_t S_max, int64_t b
  *   max_ctx) bytes (NULL when that is 0), holding nothing between calls; calls
  *   that share one must not overlap.  out: bf16 [B*S, Hq*D], not overlapping q.
  *   The entries that some query of a chunk sees have to be finite (a NaN value
- *   reaches the queries that do not see it); entries that no query sees are not
- *   read.  Deterministic; calls of another max_ctx may differ in the last bits.
+ *   reaches the queries that do not see it); entries that no query sees may hold
+ *   anything.  Deterministic; calls of another max_ctx may differ in the last bits.
  *   Limits: D == 128, Hq / Hkv <= 16, S_max <= 2^22, B * S * Hq < 2^27.
  * Replaces: the attention of NeuronQwen3MoEAttention (qwen_with_nki.py:9943-9946,
  *   10081-10109) for a checkpoint whose config sets use_sliding_window; the

@@ -227,7 +227,7 @@ __global__ __launch_bounds__(256, 2) void attn_rows_kernel(const ArArgs a) {
 // that the tile's queries see, the window's behind the first ones that stay (the
 // windows of consecutive queries are one run of rows).  Bound by the matrix pipe with the
 // softmax's VALU work beside it, as attn_rows_kernel (2 prompts of 8192 with a window of
-// 1024 + 4: 259 GFLOP in 309-314 us a call among others, 825-840 TFLOP/s, and 368 in the
+// 1024 + 4: 259 GFLOP in 303-314 us a call among others, 825-855 TFLOP/s, and 368 in the
 // first calls after a pause; without a window, on qmoe_attn_prefill's work, 1040).  A
 // tile's key steps are few in a window (17 of 64 keys): what is lost is the masked parts
 // of its first and last ones (5.5%) and the start of its pipeline (9%).  In 4 bits a step
